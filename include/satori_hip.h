@@ -35,6 +35,9 @@ typedef struct satori_hip_matrix satori_hip_matrix;
 typedef struct satori_hip_group satori_hip_group;
 typedef struct satori_hip_step satori_hip_step;
 typedef struct satori_hip_gguf satori_hip_gguf;
+typedef struct satori_hip_pages satori_hip_pages;
+typedef struct satori_hip_cache_plan satori_hip_cache_plan;
+typedef struct satori_hip_adapters satori_hip_adapters;
 
 typedef enum satori_hip_status {
     SATORI_HIP_OK = 0,
@@ -60,6 +63,12 @@ typedef enum satori_hip_format {
     SATORI_HIP_Q6_K = 3,
     SATORI_HIP_TERNARY2 = 16
 } satori_hip_format;
+
+/* Element types of key/value pages and adapters. */
+typedef enum satori_hip_element {
+    SATORI_HIP_F32 = 0,
+    SATORI_HIP_F16 = 1
+} satori_hip_element;
 
 /* ---- library ---- */
 
@@ -415,6 +424,103 @@ int satori_hip_grouped_attention_static(satori_hip_context* context, const float
  * Q8_0 / Q4_K / Q6_K matrix decoded to FP32 `columns` floats (QuantizedRow.DecodeRow), bit-identical to the
  * reference's decode. Q4_0 and Ternary2 fail with SATORI_HIP_E_NOT_SUPPORTED. */
 int satori_hip_matrix_decode_row(satori_hip_matrix* matrix, int row, float* output, void* stream);
+
+/* ---- several sequences at once: pages that sequences share ----
+ * No counterpart in the reference, whose DenseSession (src/Satori.Core/Model/DenseSession.cs:20) keeps one sequence's
+ * keys and values in arrays of its own. A key/value cache here is a pool of pages of `page_tokens` positions (32, 64, 128
+ * or 256), a page holding them for every layer; sequences list the pages they hold, and sequences forked from one another
+ * hold the same ones. satori_hip_pages keeps the lists and reference counts on the host (no device call, no context; a
+ * handle's calls exclude one another); the pages' bytes are the caller's pool on the device. Where a call says that page
+ * bytes must follow, it gives moves (source page, destination page), which the caller hands to
+ * satori_hip_cache_copy_pages before anything reads or writes the destinations. Sources and destinations of one call's
+ * moves are different pages. A call that fails changes nothing. New pages and sequence numbers are the lowest free ones. */
+int satori_hip_pages_create(int page_count, int page_tokens, satori_hip_pages** pages);
+/* Idempotent: NULL is accepted. */
+int satori_hip_pages_destroy(satori_hip_pages* pages);
+/* A new sequence without tokens. */
+int satori_hip_pages_open(satori_hip_pages* pages, int* sequence);
+/* Makes sequences[i] longer by tokens[i] (>= 0) positions that no other sequence holds. A last page that is part full and
+ * shared is replaced by one of its own, with a move; the last holder left keeps the page. At most `count` moves, and the
+ * arrays (of `capacity`) must hold that many; a sequence listed twice fails with SATORI_HIP_E_ARGUMENT, too few free
+ * pages with SATORI_HIP_E_OUT_OF_MEMORY. */
+int satori_hip_pages_extend(satori_hip_pages* pages, const int* sequences, const int* tokens, int count, int* sources,
+                            int* destinations, int capacity, int* moves);
+/* Shortens a sequence to its first `tokens` positions and gives up the pages behind them. */
+int satori_hip_pages_truncate(satori_hip_pages* pages, int sequence, int tokens);
+/* `count` new sequences with the tokens of `sequence`, in the same pages. */
+int satori_hip_pages_fork(satori_hip_pages* pages, int sequence, int count, int* forks);
+/* A new sequence with the tokens of `sequence` in pages of its own: a move per page. */
+int satori_hip_pages_copy(satori_hip_pages* pages, int sequence, int* copy, int* sources, int* destinations,
+                          int capacity, int* moves);
+/* Ends sequences; pages that nobody holds any more are free. */
+int satori_hip_pages_free(satori_hip_pages* pages, const int* sequences, int count);
+/* Moves the pages in use to the front: afterwards n pages in use are pages 0 .. n - 1. A move per page that was behind. */
+int satori_hip_pages_compact(satori_hip_pages* pages, int* sources, int* destinations, int capacity, int* moves);
+int satori_hip_pages_free_count(satori_hip_pages* pages, int* free_pages);
+/* A sequence's length and its pages in order; any out pointer may be NULL. */
+int satori_hip_pages_sequence(satori_hip_pages* pages, int sequence, int* tokens, int* table, int capacity, int* count);
+
+/* Bytes of a page: [layers][keys, values], a layer's keys [kv_heads][page_tokens][width] and its values
+ * [kv_heads][width][page_tokens] (transposed: the order in which the attention's matrix instructions take them), `width`
+ * being head_dim rounded up to 32, 64, 96, 128, 192 or 256 (SATORI_HIP_E_NOT_SUPPORTED past that), of the satori_hip_element
+ * `type`. */
+int satori_hip_cache_page_bytes(int layers, int kv_heads, int head_dim, int page_tokens, int type, int64_t* bytes);
+/* Copies page sources[i] of the pool to page destinations[i], i < count, enqueued on `stream` (NULL: the context stream).
+ * The arrays are on the host and read before the call returns (a captured call keeps what it was given). No page may be
+ * written twice, or both read and written (SATORI_HIP_E_ARGUMENT). */
+int satori_hip_cache_copy_pages(satori_hip_context* context, void* pool, int64_t page_bytes, int page_count,
+                                const int* sources, const int* destinations, int count, void* stream);
+
+/* ---- a batch over the pages ----
+ * A plan is the device's picture of one batch: which positions of which sequences its rows are, where they lie in the
+ * pool, and how their attention is divided. satori_hip_cache_plan_set makes it once for all layers of a step; the calls
+ * below then run per layer over device pointers. Rows are the last new_tokens[i] positions of sequences[i] (0: none), in
+ * that order, so extend the sequences first; a sequence listed twice fails with SATORI_HIP_E_ARGUMENT. A plan shows the
+ * pages as they were when it was set: set it again after any change to its sequences and after a compaction. The copy to
+ * the device is enqueued on `stream`, so the launches that read it must follow on that stream (or be ordered by the
+ * caller); not while capturing. A captured step reads the plan when it is replayed: capture a step once, then extend, set
+ * and replay it per token, with as many rows as its other launches were captured with. While steps read a plan, a batch
+ * that needs more memory than the largest before fails with SATORI_HIP_E_INVALID_OPERATION. Each plan owns the workspace
+ * of its attention, so calls on one plan must not overlap in time on different streams; different plans may. The pool must
+ * be 16-byte aligned and outlive the plan; destroy plans before their context. */
+int satori_hip_cache_plan_create(satori_hip_context* context, void* pool, int page_count, int layers, int query_heads,
+                                 int kv_heads, int head_dim, int page_tokens, int type, satori_hip_cache_plan** plan);
+int satori_hip_cache_plan_set(satori_hip_cache_plan* plan, satori_hip_pages* pages, const int* sequences,
+                              const int* new_tokens, int count, void* stream);
+/* Fails with SATORI_HIP_E_ARGUMENT while a step reads the plan. */
+int satori_hip_cache_plan_destroy(satori_hip_cache_plan* plan);
+/* The attention inputs of every row (satori_hip_attention_inputs, with the same values): bias adds (biases may be NULL),
+ * RopeHalf at the row's position of the query into query_out (which may be query) and of the key into its page, the value
+ * into its page, rounded once more to the pages' type. query and query_out [rows][query_heads * head_dim], key and value
+ * [rows][kv_heads * head_dim]. rope_table: satori_hip_rope_table of `rope_positions` rows for (rotary_dimensions,
+ * frequency_base), or NULL; angles of positions past it are computed in the launch. Writing to a page that several
+ * sequences hold fails with SATORI_HIP_E_INVALID_OPERATION. */
+int satori_hip_cache_append(satori_hip_cache_plan* plan, int layer, const float* query, const float* query_bias,
+                            float* query_out, const float* key, const float* key_bias, const float* value,
+                            const float* value_bias, double frequency_base, int rotary_dimensions,
+                            const double* rope_table, int rope_positions, void* stream);
+/* GroupedAttention (src/Satori.Core/TransformerOps.cs:135-179) of every row over the positions of its sequence up to its
+ * own. Pages that several sequences of the batch hold are read once for all of them: the tables are divided where they
+ * part, each part is attended by the rows below it, and the partial results are joined. FP32 scores, maxima and sums
+ * (the single-sequence attention's are FP64); of F16 pages every bit is used, and queries and probabilities keep 22. A row
+ * that sees a key or value that is not finite gives outputs that are not finite (NaN where the definition may give an
+ * infinity); what a row does not see never reaches it. query and output [rows][query_heads * head_dim], not overlapping. */
+int satori_hip_cache_attention(satori_hip_cache_plan* plan, int layer, const float* query, float* output, void* stream);
+
+/* ---- low-rank adapters of many requests beside one projection ----
+ * No counterpart in the reference. output[r] = base[r] + scale * up (down input[r]) with the adapter selection[r] of each
+ * row, or base[r] where it is -1: `base` being the shared projection's output over the same rows (output may be base).
+ * Adapter i: down[i] [ranks[i]][columns] and up[i] [rows][ranks[i]] on the device, row-major, of the satori_hip_element
+ * `type`, which the caller keeps alive; ranks 1 .. 512. selection is on the host and read before the call returns (a
+ * captured call keeps it). Sums in FP32. Applications of one handle share its workspace and must not overlap in time on
+ * different streams. Destroy adapters before their context. */
+int satori_hip_adapters_create(satori_hip_context* context, int rows, int columns, int type, int count,
+                               const void* const* down, const void* const* up, const int* ranks, const float* scales,
+                               satori_hip_adapters** adapters);
+int satori_hip_adapters_apply(satori_hip_adapters* adapters, const int* selection, int positions, const float* input,
+                              const float* base, float* output, void* stream);
+/* Fails with SATORI_HIP_E_ARGUMENT while a step applies the adapters. */
+int satori_hip_adapters_destroy(satori_hip_adapters* adapters);
 
 /* ---- GGUF containers (src/Satori.Formats.Gguf) ----
  * A GGUF v3 file mapped read-only and its catalogue parsed strictly, with the reference's limits and

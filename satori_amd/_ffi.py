@@ -15,6 +15,7 @@ P = ctypes.c_void_p
 I = ctypes.c_int
 SZ = ctypes.c_size_t
 PP = ctypes.POINTER(ctypes.c_void_p)
+PI = ctypes.POINTER(ctypes.c_int)
 
 # name -> argument types; every entry point returns int (status) except the two noted.
 SIGNATURES = {
@@ -79,6 +80,27 @@ SIGNATURES = {
     "satori_hip_add_rms_norm": (I, [P, P, P, P, ctypes.c_float, I, P, P]),
     "satori_hip_attention_inputs": (I, [P, P, P, P, P, P, P, P, P, I, I, I, I, ctypes.c_double, I, P]),
     "satori_hip_matrix_decode_row": (I, [P, I, P, P]),
+    "satori_hip_pages_create": (I, [I, I, PP]),
+    "satori_hip_pages_destroy": (I, [P]),
+    "satori_hip_pages_open": (I, [P, PI]),
+    "satori_hip_pages_extend": (I, [P, P, P, I, P, P, I, PI]),
+    "satori_hip_pages_truncate": (I, [P, I, I]),
+    "satori_hip_pages_fork": (I, [P, I, I, P]),
+    "satori_hip_pages_copy": (I, [P, I, PI, P, P, I, PI]),
+    "satori_hip_pages_free": (I, [P, P, I]),
+    "satori_hip_pages_compact": (I, [P, P, P, I, PI]),
+    "satori_hip_pages_free_count": (I, [P, PI]),
+    "satori_hip_pages_sequence": (I, [P, I, PI, P, I, PI]),
+    "satori_hip_cache_page_bytes": (I, [I, I, I, I, I, ctypes.POINTER(ctypes.c_int64)]),
+    "satori_hip_cache_copy_pages": (I, [P, P, ctypes.c_int64, I, P, P, I, P]),
+    "satori_hip_cache_plan_create": (I, [P, P, I, I, I, I, I, I, I, PP]),
+    "satori_hip_cache_plan_set": (I, [P, P, P, P, I, P]),
+    "satori_hip_cache_plan_destroy": (I, [P]),
+    "satori_hip_cache_append": (I, [P, I, P, P, P, P, P, P, P, ctypes.c_double, I, P, I, P]),
+    "satori_hip_cache_attention": (I, [P, I, P, P, P]),
+    "satori_hip_adapters_create": (I, [P, I, I, I, I, P, P, P, P, PP]),
+    "satori_hip_adapters_apply": (I, [P, P, I, P, P, P, P]),
+    "satori_hip_adapters_destroy": (I, [P]),
     "satori_hip_gguf_open": (I, [ctypes.c_char_p, PP]),
     "satori_hip_gguf_close": (I, [P]),
     "satori_hip_gguf_data_offset": (I, [P, ctypes.POINTER(ctypes.c_int64)]),

@@ -23,8 +23,8 @@ ARCH = "gfx950"
 
 SOURCES = ["satori_hip.hip", "gemv_float.hip", "gemv_t2.hip", "gemv_kint.hip", "gemv_kmfma.hip", "gemv_fbatch.hip",
            "scale_check.hip", "host_copy.hip", "upload.hip",
-           "transformer_ops.hip",
-           "host_cpu.cpp", "gguf.cpp"]
+           "transformer_ops.hip", "cache_ops.hip", "adapters.hip",
+           "host_cpu.cpp", "gguf.cpp", "pages.cpp"]
 
 COMMON = ["-O3", "-std=c++17", "-fPIC", "-ffp-contract=off", "-Wall", "-Wno-unused-function"]
 HIP_ONLY = [f"--offload-arch={ARCH}", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",

@@ -1,0 +1,234 @@
+"""Several sequences over one key/value cache: pages that sequences share (satori_hip_pages_*), the plan of a batch over
+them and its cache write and attention (satori_hip_cache_*).
+
+The reference keeps one sequence per DenseSession (src/Satori.Core/Model/DenseSession.cs:20); this is the form for hosts
+that answer several requests at once. A step of a batch: extend the sequences by their new positions, set the plan, then per
+layer append (bias, rotation, cache write) and attend; projections run over the batch's rows as positions.
+"""
+from __future__ import annotations
+
+import ctypes
+import enum
+from collections.abc import Sequence
+from dataclasses import dataclass
+
+import numpy as np
+
+from . import ArgumentException, HipContext, _check, _ffi
+
+
+class ElementType(enum.IntEnum):
+    F32 = 0
+    F16 = 1
+
+
+def _ints(values) -> np.ndarray:
+    return np.ascontiguousarray(values, dtype=np.int32).reshape(-1)
+
+
+def _at(array: np.ndarray) -> ctypes.c_void_p:
+    return ctypes.c_void_p(array.ctypes.data)
+
+
+def _pointer(address: int) -> ctypes.c_void_p:
+    return ctypes.c_void_p(address or None)
+
+
+class PageTable:
+    """Page lists and reference counts of a cache of `page_count` pages (satori_hip_pages): host only. Calls that need
+    page bytes to follow return them as moves, (sources, destinations)."""
+
+    def __init__(self, page_count: int, page_tokens: int = 32):
+        handle = ctypes.c_void_p()
+        _check(_ffi.lib().satori_hip_pages_create(page_count, page_tokens, ctypes.byref(handle)))
+        self._handle = handle
+        self.page_count, self.page_tokens = page_count, page_tokens
+
+    @property
+    def handle(self) -> ctypes.c_void_p:
+        return self._handle
+
+    def open(self) -> int:
+        sequence = ctypes.c_int()
+        _check(_ffi.lib().satori_hip_pages_open(self._handle, ctypes.byref(sequence)))
+        return sequence.value
+
+    def extend(self, sequences, tokens) -> tuple[np.ndarray, np.ndarray]:
+        ids, counts = _ints(sequences), _ints(tokens)
+        if ids.size != counts.size:
+            raise ArgumentException("Lengths differ.")
+        sources, destinations, moves = np.empty(ids.size, np.int32), np.empty(ids.size, np.int32), ctypes.c_int()
+        _check(_ffi.lib().satori_hip_pages_extend(self._handle, _at(ids), _at(counts), ids.size, _at(sources),
+                                                  _at(destinations), ids.size, ctypes.byref(moves)))
+        return sources[:moves.value], destinations[:moves.value]
+
+    def truncate(self, sequence: int, tokens: int) -> None:
+        _check(_ffi.lib().satori_hip_pages_truncate(self._handle, sequence, tokens))
+
+    def fork(self, sequence: int, count: int = 1) -> list[int]:
+        forks = np.empty(max(count, 0), np.int32)
+        _check(_ffi.lib().satori_hip_pages_fork(self._handle, sequence, count, _at(forks)))
+        return forks.tolist()
+
+    def copy(self, sequence: int) -> tuple[int, tuple[np.ndarray, np.ndarray]]:
+        most = self._describe(sequence)[1]
+        sources, destinations = np.empty(most, np.int32), np.empty(most, np.int32)
+        made, moves = ctypes.c_int(), ctypes.c_int()
+        _check(_ffi.lib().satori_hip_pages_copy(self._handle, sequence, ctypes.byref(made), _at(sources),
+                                                _at(destinations), most, ctypes.byref(moves)))
+        return made.value, (sources[:moves.value], destinations[:moves.value])
+
+    def free(self, sequences) -> None:
+        ids = _ints(sequences)
+        _check(_ffi.lib().satori_hip_pages_free(self._handle, _at(ids), ids.size))
+
+    def compact(self) -> tuple[np.ndarray, np.ndarray]:
+        most = self.page_count - self.free_pages
+        sources, destinations, moves = np.empty(most, np.int32), np.empty(most, np.int32), ctypes.c_int()
+        _check(_ffi.lib().satori_hip_pages_compact(self._handle, _at(sources), _at(destinations), most,
+                                                   ctypes.byref(moves)))
+        return sources[:moves.value], destinations[:moves.value]
+
+    @property
+    def free_pages(self) -> int:
+        count = ctypes.c_int()
+        _check(_ffi.lib().satori_hip_pages_free_count(self._handle, ctypes.byref(count)))
+        return count.value
+
+    def _describe(self, sequence: int) -> tuple[int, int]:
+        tokens, count = ctypes.c_int(), ctypes.c_int()
+        _check(_ffi.lib().satori_hip_pages_sequence(self._handle, sequence, ctypes.byref(tokens), None, 0,
+                                                    ctypes.byref(count)))
+        return tokens.value, count.value
+
+    def tokens(self, sequence: int) -> int:
+        return self._describe(sequence)[0]
+
+    def pages(self, sequence: int) -> list[int]:
+        table = np.empty(self._describe(sequence)[1], np.int32)
+        _check(_ffi.lib().satori_hip_pages_sequence(self._handle, sequence, None, _at(table), table.size, None))
+        return table.tolist()
+
+    def dispose(self) -> None:
+        _check(_ffi.lib().satori_hip_pages_destroy(self._handle))
+
+
+@dataclass(frozen=True)
+class CacheLayout:
+    """What a page holds: `page_tokens` positions' keys and values of every layer."""
+    layers: int
+    kv_heads: int
+    head_dim: int
+    page_tokens: int = 32
+    type: ElementType = ElementType.F16
+
+    @property
+    def page_bytes(self) -> int:
+        count = ctypes.c_int64()
+        _check(_ffi.lib().satori_hip_cache_page_bytes(self.layers, self.kv_heads, self.head_dim, self.page_tokens,
+                                                      int(self.type), ctypes.byref(count)))
+        return count.value
+
+
+class PagedCache:
+    """A pool of pages on the device with its page table: the calls of PageTable, with the page bytes moved on the
+    context stream. `pool` is a device pointer to page_count * layout.page_bytes bytes; 0: allocated here."""
+
+    def __init__(self, context: HipContext, layout: CacheLayout, page_count: int, pool: int = 0):
+        self.context, self.layout, self.page_count = context, layout, page_count
+        self.page_bytes = layout.page_bytes
+        self.table = PageTable(page_count, layout.page_tokens)
+        self._owned = 0
+        if not pool:
+            self._owned = pool = context.alloc(page_count * self.page_bytes)
+        self.pool = pool
+
+    def _move(self, moves: tuple[np.ndarray, np.ndarray]) -> None:
+        sources, destinations = moves
+        if sources.size:
+            _check(_ffi.lib().satori_hip_cache_copy_pages(self.context.handle, _pointer(self.pool), self.page_bytes,
+                                                          self.page_count, _at(sources), _at(destinations),
+                                                          sources.size, None))
+
+    def open(self) -> int:
+        return self.table.open()
+
+    def extend(self, sequences, tokens) -> None:
+        """Makes room for tokens[i] more positions of sequences[i]."""
+        self._move(self.table.extend(sequences, tokens))
+
+    def truncate(self, sequence: int, tokens: int) -> None:
+        self.table.truncate(sequence, tokens)
+
+    def fork(self, sequence: int, count: int = 1) -> list[int]:
+        return self.table.fork(sequence, count)
+
+    def copy(self, sequence: int) -> int:
+        made, moves = self.table.copy(sequence)
+        self._move(moves)
+        return made
+
+    def free(self, sequences) -> None:
+        self.table.free(sequences)
+
+    def compact(self) -> None:
+        self._move(self.table.compact())
+
+    def tokens(self, sequence: int) -> int:
+        return self.table.tokens(sequence)
+
+    def pages(self, sequence: int) -> list[int]:
+        return self.table.pages(sequence)
+
+    @property
+    def free_pages(self) -> int:
+        return self.table.free_pages
+
+    def plan(self, heads: int) -> "CachePlan":
+        """A plan of batches with `heads` query heads over this cache."""
+        return CachePlan(self, heads)
+
+    def dispose(self) -> None:
+        """Frees the page table and a pool allocated here; plans are disposed of first."""
+        self.table.dispose()
+        if self._owned:
+            self.context.free(self._owned)
+            self._owned = 0
+
+
+class CachePlan:
+    """One batch over a PagedCache (satori_hip_cache_plan). Device pointers are ints; `stream` 0 is the context
+    stream."""
+
+    def __init__(self, cache: PagedCache, heads: int):
+        layout = cache.layout
+        handle = ctypes.c_void_p()
+        _check(_ffi.lib().satori_hip_cache_plan_create(cache.context.handle, _pointer(cache.pool), cache.page_count,
+                                                       layout.layers, heads, layout.kv_heads, layout.head_dim,
+                                                       layout.page_tokens, int(layout.type), ctypes.byref(handle)))
+        self.cache, self.heads = cache, heads
+        self._handle = handle
+
+    def set(self, sequences: Sequence[int], new_tokens: Sequence[int], stream: int = 0) -> None:
+        """The batch's rows: the last new_tokens[i] positions of sequences[i]."""
+        ids, counts = _ints(sequences), _ints(new_tokens)
+        if ids.size != counts.size:
+            raise ArgumentException("Lengths differ.")
+        _check(_ffi.lib().satori_hip_cache_plan_set(self._handle, self.cache.table.handle, _at(ids), _at(counts),
+                                                    ids.size, _pointer(stream)))
+
+    def append(self, layer: int, q: int, q_bias: int, q_out: int, k: int, k_bias: int, v: int, v_bias: int, base: float,
+               rotary: int, rope_table: int = 0, rope_positions: int = 0, stream: int = 0) -> None:
+        """Bias, rotation and cache write of every row (biases and rope_table may be 0); q_out may be q."""
+        _check(_ffi.lib().satori_hip_cache_append(self._handle, layer, _pointer(q), _pointer(q_bias), _pointer(q_out),
+                                                  _pointer(k), _pointer(k_bias), _pointer(v), _pointer(v_bias),
+                                                  float(base), rotary, _pointer(rope_table), rope_positions,
+                                                  _pointer(stream)))
+
+    def attention(self, layer: int, q: int, out: int, stream: int = 0) -> None:
+        """Grouped attention of every row over the positions of its sequence up to its own."""
+        _check(_ffi.lib().satori_hip_cache_attention(self._handle, layer, _pointer(q), _pointer(out),
+                                                     _pointer(stream)))
+
+    def dispose(self) -> None:
+        _check(_ffi.lib().satori_hip_cache_plan_destroy(self._handle))

@@ -1,0 +1,608 @@
+// Pages of a shared key/value cache (PageTables), the plan of a batch over them (plan_batch) and the host-only entry
+// points satori_hip_pages_*. No device code.
+#include "pages.hpp"
+
+#include <algorithm>
+#include <climits>
+#include <cstring>
+#include <new>
+#include <string>
+#include <unordered_map>
+
+#include "../../include/satori_hip.h"
+#include "host_shapes.hpp"
+
+namespace satori {
+
+namespace {
+
+[[noreturn]] void out_of_range(const char* name) {
+    fail(SATORI_HIP_E_ARGUMENT_OUT_OF_RANGE,
+         std::string("Specified argument was out of the range of valid values. (Parameter '") + name + "')");
+}
+
+// push_back after this does not allocate.
+template <class T>
+void reserve_for(std::vector<T>& v, size_t n) {
+    if (v.capacity() < n) v.reserve(std::max(n, 2 * v.capacity()));
+}
+
+}  // namespace
+
+PageTables::PageTables(int pages, int page_tokens) : page_tokens_(page_tokens), free_(pages) {
+    if (pages <= 0) out_of_range("pageCount");
+    if (!valid_page_tokens(page_tokens))
+        fail(SATORI_HIP_E_ARGUMENT_OUT_OF_RANGE, "Supported page sizes: 32, 64, 128 and 256 tokens.");
+    if (static_cast<int64_t>(pages) * page_tokens > INT32_MAX)
+        fail(SATORI_HIP_E_OVERFLOW, "Arithmetic operation resulted in an overflow.");
+    references_.resize(pages);
+}
+
+const PageTables::Sequence& PageTables::at(int sequence) const {
+    if (sequence < 0 || static_cast<size_t>(sequence) >= sequences_.size() || !sequences_[sequence].open)
+        fail(SATORI_HIP_E_ARGUMENT, "There is no open sequence " + std::to_string(sequence) + ".");
+    return sequences_[sequence];
+}
+
+void PageTables::require_distinct(const int* sequences, int count) const {
+    std::vector<int> sorted(sequences, sequences + count);
+    std::sort(sorted.begin(), sorted.end());
+    if (std::adjacent_find(sorted.begin(), sorted.end()) != sorted.end())
+        fail(SATORI_HIP_E_ARGUMENT, "A sequence is listed twice.");
+    for (int s : sorted) at(s);
+}
+
+int PageTables::take_page() {
+    while (references_[lowest_] != 0) ++lowest_;
+    references_[lowest_] = 1;
+    --free_;
+    return lowest_++;
+}
+
+void PageTables::drop_page(int page) {
+    if (--references_[page] == 0) {
+        ++free_;
+        lowest_ = std::min(lowest_, page);
+    }
+}
+
+int PageTables::next_sequence() {
+    for (size_t i = 0; i < sequences_.size(); ++i)
+        if (!sequences_[i].open) return static_cast<int>(i);
+    if (sequences_.size() >= INT32_MAX) fail(SATORI_HIP_E_OVERFLOW, "Arithmetic operation resulted in an overflow.");
+    sequences_.emplace_back();
+    return static_cast<int>(sequences_.size() - 1);
+}
+
+void PageTables::close() {
+    live_ = false;
+    std::vector<int>().swap(references_);
+    std::vector<Sequence>().swap(sequences_);
+}
+
+int PageTables::open() {
+    const int s = next_sequence();
+    sequences_[s].open = true;
+    return s;
+}
+
+void PageTables::extend(const int* sequences, const int* tokens, int count, std::vector<PageMove>& moves) {
+    require_distinct(sequences, count);
+    // What the call takes, before anything changes: sequences that share a part full page are asked in order, and
+    // the last holder left keeps it.
+    int64_t need = 0;
+    std::unordered_map<int, int> left;
+    for (int i = 0; i < count; ++i) {
+        if (tokens[i] < 0) out_of_range("tokens");
+        Sequence& s = sequences_[sequences[i]];
+        const int64_t total = static_cast<int64_t>(s.tokens) + tokens[i];
+        if (total > INT32_MAX) fail(SATORI_HIP_E_OVERFLOW, "Arithmetic operation resulted in an overflow.");
+        const int pages = pages_of(total);
+        need += pages - static_cast<int>(s.table.size());
+        if (tokens[i] > 0 && s.tokens % page_tokens_ != 0 && references_[s.table.back()] > 1) {
+            auto it = left.emplace(s.table.back(), references_[s.table.back()]).first;
+            if (it->second > 1) {
+                --it->second;
+                ++need;
+            }
+        }
+    }
+    if (need > free_)
+        fail(SATORI_HIP_E_OUT_OF_MEMORY, "The cache has " + std::to_string(free_) + " free pages; " +
+                                             std::to_string(need) + " are needed.");
+    reserve_for(moves, moves.size() + count);
+    for (int i = 0; i < count; ++i) {
+        Sequence& s = sequences_[sequences[i]];
+        reserve_for(s.table, pages_of(static_cast<int64_t>(s.tokens) + tokens[i]));
+    }
+    for (int i = 0; i < count; ++i) {
+        Sequence& s = sequences_[sequences[i]];
+        if (tokens[i] > 0 && s.tokens % page_tokens_ != 0 && references_[s.table.back()] > 1) {
+            const int page = take_page();
+            moves.push_back({s.table.back(), page});
+            drop_page(s.table.back());
+            s.table.back() = page;
+        }
+        s.tokens += tokens[i];
+        while (static_cast<int>(s.table.size()) < pages_of(s.tokens)) s.table.push_back(take_page());
+    }
+}
+
+void PageTables::truncate(int sequence, int tokens) {
+    at(sequence);
+    Sequence& s = sequences_[sequence];
+    if (tokens < 0 || tokens > s.tokens) out_of_range("tokens");
+    s.tokens = tokens;
+    while (static_cast<int>(s.table.size()) > pages_of(tokens)) {
+        drop_page(s.table.back());
+        s.table.pop_back();
+    }
+}
+
+void PageTables::fork(int sequence, int count, int* forks) {
+    at(sequence);
+    if (count < 0) out_of_range("count");
+    const Sequence parent = sequences_[sequence];
+    std::vector<Sequence> made(count, parent);  // what allocates comes first
+    size_t free_numbers = 0;
+    for (const Sequence& s : sequences_) free_numbers += !s.open;
+    if (static_cast<size_t>(count) > free_numbers) reserve_for(sequences_, sequences_.size() + count - free_numbers);
+    for (int i = 0; i < count; ++i) {
+        const int s = next_sequence();
+        sequences_[s] = std::move(made[i]);
+        forks[i] = s;
+    }
+    for (int page : parent.table) references_[page] += count;
+}
+
+int PageTables::copy(int sequence, std::vector<PageMove>& moves) {
+    at(sequence);
+    const size_t pages = sequences_[sequence].table.size();
+    if (static_cast<int64_t>(pages) > free_)
+        fail(SATORI_HIP_E_OUT_OF_MEMORY, "The cache has " + std::to_string(free_) + " free pages; " +
+                                             std::to_string(pages) + " are needed.");
+    reserve_for(moves, moves.size() + pages);
+    std::vector<int> table;
+    table.reserve(pages);
+    const int s = next_sequence();
+    for (int page : sequences_[sequence].table) {
+        table.push_back(take_page());
+        moves.push_back({page, table.back()});
+    }
+    sequences_[s].open = true;
+    sequences_[s].tokens = sequences_[sequence].tokens;
+    sequences_[s].table = std::move(table);
+    return s;
+}
+
+void PageTables::release(const int* sequences, int count) {
+    require_distinct(sequences, count);
+    for (int i = 0; i < count; ++i) {
+        for (int page : sequences_[sequences[i]].table) drop_page(page);
+        sequences_[sequences[i]] = Sequence{};
+    }
+}
+
+void PageTables::compact(std::vector<PageMove>& moves) {
+    const int used = pages() - free_;
+    std::vector<int> to(pages() - used, -1);  // of the pages behind
+    int moved = 0;
+    for (int p = used; p < pages(); ++p) moved += references_[p] != 0;
+    reserve_for(moves, moves.size() + moved);
+    int gap = 0;
+    for (int p = used; p < pages(); ++p) {
+        if (references_[p] == 0) continue;
+        while (references_[gap] != 0) ++gap;
+        references_[gap] = references_[p];
+        references_[p] = 0;
+        to[p - used] = gap;
+        moves.push_back({p, gap});
+    }
+    if (moved == 0) return;
+    for (Sequence& s : sequences_)
+        for (int& page : s.table)
+            if (page >= used) page = to[page - used];
+    lowest_ = used;
+}
+
+// ---- the plan ----
+
+namespace {
+
+constexpr int kTile = 32;         // tokens a wave attends at once
+constexpr int kWaves = 4;         // of a workgroup, which take tiles in turn
+constexpr int kNarrowPairs = 16;  // pairs of a narrow workgroup
+
+// Tokens [begin, end) of the pages of `sequence`, seen by the rows of the sequences members[0 .. count).
+struct Node {
+    int begin, end;
+    std::vector<int> members;  // positions in the batch
+    int ancestors;             // node that the members share before this one, or -1
+    int chunks = 0, slot = 0, chunk = 0;
+    int pages = 0, rows = 0;   // where its lists begin
+    bool wide = false;
+};
+
+// Runs of pages that sequences share but that are shorter than this are read by each of them: one more partial result
+// per row and head (and its joining) costs about what reading so many tokens again does.
+constexpr int kLeastShared = 128;
+
+}  // namespace
+
+PlanImage plan_batch(const PageTables& tables, const int* sequences, const int* new_tokens, int count,
+                     const PlanShape& shape) {
+    PlanImage image;
+    const int P = tables.page_tokens();
+    std::vector<int> sorted(sequences, sequences + count);
+    std::sort(sorted.begin(), sorted.end());
+    if (std::adjacent_find(sorted.begin(), sorted.end()) != sorted.end())
+        fail(SATORI_HIP_E_ARGUMENT, "A sequence is listed twice.");
+    std::vector<int> first_row(count + 1);
+    std::vector<PlanRow> rows;
+    std::vector<PlanRun> runs;
+    for (int i = 0; i < count; ++i) {
+        const int tokens = tables.tokens(sequences[i]);
+        if (new_tokens[i] < 0 || new_tokens[i] > tokens)
+            fail(SATORI_HIP_E_ARGUMENT_OUT_OF_RANGE, "A sequence has fewer tokens than rows.");
+        const int64_t total = static_cast<int64_t>(first_row[i]) + new_tokens[i];
+        if (total * shape.group > INT32_MAX / 2)
+            fail(SATORI_HIP_E_OVERFLOW, "Arithmetic operation resulted in an overflow.");
+        first_row[i + 1] = static_cast<int>(total);
+        const std::vector<int>& table = tables.table(sequences[i]);
+        for (int p = tokens - new_tokens[i]; p < tokens; ++p) {
+            if (p % P == 0 || p == tokens - new_tokens[i]) {
+                runs.push_back({static_cast<int>(rows.size()), 0, table[p / P], p % P});
+                image.writable &= tables.references(table[p / P]) == 1;
+            }
+            runs.back().tokens++;
+            rows.push_back({p, 0, 0, 0});
+            image.last_position = std::max(image.last_position, p);
+        }
+    }
+
+    // The trie of the tables: a node for every run of pages that the same sequences share.
+    std::vector<Node> nodes;
+    struct Open {
+        std::vector<int> members;
+        int page, ancestors;
+    };
+    std::vector<Open> open(1);
+    open[0].page = 0;
+    open[0].ancestors = -1;
+    for (int i = 0; i < count; ++i)
+        if (new_tokens[i] > 0) open[0].members.push_back(i);
+    while (!open.empty()) {
+        Open o = std::move(open.back());
+        open.pop_back();
+        if (o.members.empty()) continue;
+        const std::vector<int>& lead = tables.table(sequences[o.members[0]]);
+        if (o.members.size() == 1) {
+            const int end = tables.tokens(sequences[o.members[0]]);
+            if (o.page * P < end) nodes.push_back({o.page * P, end, o.members, o.ancestors});
+            continue;
+        }
+        size_t common = lead.size();
+        int longest = 0;
+        for (int m : o.members) {
+            const std::vector<int>& t = tables.table(sequences[m]);
+            size_t same = o.page;
+            while (same < std::min(common, t.size()) && t[same] == lead[same]) ++same;
+            common = same;
+            longest = std::max(longest, tables.tokens(sequences[m]));
+        }
+        const int begin = o.page * P, end = std::min(static_cast<int>(common) * P, longest);
+        int from = o.page, ancestors = o.ancestors;
+        if (end - begin >= kLeastShared) {
+            nodes.push_back({begin, end, o.members, o.ancestors});
+            from = static_cast<int>(common);
+            ancestors = static_cast<int>(nodes.size()) - 1;
+        }
+        // Its members by the page that follows, in the order of their first appearance.
+        std::vector<Open> parts;
+        std::unordered_map<int, size_t> by_page;
+        for (int m : o.members) {
+            const std::vector<int>& t = tables.table(sequences[m]);
+            if (common >= t.size()) {  // nothing follows: what is left of it, if anything, is its own part
+                if (from < static_cast<int>(t.size())) parts.push_back({{m}, from, ancestors});
+                continue;
+            }
+            auto it = by_page.find(t[common]);
+            if (it == by_page.end()) {
+                it = by_page.emplace(t[common], parts.size()).first;
+                parts.push_back({{}, from, ancestors});
+            }
+            parts[it->second].members.push_back(m);
+        }
+        for (auto it = parts.rbegin(); it != parts.rend(); ++it) open.push_back(std::move(*it));
+    }
+
+    // Chunks of tokens: as many as give every CU work (kv heads and blocks of pairs count too), and no shorter than
+    // one tile per wave.
+    const auto blocks_of = [&](const Node& n) {
+        int64_t pairs = 0;
+        for (int m : n.members) pairs += static_cast<int64_t>(new_tokens[m]) * shape.group;
+        return pairs;
+    };
+    int64_t narrow_tokens = 0, wide_tokens = 0;
+    std::vector<int64_t> pairs_of(nodes.size());
+    for (size_t i = 0; i < nodes.size(); ++i) {
+        Node& n = nodes[i];
+        pairs_of[i] = blocks_of(n);
+        n.wide = pairs_of[i] > kNarrowPairs;
+        const int64_t blocks = n.wide ? (pairs_of[i] + shape.wide_pairs - 1) / shape.wide_pairs : 1;
+        (n.wide ? wide_tokens : narrow_tokens) += blocks * shape.kv_heads * (n.end - n.begin);
+    }
+    const auto chunk_for = [&](int64_t tokens, int workgroups) {
+        const int64_t step = kTile * kWaves;
+        const int64_t c = (tokens / workgroups + step - 1) / step * step;
+        return static_cast<int>(std::min<int64_t>(std::max<int64_t>(c, step), 1 << 20));
+    };
+    const int narrow_chunk = chunk_for(narrow_tokens, 1024), wide_chunk = chunk_for(wide_tokens, 256);
+
+    std::vector<int> page_list, row_list;
+    for (Node& n : nodes) {
+        n.chunk = n.wide ? wide_chunk : narrow_chunk;
+        n.chunks = (n.end - n.begin + n.chunk - 1) / n.chunk;
+        n.slot = n.ancestors < 0 ? 0 : nodes[n.ancestors].slot + nodes[n.ancestors].chunks;
+        n.pages = static_cast<int>(page_list.size());
+        const std::vector<int>& table = tables.table(sequences[n.members[0]]);
+        page_list.insert(page_list.end(), table.begin() + n.begin / P, table.begin() + (n.end + P - 1) / P);
+        n.rows = static_cast<int>(row_list.size());
+        for (int m : n.members)
+            for (int r = first_row[m]; r < first_row[m + 1]; ++r) {
+                row_list.push_back(r);
+                rows[r].slots = n.slot + n.chunks;  // a deeper node comes later
+            }
+    }
+    int64_t slots = 0;
+    for (PlanRow& r : rows) {
+        if (slots + r.slots > INT32_MAX) fail(SATORI_HIP_E_OVERFLOW, "Arithmetic operation resulted in an overflow.");
+        r.slot = static_cast<int>(slots);
+        slots += r.slots;
+        image.header.joined += r.slots > 1;
+    }
+    image.header.slots = static_cast<int>(slots);
+
+    // The workgroups. Consecutive workgroups run on different XCDs (eight, each with an L2 of its own), so the blocks of
+    // pairs that read the same tokens are put eight apart.
+    std::vector<PlanItem> narrow, wide;
+    for (size_t i = 0; i < nodes.size(); ++i) {
+        const Node& n = nodes[i];
+        const int step = n.wide ? shape.wide_pairs : kNarrowPairs;
+        const int blocks = static_cast<int>((pairs_of[i] + step - 1) / step);
+        const int64_t units = static_cast<int64_t>(n.chunks) * shape.kv_heads;
+        std::vector<PlanItem>& list = n.wide ? wide : narrow;
+        if (static_cast<int64_t>(list.size()) + units * blocks > INT32_MAX / 32)
+            fail(SATORI_HIP_E_OVERFLOW, "Arithmetic operation resulted in an overflow.");
+        for (int64_t u0 = 0; u0 < units; u0 += 8)
+            for (int b = 0; b < blocks; ++b)
+                for (int64_t u = u0; u < std::min<int64_t>(u0 + 8, units); ++u) {
+                    const int chunk = static_cast<int>(u / shape.kv_heads);
+                    PlanItem item{};
+                    item.first = n.begin + chunk * n.chunk;
+                    item.tokens = std::min(n.chunk, n.end - item.first);
+                    item.pages = n.pages + item.first / P - n.begin / P;
+                    item.rows = n.rows;
+                    item.pair = b * step;
+                    item.pairs = static_cast<int>(std::min<int64_t>(step, pairs_of[i] - item.pair));
+                    item.slot = n.slot + chunk;
+                    item.kv = static_cast<int>(u % shape.kv_heads);
+                    int least = INT_MAX, most = 0;
+                    for (int r = item.pair / shape.group; r <= (item.pair + item.pairs - 1) / shape.group; ++r) {
+                        const int position = rows[row_list[n.rows + r]].position;
+                        least = std::min(least, position);
+                        most = std::max(most, position);
+                    }
+                    item.limit = least;
+                    // Tokens behind all rows of the block are not read (an empty item still writes its partials).
+                    item.tokens = std::max(0, std::min(item.tokens, most + 1 - item.first));
+                    list.push_back(item);
+                }
+    }
+
+    const auto append = [&](const auto& v) {
+        using T = typename std::decay_t<decltype(v)>::value_type;
+        static_assert(sizeof(T) % 4 == 0, "whole words");
+        const size_t at = (image.words.size() + 3) / 4 * 4;  // 16-byte aligned
+        image.words.resize(at + v.size() * (sizeof(T) / 4));
+        if (!v.empty()) std::memcpy(image.words.data() + at, v.data(), v.size() * sizeof(T));
+        return static_cast<int>(at);
+    };
+    PlanHeader& h = image.header;
+    image.words.resize(sizeof(PlanHeader) / 4);
+    h.rows = static_cast<int>(rows.size());
+    h.narrow = static_cast<int>(narrow.size());
+    h.wide = static_cast<int>(wide.size());
+    h.runs = static_cast<int>(runs.size());
+    h.rows_at = append(rows);
+    h.narrow_at = append(narrow);
+    h.wide_at = append(wide);
+    h.runs_at = append(runs);
+    h.pages_at = append(page_list);
+    h.list_at = append(row_list);
+    image.words.resize((image.words.size() + 3) / 4 * 4);
+    std::memcpy(image.words.data(), &h, sizeof h);
+    return image;
+}
+
+}  // namespace satori
+
+struct satori_hip_pages {
+    satori::PageTables tables;
+    satori_hip_pages(int pages, int page_tokens) : tables(pages, page_tokens) {}
+};
+
+namespace satori {
+
+PageTables& page_tables(satori_hip_pages* handle) { return handle->tables; }
+
+namespace {
+
+template <class F>
+int host_call(F&& body) {
+    try {
+        body();
+        record_error("");
+        return SATORI_HIP_OK;
+    } catch (const Failure& f) {
+        record_error(f.message);
+        return f.status;
+    } catch (const std::bad_alloc&) {
+        record_error("Out of host memory.");
+        return SATORI_HIP_E_OUT_OF_MEMORY;
+    } catch (...) {
+        record_error("Unexpected failure.");
+        return SATORI_HIP_E_DEVICE;
+    }
+}
+
+void require_pointer(const void* p, const char* name) {
+    if (!p) fail(SATORI_HIP_E_ARGUMENT_NULL, std::string("Value cannot be null. (Parameter '") + name + "')");
+}
+
+template <class F>
+int pages_call(satori_hip_pages* handle, F&& body) {
+    return host_call([&] {
+        require_pointer(handle, "pages");
+        std::lock_guard<std::mutex> guard(handle->tables.lock);
+        if (!handle->tables.live())
+            fail(SATORI_HIP_E_OBJECT_DISPOSED, "Cannot access a disposed object. Object name: 'satori_hip_pages'.");
+        body(handle->tables);
+    });
+}
+
+// The caller's arrays hold `capacity` moves. `most` is what the call can need: checked before anything changes.
+void require_capacity(int64_t most, int capacity, const int* sources, const int* destinations) {
+    if (capacity < 0) out_of_range("capacity");
+    if (most > capacity)
+        fail(SATORI_HIP_E_ARGUMENT, "The move arrays hold " + std::to_string(capacity) + " of up to " +
+                                        std::to_string(most) + " moves.");
+    if (most > 0) {
+        require_pointer(sources, "sources");
+        require_pointer(destinations, "destinations");
+    }
+}
+
+void give(const std::vector<PageMove>& moves, int* sources, int* destinations, int* count) {
+    for (size_t i = 0; i < moves.size(); ++i) {
+        sources[i] = moves[i].source;
+        destinations[i] = moves[i].destination;
+    }
+    *count = static_cast<int>(moves.size());
+}
+
+}  // namespace
+}  // namespace satori
+
+using namespace satori;
+
+extern "C" {
+
+int satori_hip_pages_create(int page_count, int page_tokens, satori_hip_pages** pages) {
+    return host_call([&] {
+        require_pointer(pages, "pages");
+        *pages = nullptr;
+        *pages = new satori_hip_pages(page_count, page_tokens);
+    });
+}
+
+int satori_hip_pages_destroy(satori_hip_pages* pages) {
+    return host_call([&] {
+        if (!pages) return;
+        std::lock_guard<std::mutex> guard(pages->tables.lock);
+        pages->tables.close();  // the handle stays valid as a tombstone so a second destroy is a no-op
+    });
+}
+
+int satori_hip_pages_open(satori_hip_pages* pages, int* sequence) {
+    return pages_call(pages, [&](PageTables& t) {
+        require_pointer(sequence, "sequence");
+        *sequence = t.open();
+    });
+}
+
+int satori_hip_pages_extend(satori_hip_pages* pages, const int* sequences, const int* tokens, int count, int* sources,
+                            int* destinations, int capacity, int* moves) {
+    return pages_call(pages, [&](PageTables& t) {
+        require_pointer(moves, "moves");
+        *moves = 0;
+        if (count < 0) out_of_range("count");
+        if (count > 0) {
+            require_pointer(sequences, "sequences");
+            require_pointer(tokens, "tokens");
+        }
+        require_capacity(count, capacity, sources, destinations);
+        std::vector<PageMove> made;
+        t.extend(sequences, tokens, count, made);
+        give(made, sources, destinations, moves);
+    });
+}
+
+int satori_hip_pages_truncate(satori_hip_pages* pages, int sequence, int tokens) {
+    return pages_call(pages, [&](PageTables& t) { t.truncate(sequence, tokens); });
+}
+
+int satori_hip_pages_fork(satori_hip_pages* pages, int sequence, int count, int* forks) {
+    return pages_call(pages, [&](PageTables& t) {
+        if (count > 0) require_pointer(forks, "forks");
+        t.fork(sequence, count, forks);
+    });
+}
+
+int satori_hip_pages_copy(satori_hip_pages* pages, int sequence, int* copy, int* sources, int* destinations,
+                          int capacity, int* moves) {
+    return pages_call(pages, [&](PageTables& t) {
+        require_pointer(copy, "copy");
+        require_pointer(moves, "moves");
+        *moves = 0;
+        require_capacity(static_cast<int64_t>(t.table(sequence).size()), capacity, sources, destinations);
+        std::vector<PageMove> made;
+        *copy = t.copy(sequence, made);
+        give(made, sources, destinations, moves);
+    });
+}
+
+int satori_hip_pages_free(satori_hip_pages* pages, const int* sequences, int count) {
+    return pages_call(pages, [&](PageTables& t) {
+        if (count < 0) out_of_range("count");
+        if (count > 0) require_pointer(sequences, "sequences");
+        t.release(sequences, count);
+    });
+}
+
+int satori_hip_pages_compact(satori_hip_pages* pages, int* sources, int* destinations, int capacity, int* moves) {
+    return pages_call(pages, [&](PageTables& t) {
+        require_pointer(moves, "moves");
+        *moves = 0;
+        const int used = t.pages() - t.free_pages();
+        int64_t most = 0;
+        for (int p = used; p < t.pages(); ++p) most += t.references(p) != 0;
+        require_capacity(most, capacity, sources, destinations);
+        std::vector<PageMove> made;
+        t.compact(made);
+        give(made, sources, destinations, moves);
+    });
+}
+
+int satori_hip_pages_free_count(satori_hip_pages* pages, int* free_pages) {
+    return pages_call(pages, [&](PageTables& t) {
+        require_pointer(free_pages, "freePages");
+        *free_pages = t.free_pages();
+    });
+}
+
+int satori_hip_pages_sequence(satori_hip_pages* pages, int sequence, int* tokens, int* table, int capacity,
+                              int* count) {
+    return pages_call(pages, [&](PageTables& t) {
+        const std::vector<int>& list = t.table(sequence);
+        if (tokens) *tokens = t.tokens(sequence);
+        if (count) *count = static_cast<int>(list.size());
+        if (!table) return;
+        if (capacity < static_cast<int>(list.size()))
+            fail(SATORI_HIP_E_ARGUMENT, "The table holds " + std::to_string(capacity) + " of " +
+                                            std::to_string(list.size()) + " pages.");
+        std::copy(list.begin(), list.end(), table);
+    });
+}
+
+}  // extern "C"

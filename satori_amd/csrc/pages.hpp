@@ -1,0 +1,123 @@
+// Host bookkeeping of a paged key/value cache that sequences share, and the plan of one batch over it: which page
+// holds what, which tokens several rows have in common, and how their attention is cut into workgroups. Plain C++
+// without device calls; the device code reads the plan's image (PlanHeader and the arrays behind it).
+#pragma once
+
+#include <cstdint>
+#include <mutex>
+#include <vector>
+
+struct satori_hip_pages;
+
+namespace satori {
+
+struct PageMove {
+    int source, destination;
+};
+
+inline bool valid_page_tokens(int n) { return n == 32 || n == 64 || n == 128 || n == 256; }
+
+// Reference-counted pages of `page_tokens` positions and the sequences that hold them. Every change is all or nothing:
+// a call that fails leaves everything as it was. New pages and sequence numbers are the lowest free ones, so that the
+// same calls always give the same tables.
+class PageTables {
+public:
+    PageTables(int pages, int page_tokens);
+
+    int open();
+    // Makes room for tokens[i] more positions of sequences[i] that nobody else sees: a last page that is part full and
+    // shared is replaced by a copy of its own (a move), and pages are added behind it.
+    void extend(const int* sequences, const int* tokens, int count, std::vector<PageMove>& moves);
+    void truncate(int sequence, int tokens);
+    // `count` sequences that hold the same pages.
+    void fork(int sequence, int count, int* forks);
+    // A sequence with the same tokens in pages of its own.
+    int copy(int sequence, std::vector<PageMove>& moves);
+    void release(const int* sequences, int count);
+    // Moves every page behind the first n (n pages being in use) into a gap among those, in ascending order of both.
+    void compact(std::vector<PageMove>& moves);
+
+    int pages() const { return static_cast<int>(references_.size()); }
+    int page_tokens() const { return page_tokens_; }
+    int free_pages() const { return free_; }
+    int references(int page) const { return references_[page]; }
+    int tokens(int sequence) const { return at(sequence).tokens; }
+    const std::vector<int>& table(int sequence) const { return at(sequence).table; }
+
+    // For the handle that holds it: calls are made under `lock`, and none but live() after close().
+    std::mutex lock;
+    bool live() const { return live_; }
+    void close();
+
+private:
+    struct Sequence {
+        bool open = false;
+        int tokens = 0;
+        std::vector<int> table;
+    };
+    const Sequence& at(int sequence) const;
+    int pages_of(int64_t tokens) const { return static_cast<int>((tokens + page_tokens_ - 1) / page_tokens_); }
+    void require_distinct(const int* sequences, int count) const;
+    int take_page();
+    void drop_page(int page);
+    int next_sequence();
+
+    bool live_ = true;
+    int page_tokens_;
+    int free_;
+    int lowest_ = 0;  // no page below this one is free
+    std::vector<int> references_;
+    std::vector<Sequence> sequences_;
+};
+
+// ---- the plan of a batch ----
+
+// One query row: attends positions 0 .. position of its sequence. Its attention is the joined result of `slots` partial
+// ones, slot .. slot + slots - 1 (one: written as the output by the workgroup that computes it).
+struct PlanRow {
+    int position, slot, slots, pad;
+};
+
+// One workgroup's attention: key/value head `kv`, tokens [first, first + tokens) of the pages listed from `pages` on
+// (the first of them holds token `first`, a multiple of 32), for the (row, query head) pairs pair .. pair + pairs - 1 of
+// the rows listed from `rows` on (pair p: row p / group, head p % group of the key/value head). `slot` counts from the
+// rows' first slots; `limit` is the least position of the rows, so tokens up to it are seen by all of them.
+struct PlanItem {
+    int pages, first, tokens, rows;
+    int pair, pairs, slot, kv;
+    int limit, pad[3];
+};
+
+// Consecutive rows of one sequence whose positions lie in one page: row .. row + tokens - 1 at `offset` of the page.
+struct PlanRun {
+    int row, tokens, page, offset;
+};
+
+// At the start of the image; the offsets count 4-byte words from there.
+struct PlanHeader {
+    int rows, narrow, wide, runs;
+    int rows_at, narrow_at, wide_at, runs_at;
+    int pages_at, list_at, joined, slots;  // joined: rows of several slots; slots: of all rows
+};
+
+struct PlanShape {
+    int kv_heads, group;  // group: query heads of a key/value head
+    int wide_pairs;       // pairs of a wide workgroup; a narrow one takes 16
+};
+
+// The image of a plan and what its launches need to know.
+struct PlanImage {
+    std::vector<int> words;
+    PlanHeader header{};
+    int last_position = 0;
+    bool writable = true;  // no page that the rows lie in is shared
+};
+
+// Rows: the last new_tokens[i] positions of sequences[i], in this order.
+PlanImage plan_batch(const PageTables& tables, const int* sequences, const int* new_tokens, int count,
+                     const PlanShape& shape);
+
+// The tables behind a handle (satori_hip_pages_*).
+PageTables& page_tables(satori_hip_pages* handle);
+
+}  // namespace satori

@@ -15,6 +15,8 @@
 #include <vector>
 
 #include "../../include/satori_hip.h"
+#include "adapters.hpp"
+#include "cache_ops.hpp"
 #include "gguf.hpp"
 #include "host_shapes.hpp"
 #include "kernels.hpp"
@@ -144,6 +146,9 @@ struct satori_hip_context {
     int captured_last[2] = {-1, -1};                     // the two in turn now
     std::vector<satori_hip_matrix*> captured_matrices;
     std::vector<satori_hip_group*> captured_groups;
+    std::vector<satori_hip_cache_plan*> captured_plans;
+    std::vector<satori_hip_adapters*> captured_adapters;
+    int plans = 0, adapters = 0;  // live ones
 };
 
 struct satori_hip_matrix {
@@ -184,6 +189,30 @@ struct satori_hip_group {
     bool live = true;
 };
 
+struct satori_hip_cache_plan {
+    satori_hip_context* context = nullptr;
+    satori::CacheShape shape{};
+    int page_count = 0, layers = 0;
+    satori::PlanShape plan{};
+    satori::PlanHeader header{};     // of the image on the device; rows are 0 before the first satori_hip_cache_plan_set
+    bool set = false, writable = false;
+    satori::DeviceBuffer image, partials;
+    satori::PinnedBuffer staging[2];  // in turn; `copied` tells when the device has read one
+    hipEvent_t copied[2] = {nullptr, nullptr};
+    int turn = 0;
+    int steps = 0;                   // captured steps that read the plan
+    bool live = true;
+};
+
+struct satori_hip_adapters {
+    satori_hip_context* context = nullptr;
+    satori::AdapterShape shape{};
+    int count = 0;
+    satori::DeviceBuffer table, workspace;
+    int steps = 0;
+    bool live = true;
+};
+
 struct satori_hip_gguf {
     satori::GgufFile* file = nullptr;  // null once closed (the handle stays as a tombstone)
     bool live = true;
@@ -195,6 +224,8 @@ struct satori_hip_step {
     std::vector<satori_hip_matrix*> matrices;  // launched directly in a captured step (each counts it)
     std::vector<satori::DeviceBuffer> scratch; // partial sums of its Q8_0 / Q4_0 batches
     bool attention = false;                    // the graph uses the context's split-attention workspace
+    std::vector<satori_hip_cache_plan*> plans; // read by the graph, and what they and the adapters own
+    std::vector<satori_hip_adapters*> adapters;
     hipGraph_t graph = nullptr;
     hipGraphExec_t exec = nullptr;
     bool live = true;
@@ -917,6 +948,8 @@ int satori_hip_context_destroy(satori_hip_context* c) {
         if (!c->live) return;
         if (c->matrices > 0)
             fail(SATORI_HIP_E_ARGUMENT, "Matrices created on the context must be destroyed first.");
+        if (c->plans > 0 || c->adapters > 0)
+            fail(SATORI_HIP_E_ARGUMENT, "Cache plans and adapters created on the context must be destroyed first.");
         (void)hipSetDevice(c->device);
         (void)hipStreamSynchronize(c->stream);
         c->x.release();
@@ -1589,6 +1622,10 @@ int satori_hip_step_destroy(satori_hip_step* s) {
         }
         if (s->attention) c->attention_steps--;
         s->attention = false;
+        for (satori_hip_cache_plan* p : s->plans) p->steps--;
+        for (satori_hip_adapters* a : s->adapters) a->steps--;
+        s->plans.clear();
+        s->adapters.clear();
         s->groups.clear();
         s->matrices.clear();
         s->live = false;
@@ -1608,6 +1645,8 @@ int satori_hip_capture_begin(satori_hip_context* c) {
         c->capturing = true;
         c->captured_matrices.clear();
         c->captured_groups.clear();
+        c->captured_plans.clear();
+        c->captured_adapters.clear();
         c->captured_attention = false;
     });
 }
@@ -1625,6 +1664,10 @@ int satori_hip_capture_end(satori_hip_context* c, satori_hip_step** step) {
         std::vector<satori_hip_group*> groups;
         matrices.swap(c->captured_matrices);
         groups.swap(c->captured_groups);
+        std::vector<satori_hip_cache_plan*> plans;
+        std::vector<satori_hip_adapters*> adapters;
+        plans.swap(c->captured_plans);
+        adapters.swap(c->captured_adapters);
         struct Scratch {  // freed unless a step takes it
             std::vector<DeviceBuffer> buffers;
             ~Scratch() {
@@ -1658,6 +1701,18 @@ int satori_hip_capture_end(satori_hip_context* c, satori_hip_step** step) {
                 st->matrices.push_back(m);
                 m->groups++;
                 m->steps++;
+            }
+        }
+        for (satori_hip_cache_plan* p : plans) {
+            if (std::find(st->plans.begin(), st->plans.end(), p) == st->plans.end()) {
+                st->plans.push_back(p);
+                p->steps++;
+            }
+        }
+        for (satori_hip_adapters* a : adapters) {
+            if (std::find(st->adapters.begin(), st->adapters.end(), a) == st->adapters.end()) {
+                st->adapters.push_back(a);
+                a->steps++;
             }
         }
         st->attention = c->captured_attention;
@@ -2186,6 +2241,416 @@ int satori_hip_matrix_decode_row(satori_hip_matrix* m, int row, float* output, v
         check_hip(launch_decode_row(m->payload, s.format, s.rows, s.columns, row, output, op_stream(c, stream)),
                   "decode_row launch");
         note_launch(c, m, op_stream(c, stream));
+    });
+}
+
+}  // extern "C"
+
+namespace {
+
+void out_of_range(const char* name) {
+    fail(SATORI_HIP_E_ARGUMENT_OUT_OF_RANGE,
+         std::string("Specified argument was out of the range of valid values. (Parameter '") + name + "')");
+}
+
+void check_rotation(int head_dim, double frequency_base, int rotary_dimensions) {
+    if (!std::isfinite(frequency_base) || frequency_base <= 0) out_of_range("frequencyBase");
+    if (rotary_dimensions <= 0 || rotary_dimensions > head_dim || rotary_dimensions % 2 != 0)
+        out_of_range("rotaryDimensions");
+}
+
+int element_type(int type) {
+    if (type != SATORI_HIP_F32 && type != SATORI_HIP_F16) out_of_range("type");
+    return type;
+}
+
+// The shape of a cache without its pool.
+CacheShape cache_shape(int layers, int query_heads, int kv_heads, int head_dim, int page_tokens, int type) {
+    if (layers <= 0) out_of_range("layers");
+    if (head_dim <= 0 || query_heads <= 0 || kv_heads <= 0 || query_heads % kv_heads != 0)
+        fail(SATORI_HIP_E_ARGUMENT, "Invalid grouped-attention dimensions.");
+    if (!valid_page_tokens(page_tokens))
+        fail(SATORI_HIP_E_ARGUMENT_OUT_OF_RANGE, "Supported page sizes: 32, 64, 128 and 256 tokens.");
+    CacheShape s{};
+    s.type = element_type(type);
+    s.width = cache_width(head_dim);
+    if (s.width == 0) fail(SATORI_HIP_E_NOT_SUPPORTED, "Heads of more than 256 lanes are not kept in pages.");
+    s.heads = query_heads;
+    s.kv_heads = kv_heads;
+    s.head_dim = head_dim;
+    s.page_tokens = page_tokens;
+    while (1 << s.page_shift < page_tokens) ++s.page_shift;
+    const int64_t row = static_cast<int64_t>(kv_heads) * s.width, head = static_cast<int64_t>(query_heads) * head_dim;
+    if (row > INT32_MAX / 512 || head > INT32_MAX / 512)
+        fail(SATORI_HIP_E_OVERFLOW, "Arithmetic operation resulted in an overflow.");
+    s.layer_bytes = 2 * row * page_tokens * element_bytes(type);
+    if (s.layer_bytes > INT64_MAX / layers) fail(SATORI_HIP_E_OVERFLOW, "Arithmetic operation resulted in an overflow.");
+    s.page_bytes = s.layer_bytes * layers;
+    return s;
+}
+
+void require_pool(const void* pool) {
+    require(pool, "pool");
+    if (reinterpret_cast<uintptr_t>(pool) % 16 != 0) fail(SATORI_HIP_E_ARGUMENT, "The pool must be 16-byte aligned.");
+}
+
+// Bytes [a, a + n) and [b, b + m) overlap.
+bool bytes_overlap(const void* a, int64_t n, const void* b, int64_t m) {
+    const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+    return a && b && x < y + static_cast<uintptr_t>(m) && y < x + static_cast<uintptr_t>(n);
+}
+
+// Entry-point frame of the calls on a plan, or on adapters.
+template <class H, class F>
+int handle_call(H* handle, const char* parameter, const char* name, F&& body) {
+    return guarded([&] {
+        require(handle, parameter);
+        satori_hip_context* c = handle->context;
+        std::lock_guard<std::mutex> guard(c->lock);
+        if (!handle->live || !c->live)
+            fail(SATORI_HIP_E_OBJECT_DISPOSED, std::string("Cannot access a disposed object. Object name: '") + name + "'.");
+        set_device(c);
+        body(c);
+    });
+}
+
+template <class F>
+int plan_call(satori_hip_cache_plan* p, F&& body) {
+    return handle_call(p, "plan", "satori_hip_cache_plan", [&](satori_hip_context* c) { body(c); });
+}
+
+// Grows a buffer of the plan, unless a captured step reads it.
+void reserve_for_plan(satori_hip_cache_plan* p, DeviceBuffer& buffer, size_t need) {
+    if (need <= buffer.bytes) return;
+    if (p->steps > 0)
+        fail(SATORI_HIP_E_INVALID_OPERATION,
+             "The memory of this plan cannot grow while a captured step reads it: destroy the step, or set the largest "
+             "batch before capturing.");
+    check_hip(hipDeviceSynchronize(), "device");  // earlier launches on any stream may read the old one
+    buffer.reserve(need + need / 2);
+}
+
+void free_plan(satori_hip_cache_plan* p) {
+    p->image.release();
+    p->partials.release();
+    for (PinnedBuffer& b : p->staging) b.release();
+    for (hipEvent_t& e : p->copied) {
+        if (e) (void)hipEventDestroy(e);
+        e = nullptr;
+    }
+}
+
+// What the calls on a plan ask of it, and whether the launch becomes part of a captured step.
+bool note_plan(satori_hip_context* c, satori_hip_cache_plan* p, int layer, hipStream_t stream) {
+    if (!p->set) fail(SATORI_HIP_E_INVALID_OPERATION, "Set the plan's batch first.");
+    if (layer < 0 || layer >= p->layers) out_of_range("layer");
+    const bool captured = c->capturing && stream == c->stream;
+    if (captured) c->captured_plans.push_back(p);
+    return captured || captured_elsewhere(c, stream);
+}
+
+}  // namespace
+
+extern "C" {
+
+int satori_hip_cache_page_bytes(int layers, int kv_heads, int head_dim, int page_tokens, int type, int64_t* bytes) {
+    return guarded([&] {
+        require(bytes, "bytes");
+        *bytes = cache_shape(layers, kv_heads, kv_heads, head_dim, page_tokens, type).page_bytes;
+    });
+}
+
+int satori_hip_cache_copy_pages(satori_hip_context* c, void* pool, int64_t page_bytes, int page_count,
+                                const int* sources, const int* destinations, int count, void* stream) {
+    return op_call(c, [&] {
+        require_pool(pool);
+        if (page_count <= 0) out_of_range("pageCount");
+        if (page_bytes <= 0 || page_bytes % 16 != 0 || page_bytes > (int64_t(1) << 40)) out_of_range("pageBytes");
+        if (count < 0 || count > page_count) out_of_range("count");
+        if (count == 0) return;
+        require(sources, "sources");
+        require(destinations, "destinations");
+        std::vector<uint8_t> role(page_count);
+        for (int i = 0; i < count; ++i) {
+            if (sources[i] < 0 || sources[i] >= page_count) out_of_range("sources");
+            if (destinations[i] < 0 || destinations[i] >= page_count) out_of_range("destinations");
+            role[sources[i]] = 1;
+        }
+        for (int i = 0; i < count; ++i) {
+            if (role[destinations[i]])
+                fail(SATORI_HIP_E_ARGUMENT, "A page is written twice, or read and written.");
+            role[destinations[i]] = 2;
+        }
+        for (int i0 = 0; i0 < count; i0 += kMovesPerLaunch) {
+            PageMoves moves{};
+            moves.count = std::min(kMovesPerLaunch, count - i0);
+            std::copy(sources + i0, sources + i0 + moves.count, moves.source);
+            std::copy(destinations + i0, destinations + i0 + moves.count, moves.destination);
+            check_hip(launch_copy_pages(static_cast<uint8_t*>(pool), page_bytes, moves, op_stream(c, stream)),
+                      "page copy launch");
+        }
+    });
+}
+
+int satori_hip_cache_plan_create(satori_hip_context* c, void* pool, int page_count, int layers, int query_heads,
+                                 int kv_heads, int head_dim, int page_tokens, int type, satori_hip_cache_plan** plan) {
+    return guarded([&] {
+        require(plan, "plan");
+        *plan = nullptr;
+        require_live(c);
+        std::lock_guard<std::mutex> guard(c->lock);
+        require_live(c);
+        require_not_capturing(c);
+        require_pool(pool);
+        if (page_count <= 0) out_of_range("pageCount");
+        CacheShape shape = cache_shape(layers, query_heads, kv_heads, head_dim, page_tokens, type);
+        if (static_cast<int64_t>(page_count) * page_tokens > INT32_MAX || shape.page_bytes > INT64_MAX / page_count)
+            fail(SATORI_HIP_E_OVERFLOW, "Arithmetic operation resulted in an overflow.");
+        shape.pool = static_cast<uint8_t*>(pool);
+        set_device(c);
+        auto* p = new satori_hip_cache_plan();
+        p->context = c;
+        p->shape = shape;
+        p->page_count = page_count;
+        p->layers = layers;
+        p->plan.kv_heads = kv_heads;
+        p->plan.group = query_heads / kv_heads;
+        p->plan.wide_pairs = cache_wide_pairs(type, shape.width);
+        try {
+            for (hipEvent_t& e : p->copied) check_hip(hipEventCreateWithFlags(&e, hipEventDisableTiming), "hipEventCreate");
+            p->image.reserve(size_t(256) << 10);
+            p->partials.reserve(size_t(4) << 20);
+        } catch (...) {
+            free_plan(p);
+            delete p;
+            throw;
+        }
+        c->plans++;
+        *plan = p;
+    });
+}
+
+int satori_hip_cache_plan_destroy(satori_hip_cache_plan* p) {
+    return guarded([&] {
+        if (!p) return;
+        satori_hip_context* c = p->context;
+        std::lock_guard<std::mutex> guard(c->lock);
+        require_not_capturing(c);
+        if (!p->live) return;
+        if (p->steps > 0) fail(SATORI_HIP_E_ARGUMENT, "Steps that read the plan must be destroyed first.");
+        (void)hipSetDevice(c->device);
+        (void)hipStreamSynchronize(c->stream);
+        free_plan(p);
+        p->live = false;
+        c->plans--;
+    });
+}
+
+int satori_hip_cache_plan_set(satori_hip_cache_plan* p, satori_hip_pages* pages, const int* sequences,
+                              const int* new_tokens, int count, void* stream) {
+    return plan_call(p, [&](satori_hip_context* c) {
+        require(pages, "pages");
+        if (count < 0) out_of_range("count");
+        if (count > 0) {
+            require(sequences, "sequences");
+            require(new_tokens, "newTokens");
+        }
+        const hipStream_t st = op_stream(c, stream);
+        require_not_capturing(c);
+        if (captured_elsewhere(c, st))
+            fail(SATORI_HIP_E_INVALID_OPERATION, "A plan cannot be set while its stream is being captured.");
+        PlanImage image;
+        {
+            PageTables& tables = page_tables(pages);
+            std::lock_guard<std::mutex> tables_guard(tables.lock);
+            if (!tables.live())
+                fail(SATORI_HIP_E_OBJECT_DISPOSED, "Cannot access a disposed object. Object name: 'satori_hip_pages'.");
+            if (tables.pages() != p->page_count || tables.page_tokens() != p->shape.page_tokens)
+                fail(SATORI_HIP_E_ARGUMENT, "The pages are not those of the plan's pool.");
+            image = plan_batch(tables, sequences, new_tokens, count, p->plan);
+        }
+        const size_t bytes = image.words.size() * 4;
+        reserve_for_plan(p, p->image, bytes);
+        reserve_for_plan(p, p->partials, cache_partial_bytes(p->shape, image.header.slots));
+        const int turn = p->turn;
+        check_hip(hipEventSynchronize(p->copied[turn]), "plan copy");  // (done at once where none was recorded)
+        p->staging[turn].reserve(std::max(bytes, p->image.bytes));
+        std::memcpy(p->staging[turn].ptr, image.words.data(), bytes);
+        if (bytes <= kKernelCopyMaxBytes)
+            check_hip(launch_copy_words(p->staging[turn].ptr, p->image.ptr, bytes, st), "plan copy");
+        else
+            check_hip(hipMemcpyAsync(p->image.ptr, p->staging[turn].ptr, bytes, hipMemcpyHostToDevice, st), "plan copy");
+        check_hip(hipEventRecord(p->copied[turn], st), "plan copy");
+        p->turn ^= 1;
+        p->header = image.header;
+        p->writable = image.writable;
+        p->set = true;
+    });
+}
+
+int satori_hip_cache_append(satori_hip_cache_plan* p, int layer, const float* query, const float* query_bias,
+                            float* query_out, const float* key, const float* key_bias, const float* value,
+                            const float* value_bias, double frequency_base, int rotary_dimensions,
+                            const double* rope_table, int rope_positions, void* stream) {
+    return plan_call(p, [&](satori_hip_context* c) {
+        require(query, "query");
+        require(query_out, "queryOut");
+        require(key, "key");
+        require(value, "value");
+        const CacheShape& s = p->shape;
+        check_rotation(s.head_dim, frequency_base, rotary_dimensions);
+        if (rope_positions < 0) out_of_range("ropePositions");
+        const hipStream_t st = op_stream(c, stream);
+        if (!p->set) fail(SATORI_HIP_E_INVALID_OPERATION, "Set the plan's batch first.");
+        if (!p->writable)
+            fail(SATORI_HIP_E_INVALID_OPERATION, "The rows lie in pages that other sequences hold: extend their sequences.");
+        const int64_t rows = p->header.rows, qb = rows * s.heads * s.head_dim * 4, kb = rows * s.kv_heads * s.head_dim * 4;
+        const int64_t pool = s.page_bytes * p->page_count;
+        if ((bytes_overlap(query, qb, query_out, qb) && query != query_out) || bytes_overlap(key, kb, query_out, qb) ||
+            bytes_overlap(value, kb, query_out, qb) || bytes_overlap(query, qb, s.pool, pool) ||
+            bytes_overlap(query_out, qb, s.pool, pool) || bytes_overlap(key, kb, s.pool, pool) ||
+            bytes_overlap(value, kb, s.pool, pool))
+            fail(SATORI_HIP_E_ARGUMENT, "Partial overlap.");
+        const bool captured = note_plan(c, p, layer, st);
+        const AppendArgs args{query, query_bias, key, key_bias, value, value_bias, query_out, frequency_base,
+                              rotary_dimensions, rope_table, rope_table ? rope_positions : 0, layer};
+        check_hip(launch_cache_append(s, static_cast<const int*>(p->image.ptr), captured ? 256 : p->header.runs, args, st),
+                  "cache append launch");
+    });
+}
+
+int satori_hip_cache_attention(satori_hip_cache_plan* p, int layer, const float* query, float* output, void* stream) {
+    return plan_call(p, [&](satori_hip_context* c) {
+        require(query, "query");
+        require(output, "output");
+        const CacheShape& s = p->shape;
+        const hipStream_t st = op_stream(c, stream);
+        const int64_t bytes = static_cast<int64_t>(p->header.rows) * s.heads * s.head_dim * 4;
+        const int64_t pool = s.page_bytes * p->page_count;
+        if (bytes_overlap(query, bytes, output, bytes) || bytes_overlap(output, bytes, s.pool, pool))
+            fail(SATORI_HIP_E_ARGUMENT, "Attention output overlaps input.");
+        const bool captured = note_plan(c, p, layer, st);
+        check_hip(launch_cache_attention(s, static_cast<const int*>(p->image.ptr), p->header, captured, layer, query, output,
+                                         static_cast<float*>(p->partials.ptr), st),
+                  "cache attention launch");
+    });
+}
+
+int satori_hip_adapters_create(satori_hip_context* c, int rows, int columns, int type, int count,
+                               const void* const* down, const void* const* up, const int* ranks, const float* scales,
+                               satori_hip_adapters** adapters) {
+    return guarded([&] {
+        require(adapters, "adapters");
+        *adapters = nullptr;
+        require_live(c);
+        std::lock_guard<std::mutex> guard(c->lock);
+        require_live(c);
+        require_not_capturing(c);
+        if (rows <= 0 || rows > (1 << 23)) out_of_range("rows");
+        if (columns <= 0 || columns > (1 << 24)) out_of_range("columns");
+        if (count <= 0 || count >= kMaxAdapters) out_of_range("count");
+        element_type(type);
+        require(down, "down");
+        require(up, "up");
+        require(ranks, "ranks");
+        require(scales, "scales");
+        AdapterShape shape{};
+        shape.rows = rows;
+        shape.columns = columns;
+        shape.type = type;
+        const uintptr_t unit = element_bytes(type);
+        shape.aligned = columns * unit % 16 == 0 && columns % 4 == 0;
+        std::vector<Adapter> table(count);
+        for (int i = 0; i < count; ++i) {
+            require(down[i], "down");
+            require(up[i], "up");
+            if (ranks[i] <= 0 || ranks[i] > kMaxRank) out_of_range("ranks");
+            if (reinterpret_cast<uintptr_t>(down[i]) % unit != 0 || reinterpret_cast<uintptr_t>(up[i]) % unit != 0)
+                fail(SATORI_HIP_E_ARGUMENT, "Adapter weights must be aligned to their elements.");
+            table[i] = Adapter{down[i], up[i], ranks[i], scales[i]};
+            shape.rank_most = std::max(shape.rank_most, (ranks[i] + 15) / 16 * 16);
+            shape.aligned &= reinterpret_cast<uintptr_t>(down[i]) % 16 == 0;
+        }
+        set_device(c);
+        auto* a = new satori_hip_adapters();
+        a->context = c;
+        a->count = count;
+        try {
+            a->table.reserve(table.size() * sizeof(Adapter));
+            a->workspace.reserve(adapter_workspace_bytes(shape));
+            check_hip(hipMemcpyAsync(a->table.ptr, table.data(), table.size() * sizeof(Adapter), hipMemcpyHostToDevice,
+                                     c->stream),
+                      "adapter table copy");
+            check_hip(hipStreamSynchronize(c->stream), "stream");
+        } catch (...) {
+            a->table.release();
+            a->workspace.release();
+            delete a;
+            throw;
+        }
+        shape.adapters = static_cast<const Adapter*>(a->table.ptr);
+        a->shape = shape;
+        c->adapters++;
+        *adapters = a;
+    });
+}
+
+int satori_hip_adapters_destroy(satori_hip_adapters* a) {
+    return guarded([&] {
+        if (!a) return;
+        satori_hip_context* c = a->context;
+        std::lock_guard<std::mutex> guard(c->lock);
+        require_not_capturing(c);
+        if (!a->live) return;
+        if (a->steps > 0) fail(SATORI_HIP_E_ARGUMENT, "Steps that apply the adapters must be destroyed first.");
+        (void)hipSetDevice(c->device);
+        (void)hipStreamSynchronize(c->stream);
+        a->table.release();
+        a->workspace.release();
+        a->live = false;
+        c->adapters--;
+    });
+}
+
+int satori_hip_adapters_apply(satori_hip_adapters* a, const int* selection, int positions, const float* input,
+                              const float* base, float* output, void* stream) {
+    return handle_call(a, "adapters", "satori_hip_adapters", [&](satori_hip_context* c) {
+        require(selection, "selection");
+        require(input, "input");
+        require(base, "base");
+        require(output, "output");
+        if (positions <= 0) out_of_range("positions");
+        const AdapterShape& s = a->shape;
+        for (int i = 0; i < positions; ++i)
+            if (selection[i] < -1 || selection[i] >= a->count) out_of_range("selection");
+        const int64_t in = static_cast<int64_t>(positions) * s.columns * 4, out = static_cast<int64_t>(positions) * s.rows * 4;
+        if (bytes_overlap(input, in, output, out) || (bytes_overlap(base, out, output, out) && base != output))
+            fail(SATORI_HIP_E_ARGUMENT, "Partial overlap.");
+        const hipStream_t st = op_stream(c, stream);
+        if (c->capturing && st == c->stream) c->captured_adapters.push_back(a);
+        for (int p0 = 0; p0 < positions; p0 += kAdapterRows) {
+            AdapterTiles tiles{};
+            tiles.positions = std::min(kAdapterRows, positions - p0);
+            const int* chosen = selection + p0;
+            for (int i = 0; i < tiles.positions; ++i) tiles.order[i] = static_cast<uint8_t>(i);
+            std::stable_sort(tiles.order, tiles.order + tiles.positions,
+                             [&](uint8_t x, uint8_t y) { return chosen[x] < chosen[y]; });
+            for (int i = 0; i < tiles.positions; ++i) {
+                const int mine = chosen[tiles.order[i]];
+                // Rows without an adapter keep what they have where the output is the base.
+                if (mine < 0 && base == output) continue;
+                const uint16_t id = mine < 0 ? kNoAdapter : static_cast<uint16_t>(mine);
+                if (tiles.tiles == 0 || tiles.adapter[tiles.tiles - 1] != id || i - tiles.begin[tiles.tiles - 1] == 16) {
+                    tiles.adapter[tiles.tiles] = id;
+                    tiles.begin[tiles.tiles++] = static_cast<uint16_t>(i);
+                }
+                tiles.begin[tiles.tiles] = static_cast<uint16_t>(i + 1);
+            }
+            const int64_t at = p0;
+            check_hip(launch_adapters(s, tiles, input + at * s.columns, base + at * s.rows, output + at * s.rows,
+                                      static_cast<float*>(a->workspace.ptr), st),
+                      "adapters launch");
+        }
     });
 }
 

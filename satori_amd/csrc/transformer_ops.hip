@@ -16,6 +16,7 @@
 #include "kernels.hpp"
 #include "ops_device.hpp"
 #include "q8k_device.hpp"
+#include "rope_device.hpp"
 
 // Split-attention partials of the no-allocation entry point: one copy per device, alive until the process
 // ends, shared by every such call on that device (calls that overlap in time race on it). Host code never
@@ -110,30 +111,6 @@ __global__ __launch_bounds__(kThreads) void add_rms_norm_q8k_kernel(float* resid
 // v + v_bias (when the biases are given), then RopeHalf of q and of the key, the key and value written to
 // their cache slots. Same per-element operations as Add and RopeHalf, so the outputs equal the separate
 // calls bit for bit. Threads: q pairs, key pairs, then the unrotated q and key lanes, then the values.
-__device__ __forceinline__ float biased(const float* x, const float* bias, int i) {
-    return bias ? __fadd_rn(x[i], bias[i]) : x[i];
-}
-
-// RopeHalf of lane pair (kk, kk + rotary / 2) of one head (TransformerOps.cs:94-114): the angle
-// position / base^(2 kk / rotary) in FP64, then both rotated lanes in FP64, each rounded once.
-__device__ __forceinline__ void rope_angle(int kk, int position, double base, int rotary, double& sn, double& cs) {
-    const double angle = position / pow(base, 2.0 * kk / rotary);
-    sn = sin(angle);
-    cs = cos(angle);
-}
-
-__device__ __forceinline__ void rope_apply(double x, double y, double sn, double cs, float& a, float& b) {
-    a = static_cast<float>(x * cs - y * sn);
-    b = static_cast<float>(x * sn + y * cs);
-}
-
-__device__ __forceinline__ void rope_pair(double x, double y, int kk, int position, double base, int rotary, float& a,
-                                          float& b) {
-    double sn, cs;
-    rope_angle(kk, position, base, rotary, sn, cs);
-    rope_apply(x, y, sn, cs, a, b);
-}
-
 __global__ __launch_bounds__(kThreads) void attention_inputs_kernel(float* q, const float* q_bias, const float* k,
                                                                     const float* k_bias, float* k_out, const float* v,
                                                                     const float* v_bias, float* v_out, int heads,
