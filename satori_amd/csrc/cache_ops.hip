@@ -34,58 +34,90 @@ __global__ __launch_bounds__(kThreads) void copy_pages_kernel(uint8_t* pool, int
 
 // ---- the write of new positions ----
 
+template <typename T, int N>
+__device__ __forceinline__ void store_as(T* p, const float (&v)[N]) {
+    typedef T pack __attribute__((ext_vector_type(N)));
+    pack out;
+#pragma unroll
+    for (int i = 0; i < N; ++i) out[i] = static_cast<T>(v[i]);
+    *(SATORI_GLOBAL pack*)(p) = out;
+}
 template <typename T>
-__device__ __forceinline__ void store_as(T* p, float v) {
-    *(SATORI_GLOBAL T*)(p) = static_cast<T>(v);
+__device__ __forceinline__ void store_as(T* p, const float (&v)[1]) {
+    *(SATORI_GLOBAL T*)(p) = static_cast<T>(v[0]);
 }
 
-// A run's (query and key head, lane pair) items, then its lanes behind the rotated ones and the keys' padding, then its
-// values, spread over gridDim.y workgroups.
-template <typename T>
+// N values of a row with their bias (biased()), in one load each.
+template <int N>
+__device__ __forceinline__ void load_biased(const float* x, const float* bias, int64_t at, int lane, float (&out)[N]) {
+    typedef float pack __attribute__((ext_vector_type(N)));
+    if constexpr (N == 1) {
+        out[0] = biased(x + at, bias, lane);
+    } else {
+        const pack v = *(const SATORI_GLOBAL pack*)(x + at + lane);
+        pack b{};
+        if (bias) b = *(const SATORI_GLOBAL pack*)(bias + lane);
+#pragma unroll
+        for (int i = 0; i < N; ++i) out[i] = bias ? __fadd_rn(v[i], b[i]) : v[i];
+    }
+}
+
+constexpr int kGroupTokens = 8;  // positions whose values a thread stores at once
+
+// The rows of a run, spread over gridDim.y workgroups: N rotated lane pairs of a query or key head per thread and turn,
+// then the lanes behind the rotated ones and the keys' padding, then the values. A page's values lie [lane][position], so a
+// thread gathers one lane of up to eight positions (its neighbours the next lanes: the reads are whole lines) and stores
+// them together where they fill an aligned group.
+template <typename T, int N>
 __global__ __launch_bounds__(kThreads) void cache_append_kernel(CacheShape s, const int* __restrict__ plan,
                                                                 AppendArgs a) {
     const PlanHeader& h = *reinterpret_cast<const PlanHeader*>(plan);
     const PlanRun* runs = reinterpret_cast<const PlanRun*>(plan + h.runs_at);
     const PlanRow* rows = reinterpret_cast<const PlanRow*>(plan + h.rows_at);
     const int pairs = a.rotary / 2, D = s.head_dim, both = s.heads + s.kv_heads;
-    const int64_t head_bytes = static_cast<int64_t>(s.page_tokens) * s.width;
+    const int64_t head_size = static_cast<int64_t>(s.page_tokens) * s.width;
     for (int u = blockIdx.x; u < h.runs; u += gridDim.x) {
         const PlanRun run = runs[u];
+        const int position0 = rows[run.row].position;
         T* keys = reinterpret_cast<T*>(s.pool + run.page * s.page_bytes + a.layer * s.layer_bytes);
-        T* values = keys + s.kv_heads * head_bytes;
+        T* values = keys + s.kv_heads * head_size;
         const int start = blockIdx.y * kThreads + threadIdx.x, stride = gridDim.y * kThreads;
-        for (int i = start; i < run.tokens * both * pairs; i += stride) {
-            const int kk = i % pairs, head = i / pairs % both, t = i / pairs / both;
-            const int64_t row = run.row + t;
-            const int position = rows[row].position;
-            double sn, cs;
-            if (a.rope && position < a.rope_positions) {
-                sn = a.rope[static_cast<int64_t>(position) * a.rotary + kk];
-                cs = a.rope[static_cast<int64_t>(position) * a.rotary + pairs + kk];
-            } else {
-                rope_angle(kk, position, a.base, a.rotary, sn, cs);
+        const int packs = pairs / N;
+        for (int i = start; i < run.tokens * both * packs; i += stride) {
+            const int kk = i % packs * N, rest = i / packs, head = rest % both, t = rest / both;
+            const int position = position0 + t;
+            const bool is_query = head < s.heads;
+            const int lane = (is_query ? head : head - s.heads) * D + kk;
+            const int64_t at = static_cast<int64_t>(run.row + t) * (is_query ? s.heads : s.kv_heads) * D;
+            float x[N], y[N];
+            load_biased(is_query ? a.query : a.key, is_query ? a.query_bias : a.key_bias, at, lane, x);
+            load_biased(is_query ? a.query : a.key, is_query ? a.query_bias : a.key_bias, at, lane + pairs, y);
+            const bool listed = a.rope && position < a.rope_positions;
+            const double* angles = a.rope + static_cast<int64_t>(position) * a.rotary + kk;
+#pragma unroll
+            for (int j = 0; j < N; ++j) {
+                double sn, cs;
+                if (listed) {
+                    sn = angles[j];
+                    cs = angles[pairs + j];
+                } else {
+                    rope_angle(kk + j, position, a.base, a.rotary, sn, cs);
+                }
+                rope_apply(x[j], y[j], sn, cs, x[j], y[j]);
             }
-            float x, y;
-            if (head < s.heads) {
-                const float* q = a.query + row * s.heads * D;
-                const int e = head * D + kk;
-                rope_apply(biased(q, a.query_bias, e), biased(q, a.query_bias, e + pairs), sn, cs, x, y);
-                float* out = a.query_out + row * s.heads * D;
-                store_f32(out + e, x);
-                store_f32(out + e + pairs, y);
+            if (is_query) {
+                store_as(a.query_out + at + lane, x);
+                store_as(a.query_out + at + lane + pairs, y);
             } else {
-                const float* k = a.key + row * s.kv_heads * D;
-                const int e = (head - s.heads) * D + kk;
-                rope_apply(biased(k, a.key_bias, e), biased(k, a.key_bias, e + pairs), sn, cs, x, y);
-                T* out = keys + (head - s.heads) * head_bytes + static_cast<int64_t>(run.offset + t) * s.width;
-                store_as(out + kk, x);
-                store_as(out + kk + pairs, y);
+                T* out = keys + (head - s.heads) * head_size + static_cast<int64_t>(run.offset + t) * s.width + kk;
+                store_as(out, x);
+                store_as(out + pairs, y);
             }
         }
-        const int rest = s.width - a.rotary;
-        if (rest > 0)
-            for (int i = start; i < run.tokens * both * rest; i += stride) {
-                const int lane = a.rotary + i % rest, head = i / rest % both, t = i / rest / both;
+        const int behind = s.width - a.rotary;
+        if (behind > 0)
+            for (int i = start; i < run.tokens * both * behind; i += stride) {
+                const int lane = a.rotary + i % behind, head = i / behind % both, t = i / behind / both;
                 const int64_t row = run.row + t;
                 if (head < s.heads) {
                     if (lane < D)
@@ -93,15 +125,28 @@ __global__ __launch_bounds__(kThreads) void cache_append_kernel(CacheShape s, co
                                   biased(a.query + row * s.heads * D, a.query_bias, head * D + lane));
                 } else {
                     const int kh = head - s.heads;
-                    const float v = lane < D ? biased(a.key + row * s.kv_heads * D, a.key_bias, kh * D + lane) : 0.0f;
-                    store_as(keys + kh * head_bytes + static_cast<int64_t>(run.offset + t) * s.width + lane, v);
+                    const float v[1] = {lane < D ? biased(a.key + row * s.kv_heads * D, a.key_bias, kh * D + lane) : 0.0f};
+                    store_as(keys + kh * head_size + static_cast<int64_t>(run.offset + t) * s.width + lane, v);
                 }
             }
-        for (int i = start; i < run.tokens * s.kv_heads * D; i += stride) {
-            const int lane = i % (s.kv_heads * D), t = i / (s.kv_heads * D);
-            const int kh = lane / D, dim = lane % D;
-            const float v = biased(a.value + static_cast<int64_t>(run.row + t) * s.kv_heads * D, a.value_bias, lane);
-            store_as(values + kh * head_bytes + static_cast<int64_t>(dim) * s.page_tokens + run.offset + t, v);
+        const int first = run.offset / kGroupTokens, groups = (run.offset + run.tokens - 1) / kGroupTokens - first + 1;
+        for (int i = start; i < groups * s.kv_heads * D; i += stride) {
+            const int lane = i % (s.kv_heads * D), group = first + i / (s.kv_heads * D);
+            const int t0 = group * kGroupTokens - run.offset;  // of the run
+            T* out = values + lane / D * head_size + static_cast<int64_t>(lane % D) * s.page_tokens + group * kGroupTokens;
+            float v[kGroupTokens];
+#pragma unroll
+            for (int j = 0; j < kGroupTokens; ++j)
+                v[j] = t0 + j >= 0 && t0 + j < run.tokens
+                           ? biased(a.value + static_cast<int64_t>(run.row + t0 + j) * s.kv_heads * D, a.value_bias, lane)
+                           : 0.0f;
+            if (t0 >= 0 && t0 + kGroupTokens <= run.tokens) {
+                store_as(out, v);
+            } else {
+#pragma unroll
+                for (int j = 0; j < kGroupTokens; ++j)
+                    if (t0 + j >= 0 && t0 + j < run.tokens) *(SATORI_GLOBAL T*)(out + j) = static_cast<T>(v[j]);
+            }
         }
     }
 }
@@ -585,14 +630,24 @@ hipError_t launch_copy_pages(uint8_t* pool, int64_t page_bytes, const PageMoves&
     return hipGetLastError();
 }
 
-hipError_t launch_cache_append(const CacheShape& shape, const int* plan, int runs, const AppendArgs& args,
-                               hipStream_t stream) {
-    if (runs == 0) return hipSuccess;
-    const dim3 grid(runs, 4);
-    if (shape.type == kF32)
-        cache_append_kernel<float><<<grid, kThreads, 0, stream>>>(shape, plan, args);
+hipError_t launch_cache_append(const CacheShape& s, const int* plan, const PlanHeader& now, bool all,
+                               const AppendArgs& args, hipStream_t stream) {
+    if (now.runs == 0 && !all) return hipSuccess;
+    // Four lane pairs a thread and access where every row allows it.
+    const auto whole = [](const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; };
+    const bool packed = args.rotary % 8 == 0 && s.head_dim % 4 == 0 && whole(args.query) && whole(args.query_bias) &&
+                        whole(args.query_out) && whole(args.key) && whole(args.key_bias);
+    // One turn a thread for the longest run's rotations, and what a run of a few positions needs for its values.
+    const int longest = all ? 8 : now.longest_run;
+    const int64_t turns = static_cast<int64_t>(longest) * (s.heads + s.kv_heads) * (args.rotary / (packed ? 8 : 2));
+    const int64_t values = (static_cast<int64_t>(longest) / kGroupTokens + 1) * s.kv_heads * s.head_dim;
+    const int y = static_cast<int>(std::min<int64_t>((std::max(turns, values) + kThreads - 1) / kThreads, 1024));
+    const dim3 grid(all ? 256 : now.runs, y);
+    const auto launch = [&](auto kernel) { kernel<<<grid, kThreads, 0, stream>>>(s, plan, args); };
+    if (s.type == kF32)
+        packed ? launch(cache_append_kernel<float, 4>) : launch(cache_append_kernel<float, 1>);
     else
-        cache_append_kernel<_Float16><<<grid, kThreads, 0, stream>>>(shape, plan, args);
+        packed ? launch(cache_append_kernel<_Float16, 4>) : launch(cache_append_kernel<_Float16, 1>);
     return hipGetLastError();
 }
 

@@ -54,9 +54,10 @@ struct AppendArgs {
     int rope_positions;
     int layer;
 };
-// `plan`: the image on the device; `runs` of it now, or at most in later replays (the grid covers any).
-hipError_t launch_cache_append(const CacheShape& shape, const int* plan, int runs, const AppendArgs& args,
-                               hipStream_t stream);
+// `plan`: the image on the device, `now` its header. `all`: the launch is captured and replays may read any plan, so its
+// grid must do for any.
+hipError_t launch_cache_append(const CacheShape& shape, const int* plan, const PlanHeader& now, bool all,
+                               const AppendArgs& args, hipStream_t stream);
 
 // `partials`: cache_partial_bytes for the plan's slots. Launches with no work now are left out unless `all` (captured:
 // replays may have some).

@@ -254,7 +254,7 @@ PlanImage plan_batch(const PageTables& tables, const int* sequences, const int* 
                 runs.push_back({static_cast<int>(rows.size()), 0, table[p / P], p % P});
                 image.writable &= tables.references(table[p / P]) == 1;
             }
-            runs.back().tokens++;
+            image.header.longest_run = std::max(image.header.longest_run, ++runs.back().tokens);
             rows.push_back({p, 0, 0, 0});
             image.last_position = std::max(image.last_position, p);
         }

@@ -98,6 +98,7 @@ struct PlanHeader {
     int rows, narrow, wide, runs;
     int rows_at, narrow_at, wide_at, runs_at;
     int pages_at, list_at, joined, slots;  // joined: rows of several slots; slots: of all rows
+    int longest_run, pad[3];
 };
 
 struct PlanShape {

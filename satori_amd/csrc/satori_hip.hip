@@ -2514,7 +2514,7 @@ int satori_hip_cache_append(satori_hip_cache_plan* p, int layer, const float* qu
         const bool captured = note_plan(c, p, layer, st);
         const AppendArgs args{query, query_bias, key, key_bias, value, value_bias, query_out, frequency_base,
                               rotary_dimensions, rope_table, rope_table ? rope_positions : 0, layer};
-        check_hip(launch_cache_append(s, static_cast<const int*>(p->image.ptr), captured ? 256 : p->header.runs, args, st),
+        check_hip(launch_cache_append(s, static_cast<const int*>(p->image.ptr), p->header, captured, args, st),
                   "cache append launch");
     });
 }
