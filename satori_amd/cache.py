@@ -23,7 +23,9 @@ class ElementType(enum.IntEnum):
 
 
 def _ints(values) -> np.ndarray:
-    return np.ascontiguousarray(values, dtype=np.int32).reshape(-1)
+    if isinstance(values, np.ndarray) and values.dtype == np.int32 and values.flags.c_contiguous:
+        return values.reshape(-1)
+    return np.array(values, dtype=np.int32).reshape(-1)
 
 
 def _at(array: np.ndarray) -> ctypes.c_void_p:
@@ -38,11 +40,18 @@ class PageTable:
     """Page lists and reference counts of a cache of `page_count` pages (satori_hip_pages): host only. Calls that need
     page bytes to follow return them as moves, (sources, destinations)."""
 
+    # A table's read returns a few dozen page numbers and takes about a microsecond, most of it building ctypes arguments,
+    # so the small calls pass plain addresses of one array per call (of its own: threads may call at once).
+
     def __init__(self, page_count: int, page_tokens: int = 32):
         handle = ctypes.c_void_p()
-        _check(_ffi.lib().satori_hip_pages_create(page_count, page_tokens, ctypes.byref(handle)))
+        lib = _ffi.lib()
+        _check(lib.satori_hip_pages_create(page_count, page_tokens, ctypes.byref(handle)))
         self._handle = handle
         self.page_count, self.page_tokens = page_count, page_tokens
+        self._read, self._address = lib.satori_hip_pages_sequence, handle.value
+        self._room = min(page_count, 256)
+        self._array = ctypes.c_int * (self._room + 1)  # and the count
 
     @property
     def handle(self) -> ctypes.c_void_p:
@@ -55,20 +64,23 @@ class PageTable:
 
     def extend(self, sequences, tokens) -> tuple[np.ndarray, np.ndarray]:
         ids, counts = _ints(sequences), _ints(tokens)
-        if ids.size != counts.size:
+        n = ids.size
+        if n != counts.size:
             raise ArgumentException("Lengths differ.")
-        sources, destinations, moves = np.empty(ids.size, np.int32), np.empty(ids.size, np.int32), ctypes.c_int()
-        _check(_ffi.lib().satori_hip_pages_extend(self._handle, _at(ids), _at(counts), ids.size, _at(sources),
-                                                  _at(destinations), ids.size, ctypes.byref(moves)))
-        return sources[:moves.value], destinations[:moves.value]
+        moves = np.empty(2 * n + 1, np.int32)
+        at = moves.ctypes.data
+        _check(_ffi.lib().satori_hip_pages_extend(self._handle, ids.ctypes.data, counts.ctypes.data, n, at, at + 4 * n, n,
+                                                  at + 8 * n))
+        made = int(moves[2 * n])
+        return moves[:made], moves[n:n + made]
 
     def truncate(self, sequence: int, tokens: int) -> None:
         _check(_ffi.lib().satori_hip_pages_truncate(self._handle, sequence, tokens))
 
     def fork(self, sequence: int, count: int = 1) -> list[int]:
-        forks = np.empty(max(count, 0), np.int32)
-        _check(_ffi.lib().satori_hip_pages_fork(self._handle, sequence, count, _at(forks)))
-        return forks.tolist()
+        forks = np.empty(max(count, 1), np.int32)
+        _check(_ffi.lib().satori_hip_pages_fork(self._handle, sequence, count, forks.ctypes.data))
+        return forks[:count].tolist()
 
     def copy(self, sequence: int) -> tuple[int, tuple[np.ndarray, np.ndarray]]:
         most = self._describe(sequence)[1]
@@ -80,7 +92,7 @@ class PageTable:
 
     def free(self, sequences) -> None:
         ids = _ints(sequences)
-        _check(_ffi.lib().satori_hip_pages_free(self._handle, _at(ids), ids.size))
+        _check(_ffi.lib().satori_hip_pages_free(self._handle, ids.ctypes.data, ids.size))
 
     def compact(self) -> tuple[np.ndarray, np.ndarray]:
         most = self.page_count - self.free_pages
@@ -105,9 +117,16 @@ class PageTable:
         return self._describe(sequence)[0]
 
     def pages(self, sequence: int) -> list[int]:
-        table = np.empty(self._describe(sequence)[1], np.int32)
-        _check(_ffi.lib().satori_hip_pages_sequence(self._handle, sequence, None, _at(table), table.size, None))
-        return table.tolist()
+        array, room = self._array(), self._room
+        at = ctypes.addressof(array)
+        status = self._read(self._address, sequence, None, at, room, at + 4 * room)
+        count = array[room]
+        if count > room:  # a long table: a call of its own size
+            array = (ctypes.c_int * count)()
+            status = self._read(self._address, sequence, None, ctypes.addressof(array), count, None)
+        if status:
+            _check(status)
+        return array[:count]
 
     def dispose(self) -> None:
         _check(_ffi.lib().satori_hip_pages_destroy(self._handle))
@@ -146,9 +165,9 @@ class PagedCache:
     def _move(self, moves: tuple[np.ndarray, np.ndarray]) -> None:
         sources, destinations = moves
         if sources.size:
-            _check(_ffi.lib().satori_hip_cache_copy_pages(self.context.handle, _pointer(self.pool), self.page_bytes,
-                                                          self.page_count, _at(sources), _at(destinations),
-                                                          sources.size, None))
+            _check(_ffi.lib().satori_hip_cache_copy_pages(self.context.handle, self.pool, self.page_bytes, self.page_count,
+                                                          sources.ctypes.data, destinations.ctypes.data, sources.size,
+                                                          None))
 
     def open(self) -> int:
         return self.table.open()
