@@ -2,6 +2,7 @@
 // sequences share pages.
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 #include "cache_ops.hpp"
 #include "device_common.hpp"
@@ -30,6 +31,21 @@ __global__ __launch_bounds__(kThreads) void copy_pages_kernel(uint8_t* pool, int
 #pragma unroll
     for (int i = 0; i < 4; ++i)
         if (at + i * kThreads * 16 < page_bytes) *(SATORI_GLOBAL u32x4*)(dst + at + i * kThreads * 16) = v[i];
+}
+
+// ---- a plan's copy ----
+
+constexpr int kPlanParts = 7;
+struct PlanParts {
+    int at[kPlanParts], end[kPlanParts];  // 16-byte units; end: of the parts up to this one, counted through
+};
+
+__global__ __launch_bounds__(kThreads) void plan_copy_kernel(const u32x4* from, u32x4* to, PlanParts parts) {
+    int n = blockIdx.x * kThreads + threadIdx.x, part = 0;
+    if (n >= parts.end[kPlanParts - 1]) return;
+    while (n >= parts.end[part]) ++part;
+    n += parts.at[part] - (part ? parts.end[part - 1] : 0);
+    to[n] = from[n];
 }
 
 // ---- the write of new positions ----
@@ -69,16 +85,15 @@ constexpr int kGroupTokens = 8;  // positions whose values a thread stores at on
 // thread gathers one lane of up to eight positions (its neighbours the next lanes: the reads are whole lines) and stores
 // them together where they fill an aligned group.
 template <typename T, int N>
-__global__ __launch_bounds__(kThreads) void cache_append_kernel(CacheShape s, const int* __restrict__ plan,
+__global__ __launch_bounds__(kThreads) void cache_append_kernel(CacheShape s, const int* __restrict__ image, int runs_at,
                                                                 AppendArgs a) {
-    const PlanHeader& h = *reinterpret_cast<const PlanHeader*>(plan);
-    const PlanRun* runs = reinterpret_cast<const PlanRun*>(plan + h.runs_at);
-    const PlanRow* rows = reinterpret_cast<const PlanRow*>(plan + h.rows_at);
+    const int count = reinterpret_cast<const PlanHeader*>(image)->runs;
+    const PlanRun* runs = reinterpret_cast<const PlanRun*>(image + runs_at);
     const int pairs = a.rotary / 2, D = s.head_dim, both = s.heads + s.kv_heads;
     const int64_t head_size = static_cast<int64_t>(s.page_tokens) * s.width;
-    for (int u = blockIdx.x; u < h.runs; u += gridDim.x) {
+    for (int u = blockIdx.x; u < count; u += gridDim.x) {
         const PlanRun run = runs[u];
-        const int position0 = rows[run.row].position;
+        const int position0 = run.position;
         T* keys = reinterpret_cast<T*>(s.pool + run.page * s.page_bytes + a.layer * s.layer_bytes);
         T* values = keys + s.kv_heads * head_size;
         const int start = blockIdx.y * kThreads + threadIdx.x, stride = gridDim.y * kThreads;
@@ -153,94 +168,82 @@ __global__ __launch_bounds__(kThreads) void cache_append_kernel(CacheShape s, co
 
 // ---- attention ----
 //
-// A workgroup attends the tokens of one item for up to 16 * NB (row, query head) pairs of one key/value head; its four
-// waves take tiles of 32 tokens in turn. With S^T = K Q^T and O^T = V^T P^T, both computed by 16 x 16 matrix tiles, a
-// column of either product is a pair, so the running maximum and sum of a pair live in the lanes of its column
-// (lane % 16), and what the first product leaves in a lane (four tokens of a pair per tile) is what the second takes
-// from it: the tokens of the key tiles are numbered so that no value changes lanes (F16: row m of tile a is token
-// 8 * (m / 4) + 4 * a + m % 4, which leaves lane group g the tokens 8 g .. 8 g + 7).
+// With S^T = K Q^T and O^T = V^T P^T, both computed by 16 x 16 matrix tiles, a column of either product is a (row, query
+// head) pair, so the running maximum and sum of a pair live in the lanes of its column (lane % 16), and what the first
+// product leaves in a lane (four tokens of a pair per tile) is what the second takes from it: the tokens of the key tiles
+// are numbered so that no value changes lanes (F16: row m of tile a is token 8 * (m / 4) + 4 * a + m % 4, which leaves lane
+// group g the tokens 8 g .. 8 g + 7; F32: row m of tile a is token 16 * a + m).
 //
 // F16 keys and values are exact in the matrix instructions; what they meet is not, so queries and probabilities go in as
 // two halves of 11 bits, x = hi + lo, both products summed in the same FP32 accumulator: 2^-22 of a value is lost. Their
 // scale is a power of two that puts the largest query lane of a pair (and a probability of one) at 2^14, far from
 // where halves lose bits. F32 caches use the FP32 matrix instructions.
 
-constexpr int kWaves = 4;
-constexpr int kTileTokens = 32;
+constexpr int kTile = 32;  // tokens that a wave attends at once
 constexpr float kLog2e = 1.44269504088896340736f;
 
 // Maximum and sum over the four lanes that hold one column (lane, lane ^ 16, lane ^ 32, lane ^ 48).
 __device__ __forceinline__ float column_max(float v) {
-    v = fmaxf(v, __shfl_xor(v, 16, 64));
-    return fmaxf(v, __shfl_xor(v, 32, 64));
+    auto p = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = fmaxf(__uint_as_float(p[0]), __uint_as_float(p[1]));
+    p = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(p[0]), __uint_as_float(p[1]));
 }
 __device__ __forceinline__ float column_sum(float v) {
     v += __shfl_xor(v, 16, 64);
     return v + __shfl_xor(v, 32, 64);
 }
 
-__device__ __forceinline__ f32x4 mfma16(f16x8 a, f16x8 b, f32x4 c) {
-    return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
-}
-__device__ __forceinline__ f32x4 mfma32(float a, float b, f32x4 c) {
-    return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0);
+// N lanes of a query from d on, zero from head_dim on and where `is` does not hold. `row` is a row's address in any case.
+template <int N>
+__device__ __forceinline__ void load_lanes(const float* row, int d, int head_dim, bool quads, bool is, float (&x)[N]) {
+#pragma unroll
+    for (int j = 0; j < N; j += 4) {
+        if (quads) {  // (heads of whole 16-byte pieces)
+            const f32x4 v = *(const SATORI_GLOBAL f32x4*)(row + min(d + j, head_dim - 4));
+#pragma unroll
+            for (int k = 0; k < 4; ++k) x[j + k] = is && d + j < head_dim ? v[k] : 0.0f;
+        } else {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const float v = load_f32(row + min(d + j + k, head_dim - 1));
+                x[j + k] = is && d + j + k < head_dim ? v : 0.0f;
+            }
+        }
+    }
 }
 
-// Operands of one wave's tile, by element type. Tokens are counted from the tile's first; token(i) is the i-th (of 8)
-// that this lane's scores belong to.
+// The arithmetic of an element type: W lanes a head. Lane (c, g) = (lane % 16, lane / 16).
 template <typename T, int W>
-struct Tile;
+struct Math;
 
 template <int W>
-struct Tile<_Float16, W> {
-    static constexpr float kTop = 14.0f;  // log2 of a probability of one, as the second product takes it
+struct Math<_Float16, W> {
+    static constexpr float kTop = 14.0f;        // log2 of a probability of one, as the second product takes it
+    static constexpr int kKeyParts = W / 32;    // fragments of a key tile's 16 rows, of a value tile's 16 lanes
+    static constexpr int kValueParts = 1;
+    typedef f16x8 Fragment;                     // 16 bytes: lanes 32 s + 8 g .. of a key, tokens 8 g .. of a value lane
     struct Query {
         f16x8 hi[W / 32], lo[W / 32];
         float factor;  // of a score: 1 / sqrt(head_dim), the base of exp2 and the query's own scale
     };
-    f16x8 k[2][W / 32], v[W / 16];
+    struct Weights {
+        f16x8 hi, lo;
+    };
 
-    static __device__ __forceinline__ int token(int g, int i) { return 8 * g + i; }
-
-    __device__ __forceinline__ void load_keys(const uint8_t* page, int c, int g) {
-        const _Float16* p = reinterpret_cast<const _Float16*>(page) + (8 * (c >> 2) + (c & 3)) * W + 8 * g;
-#pragma unroll
-        for (int a = 0; a < 2; ++a)
-#pragma unroll
-            for (int s = 0; s < W / 32; ++s) k[a][s] = *(const SATORI_GLOBAL f16x8*)(p + 4 * a * W + 32 * s);
-    }
-    __device__ __forceinline__ void load_values(const uint8_t* page, int page_tokens, int c, int g) {
-        const _Float16* p = reinterpret_cast<const _Float16*>(page) + c * page_tokens + 8 * g;
-#pragma unroll
-        for (int d = 0; d < W / 16; ++d) v[d] = *(const SATORI_GLOBAL f16x8*)(p + 16 * d * page_tokens);
-    }
-    // Values of tokens from `end` on become zero (they are nobody's, and may hold anything).
-    __device__ __forceinline__ void clip_values(int end, int g) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-            if (8 * g + i >= end)
-#pragma unroll
-                for (int d = 0; d < W / 16; ++d) v[d][i] = 0;
-    }
-    __device__ __forceinline__ bool values_finite() const {
-        bool finite = true;
-#pragma unroll
-        for (int d = 0; d < W / 16; ++d)
-#pragma unroll
-            for (int i = 0; i < 8; ++i) finite &= __builtin_isfinite(static_cast<float>(v[d][i]));
-        return finite;
-    }
-    static __device__ __forceinline__ void load_query(Query& q, const float* row, int head_dim, float scale, int g) {
+    static __device__ __forceinline__ int token(int g, int i) { return 8 * g + i; }     // of score i (of 8)
+    static __device__ __forceinline__ int key_token(int a, int m) { return 8 * (m >> 2) + 4 * a + (m & 3); }
+    static __device__ __forceinline__ int key_row(int t) { return 16 * ((t >> 2) & 1) + 4 * (t >> 3) + (t & 3); }
+    static __device__ __forceinline__ void load_query(Query& q, const float* row, bool is, int head_dim, bool quads,
+                                                      float scale, int g) {
         float x[W / 32][8];
         float top = 0;
 #pragma unroll
+        for (int s = 0; s < W / 32; ++s) load_lanes(row, 32 * s + 8 * g, head_dim, quads, is, x[s]);
+#pragma unroll
         for (int s = 0; s < W / 32; ++s)
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const int d = 32 * s + 8 * g + j;
-                x[s][j] = row && d < head_dim ? load_f32(row + d) : 0.0f;
-                top = fmaxf(top, fabsf(x[s][j]));
-            }
+            for (int j = 0; j < 8; ++j) top = fmaxf(top, fabsf(x[s][j]));
         top = column_max(top);
         const int exponent = static_cast<int>(__float_as_uint(top) >> 23) - 127;
         const int shift = top > 0 && exponent < 128 ? (14 - exponent < 100 ? 14 - exponent : 100) : 0;
@@ -254,290 +257,390 @@ struct Tile<_Float16, W> {
                 q.lo[s][j] = static_cast<_Float16>(y - static_cast<float>(q.hi[s][j]));
             }
     }
-    __device__ __forceinline__ void scores(const Query& q, f32x4 (&out)[2]) const {
-#pragma unroll
-        for (int a = 0; a < 2; ++a) out[a] = f32x4{0, 0, 0, 0};
-#pragma unroll
-        for (int s = 0; s < W / 32; ++s) {
-#pragma unroll
-            for (int a = 0; a < 2; ++a) out[a] = mfma16(k[a][s], q.hi[s], out[a]);
-#pragma unroll
-            for (int a = 0; a < 2; ++a) out[a] = mfma16(k[a][s], q.lo[s], out[a]);
-        }
+    static constexpr int kTerms = 2;  // products of a fragment: with the high halves, with the low ones
+    static __device__ __forceinline__ f32x4 score(Fragment k, const Query& q, int s, int term, f32x4 sum) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(k, term ? q.lo[s] : q.hi[s], sum, 0, 0, 0);
     }
-    static __device__ __forceinline__ void halves(const float (&p)[8], f16x8& hi, f16x8& lo) {
+    static __device__ __forceinline__ void weights(const float (&p)[8], Weights& w) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            hi[i] = static_cast<_Float16>(p[i]);
-            lo[i] = static_cast<_Float16>(p[i] - static_cast<float>(hi[i]));
+            w.hi[i] = static_cast<_Float16>(p[i]);
+            w.lo[i] = static_cast<_Float16>(p[i] - static_cast<float>(w.hi[i]));
         }
     }
-    __device__ __forceinline__ void weigh(const float (&p)[8], f32x4 (&o)[W / 16]) const {
-        f16x8 hi, lo;
-        halves(p, hi, lo);
-#pragma unroll
-        for (int d = 0; d < W / 16; ++d) o[d] = mfma16(v[d], hi, o[d]);
-#pragma unroll
-        for (int d = 0; d < W / 16; ++d) o[d] = mfma16(v[d], lo, o[d]);
-    }
-    // The same for token t of the tile alone, added where `seen`.
-    __device__ __forceinline__ void weigh_one(const float (&p)[8], int t, int g, bool seen, f32x4 (&o)[W / 16]) const {
-        f16x8 hi, lo;
-        halves(p, hi, lo);
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-            if (8 * g + i != t) hi[i] = lo[i] = 0;
-#pragma unroll
-        for (int d = 0; d < W / 16; ++d) {
-            f16x8 one;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) one[i] = 8 * g + i == t ? v[d][i] : static_cast<_Float16>(0);
-            const f32x4 add = mfma16(one, lo, mfma16(one, hi, f32x4{0, 0, 0, 0}));
-            if (seen) o[d] = o[d] + add;
-        }
+    static __device__ __forceinline__ f32x4 weigh(Fragment v, const Weights& w, int, int term, f32x4 sum) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(v, term ? w.lo : w.hi, sum, 0, 0, 0);
     }
 };
 
 template <int W>
-struct Tile<float, W> {
+struct Math<float, W> {
     static constexpr float kTop = 0.0f;
+    static constexpr int kKeyParts = W / 16;
+    static constexpr int kValueParts = 2;
+    typedef f32x4 Fragment;  // lanes 16 s + 4 g .. of a key, tokens 16 a + 4 g .. of a value lane
     struct Query {
         f32x4 x[W / 16];
         float factor;
     };
-    f32x4 k[2][W / 16], v[W / 16][2];
+    struct Weights {
+        float p[8];
+    };
 
     static __device__ __forceinline__ int token(int g, int i) { return 16 * (i >> 2) + 4 * g + (i & 3); }
-
-    __device__ __forceinline__ void load_keys(const uint8_t* page, int c, int g) {
-        const float* p = reinterpret_cast<const float*>(page) + c * W + 4 * g;
+    static __device__ __forceinline__ int key_token(int a, int m) { return 16 * a + m; }
+    static __device__ __forceinline__ int key_row(int t) { return t; }
+    static __device__ __forceinline__ void load_query(Query& q, const float* row, bool is, int head_dim, bool quads,
+                                                      float scale, int g) {
+        float x[W / 16][4];
 #pragma unroll
-        for (int a = 0; a < 2; ++a)
+        for (int s = 0; s < W / 16; ++s) load_lanes(row, 16 * s + 4 * g, head_dim, quads, is, x[s]);
 #pragma unroll
-            for (int s = 0; s < W / 16; ++s) k[a][s] = *(const SATORI_GLOBAL f32x4*)(p + 16 * a * W + 16 * s);
-    }
-    __device__ __forceinline__ void load_values(const uint8_t* page, int page_tokens, int c, int g) {
-        const float* p = reinterpret_cast<const float*>(page) + c * page_tokens + 4 * g;
-#pragma unroll
-        for (int d = 0; d < W / 16; ++d)
-#pragma unroll
-            for (int a = 0; a < 2; ++a) v[d][a] = *(const SATORI_GLOBAL f32x4*)(p + 16 * d * page_tokens + 16 * a);
-    }
-    __device__ __forceinline__ void clip_values(int end, int g) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-            if (token(g, i) >= end)
-#pragma unroll
-                for (int d = 0; d < W / 16; ++d) v[d][i >> 2][i & 3] = 0;
-    }
-    __device__ __forceinline__ bool values_finite() const {
-        bool finite = true;
-#pragma unroll
-        for (int d = 0; d < W / 16; ++d)
-#pragma unroll
-            for (int i = 0; i < 8; ++i) finite &= __builtin_isfinite(v[d][i >> 2][i & 3]);
-        return finite;
-    }
-    static __device__ __forceinline__ void load_query(Query& q, const float* row, int head_dim, float scale, int g) {
-#pragma unroll
-        for (int s = 0; s < W / 16; ++s)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const int d = 16 * s + 4 * g + j;
-                q.x[s][j] = row && d < head_dim ? load_f32(row + d) : 0.0f;
-            }
+        for (int s = 0; s < W / 16; ++s) q.x[s] = f32x4{x[s][0], x[s][1], x[s][2], x[s][3]};
         q.factor = scale;
     }
-    __device__ __forceinline__ void scores(const Query& q, f32x4 (&out)[2]) const {
-#pragma unroll
-        for (int a = 0; a < 2; ++a) out[a] = f32x4{0, 0, 0, 0};
-#pragma unroll
-        for (int s = 0; s < W / 16; ++s)
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-#pragma unroll
-                for (int a = 0; a < 2; ++a) out[a] = mfma32(k[a][s][j], q.x[s][j], out[a]);
+    static constexpr int kTerms = 4;  // products of a fragment: one per element
+    static __device__ __forceinline__ f32x4 score(Fragment k, const Query& q, int s, int term, f32x4 sum) {
+        return __builtin_amdgcn_mfma_f32_16x16x4f32(k[term], q.x[s][term], sum, 0, 0, 0);
     }
-    __device__ __forceinline__ void weigh(const float (&p)[8], f32x4 (&o)[W / 16]) const {
+    static __device__ __forceinline__ void weights(const float (&p)[8], Weights& w) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-#pragma unroll
-            for (int d = 0; d < W / 16; ++d) o[d] = mfma32(v[d][i >> 2][i & 3], p[i], o[d]);
+        for (int i = 0; i < 8; ++i) w.p[i] = p[i];
     }
-    __device__ __forceinline__ void weigh_one(const float (&p)[8], int t, int g, bool seen, f32x4 (&o)[W / 16]) const {
-#pragma unroll
-        for (int d = 0; d < W / 16; ++d) {
-            f32x4 add{0, 0, 0, 0};
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const bool mine = token(g, i) == t;
-                add = mfma32(mine ? v[d][i >> 2][i & 3] : 0.0f, mine ? p[i] : 0.0f, add);
-            }
-            if (seen) o[d] = o[d] + add;
-        }
+    static __device__ __forceinline__ f32x4 weigh(Fragment v, const Weights& w, int part, int term, f32x4 sum) {
+        return __builtin_amdgcn_mfma_f32_16x16x4f32(v[term], w.p[4 * part + term], sum, 0, 0, 0);
     }
 };
 
-// Partial results: [slots][heads][width] values, then [slots][heads] (maximum, sum) pairs, in units of exp2.
-__device__ __forceinline__ float* partial_values(float* partials, int width, int64_t index) {
-    return partials + index * width;
+// The state of 16 pairs: maximum (in units of exp2), the lane's part of the sum, and O^T: lane (c, g) holds lanes
+// 16 d + 4 g .. 16 d + 4 g + 3 of pair c.
+template <int W>
+struct Softmax {
+    float m, l;
+    f32x4 o[W / 16];
+
+    __device__ __forceinline__ void clear() {
+        m = -INFINITY;
+        l = 0;
+#pragma unroll
+        for (int d = 0; d < W / 16; ++d) o[d] = f32x4{0, 0, 0, 0};
+    }
+    // Takes a tile's scores (as they leave the first product) and gives their weights.
+    __device__ __forceinline__ void take(const f32x4 (&score)[2], float factor, float top_weight, float (&p)[8]) {
+        float top = fmaxf(fmaxf(fmaxf(score[0][0], score[0][1]), fmaxf(score[0][2], score[0][3])),
+                          fmaxf(fmaxf(score[1][0], score[1][1]), fmaxf(score[1][2], score[1][3])));
+        top = column_max(top) * factor;
+        if (__any(top > m)) {
+            const float now = fmaxf(m, top);
+            const float shrink = __builtin_amdgcn_exp2f(m - (now == -INFINITY ? 0.0f : now));
+            m = now;
+            l *= shrink;
+#pragma unroll
+            for (int d = 0; d < W / 16; ++d) o[d] = o[d] * shrink;
+        }
+        const float from = top_weight - (m == -INFINITY ? 0.0f : m);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) p[i] = __builtin_amdgcn_exp2f(__fmaf_rn(score[i >> 2][i & 3], factor, from));
+        l += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
+    }
+};
+
+// The scores of the tokens that a pair does not see become -infinity: those from `seen` on, of the tile.
+template <typename M>
+__device__ __forceinline__ void hide(f32x4 (&score)[2], int seen, int g) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+        if (M::token(g, i) >= seen) score[i >> 2][i & 3] = -INFINITY;
 }
-__device__ __forceinline__ float* partial_sums(float* partials, int width, int64_t all, int64_t index) {
-    return partials + all * width + index * 2;
+
+// Values that are not finite. Where some pairs see a token and others must not, the second product would spoil the others'
+// sums (0 * infinity), so such a tile's values get zeros in those places, and the sum of each (pair, lane) that sees one
+// becomes NaN: here, with values in registers, a product tells which.
+template <typename F>
+__device__ __forceinline__ bool all_finite(F v) {
+    bool all = true;
+#pragma unroll
+    for (int i = 0; i < static_cast<int>(sizeof(F) / sizeof(v[0])); ++i) all &= __builtin_isfinite(static_cast<float>(v[i]));
+    return all;
 }
+template <typename F>
+__device__ __forceinline__ F take_spoiled(F& v) {
+    F spoiled;
+#pragma unroll
+    for (int i = 0; i < static_cast<int>(sizeof(F) / sizeof(v[0])); ++i) {
+        const bool fine = __builtin_isfinite(static_cast<float>(v[i]));
+        spoiled[i] = fine ? 0 : 1;
+        v[i] = fine ? v[i] : 0;
+    }
+    return spoiled;
+}
+template <typename M>
+__device__ __forceinline__ void spoil(typename M::Fragment spoiled, int seen, int part, int g, f32x4& o) {
+    float one[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) one[i] = M::token(g, i) < seen ? 1.0f : 0.0f;
+    typename M::Weights w;
+    M::weights(one, w);
+    f32x4 hit{0, 0, 0, 0};
+#pragma unroll
+    for (int term = 0; term < M::kTerms; ++term) hit = M::weigh(spoiled, w, part, term, hit);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) o[j] = hit[j] > 0 ? NAN : o[j];
+}
+
+// Partial results: [slots][heads][width] values, then [slots][heads] (maximum, sum) pairs, in units of exp2; `all`: slots
+// times heads that there is room for.
+struct Partials {
+    float* at;
+    int64_t all;
+    __device__ __forceinline__ float* values(int width, int64_t index) const { return at + index * width; }
+    __device__ __forceinline__ float* sums(int width, int64_t index) const { return at + all * width + index * 2; }
+};
+
+struct AttentionArgs {
+    CacheShape s;
+    const int* image;
+    PlanLayout at;
+    int layer;
+    const float* query;
+    float* output;
+    Partials partials;
+    float scale;
+    bool quads;  // heads of a query start at multiples of 16 bytes and are whole 16-byte pieces
+};
+
+// What a lane knows of pair `p` of an item: its row and query head.
+struct Pair {
+    PlanRow row;
+    int head;
+    bool is;
+};
+
+__device__ __forceinline__ Pair pair_of(const AttentionArgs& a, const PlanItem& item, int p) {
+    Pair r;
+    r.is = p < item.pairs;
+    const int group = a.s.heads / a.s.kv_heads, of = item.pair + (r.is ? p : 0);
+    r.row = reinterpret_cast<const PlanRow*>(a.image + a.at.list_at)[item.rows + of / group];
+    r.head = item.kv * group + of % group;
+    return r;
+}
+
+__device__ __forceinline__ const float* query_of(const AttentionArgs& a, const Pair& p) {
+    return a.query + (static_cast<int64_t>(p.row.row) * a.s.heads + p.head) * a.s.head_dim;
+}
+
+// One joined result of a pair, four lanes from `d` on: the output where it is the row's only one.
+template <int W>
+__device__ __forceinline__ void give(const AttentionArgs& a, const PlanItem& item, const Pair& p, int d, f32x4 o,
+                                     float total) {
+    if (p.row.slots > 1) {
+        const int64_t index = static_cast<int64_t>(p.row.slot + item.slot) * a.s.heads + p.head;
+        *reinterpret_cast<f32x4*>(a.partials.values(W, index) + d) = o;
+        return;
+    }
+    float* out = a.output + (static_cast<int64_t>(p.row.row) * a.s.heads + p.head) * a.s.head_dim + d;
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+        if (d + j < a.s.head_dim) store_f32(out + j, o[j] / total);
+}
+template <int W>
+__device__ __forceinline__ void give_sums(const AttentionArgs& a, const PlanItem& item, const Pair& p, float m, float l) {
+    if (p.row.slots <= 1) return;
+    float* sums = a.partials.sums(W, static_cast<int64_t>(p.row.slot + item.slot) * a.s.heads + p.head);
+    sums[0] = m;
+    sums[1] = l;
+}
+
+// Reads of what no kernel writes, at addresses that a wave has in common: through the scalar cache.
+template <typename T>
+__device__ __forceinline__ T scalar_load(const T* p) {
+    const auto* words = (const __attribute__((address_space(4))) int*)(p);
+    int w[sizeof(T) / 4];
+#pragma unroll
+    for (int i = 0; i < static_cast<int>(sizeof(T) / 4); ++i) w[i] = words[i];
+    T out;
+    __builtin_memcpy(&out, w, sizeof(T));
+    return out;
+}
+
+// The same value, of which the compiler knows nothing: what is computed from it inside a loop stays there (hundreds of
+// lane masks and addresses, moved out of the loop over items, would fill the registers).
+__device__ __forceinline__ int unknown(int v) {
+    __asm__ volatile("" : "+v"(v));
+    return v;
+}
+__device__ __forceinline__ int unknown_scalar(int v) {
+    __asm__ volatile("" : "+s"(v));
+    return v;
+}
+
+// The pages of an item's tokens for one layer and key/value head.
+struct Pages {
+    const uint8_t* base;
+    const int* list;
+    int64_t page_bytes, head_bytes;
+    int first, tokens, shift, kv_heads;
+    __device__ __forceinline__ Pages(const AttentionArgs& a, const PlanItem& item, int64_t head) {
+        head_bytes = head;
+        base = a.s.pool + a.layer * a.s.layer_bytes + item.kv * head_bytes;
+        list = a.image + a.at.pages_at + item.pages;
+        page_bytes = a.s.page_bytes;
+        tokens = a.s.page_tokens;
+        first = item.first & (tokens - 1);
+        shift = a.s.page_shift;
+        kv_heads = a.s.kv_heads;
+    }
+    // Page number of the item's token t, and the bytes of the keys and values from a token within it.
+    __device__ __forceinline__ int page(int t) const { return scalar_load(list + ((first + t) >> shift)); }
+    __device__ __forceinline__ int within(int t) const { return (first + t) & (tokens - 1); }
+    __device__ __forceinline__ const uint8_t* keys(int page) const { return base + page * page_bytes; }
+    __device__ __forceinline__ const uint8_t* values(int page) const { return keys(page) + kv_heads * head_bytes; }
+};
+
+// Few pairs (16 * NB at most): each of four waves takes tiles of its own in turn, keys and values straight from the cache
+// into registers (nobody else in the workgroup wants them), and the waves' results are joined through LDS.
+constexpr int kNarrowWaves = 4;
 
 template <typename T, int W, int NB>
-__global__ __launch_bounds__(kWaves * 64, NB == 1 && W <= 128 ? 2 : 1) void cache_attention_kernel(CacheShape s, const int* __restrict__ plan,
-                                                                      int layer, const float* __restrict__ query,
-                                                                      float* __restrict__ output, float* partials,
-                                                                      float scale, int wide) {
+__global__ __launch_bounds__(kNarrowWaves * 64, W <= 128 ? 2 : 1) void cache_attention_narrow_kernel(AttentionArgs a) {
+    using M = Math<T, W>;
+    using Fragment = typename M::Fragment;
     constexpr int kPart = W < 128 ? W : 128;  // lanes joined at once
-    static_assert(W % 16 == 0 && (W <= 128 || W % 64 == 0), "widths");
-    __shared__ float joined[kWaves][16][kPart + 4];
-    __shared__ float stats[kWaves][16][2];
-    const PlanHeader& h = *reinterpret_cast<const PlanHeader*>(plan);
-    const PlanRow* rows = reinterpret_cast<const PlanRow*>(plan + h.rows_at);
-    const PlanItem* items = reinterpret_cast<const PlanItem*>(plan + (wide ? h.wide_at : h.narrow_at));
-    const int count = wide ? h.wide : h.narrow;
+    constexpr int kKeyUnit = sizeof(T) == 2 ? 32 : 16;  // lanes a key fragment's step covers
+    constexpr int kGroupLanes = 16 / sizeof(T);         // elements of a fragment
+    __shared__ float joined[kNarrowWaves][16][kPart + 4];
+    __shared__ float stats[kNarrowWaves][16][2];
+    const int count = reinterpret_cast<const PlanHeader*>(a.image)->narrow;
+    const PlanItem* items = reinterpret_cast<const PlanItem*>(a.image + a.at.narrow_at);
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
-    const int group = s.heads / s.kv_heads;
-    const int64_t head_bytes = static_cast<int64_t>(s.page_tokens) * W * sizeof(T);
-    const int64_t partial_rows = static_cast<int64_t>(h.slots) * s.heads;
     for (int u = blockIdx.x; u < count; u += gridDim.x) {
-        const PlanItem item = items[u];
-        const int* pages = plan + h.pages_at + item.pages;
-        const int* list = plan + h.list_at + item.rows;
-        const uint8_t* base = s.pool + layer * s.layer_bytes + item.kv * head_bytes;
+        const PlanItem item = scalar_load(items + u);
+        const int thread = unknown(threadIdx.x), lane = thread & 63, c = lane & 15, g = lane >> 4;
+        const int head_dim = unknown_scalar(a.s.head_dim);
+        const Pages pages(a, item, static_cast<int64_t>(a.s.page_tokens) * W * sizeof(T));
         const int blocks = (item.pairs + 15) / 16;
-
-        typename Tile<T, W>::Query q[NB];
-        f32x4 o[NB][W / 16];
-        float m[NB], l[NB];
+        Fragment k[2][M::kKeyParts], v[W / 16][M::kValueParts];
+        const auto load_keys = [&](int t) {
+            const T* p = reinterpret_cast<const T*>(pages.keys(pages.page(t))) + pages.within(t) * W + kGroupLanes * g;
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int s = 0; s < M::kKeyParts; ++s)
+                    k[h][s] = *(const SATORI_GLOBAL Fragment*)(p + M::key_token(h, c) * W + kKeyUnit * s);
+        };
+        int t = wave * kTile;
+        if (t < item.tokens) load_keys(t);
+        typename M::Query q[NB];
+        Softmax<W> x[NB];
         int limit[NB];
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
-            const int p = item.pair + 16 * b + c;
-            const float* row = nullptr;
+            x[b].clear();
             limit[b] = -1;
-            if (16 * b + c < item.pairs) {
-                const int r = list[p / group];
-                row = query + (static_cast<int64_t>(r) * s.heads + item.kv * group + p % group) * s.head_dim;
-                limit[b] = rows[r].position - item.first;
-            }
-            if (b < blocks) Tile<T, W>::load_query(q[b], row, s.head_dim, scale, g);
-            m[b] = -INFINITY;
-            l[b] = 0;
-#pragma unroll
-            for (int d = 0; d < W / 16; ++d) o[b][d] = f32x4{0, 0, 0, 0};
+            const Pair p = pair_of(a, item, 16 * b + c);
+            if (p.is) limit[b] = p.row.position - item.first;
+            M::load_query(q[b], query_of(a, p), p.is, head_dim, a.quads, a.scale, g);
         }
-
-        Tile<T, W> tile;
-        const auto page_of = [&](int t) {  // the page and place of token item.first + t
-            const int at = (item.first & (s.page_tokens - 1)) + t;
-            return base + pages[at >> s.page_shift] * s.page_bytes;
-        };
-        const auto within = [&](int t) { return (item.first + t) & (s.page_tokens - 1); };
-        int t = wave * kTileTokens;
-        if (t < item.tokens) tile.load_keys(page_of(t) + static_cast<int64_t>(within(t)) * W * sizeof(T), c, g);
-        for (; t < item.tokens; t += kWaves * kTileTokens) {
-            tile.load_values(page_of(t) + s.kv_heads * head_bytes + within(t) * sizeof(T), s.page_tokens, c, g);
-            f32x4 sc[NB][2];
+        for (; t < item.tokens; t += kNarrowWaves * kTile) {
+            const T* vp = reinterpret_cast<const T*>(pages.values(pages.page(t))) + pages.within(t);
 #pragma unroll
-            for (int b = 0; b < NB; ++b)
-                if (b < blocks) tile.scores(q[b], sc[b]);
-            const int next = t + kWaves * kTileTokens;
-            if (next < item.tokens)
-                tile.load_keys(page_of(next) + static_cast<int64_t>(within(next)) * W * sizeof(T), c, g);
+            for (int d = 0; d < W / 16; ++d)
+#pragma unroll
+                for (int h = 0; h < M::kValueParts; ++h)
+                    v[d][h] = *(const SATORI_GLOBAL Fragment*)(vp + static_cast<int64_t>(16 * d + c) * pages.tokens +
+                                                               16 * h + kGroupLanes * g);
+            f32x4 score[NB][2];
+#pragma unroll
+            for (int b = 0; b < NB; ++b) score[b][0] = score[b][1] = f32x4{0, 0, 0, 0};
+#pragma unroll
+            for (int s = 0; s < M::kKeyParts; ++s)
+#pragma unroll
+                for (int term = 0; term < M::kTerms; ++term)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h)
+#pragma unroll
+                        for (int b = 0; b < NB; ++b) score[b][h] = M::score(k[h][s], q[b], s, term, score[b][h]);
+            if (t + kNarrowWaves * kTile < item.tokens) load_keys(t + kNarrowWaves * kTile);
             const int end = item.tokens - t;  // tokens of this tile that exist
-            const bool hides = item.first + t + kTileTokens - 1 > item.limit;
-            if (end < kTileTokens) tile.clip_values(end, g);
-            // A value that one row sees and another must not can only spoil the other's sums if it is not finite.
-            const bool one_by_one = hides && !__all(tile.values_finite());
+            const bool hides = item.first + t + kTile - 1 > item.limit;
+            if (end < kTile) {
+                // Values of tokens behind the end become zero (they are nobody's, and may hold anything).
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    if (M::token(g, i) >= end)
+#pragma unroll
+                        for (int d = 0; d < W / 16; ++d) v[d][i / kGroupLanes][i % kGroupLanes] = 0;
+            }
+            if (hides) {
+                bool finite = true;
+#pragma unroll
+                for (int d = 0; d < W / 16; ++d)
+#pragma unroll
+                    for (int h = 0; h < M::kValueParts; ++h) finite &= all_finite(v[d][h]);
+                if (!__all(finite))
+#pragma unroll
+                    for (int d = 0; d < W / 16; ++d)
+#pragma unroll
+                        for (int h = 0; h < M::kValueParts; ++h) {
+                            const Fragment spoiled = take_spoiled(v[d][h]);
+#pragma unroll
+                            for (int b = 0; b < NB; ++b) spoil<M>(spoiled, min(limit[b] - t + 1, end), h, g, x[b].o[d]);
+                        }
+            }
 #pragma unroll
             for (int b = 0; b < NB; ++b) {
-                if (b >= blocks) continue;
-                float x[8];
+                if (hides || end < kTile) hide<M>(score[b], min(limit[b] - t + 1, end), g);
+                float p[8];
+                x[b].take(score[b], q[b].factor, M::kTop, p);
+                typename M::Weights w;
+                M::weights(p, w);
 #pragma unroll
-                for (int i = 0; i < 8; ++i) x[i] = sc[b][i >> 2][i & 3] * q[b].factor;
-                if (hides || end < kTileTokens) {
-                    const int seen = min(limit[b] - t + 1, end);
+                for (int h = 0; h < M::kValueParts; ++h)
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) x[i] = Tile<T, W>::token(g, i) < seen ? x[i] : -INFINITY;
-                }
-                float top = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])),
-                                  fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
-                top = column_max(top);
-                if (__any(top > m[b])) {
-                    const float now = fmaxf(m[b], top);
-                    const float shrink = __builtin_amdgcn_exp2f(m[b] - (now == -INFINITY ? 0.0f : now));
-                    m[b] = now;
-                    l[b] *= shrink;
+                    for (int term = 0; term < M::kTerms; ++term)
 #pragma unroll
-                    for (int d = 0; d < W / 16; ++d) o[b][d] = o[b][d] * shrink;
-                }
-                const float from = Tile<T, W>::kTop - (m[b] == -INFINITY ? 0.0f : m[b]);
-#pragma unroll
-                for (int i = 0; i < 8; ++i) x[i] = __builtin_amdgcn_exp2f(x[i] + from);
-                l[b] += ((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7]));
-                if (!one_by_one) {
-                    tile.weigh(x, o[b]);
-                } else {
-                    for (int k = 0; k < min(end, kTileTokens); ++k) tile.weigh_one(x, k, g, t + k <= limit[b], o[b]);
-                }
+                        for (int d = 0; d < W / 16; ++d) x[b].o[d] = M::weigh(v[d][h], w, h, term, x[b].o[d]);
             }
         }
 
-        // The four waves' results joined, 16 pairs and up to 128 lanes at a time.
+        // The waves' results joined, 16 pairs and up to 128 lanes at a time.
+        __syncthreads();
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
             if (b >= blocks) continue;
-            const float sum = column_sum(l[b]);
+            const float sum = column_sum(x[b].l);
             if (g == 0) {
-                stats[wave][c][0] = m[b];
+                stats[wave][c][0] = x[b].m;
                 stats[wave][c][1] = sum;
             }
 #pragma unroll
             for (int part = 0; part < (W + kPart - 1) / kPart; ++part) {
-                constexpr int kTiles = kPart / 16;
 #pragma unroll
-                for (int d = 0; d < kTiles; ++d) {
-                    const int of = part * kTiles + d;
-                    if (of < W / 16) *reinterpret_cast<f32x4*>(&joined[wave][c][16 * d + 4 * g]) = o[b][of < W / 16 ? of : 0];
+                for (int d = 0; d < kPart / 16; ++d) {
+                    const int of = part * (kPart / 16) + d;
+                    if (of < W / 16) *reinterpret_cast<f32x4*>(&joined[wave][c][16 * d + 4 * g]) = x[b].o[of < W / 16 ? of : 0];
                 }
                 __syncthreads();
-                const int pair = threadIdx.x >> 4;  // 16 threads a pair
-                if (16 * b + pair < item.pairs) {
-                    float top = -INFINITY, total = 0;
+                const int pair = threadIdx.x >> 4;  // 16 threads a pair, four lanes each and turn
+                const Pair p = pair_of(a, item, 16 * b + pair);
+                if (p.is) {
+                    float top = -INFINITY, total = 0, weight[kNarrowWaves];
 #pragma unroll
-                    for (int w = 0; w < kWaves; ++w) top = fmaxf(top, stats[w][pair][0]);
-                    float weight[kWaves];
+                    for (int w = 0; w < kNarrowWaves; ++w) top = fmaxf(top, stats[w][pair][0]);
 #pragma unroll
-                    for (int w = 0; w < kWaves; ++w) {
-                        // (a NaN maximum never arises; a NaN score leaves a NaN sum)
+                    for (int w = 0; w < kNarrowWaves; ++w) {
                         weight[w] = __builtin_amdgcn_exp2f(stats[w][pair][0] - (top == -INFINITY ? 0.0f : top));
                         total += weight[w] * stats[w][pair][1];
                     }
-                    const int p = item.pair + 16 * b + pair;
-                    const int r = list[p / group], head = item.kv * group + p % group;
-                    const PlanRow row = rows[r];
-                    const int64_t index = static_cast<int64_t>(row.slot + item.slot) * s.heads + head;
                     const int left = W - part * kPart < kPart ? W - part * kPart : kPart;
-                    for (int d = threadIdx.x & 15; d < left; d += 16) {
-                        float v = 0;
+                    for (int d = 4 * (threadIdx.x & 15); d < left; d += 64) {
+                        f32x4 o{0, 0, 0, 0};
 #pragma unroll
-                        for (int w = 0; w < kWaves; ++w) v += weight[w] * joined[w][pair][d];
-                        const int lane_of = part * kPart + d;
-                        if (row.slots > 1)
-                            partial_values(partials, W, index)[lane_of] = v;
-                        else if (lane_of < s.head_dim)
-                            output[(static_cast<int64_t>(r) * s.heads + head) * s.head_dim + lane_of] = v / total;
+                        for (int w = 0; w < kNarrowWaves; ++w)
+                            o = o + *reinterpret_cast<const f32x4*>(&joined[w][pair][d]) * weight[w];
+                        give<W>(a, item, p, part * kPart + d, o, total);
                     }
-                    if (row.slots > 1 && part == 0 && (threadIdx.x & 15) == 0) {
-                        float* sums = partial_sums(partials, W, partial_rows, index);
-                        sums[0] = top;
-                        sums[1] = total;
-                    }
+                    if (part == 0 && (threadIdx.x & 15) == 0) give_sums<W>(a, item, p, top, total);
                 }
                 __syncthreads();
             }
@@ -545,83 +648,387 @@ __global__ __launch_bounds__(kWaves * 64, NB == 1 && W <= 128 ? 2 : 1) void cach
     }
 }
 
-// The partial results of one (row, head), joined by a wave: weight 2^(m_i - m) each.
-__global__ __launch_bounds__(kThreads) void cache_join_kernel(CacheShape s, const int* __restrict__ plan,
-                                                              float* partials, float* __restrict__ output) {
-    const PlanHeader& h = *reinterpret_cast<const PlanHeader*>(plan);
-    const PlanRow* rows = reinterpret_cast<const PlanRow*>(plan + h.rows_at);
+// Many pairs: PG groups of 16 * NB pairs, one per wave, share the tiles, which pass through LDS (two buffers: while one is
+// attended, the next steps' bytes are on their way in registers); TG such sets of waves take tiles in turn and are joined
+// at the end. Rows of a tile are 16-byte pieces, put where the 16 lanes that read a column of them reach different banks:
+// piece p of row r lies at p ^ (r's bits that its place in a 256-byte line leaves open).
+template <int PIECES>
+__device__ __forceinline__ int piece_at(int row, int piece) {
+    constexpr int kWhole = (PIECES & -PIECES) < 16 ? (PIECES & -PIECES) : 16;  // pieces that an XOR may permute
+    constexpr int kShift = kWhole == 16 ? 0 : kWhole == 8 ? 1 : 2;
+    return row * PIECES + (piece ^ ((row >> kShift) & (kWhole - 1)));
+}
+
+template <typename T, int W, int NB, int PG, int TG>
+struct Wide {
+    static constexpr int kThreads = 64 * PG * TG;
+    static constexpr int kPairs = 16 * NB * PG;
+    static constexpr int kKeyPieces = W * sizeof(T) / 16, kValuePieces = kTile * sizeof(T) / 16;
+    static constexpr int kKeys = kTile * kKeyPieces, kValues = W * kValuePieces;  // pieces of a tile
+    static constexpr int kPieces = kKeys + kValues;
+    static constexpr int kPer = (kPieces * TG + kThreads - 1) / kThreads;         // pieces a thread moves per step
+    // Whether all threads' i-th pieces belong to one tile, and to its keys or its values.
+    static constexpr bool kEven = kKeys % kThreads == 0 && kValues % kThreads == 0;
+    static constexpr size_t kBuffers = size_t(2) * TG * kPieces * 16;
+    static constexpr size_t kJoin = size_t(TG - 1) * PG * NB * 16 * (W + 4 + 2) * sizeof(float);
+    static constexpr size_t kTiles = kBuffers > kJoin ? kBuffers : kJoin;
+    static constexpr size_t kLds = kTiles + size_t(2) * TG * W * sizeof(uint32_t);
+};
+
+template <typename T, int W, int NB, int PG, int TG>
+__global__ __launch_bounds__(64 * PG * TG, 2) void cache_attention_wide_kernel(AttentionArgs a) {
+    using M = Math<T, W>;
+    using S = Wide<T, W, NB, PG, TG>;
+    using Fragment = typename M::Fragment;
+    extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
+    const int count = reinterpret_cast<const PlanHeader*>(a.image)->wide;
+    const PlanItem* items = reinterpret_cast<const PlanItem*>(a.image + a.at.wide_at);
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int pg = wave / TG, tg = wave % TG;
+    uint32_t* spoiled = reinterpret_cast<uint32_t*>(lds + S::kTiles);  // [2][TG][W]
+    for (int u = blockIdx.x; u < count; u += gridDim.x) {
+        const PlanItem item = scalar_load(items + u);
+        const int thread = unknown(threadIdx.x), lane = thread & 63, c = lane & 15, g = lane >> 4;
+        const int head_dim = unknown_scalar(a.s.head_dim);
+        const Pages pages(a, item, static_cast<int64_t>(a.s.page_tokens) * W * sizeof(T));
+        const int tiles = (item.tokens + kTile - 1) / kTile, steps = (tiles + TG - 1) / TG;
+        const int blocks = min(NB, (item.pairs - 16 * NB * pg + 15) / 16);  // of this wave; none or less: it only carries
+
+        u32x4 moved[S::kPer];
+        int of_set[TG];  // the pages of the step that is fetched next, read a step before
+        const auto look = [&](int step) {
+#pragma unroll
+            for (int k = 0; k < TG; ++k) of_set[k] = pages.page(min(step * TG + k, tiles - 1) * kTile);
+        };
+        const auto fetch = [&](int step) {
+#pragma unroll
+            for (int i = 0; i < S::kPer; ++i) {
+                const int n = thread + i * S::kThreads;
+                const int set = S::kEven ? i * S::kThreads / S::kPieces : n / S::kPieces;
+                const int piece = S::kEven ? thread + i * S::kThreads % S::kPieces : n % S::kPieces;
+                const int tile = step * TG + set;
+                if ((S::kPieces * TG % S::kThreads != 0 && n >= S::kPieces * TG) || tile >= tiles) continue;
+                int page = of_set[0];
+#pragma unroll
+                for (int k = 1; k < TG; ++k) page = set == k ? of_set[k] : page;
+                const uint8_t* from;
+                if (S::kEven ? i * S::kThreads % S::kPieces < S::kKeys : piece < S::kKeys) {
+                    from = pages.keys(page) + pages.within(tile * kTile) * (W * static_cast<int>(sizeof(T))) + piece * 16;
+                } else {
+                    const int row = (piece - S::kKeys) / S::kValuePieces, of = (piece - S::kKeys) % S::kValuePieces;
+                    from = pages.values(page) + (row * pages.tokens + pages.within(tile * kTile)) * static_cast<int>(sizeof(T)) + of * 16;
+                }
+                moved[i] = *(const SATORI_GLOBAL u32x4*)(from);
+            }
+        };
+        const auto put = [&](int step) {
+            u32x4* buffer = reinterpret_cast<u32x4*>(lds) + (step & 1) * TG * S::kPieces;
+#pragma unroll
+            for (int i = 0; i < S::kPer; ++i) {
+                const int n = thread + i * S::kThreads;
+                const int set = S::kEven ? i * S::kThreads / S::kPieces : n / S::kPieces;
+                const int piece = S::kEven ? thread + i * S::kThreads % S::kPieces : n % S::kPieces;
+                if (S::kPieces * TG % S::kThreads != 0 && n >= S::kPieces * TG) continue;
+                if (S::kEven ? i * S::kThreads % S::kPieces < S::kKeys : piece < S::kKeys) {
+                    const int row = M::key_row(piece / S::kKeyPieces);
+                    buffer[set * S::kPieces + piece_at<S::kKeyPieces>(row, piece % S::kKeyPieces)] = moved[i];
+                } else {
+                    const int row = (piece - S::kKeys) / S::kValuePieces, of = (piece - S::kKeys) % S::kValuePieces;
+                    buffer[set * S::kPieces + S::kKeys + piece_at<S::kValuePieces>(row, of)] = moved[i];
+                }
+            }
+        };
+
+        if (tiles > 0) {
+            look(0);
+            fetch(0);
+            look(1);
+        }
+        typename M::Query q[NB];
+        Softmax<W> x[NB];
+        int limit[NB];
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+            x[b].clear();
+            limit[b] = -1;
+            const Pair p = pair_of(a, item, 16 * (NB * pg + b) + c);
+            if (p.is) limit[b] = p.row.position - item.first;
+            M::load_query(q[b], query_of(a, p), p.is, head_dim, a.quads, a.scale, g);
+        }
+        // Tiles that some pair does not see whole, once they are in LDS: values of tokens behind the item's end become zero
+        // (they are nobody's, and may hold anything), and so do values that are not finite, whose places are kept as a bit
+        // per token of every lane: 0 * infinity would spoil the sums of pairs that must not see them.
+        const auto partial = [&](int tile) {
+            return tile < tiles && (item.first + tile * kTile + kTile - 1 > item.limit || tile * kTile + kTile > item.tokens);
+        };
+        const auto settle = [&](int step) {
+            if (!partial(min(step * TG + TG, tiles) - 1)) return;  // (the later a tile, the more it hides)
+            __syncthreads();
+            constexpr int kOf = 16 / sizeof(T);
+#pragma unroll 1
+            for (int n = thread; n < TG * W; n += S::kThreads) {
+                const int set = n / W, row = n % W, tile = step * TG + set, left = item.tokens - tile * kTile;
+                if (!partial(tile)) continue;
+                Fragment* values = reinterpret_cast<Fragment*>(lds) + ((step & 1) * TG + set) * S::kPieces + S::kKeys;
+                uint32_t where = 0;
+#pragma unroll 1
+                for (int piece = 0; piece < S::kValuePieces; ++piece) {
+                    Fragment v = values[piece_at<S::kValuePieces>(row, piece)];
+#pragma unroll
+                    for (int j = 0; j < kOf; ++j) {
+                        const int token = piece * kOf + j;
+                        const bool fine = __builtin_isfinite(static_cast<float>(v[j]));
+                        if (!fine && token < left) where |= 1u << token;
+                        v[j] = fine && token < left ? v[j] : 0;
+                    }
+                    values[piece_at<S::kValuePieces>(row, piece)] = v;
+                }
+                spoiled[((step & 1) * TG + set) * W + row] = where;
+            }
+        };
+
+        if (tiles > 0) {
+            put(0);
+            settle(0);
+        }
+        __syncthreads();
+        for (int step = 0; step < steps; ++step) {
+            if (step + 1 < steps) {
+                fetch(step + 1);
+                look(step + 2);
+            }
+            const int t = (step * TG + tg) * kTile;
+            if (t < item.tokens && blocks > 0) {
+                const Fragment* keys = reinterpret_cast<const Fragment*>(lds) + ((step & 1) * TG + tg) * S::kPieces;
+                const Fragment* values = keys + S::kKeys;
+                f32x4 score[NB][2];
+#pragma unroll
+                for (int b = 0; b < NB; ++b) score[b][0] = score[b][1] = f32x4{0, 0, 0, 0};
+#pragma unroll
+                for (int s = 0; s < M::kKeyParts; ++s) {
+                    Fragment k[2];
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) k[h] = keys[piece_at<S::kKeyPieces>(16 * h + c, 4 * s + g)];
+#pragma unroll
+                    for (int term = 0; term < M::kTerms; ++term)
+#pragma unroll
+                        for (int h = 0; h < 2; ++h)
+#pragma unroll
+                            for (int b = 0; b < NB; ++b) score[b][h] = M::score(k[h], q[b], s, term, score[b][h]);
+                }
+                __builtin_amdgcn_sched_barrier(0);  // (the scheduler would hold both products' fragments at once, and spill)
+                const int end = item.tokens - t;
+                const bool hides = item.first + t + kTile - 1 > item.limit;
+                const auto value = [&](int d, int h) { return values[piece_at<S::kValuePieces>(16 * d + c, 4 * h + g)]; };
+                typename M::Weights w[NB];
+#pragma unroll
+                for (int b = 0; b < NB; ++b) {
+                    if (hides || end < kTile) hide<M>(score[b], min(limit[b] - t + 1, end), g);
+                    float p[8];
+                    x[b].take(score[b], q[b].factor, M::kTop, p);
+                    M::weights(p, w[b]);
+                    if (hides) {
+                        const int seen = min(limit[b] - t + 1, kTile);
+                        const uint32_t sees = seen <= 0 ? 0u : ~0u >> (kTile - seen);
+                        const u32x4* bits = reinterpret_cast<const u32x4*>(spoiled + ((step & 1) * TG + tg) * W);
+#pragma unroll
+                        for (int d = 0; d < W / 16; ++d) {
+                            const u32x4 where = bits[4 * d + g];
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) x[b].o[d][j] = where[j] & sees ? NAN : x[b].o[d][j];
+                        }
+                    }
+                }
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int h = 0; h < M::kValueParts; ++h)
+#pragma unroll
+                    for (int d = 0; d < W / 16; ++d) {
+                        const Fragment v = value(d, h);
+#pragma unroll
+                        for (int term = 0; term < M::kTerms; ++term)
+#pragma unroll
+                            for (int b = 0; b < NB; ++b) x[b].o[d] = M::weigh(v, w[b], h, term, x[b].o[d]);
+                    }
+            }
+            if (step + 1 < steps) {
+                put(step + 1);
+                settle(step + 1);
+            }
+            __syncthreads();
+        }
+
+        // The sets joined by the first of each pair group, in order.
+        constexpr int kRow = W + 4 + 2;
+        float* joined = reinterpret_cast<float*>(lds);
+#pragma unroll
+        for (int b = 0; b < NB; ++b) x[b].l = column_sum(x[b].l);
+        if (TG > 1) {
+            if (tg > 0 && blocks > 0) {
+#pragma unroll
+                for (int b = 0; b < NB; ++b) {
+                    float* to = joined + (((tg - 1) * PG + pg) * NB * 16 + 16 * b + c) * kRow;
+#pragma unroll
+                    for (int d = 0; d < W / 16; ++d)
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) to[16 * d + 4 * g + j] = x[b].o[d][j];
+                    if (g == 0) {
+                        to[W] = x[b].m;
+                        to[W + 1] = x[b].l;
+                    }
+                }
+            }
+            __syncthreads();
+        }
+        if (tg == 0 && blocks > 0) {
+#pragma unroll
+            for (int b = 0; b < NB; ++b) {
+                if (b >= blocks) continue;
+                float top = x[b].m;
+#pragma unroll
+                for (int k = 1; k < TG; ++k) top = fmaxf(top, joined[(((k - 1) * PG + pg) * NB * 16 + 16 * b + c) * kRow + W]);
+                const float from = top == -INFINITY ? 0.0f : top;
+                const float own = __builtin_amdgcn_exp2f(x[b].m - from);
+                float total = own * x[b].l;
+#pragma unroll
+                for (int d = 0; d < W / 16; ++d) x[b].o[d] = x[b].o[d] * own;
+#pragma unroll
+                for (int k = 1; k < TG; ++k) {
+                    const float* of = joined + (((k - 1) * PG + pg) * NB * 16 + 16 * b + c) * kRow;
+                    const float weight = __builtin_amdgcn_exp2f(of[W] - from);
+                    total += weight * of[W + 1];
+#pragma unroll
+                    for (int d = 0; d < W / 16; ++d)
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) x[b].o[d][j] += weight * of[16 * d + 4 * g + j];
+                }
+                const Pair p = pair_of(a, item, 16 * (NB * pg + b) + c);
+                if (p.is) {
+#pragma unroll
+                    for (int d = 0; d < W / 16; ++d) give<W>(a, item, p, 16 * d + 4 * g, x[b].o[d], total);
+                    if (g == 0) give_sums<W>(a, item, p, top, total);
+                }
+            }
+        }
+        __syncthreads();  // the next item's tiles go where the sets' results are
+    }
+}
+
+// The partial results of one (row, head), joined by a wave with weights 2^(m_i - m): lanes first take a part each for the
+// maximum and the sum, then four lanes of the head each, several parts at once.
+__global__ __launch_bounds__(kThreads) void cache_join_kernel(AttentionArgs a) {
+    const CacheShape& s = a.s;
+    const PlanRow* rows = reinterpret_cast<const PlanRow*>(a.image + a.at.rows_at);
     const int lane = threadIdx.x & 63;
-    const int64_t units = static_cast<int64_t>(h.rows) * s.heads;
-    const int64_t partial_rows = static_cast<int64_t>(h.slots) * s.heads;
-    for (int64_t u = static_cast<int64_t>(blockIdx.x) * kWaves + (threadIdx.x >> 6); u < units; u += gridDim.x * kWaves) {
-        const int r = static_cast<int>(u / s.heads), head = static_cast<int>(u % s.heads);
-        const PlanRow row = rows[r];
+    const int64_t units = static_cast<int64_t>(reinterpret_cast<const PlanHeader*>(a.image)->rows) * s.heads;
+    const int quads = s.width / 4;                          // 8 .. 64 lanes take a part's values
+    const int at_once = 64 / quads, mine = lane / quads;    // parts read at once by the wave
+    const int d = lane % quads * 4;
+    for (int64_t u = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6); u < units; u += gridDim.x * 4) {
+        const int head = static_cast<int>(u % s.heads);
+        const PlanRow row = rows[u / s.heads];
         if (row.slots <= 1) continue;
         const int64_t first = static_cast<int64_t>(row.slot) * s.heads + head;
         float top = -INFINITY;
-        for (int i = 0; i < row.slots; ++i)
-            top = fmaxf(top, partial_sums(partials, s.width, partial_rows, first + static_cast<int64_t>(i) * s.heads)[0]);
+        for (int i = lane; i < row.slots; i += 64)
+            top = fmaxf(top, a.partials.sums(s.width, first + static_cast<int64_t>(i) * s.heads)[0]);
+#pragma unroll
+        for (int k = 32; k > 0; k >>= 1) top = fmaxf(top, __shfl_xor(top, k, 64));
         const float from = top == -INFINITY ? 0.0f : top;
-        float total = 0, v[4] = {0, 0, 0, 0};
-        for (int i = 0; i < row.slots; ++i) {
-            const int64_t index = first + static_cast<int64_t>(i) * s.heads;
-            const float* sums = partial_sums(partials, s.width, partial_rows, index);
-            const float weight = __builtin_amdgcn_exp2f(sums[0] - from);
-            total += weight * sums[1];
+        float total = 0;
+        f32x4 o{0, 0, 0, 0};
+        if (mine < at_once) {
+#pragma unroll 4
+            for (int i = mine; i < row.slots; i += at_once) {
+                const int64_t index = first + static_cast<int64_t>(i) * s.heads;
+                const float* sums = a.partials.sums(s.width, index);
+                const float weight = __builtin_amdgcn_exp2f(sums[0] - from);
+                total += weight * sums[1];
+                o = o + *reinterpret_cast<const f32x4*>(a.partials.values(s.width, index) + d) * weight;
+            }
+        }
+        // The groups of lanes added to the first, in order.
+        float all = 0;
+        f32x4 sum{0, 0, 0, 0};
+        for (int k = 0; k < at_once; ++k) {
+            all += __shfl(total, k * quads + lane % quads, 64);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) sum[j] += __shfl(o[j], k * quads + lane % quads, 64);
+        }
+        if (mine == 0)
 #pragma unroll
             for (int j = 0; j < 4; ++j)
-                if (lane + 64 * j < s.width) v[j] += weight * partial_values(partials, s.width, index)[lane + 64 * j];
-        }
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-            if (lane + 64 * j < s.head_dim) output[u * s.head_dim + lane + 64 * j] = v[j] / total;
+                if (d + j < s.head_dim) store_f32(a.output + u * s.head_dim + d + j, sum[j] / all);
     }
 }
 
-// Blocks of 16 pairs of a wide workgroup: what its registers hold beside a tile.
-constexpr int wide_blocks(bool, int width) { return width <= 64 ? 4 : width <= 128 ? 2 : 1; }
+// The wide kernel of a type and width: its pair groups are as wide as a wave's registers allow with two waves a SIMD, its
+// sets of waves as many as LDS holds two buffers for.
+template <typename T, int W>
+using WideOf = Wide<T, W, sizeof(T) * W <= 256 ? 2 : 1, sizeof(T) * W <= 512 ? 4 : 8, sizeof(T) * W <= 256 ? 2 : 1>;
+constexpr int kNarrowBlocks = 1;
+constexpr int kMostGroups = 1024;  // workgroups of a launch whose work is only known when it is replayed
 
-constexpr int kMostGroups = 2048;  // workgroups of a launch whose work is only known when it is replayed
-
-struct AttentionCall {
-    const int* plan;
-    PlanHeader now;
-    bool all;
-    int layer;
-    const float* query;
-    float *output, *partials;
-    hipStream_t stream;
-};
+template <typename T, int W, int NB, int PG, int TG>
+hipError_t launch_wide(Wide<T, W, NB, PG, TG>, int groups, const AttentionArgs& a, hipStream_t stream) {
+    using S = Wide<T, W, NB, PG, TG>;
+    const auto kernel = cache_attention_wide_kernel<T, W, NB, PG, TG>;
+    // (more than 64 KB of LDS; set for the current device, where it is a table lookup after the first time)
+    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize,
+                                             static_cast<int>(S::kLds));
+    if (e != hipSuccess) return e;
+    kernel<<<groups, S::kThreads, S::kLds, stream>>>(a);
+    return hipGetLastError();
+}
 
 template <typename T, int W>
-void attention_of_width(const CacheShape& s, const AttentionCall& a) {
-    const float scale = static_cast<float>(static_cast<double>(kLog2e) / std::sqrt(static_cast<double>(s.head_dim)));
-    if (a.now.wide || a.all)
-        cache_attention_kernel<T, W, wide_blocks(sizeof(T) == 4, W)>
-            <<<a.all ? kMostGroups : a.now.wide, kWaves * 64, 0, a.stream>>>(s, a.plan, a.layer, a.query, a.output,
-                                                                             a.partials, scale, 1);
-    if (a.now.narrow || a.all)
-        cache_attention_kernel<T, W, 1><<<a.all ? kMostGroups : a.now.narrow, kWaves * 64, 0, a.stream>>>(
-            s, a.plan, a.layer, a.query, a.output, a.partials, scale, 0);
+hipError_t attention_of_width(AttentionArgs a, const PlanHeader& now, bool all, hipStream_t stream) {
+    if (now.wide || all)
+        if (const hipError_t e = launch_wide(WideOf<T, W>{}, all ? kMostGroups : now.wide, a, stream); e != hipSuccess) return e;
+    if (now.narrow || all)
+        cache_attention_narrow_kernel<T, W, kNarrowBlocks>
+            <<<all ? kMostGroups : now.narrow, kNarrowWaves * 64, 0, stream>>>(a);
+    return hipGetLastError();
 }
 
-template <typename T>
-hipError_t attention_of_type(const CacheShape& s, const AttentionCall& a) {
-    switch (s.width) {
-        case 32: attention_of_width<T, 32>(s, a); break;
-        case 64: attention_of_width<T, 64>(s, a); break;
-        case 96: attention_of_width<T, 96>(s, a); break;
-        case 128: attention_of_width<T, 128>(s, a); break;
-        case 192: attention_of_width<T, 192>(s, a); break;
-        case 256: attention_of_width<T, 256>(s, a); break;
-        default: return hipErrorInvalidValue;
-    }
-    return hipGetLastError();
+// Calls f with the type and width of a shape as template arguments.
+template <typename F>
+auto of_shape(int type, int width, F&& f) {
+    const auto of_type = [&](auto t) {
+        switch (width) {
+            case 32: return f(t, std::integral_constant<int, 32>{});
+            case 64: return f(t, std::integral_constant<int, 64>{});
+            case 96: return f(t, std::integral_constant<int, 96>{});
+            case 128: return f(t, std::integral_constant<int, 128>{});
+            case 192: return f(t, std::integral_constant<int, 192>{});
+            default: return f(t, std::integral_constant<int, 256>{});
+        }
+    };
+    return type == kF32 ? of_type(float{}) : of_type(_Float16{});
 }
 
 }  // namespace
 
-int cache_wide_pairs(int type, int width) { return 16 * wide_blocks(type == kF32, width); }
+int cache_wide_pairs(int type, int width) {
+    return of_shape(type, width, [](auto t, auto w) { return WideOf<decltype(t), decltype(w)::value>::kPairs; });
+}
+
+hipError_t launch_plan_copy(const int* from, int* to, const PlanLayout& layout, const PlanLayout& used, hipStream_t stream) {
+    const int at[kPlanParts] = {0, layout.rows_at, layout.narrow_at, layout.wide_at, layout.runs_at, layout.pages_at,
+                                layout.list_at};
+    const size_t words[kPlanParts] = {sizeof(PlanHeader) / 4, used.rows * sizeof(PlanRow) / 4, used.narrow * sizeof(PlanItem) / 4,
+                                      used.wide * sizeof(PlanItem) / 4, used.runs * sizeof(PlanRun) / 4,
+                                      static_cast<size_t>(used.pages), used.list * sizeof(PlanRow) / 4};
+    PlanParts parts;
+    int end = 0;
+    for (int i = 0; i < kPlanParts; ++i) {
+        parts.at[i] = at[i] / 4;
+        parts.end[i] = end += static_cast<int>((words[i] + 3) / 4);
+    }
+    plan_copy_kernel<<<(end + kThreads - 1) / kThreads, kThreads, 0, stream>>>(reinterpret_cast<const u32x4*>(from),
+                                                                              reinterpret_cast<u32x4*>(to), parts);
+    return hipGetLastError();
+}
 
 hipError_t launch_copy_pages(uint8_t* pool, int64_t page_bytes, const PageMoves& moves, hipStream_t stream) {
     if (moves.count == 0) return hipSuccess;
@@ -630,8 +1037,8 @@ hipError_t launch_copy_pages(uint8_t* pool, int64_t page_bytes, const PageMoves&
     return hipGetLastError();
 }
 
-hipError_t launch_cache_append(const CacheShape& s, const int* plan, const PlanHeader& now, bool all,
-                               const AppendArgs& args, hipStream_t stream) {
+hipError_t launch_cache_append(const CacheShape& s, const int* image, const PlanLayout& layout, const PlanHeader& now,
+                               bool all, const AppendArgs& args, hipStream_t stream) {
     if (now.runs == 0 && !all) return hipSuccess;
     // Four lane pairs a thread and access where every row allows it.
     const auto whole = [](const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; };
@@ -643,7 +1050,7 @@ hipError_t launch_cache_append(const CacheShape& s, const int* plan, const PlanH
     const int64_t values = (static_cast<int64_t>(longest) / kGroupTokens + 1) * s.kv_heads * s.head_dim;
     const int y = static_cast<int>(std::min<int64_t>((std::max(turns, values) + kThreads - 1) / kThreads, 1024));
     const dim3 grid(all ? 256 : now.runs, y);
-    const auto launch = [&](auto kernel) { kernel<<<grid, kThreads, 0, stream>>>(s, plan, args); };
+    const auto launch = [&](auto kernel) { kernel<<<grid, kThreads, 0, stream>>>(s, image, layout.runs_at, args); };
     if (s.type == kF32)
         packed ? launch(cache_append_kernel<float, 4>) : launch(cache_append_kernel<float, 1>);
     else
@@ -655,16 +1062,20 @@ size_t cache_partial_bytes(const CacheShape& shape, int64_t slots) {
     return static_cast<size_t>(slots) * shape.heads * (shape.width + 2) * sizeof(float);
 }
 
-hipError_t launch_cache_attention(const CacheShape& shape, const int* plan, const PlanHeader& now, bool all, int layer,
-                                  const float* query, float* output, float* partials, hipStream_t stream) {
+hipError_t launch_cache_attention(const CacheShape& shape, const int* image, const PlanLayout& layout, const PlanHeader& now,
+                                  bool all, int layer, const float* query, float* output, float* partials, size_t bytes,
+                                  hipStream_t stream) {
     if (now.rows == 0 && !all) return hipSuccess;
-    const AttentionCall call{plan, now, all, layer, query, output, partials, stream};
-    const hipError_t e = shape.type == kF32 ? attention_of_type<float>(shape, call)
-                                            : attention_of_type<_Float16>(shape, call);
+    const int64_t room = static_cast<int64_t>(bytes / cache_partial_bytes(shape, 1)) * shape.heads;
+    const float scale = static_cast<float>(static_cast<double>(kLog2e) / std::sqrt(static_cast<double>(shape.head_dim)));
+    const AttentionArgs a{shape, image, layout, layer, query, output, Partials{partials, room}, scale,
+                          shape.head_dim % 4 == 0 && reinterpret_cast<uintptr_t>(query) % 16 == 0};
+    const hipError_t e = of_shape(shape.type, shape.width, [&](auto t, auto w) {
+        return attention_of_width<decltype(t), decltype(w)::value>(a, now, all, stream);
+    });
     if (e != hipSuccess || (now.joined == 0 && !all)) return e;
-    const int64_t groups = (static_cast<int64_t>(now.rows) * shape.heads + kWaves - 1) / kWaves;
-    cache_join_kernel<<<all ? kMostGroups : static_cast<int>(std::min<int64_t>(groups, 65536)), kThreads, 0, stream>>>(
-        shape, plan, partials, output);
+    const int64_t groups = (static_cast<int64_t>(now.rows) * shape.heads + 3) / 4;
+    cache_join_kernel<<<all ? kMostGroups : static_cast<int>(std::min<int64_t>(groups, 65536)), kThreads, 0, stream>>>(a);
     return hipGetLastError();
 }
 

@@ -37,6 +37,9 @@ struct CacheShape {
 // Pairs of a wide attention workgroup (PlanShape::wide_pairs).
 int cache_wide_pairs(int type, int width);
 
+// Copies what a plan's arrays hold from pinned host memory to the same places of the image on the device.
+hipError_t launch_plan_copy(const int* from, int* to, const PlanLayout& layout, const PlanLayout& used, hipStream_t stream);
+
 constexpr int kMovesPerLaunch = 224;  // pairs of page numbers in a launch's arguments
 struct PageMoves {
     int count, pad;
@@ -54,15 +57,15 @@ struct AppendArgs {
     int rope_positions;
     int layer;
 };
-// `plan`: the image on the device, `now` its header. `all`: the launch is captured and replays may read any plan, so its
+// `image`: a plan's on the device, `now` its header. `all`: the launch is captured and replays may read any plan, so its
 // grid must do for any.
-hipError_t launch_cache_append(const CacheShape& shape, const int* plan, const PlanHeader& now, bool all,
-                               const AppendArgs& args, hipStream_t stream);
+hipError_t launch_cache_append(const CacheShape& shape, const int* image, const PlanLayout& layout, const PlanHeader& now,
+                               bool all, const AppendArgs& args, hipStream_t stream);
 
-// `partials`: cache_partial_bytes for the plan's slots. Launches with no work now are left out unless `all` (captured:
-// replays may have some).
+// `partials`: at least cache_partial_bytes for the plan's slots. Launches with no work now are left out unless `all`.
 size_t cache_partial_bytes(const CacheShape& shape, int64_t slots);
-hipError_t launch_cache_attention(const CacheShape& shape, const int* plan, const PlanHeader& now, bool all, int layer,
-                                  const float* query, float* output, float* partials, hipStream_t stream);
+hipError_t launch_cache_attention(const CacheShape& shape, const int* image, const PlanLayout& layout, const PlanHeader& now,
+                                  bool all, int layer, const float* query, float* output, float* partials, size_t bytes,
+                                  hipStream_t stream);
 
 }  // namespace satori

@@ -238,8 +238,8 @@ PlanImage plan_batch(const PageTables& tables, const int* sequences, const int* 
     if (std::adjacent_find(sorted.begin(), sorted.end()) != sorted.end())
         fail(SATORI_HIP_E_ARGUMENT, "A sequence is listed twice.");
     std::vector<int> first_row(count + 1);
-    std::vector<PlanRow> rows;
-    std::vector<PlanRun> runs;
+    std::vector<PlanRow>& rows = image.rows;
+    std::vector<PlanRun>& runs = image.runs;
     for (int i = 0; i < count; ++i) {
         const int tokens = tables.tokens(sequences[i]);
         if (new_tokens[i] < 0 || new_tokens[i] > tokens)
@@ -251,12 +251,11 @@ PlanImage plan_batch(const PageTables& tables, const int* sequences, const int* 
         const std::vector<int>& table = tables.table(sequences[i]);
         for (int p = tokens - new_tokens[i]; p < tokens; ++p) {
             if (p % P == 0 || p == tokens - new_tokens[i]) {
-                runs.push_back({static_cast<int>(rows.size()), 0, table[p / P], p % P});
+                runs.push_back({static_cast<int>(rows.size()), 0, table[p / P], p % P, p, {}});
                 image.writable &= tables.references(table[p / P]) == 1;
             }
             image.header.longest_run = std::max(image.header.longest_run, ++runs.back().tokens);
-            rows.push_back({p, 0, 0, 0});
-            image.last_position = std::max(image.last_position, p);
+            rows.push_back({p, 0, 0, static_cast<int>(rows.size())});
         }
     }
 
@@ -339,7 +338,8 @@ PlanImage plan_batch(const PageTables& tables, const int* sequences, const int* 
     };
     const int narrow_chunk = chunk_for(narrow_tokens, 1024), wide_chunk = chunk_for(wide_tokens, 256);
 
-    std::vector<int> page_list, row_list;
+    std::vector<int>& page_list = image.pages;
+    std::vector<int> row_list;
     for (Node& n : nodes) {
         n.chunk = n.wide ? wide_chunk : narrow_chunk;
         n.chunks = (n.end - n.begin + n.chunk - 1) / n.chunk;
@@ -365,10 +365,13 @@ PlanImage plan_batch(const PageTables& tables, const int* sequences, const int* 
 
     // The workgroups. Consecutive workgroups run on different XCDs (eight, each with an L2 of its own), so the blocks of
     // pairs that read the same tokens are put eight apart.
-    std::vector<PlanItem> narrow, wide;
+    std::vector<PlanItem>&narrow = image.narrow, &wide = image.wide;
     for (size_t i = 0; i < nodes.size(); ++i) {
         const Node& n = nodes[i];
-        const int step = n.wide ? shape.wide_pairs : kNarrowPairs;
+        // Blocks of pairs, as even as whole matrix tiles of 16 make them.
+        const int most = n.wide ? shape.wide_pairs : kNarrowPairs;
+        const int64_t least = (pairs_of[i] + most - 1) / most;
+        const int step = static_cast<int>((pairs_of[i] + 16 * least - 1) / (16 * least) * 16);
         const int blocks = static_cast<int>((pairs_of[i] + step - 1) / step);
         const int64_t units = static_cast<int64_t>(n.chunks) * shape.kv_heads;
         std::vector<PlanItem>& list = n.wide ? wide : narrow;
@@ -400,29 +403,82 @@ PlanImage plan_batch(const PageTables& tables, const int* sequences, const int* 
                 }
     }
 
-    const auto append = [&](const auto& v) {
-        using T = typename std::decay_t<decltype(v)>::value_type;
-        static_assert(sizeof(T) % 4 == 0, "whole words");
-        const size_t at = (image.words.size() + 3) / 4 * 4;  // 16-byte aligned
-        image.words.resize(at + v.size() * (sizeof(T) / 4));
-        if (!v.empty()) std::memcpy(image.words.data() + at, v.data(), v.size() * sizeof(T));
-        return static_cast<int>(at);
-    };
+    image.list.reserve(row_list.size());
+    for (int r : row_list) image.list.push_back(rows[r]);
     PlanHeader& h = image.header;
-    image.words.resize(sizeof(PlanHeader) / 4);
     h.rows = static_cast<int>(rows.size());
     h.narrow = static_cast<int>(narrow.size());
     h.wide = static_cast<int>(wide.size());
     h.runs = static_cast<int>(runs.size());
-    h.rows_at = append(rows);
-    h.narrow_at = append(narrow);
-    h.wide_at = append(wide);
-    h.runs_at = append(runs);
-    h.pages_at = append(page_list);
-    h.list_at = append(row_list);
-    image.words.resize((image.words.size() + 3) / 4 * 4);
-    std::memcpy(image.words.data(), &h, sizeof h);
     return image;
+}
+
+bool PlanLayout::grow(const PlanLayout& least) {
+    bool moved = words == 0;
+    const auto room = [&](int& have, int need) {
+        if (need <= have) return;
+        have = static_cast<int>(std::min<int64_t>(static_cast<int64_t>(need) + need / 2 + 16, INT32_MAX / 64));
+        have = std::max(have, need);
+        moved = true;
+    };
+    room(rows, least.rows);
+    room(narrow, least.narrow);
+    room(wide, least.wide);
+    room(runs, least.runs);
+    room(pages, least.pages);
+    room(list, least.list);
+    if (!moved) return false;
+    int64_t at = sizeof(PlanHeader) / 4;
+    const auto place = [&](int& where, int64_t entries, size_t size) {
+        where = static_cast<int>(at);
+        at = (at + entries * static_cast<int64_t>(size / 4) + 3) / 4 * 4;  // 16-byte aligned
+        if (at > INT32_MAX / 8) fail(SATORI_HIP_E_OVERFLOW, "Arithmetic operation resulted in an overflow.");
+    };
+    place(rows_at, rows, sizeof(PlanRow));
+    place(narrow_at, narrow, sizeof(PlanItem));
+    place(wide_at, wide, sizeof(PlanItem));
+    place(runs_at, runs, sizeof(PlanRun));
+    place(pages_at, pages, sizeof(int));
+    place(list_at, list, sizeof(PlanRow));
+    words = static_cast<int>(at);
+    return true;
+}
+
+PlanLayout PlanLayout::first() {
+    PlanLayout least, layout;
+    least.rows = least.runs = 256;
+    least.narrow = least.wide = 1024;
+    least.pages = 16384;
+    least.list = 1024;
+    layout.grow(least);
+    return layout;
+}
+
+PlanLayout PlanImage::least() const {
+    PlanLayout l;
+    l.rows = static_cast<int>(rows.size());
+    l.narrow = static_cast<int>(narrow.size());
+    l.wide = static_cast<int>(wide.size());
+    l.runs = static_cast<int>(runs.size());
+    l.pages = static_cast<int>(pages.size());
+    l.list = static_cast<int>(list.size());
+    return l;
+}
+
+void PlanImage::write(const PlanLayout& layout, int* words) const {
+    static_assert(sizeof(PlanHeader) % 16 == 0 && sizeof(PlanRow) % 16 == 0 && sizeof(PlanItem) % 16 == 0 &&
+                      sizeof(PlanRun) % 16 == 0,
+                  "16-byte entries");
+    std::memcpy(words, &header, sizeof header);
+    const auto put = [&](int at, const auto& v) {
+        if (!v.empty()) std::memcpy(words + at, v.data(), v.size() * sizeof(v[0]));
+    };
+    put(layout.rows_at, rows);
+    put(layout.narrow_at, narrow);
+    put(layout.wide_at, wide);
+    put(layout.runs_at, runs);
+    put(layout.pages_at, pages);
+    put(layout.list_at, list);
 }
 
 }  // namespace satori

@@ -75,7 +75,7 @@ private:
 // One query row: attends positions 0 .. position of its sequence. Its attention is the joined result of `slots` partial
 // ones, slot .. slot + slots - 1 (one: written as the output by the workgroup that computes it).
 struct PlanRow {
-    int position, slot, slots, pad;
+    int position, slot, slots, row;
 };
 
 // One workgroup's attention: key/value head `kv`, tokens [first, first + tokens) of the pages listed from `pages` on
@@ -88,17 +88,29 @@ struct PlanItem {
     int limit, pad[3];
 };
 
-// Consecutive rows of one sequence whose positions lie in one page: row .. row + tokens - 1 at `offset` of the page.
+// Consecutive rows of one sequence whose positions lie in one page: row .. row + tokens - 1, from `position` on, at `offset`
+// of the page.
 struct PlanRun {
     int row, tokens, page, offset;
+    int position, pad[3];
 };
 
-// At the start of the image; the offsets count 4-byte words from there.
+// At the start of the image.
 struct PlanHeader {
     int rows, narrow, wide, runs;
-    int rows_at, narrow_at, wide_at, runs_at;
-    int pages_at, list_at, joined, slots;  // joined: rows of several slots; slots: of all rows
-    int longest_run, pad[3];
+    int joined, slots, longest_run, pad;  // joined: rows of several slots; slots: of all rows
+};
+
+// Where the arrays lie in the image (in 4-byte words from its start) and how many entries each has room for. Launches
+// take it by value, so that a launch finds an array without reading where it is; room only grows.
+struct PlanLayout {
+    int rows_at = 0, narrow_at = 0, wide_at = 0, runs_at = 0, pages_at = 0, list_at = 0, words = 0;
+    int rows = 0, narrow = 0, wide = 0, runs = 0, pages = 0, list = 0;
+    // Room for at least these; whether anything moved.
+    bool grow(const PlanLayout& least);
+    // What a plan begins with: a batch of a few hundred rows over long sequences, so that a captured step has room to
+    // follow it.
+    static PlanLayout first();
 };
 
 struct PlanShape {
@@ -106,12 +118,16 @@ struct PlanShape {
     int wide_pairs;       // pairs of a wide workgroup; a narrow one takes 16
 };
 
-// The image of a plan and what its launches need to know.
+// A plan's arrays, and what its launches need to know.
 struct PlanImage {
-    std::vector<int> words;
     PlanHeader header{};
-    int last_position = 0;
+    std::vector<PlanRow> rows, list;  // list: the rows of every item's part of the tree
+    std::vector<PlanItem> narrow, wide;
+    std::vector<PlanRun> runs;
+    std::vector<int> pages;
     bool writable = true;  // no page that the rows lie in is shared
+    PlanLayout least() const;  // the room they take
+    void write(const PlanLayout& layout, int* words) const;
 };
 
 // Rows: the last new_tokens[i] positions of sequences[i], in this order.

@@ -194,7 +194,8 @@ struct satori_hip_cache_plan {
     satori::CacheShape shape{};
     int page_count = 0, layers = 0;
     satori::PlanShape plan{};
-    satori::PlanHeader header{};     // of the image on the device; rows are 0 before the first satori_hip_cache_plan_set
+    satori::PlanHeader header{};     // of the image on the device
+    satori::PlanLayout layout;       // of the image; it does not move while steps read it
     bool set = false, writable = false;
     satori::DeviceBuffer image, partials;
     satori::PinnedBuffer staging[2];  // in turn; `copied` tells when the device has read one
@@ -2319,13 +2320,16 @@ int plan_call(satori_hip_cache_plan* p, F&& body) {
     return handle_call(p, "plan", "satori_hip_cache_plan", [&](satori_hip_context* c) { body(c); });
 }
 
+[[noreturn]] void plan_held() {
+    fail(SATORI_HIP_E_INVALID_OPERATION,
+         "The memory of this plan cannot grow while a captured step reads it: destroy the step, or set the largest batch "
+         "before capturing.");
+}
+
 // Grows a buffer of the plan, unless a captured step reads it.
 void reserve_for_plan(satori_hip_cache_plan* p, DeviceBuffer& buffer, size_t need) {
     if (need <= buffer.bytes) return;
-    if (p->steps > 0)
-        fail(SATORI_HIP_E_INVALID_OPERATION,
-             "The memory of this plan cannot grow while a captured step reads it: destroy the step, or set the largest "
-             "batch before capturing.");
+    if (p->steps > 0) plan_held();
     check_hip(hipDeviceSynchronize(), "device");  // earlier launches on any stream may read the old one
     buffer.reserve(need + need / 2);
 }
@@ -2418,7 +2422,8 @@ int satori_hip_cache_plan_create(satori_hip_context* c, void* pool, int page_cou
         p->plan.wide_pairs = cache_wide_pairs(type, shape.width);
         try {
             for (hipEvent_t& e : p->copied) check_hip(hipEventCreateWithFlags(&e, hipEventDisableTiming), "hipEventCreate");
-            p->image.reserve(size_t(256) << 10);
+            p->layout = PlanLayout::first();
+            p->image.reserve(static_cast<size_t>(p->layout.words) * 4);
             p->partials.reserve(size_t(4) << 20);
         } catch (...) {
             free_plan(p);
@@ -2469,19 +2474,21 @@ int satori_hip_cache_plan_set(satori_hip_cache_plan* p, satori_hip_pages* pages,
                 fail(SATORI_HIP_E_ARGUMENT, "The pages are not those of the plan's pool.");
             image = plan_batch(tables, sequences, new_tokens, count, p->plan);
         }
-        const size_t bytes = image.words.size() * 4;
+        PlanLayout layout = p->layout;
+        const PlanLayout used = image.least();
+        if (layout.grow(used) && p->steps > 0) plan_held();
+        const size_t bytes = static_cast<size_t>(layout.words) * 4;
         reserve_for_plan(p, p->image, bytes);
         reserve_for_plan(p, p->partials, cache_partial_bytes(p->shape, image.header.slots));
         const int turn = p->turn;
         check_hip(hipEventSynchronize(p->copied[turn]), "plan copy");  // (done at once where none was recorded)
-        p->staging[turn].reserve(std::max(bytes, p->image.bytes));
-        std::memcpy(p->staging[turn].ptr, image.words.data(), bytes);
-        if (bytes <= kKernelCopyMaxBytes)
-            check_hip(launch_copy_words(p->staging[turn].ptr, p->image.ptr, bytes, st), "plan copy");
-        else
-            check_hip(hipMemcpyAsync(p->image.ptr, p->staging[turn].ptr, bytes, hipMemcpyHostToDevice, st), "plan copy");
+        p->staging[turn].reserve(p->image.bytes);
+        int* staging = static_cast<int*>(p->staging[turn].ptr);
+        image.write(layout, staging);
+        check_hip(launch_plan_copy(staging, static_cast<int*>(p->image.ptr), layout, used, st), "plan copy");
         check_hip(hipEventRecord(p->copied[turn], st), "plan copy");
         p->turn ^= 1;
+        p->layout = layout;
         p->header = image.header;
         p->writable = image.writable;
         p->set = true;
@@ -2514,7 +2521,7 @@ int satori_hip_cache_append(satori_hip_cache_plan* p, int layer, const float* qu
         const bool captured = note_plan(c, p, layer, st);
         const AppendArgs args{query, query_bias, key, key_bias, value, value_bias, query_out, frequency_base,
                               rotary_dimensions, rope_table, rope_table ? rope_positions : 0, layer};
-        check_hip(launch_cache_append(s, static_cast<const int*>(p->image.ptr), p->header, captured, args, st),
+        check_hip(launch_cache_append(s, static_cast<const int*>(p->image.ptr), p->layout, p->header, captured, args, st),
                   "cache append launch");
     });
 }
@@ -2530,8 +2537,8 @@ int satori_hip_cache_attention(satori_hip_cache_plan* p, int layer, const float*
         if (bytes_overlap(query, bytes, output, bytes) || bytes_overlap(output, bytes, s.pool, pool))
             fail(SATORI_HIP_E_ARGUMENT, "Attention output overlaps input.");
         const bool captured = note_plan(c, p, layer, st);
-        check_hip(launch_cache_attention(s, static_cast<const int*>(p->image.ptr), p->header, captured, layer, query, output,
-                                         static_cast<float*>(p->partials.ptr), st),
+        check_hip(launch_cache_attention(s, static_cast<const int*>(p->image.ptr), p->layout, p->header, captured, layer, query,
+                                         output, static_cast<float*>(p->partials.ptr), p->partials.bytes, st),
                   "cache attention launch");
     });
 }

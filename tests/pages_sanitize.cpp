@@ -36,22 +36,27 @@ void expect(bool ok, const char* what, int round) {
 }
 
 template <class T>
-std::vector<T> section(const PlanImage& image, int at, int count, int round) {
-    const size_t words = static_cast<size_t>(count) * (sizeof(T) / 4);
-    expect(at >= 0 && at + words <= image.words.size(), "a section lies outside the image", round);
+std::vector<T> section(const std::vector<int>& words, int at, int count, int round) {
+    const size_t n = static_cast<size_t>(count) * (sizeof(T) / 4);
+    expect(at % 4 == 0 && at >= 0 && at + n <= words.size(), "a section lies outside the image", round);
     std::vector<T> out(count);
-    if (count) std::memcpy(out.data(), image.words.data() + at, words * 4);
+    if (count) std::memcpy(out.data(), words.data() + at, n * 4);
     return out;
 }
 
 void check_plan(const PageTables& tables, const std::vector<int>& sequences, const std::vector<int>& fresh,
-                const PlanShape& shape, int round) {
+                const PlanShape& shape, PlanLayout& at, int round) {
     const PlanImage image = plan_batch(tables, sequences.data(), fresh.data(), static_cast<int>(sequences.size()), shape);
+    const PlanLayout before = at;
+    if (!at.grow(image.least())) expect(std::memcmp(&before, &at, sizeof at) == 0, "a layout that stays", round);
+    std::vector<int> words(at.words);
+    image.write(at, words.data());
     PlanHeader h;
-    std::memcpy(&h, image.words.data(), sizeof h);
-    expect(std::memcmp(&h, &image.header, sizeof h) == 0, "the image's header", round);
-    expect(image.words.size() % 4 == 0, "whole 16-byte words", round);
-    const auto rows = section<PlanRow>(image, h.rows_at, h.rows, round);
+    std::memcpy(&h, words.data(), sizeof h);
+    expect(words.size() % 4 == 0, "whole 16-byte words", round);
+    expect(h.rows <= at.rows && h.narrow <= at.narrow && h.wide <= at.wide && h.runs <= at.runs, "room", round);
+    const auto rows = section<PlanRow>(words, at.rows_at, h.rows, round);
+    for (size_t r = 0; r < rows.size(); ++r) expect(rows[r].row == static_cast<int>(r), "a row's number", round);
     const int P = tables.page_tokens();
     std::vector<std::pair<int, int>> of_row;  // sequence, position
     for (size_t i = 0; i < sequences.size(); ++i)
@@ -61,8 +66,9 @@ void check_plan(const PageTables& tables, const std::vector<int>& sequences, con
     // Runs.
     std::vector<int> written(rows.size());
     bool writable = true;
-    for (const PlanRun& run : section<PlanRun>(image, h.runs_at, h.runs, round)) {
+    for (const PlanRun& run : section<PlanRun>(words, at.runs_at, h.runs, round)) {
         expect(run.tokens > 0 && run.offset >= 0 && run.offset + run.tokens <= P, "a run within a page", round);
+        expect(run.position == of_row.at(run.row).second && run.tokens <= h.longest_run, "a run's positions", round);
         for (int t = 0; t < run.tokens; ++t) {
             const auto [s, p] = of_row.at(run.row + t);
             expect(rows[run.row + t].position == p, "a row's position", round);
@@ -76,23 +82,27 @@ void check_plan(const PageTables& tables, const std::vector<int>& sequences, con
     // Items: (row, kv, head of the group) -> positions seen, and slots written.
     std::map<std::tuple<int, int, int>, std::pair<std::vector<int>, std::set<int>>> seen;
     for (int wide = 0; wide < 2; ++wide)
-        for (const PlanItem& item : section<PlanItem>(image, wide ? h.wide_at : h.narrow_at, wide ? h.wide : h.narrow, round)) {
+        for (const PlanItem& item : section<PlanItem>(words, wide ? at.wide_at : at.narrow_at, wide ? h.wide : h.narrow, round)) {
             expect(item.first % 32 == 0 && item.tokens >= 0, "an item's tokens", round);
             expect(item.pairs > 0 && item.pairs <= (wide ? shape.wide_pairs : 16), "an item's pairs", round);
             expect(item.kv >= 0 && item.kv < shape.kv_heads, "an item's head", round);
             int least = INT32_MAX;
             for (int p = item.pair; p < item.pair + item.pairs; ++p) {
-                const size_t list_at = static_cast<size_t>(h.list_at) + item.rows + p / shape.group;
-                expect(list_at < image.words.size(), "a row list inside the image", round);
-                const int r = image.words.at(list_at);
+                const int entry = item.rows + p / shape.group;
+                expect(entry >= 0 && entry < at.list, "a row list inside its room", round);
+                PlanRow listed;
+                std::memcpy(&listed, words.data() + at.list_at + 4 * entry, sizeof listed);
+                const int r = listed.row;
+                expect(std::memcmp(&listed, &rows.at(r), sizeof listed) == 0, "a listed row", round);
                 const auto [s, position] = of_row.at(r);
                 least = std::min(least, position);
                 auto& [positions, slots] = seen[{r, item.kv, p % shape.group}];
                 expect(item.slot >= 0 && item.slot < rows[r].slots, "a slot of the row", round);
                 expect(slots.insert(item.slot).second, "a slot is written once", round);
                 for (int t = item.first; t < item.first + item.tokens; ++t) {
-                    const size_t page_at = static_cast<size_t>(h.pages_at) + item.pages + t / P - item.first / P;
-                    const int page = image.words.at(page_at);
+                    const int entry = item.pages + t / P - item.first / P;
+                    expect(entry >= 0 && entry < at.pages, "a page list inside its room", round);
+                    const int page = words.at(at.pages_at + entry);
                     expect(page >= 0 && page < tables.pages(), "a page of the pool", round);
                     if (t > position) continue;  // hidden
                     expect(page == tables.table(s).at(t / P), "the page of a position", round);
@@ -128,6 +138,7 @@ int main() {
         const int P = 32 << up_to(3), pages = 4 + up_to(60);
         PageTables tables(pages, P);
         std::vector<int> open;
+        PlanLayout layout;
         for (int step = 0; step < 25; ++step) {
             try {
                 std::vector<PageMove> moves;
@@ -178,7 +189,7 @@ int main() {
                     batch.push_back(id);
                     fresh.push_back(std::min(tables.tokens(id), up_to(2) ? 1 : up_to(40)));
                 }
-            check_plan(tables, batch, fresh, PlanShape{1 + up_to(2), 1 + up_to(6), 16 << up_to(2)}, round);
+            check_plan(tables, batch, fresh, PlanShape{1 + up_to(2), 1 + up_to(6), 16 << up_to(2)}, layout, round);
         }
     }
     // Long sequences, many chunks.
@@ -197,7 +208,8 @@ int main() {
             fresh.push_back(1 + up_to(2));
             if (fresh.back() > n) fresh.back() = n;
         }
-        check_plan(tables, batch, fresh, PlanShape{2, 3, 64}, round);
+        PlanLayout layout;
+        check_plan(tables, batch, fresh, PlanShape{2, 3, 64}, layout, round);
     }
     if (failures) return 1;
     std::puts("ok");
