@@ -12,6 +12,8 @@ namespace satori {
 namespace {
 
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
 
 constexpr int kThreads = 256;
 
@@ -176,10 +178,11 @@ __global__ __launch_bounds__(kThreads) void cache_append_kernel(CacheShape s, co
 //
 // F16 keys and values are exact in the matrix instructions; what they meet is not, so queries and probabilities go in as
 // two halves of 11 bits, x = hi + lo, both products summed in the same FP32 accumulator: 2^-22 of a value is lost. Their
-// scale is a power of two that puts the largest query lane of a pair (and a probability of one) at 2^14, far from
-// where halves lose bits. F32 caches use the FP32 matrix instructions.
+// scale is a power of two that puts the largest query lane of a pair at 2^14 and a probability of one between 2^6 and 2^14,
+// far from where halves lose bits. F32 caches use the FP32 matrix instructions.
 
 constexpr int kTile = 32;  // tokens that a wave attends at once
+constexpr float kSlack = 8.0f;
 constexpr float kLog2e = 1.44269504088896340736f;
 
 // Maximum and sum over the four lanes that hold one column (lane, lane ^ 16, lane ^ 32, lane ^ 48).
@@ -219,7 +222,7 @@ struct Math;
 
 template <int W>
 struct Math<_Float16, W> {
-    static constexpr float kTop = 14.0f;        // log2 of a probability of one, as the second product takes it
+    static constexpr float kTop = 6.0f;         // log2 of a probability of one, as the second product takes it
     static constexpr int kKeyParts = W / 32;    // fragments of a key tile's 16 rows, of a value tile's 16 lanes
     static constexpr int kValueParts = 1;
     typedef f16x8 Fragment;                     // 16 bytes: lanes 32 s + 8 g .. of a key, tokens 8 g .. of a value lane
@@ -263,9 +266,12 @@ struct Math<_Float16, W> {
     }
     static __device__ __forceinline__ void weights(const float (&p)[8], Weights& w) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            w.hi[i] = static_cast<_Float16>(p[i]);
-            w.lo[i] = static_cast<_Float16>(p[i] - static_cast<float>(w.hi[i]));
+        for (int i = 0; i < 8; i += 2) {  // in pairs, as the conversion takes them; the difference is one mixed multiply-add
+            const f16x2 hi = __builtin_convertvector((f32x2{p[i], p[i + 1]}), f16x2);
+            const f32x2 rest{__fmaf_rn(static_cast<float>(hi[0]), -1.0f, p[i]), __fmaf_rn(static_cast<float>(hi[1]), -1.0f, p[i + 1])};
+            const f16x2 lo = __builtin_convertvector(rest, f16x2);
+            w.hi[i] = hi[0], w.hi[i + 1] = hi[1];
+            w.lo[i] = lo[0], w.lo[i + 1] = lo[1];
         }
     }
     static __device__ __forceinline__ f32x4 weigh(Fragment v, const Weights& w, int, int term, f32x4 sum) {
@@ -330,7 +336,9 @@ struct Softmax {
         float top = fmaxf(fmaxf(fmaxf(score[0][0], score[0][1]), fmaxf(score[0][2], score[0][3])),
                           fmaxf(fmaxf(score[1][0], score[1][1]), fmaxf(score[1][2], score[1][3])));
         top = column_max(top) * factor;
-        if (__any(top > m)) {
+        // The maximum may fall behind by a factor of 2^kSlack before everything is scaled again (in the first tiles of random
+        // scores some pair of a wave has a new maximum almost every time).
+        if (__any(top > m + kSlack)) {
             const float now = fmaxf(m, top);
             const float shrink = __builtin_amdgcn_exp2f(m - (now == -INFINITY ? 0.0f : now));
             m = now;
@@ -667,6 +675,8 @@ struct Wide {
     static constexpr int kKeys = kTile * kKeyPieces, kValues = W * kValuePieces;  // pieces of a tile
     static constexpr int kPieces = kKeys + kValues;
     static constexpr int kPer = (kPieces * TG + kThreads - 1) / kThreads;         // pieces a thread moves per step
+    // Steps whose bytes are on their way while one is attended: two where the registers allow it.
+    static constexpr int kAhead = W * sizeof(T) <= 512 && W < 256 ? 2 : 1;
     // Whether all threads' i-th pieces belong to one tile, and to its keys or its values.
     static constexpr bool kEven = kKeys % kThreads == 0 && kValues % kThreads == 0;
     static constexpr size_t kBuffers = size_t(2) * TG * kPieces * 16;
@@ -694,13 +704,12 @@ __global__ __launch_bounds__(64 * PG * TG, 2) void cache_attention_wide_kernel(A
         const int tiles = (item.tokens + kTile - 1) / kTile, steps = (tiles + TG - 1) / TG;
         const int blocks = min(NB, (item.pairs - 16 * NB * pg + 15) / 16);  // of this wave; none or less: it only carries
 
-        u32x4 moved[S::kPer];
         int of_set[TG];  // the pages of the step that is fetched next, read a step before
         const auto look = [&](int step) {
 #pragma unroll
             for (int k = 0; k < TG; ++k) of_set[k] = pages.page(min(step * TG + k, tiles - 1) * kTile);
         };
-        const auto fetch = [&](int step) {
+        const auto fetch = [&](int step, u32x4 (&moved)[S::kPer]) {
 #pragma unroll
             for (int i = 0; i < S::kPer; ++i) {
                 const int n = thread + i * S::kThreads;
@@ -721,7 +730,7 @@ __global__ __launch_bounds__(64 * PG * TG, 2) void cache_attention_wide_kernel(A
                 moved[i] = *(const SATORI_GLOBAL u32x4*)(from);
             }
         };
-        const auto put = [&](int step) {
+        const auto put = [&](int step, const u32x4 (&moved)[S::kPer]) {
             u32x4* buffer = reinterpret_cast<u32x4*>(lds) + (step & 1) * TG * S::kPieces;
 #pragma unroll
             for (int i = 0; i < S::kPer; ++i) {
@@ -739,10 +748,15 @@ __global__ __launch_bounds__(64 * PG * TG, 2) void cache_attention_wide_kernel(A
             }
         };
 
+        u32x4 moved[S::kAhead][S::kPer];
         if (tiles > 0) {
             look(0);
-            fetch(0);
+            fetch(0, moved[0]);
             look(1);
+            if (S::kAhead > 1 && steps > 1) {
+                fetch(1, moved[S::kAhead - 1]);
+                look(2);
+            }
         }
         typename M::Query q[NB];
         Softmax<W> x[NB];
@@ -788,14 +802,14 @@ __global__ __launch_bounds__(64 * PG * TG, 2) void cache_attention_wide_kernel(A
         };
 
         if (tiles > 0) {
-            put(0);
+            put(0, moved[0]);
             settle(0);
         }
         __syncthreads();
-        for (int step = 0; step < steps; ++step) {
-            if (step + 1 < steps) {
-                fetch(step + 1);
-                look(step + 2);
+        const auto attend = [&](int step, u32x4 (&free)[S::kPer], const u32x4 (&next)[S::kPer]) {
+            if (step + S::kAhead < steps) {
+                fetch(step + S::kAhead, free);
+                look(step + S::kAhead + 1);
             }
             const int t = (step * TG + tg) * kTile;
             if (t < item.tokens && blocks > 0) {
@@ -852,10 +866,14 @@ __global__ __launch_bounds__(64 * PG * TG, 2) void cache_attention_wide_kernel(A
                     }
             }
             if (step + 1 < steps) {
-                put(step + 1);
+                put(step + 1, next);
                 settle(step + 1);
             }
             __syncthreads();
+        };
+        for (int step = 0; step < steps; step += S::kAhead) {
+            attend(step, moved[0], moved[S::kAhead - 1]);
+            if (S::kAhead > 1 && step + 1 < steps) attend(step + 1, moved[S::kAhead - 1], moved[0]);
         }
 
         // The sets joined by the first of each pair group, in order.
