@@ -409,6 +409,7 @@ struct AttentionArgs {
     CacheShape s;
     const int* image;
     PlanLayout at;
+    int wide, narrow, rows;  // of the plan; -1: as its header says when the launch runs (a captured one)
     int layer;
     const float* query;
     float* output;
@@ -417,19 +418,21 @@ struct AttentionArgs {
     bool quads;  // heads of a query start at multiples of 16 bytes and are whole 16-byte pieces
 };
 
-// What a lane knows of pair `p` of an item: its row and query head.
+// A (row, query head) pair of an item, by its number; those past the item's last are the first, and not `is`.
 struct Pair {
     PlanRow row;
     int head;
     bool is;
 };
 
+__device__ __forceinline__ int pair_place(const PlanItem& item, int p) { return item.pair + (p < item.pairs ? p : 0); }
+
 __device__ __forceinline__ Pair pair_of(const AttentionArgs& a, const PlanItem& item, int p) {
+    const int group = a.s.heads / a.s.kv_heads, of = pair_place(item, p);
     Pair r;
-    r.is = p < item.pairs;
-    const int group = a.s.heads / a.s.kv_heads, of = item.pair + (r.is ? p : 0);
     r.row = reinterpret_cast<const PlanRow*>(a.image + a.at.list_at)[item.rows + of / group];
     r.head = item.kv * group + of % group;
+    r.is = p < item.pairs;
     return r;
 }
 
@@ -443,7 +446,7 @@ __device__ __forceinline__ void give(const AttentionArgs& a, const PlanItem& ite
                                      float total) {
     if (p.row.slots > 1) {
         const int64_t index = static_cast<int64_t>(p.row.slot + item.slot) * a.s.heads + p.head;
-        *reinterpret_cast<f32x4*>(a.partials.values(W, index) + d) = o;
+        *(SATORI_GLOBAL f32x4*)(a.partials.values(W, index) + d) = o;
         return;
     }
     float* out = a.output + (static_cast<int64_t>(p.row.row) * a.s.heads + p.head) * a.s.head_dim + d;
@@ -455,8 +458,8 @@ template <int W>
 __device__ __forceinline__ void give_sums(const AttentionArgs& a, const PlanItem& item, const Pair& p, float m, float l) {
     if (p.row.slots <= 1) return;
     float* sums = a.partials.sums(W, static_cast<int64_t>(p.row.slot + item.slot) * a.s.heads + p.head);
-    sums[0] = m;
-    sums[1] = l;
+    store_f32(sums, m);
+    store_f32(sums + 1, l);
 }
 
 // Reads of what no kernel writes, at addresses that a wave has in common: through the scalar cache.
@@ -505,161 +508,17 @@ struct Pages {
     __device__ __forceinline__ const uint8_t* values(int page) const { return keys(page) + kv_heads * head_bytes; }
 };
 
-// Few pairs (16 * NB at most): each of four waves takes tiles of its own in turn, keys and values straight from the cache
-// into registers (nobody else in the workgroup wants them), and the waves' results are joined through LDS.
-constexpr int kNarrowWaves = 4;
+// A workgroup of four waves attends one item, in one of two ways.
+//
+// Few pairs (16 at most): each wave takes tiles of its own in turn, keys and values straight from the cache into registers
+// (nobody else in the workgroup wants them), and the waves' results are joined through LDS.
+//
+// Many pairs: each wave has 16 * kBlocks of them, and the tiles that all four want pass through LDS, in two buffers: while
+// one is attended, the bytes of the next two are on their way in registers. Rows of a tile are 16-byte pieces, put where the
+// 16 lanes that read a column of them reach different banks: piece p of row r lies at p ^ (r's bits that its place in a
+// 256-byte line leaves open).
+constexpr int kWaves = 4;
 
-template <typename T, int W, int NB>
-__global__ __launch_bounds__(kNarrowWaves * 64, W <= 128 ? 2 : 1) void cache_attention_narrow_kernel(AttentionArgs a) {
-    using M = Math<T, W>;
-    using Fragment = typename M::Fragment;
-    constexpr int kPart = W < 128 ? W : 128;  // lanes joined at once
-    constexpr int kKeyUnit = sizeof(T) == 2 ? 32 : 16;  // lanes a key fragment's step covers
-    constexpr int kGroupLanes = 16 / sizeof(T);         // elements of a fragment
-    __shared__ float joined[kNarrowWaves][16][kPart + 4];
-    __shared__ float stats[kNarrowWaves][16][2];
-    const int count = reinterpret_cast<const PlanHeader*>(a.image)->narrow;
-    const PlanItem* items = reinterpret_cast<const PlanItem*>(a.image + a.at.narrow_at);
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    for (int u = blockIdx.x; u < count; u += gridDim.x) {
-        const PlanItem item = scalar_load(items + u);
-        const int thread = unknown(threadIdx.x), lane = thread & 63, c = lane & 15, g = lane >> 4;
-        const int head_dim = unknown_scalar(a.s.head_dim);
-        const Pages pages(a, item, static_cast<int64_t>(a.s.page_tokens) * W * sizeof(T));
-        const int blocks = (item.pairs + 15) / 16;
-        Fragment k[2][M::kKeyParts], v[W / 16][M::kValueParts];
-        const auto load_keys = [&](int t) {
-            const T* p = reinterpret_cast<const T*>(pages.keys(pages.page(t))) + pages.within(t) * W + kGroupLanes * g;
-#pragma unroll
-            for (int h = 0; h < 2; ++h)
-#pragma unroll
-                for (int s = 0; s < M::kKeyParts; ++s)
-                    k[h][s] = *(const SATORI_GLOBAL Fragment*)(p + M::key_token(h, c) * W + kKeyUnit * s);
-        };
-        int t = wave * kTile;
-        if (t < item.tokens) load_keys(t);
-        typename M::Query q[NB];
-        Softmax<W> x[NB];
-        int limit[NB];
-#pragma unroll
-        for (int b = 0; b < NB; ++b) {
-            x[b].clear();
-            limit[b] = -1;
-            const Pair p = pair_of(a, item, 16 * b + c);
-            if (p.is) limit[b] = p.row.position - item.first;
-            M::load_query(q[b], query_of(a, p), p.is, head_dim, a.quads, a.scale, g);
-        }
-        for (; t < item.tokens; t += kNarrowWaves * kTile) {
-            const T* vp = reinterpret_cast<const T*>(pages.values(pages.page(t))) + pages.within(t);
-#pragma unroll
-            for (int d = 0; d < W / 16; ++d)
-#pragma unroll
-                for (int h = 0; h < M::kValueParts; ++h)
-                    v[d][h] = *(const SATORI_GLOBAL Fragment*)(vp + static_cast<int64_t>(16 * d + c) * pages.tokens +
-                                                               16 * h + kGroupLanes * g);
-            f32x4 score[NB][2];
-#pragma unroll
-            for (int b = 0; b < NB; ++b) score[b][0] = score[b][1] = f32x4{0, 0, 0, 0};
-#pragma unroll
-            for (int s = 0; s < M::kKeyParts; ++s)
-#pragma unroll
-                for (int term = 0; term < M::kTerms; ++term)
-#pragma unroll
-                    for (int h = 0; h < 2; ++h)
-#pragma unroll
-                        for (int b = 0; b < NB; ++b) score[b][h] = M::score(k[h][s], q[b], s, term, score[b][h]);
-            if (t + kNarrowWaves * kTile < item.tokens) load_keys(t + kNarrowWaves * kTile);
-            const int end = item.tokens - t;  // tokens of this tile that exist
-            const bool hides = item.first + t + kTile - 1 > item.limit;
-            if (end < kTile) {
-                // Values of tokens behind the end become zero (they are nobody's, and may hold anything).
-#pragma unroll
-                for (int i = 0; i < 8; ++i)
-                    if (M::token(g, i) >= end)
-#pragma unroll
-                        for (int d = 0; d < W / 16; ++d) v[d][i / kGroupLanes][i % kGroupLanes] = 0;
-            }
-            if (hides) {
-                bool finite = true;
-#pragma unroll
-                for (int d = 0; d < W / 16; ++d)
-#pragma unroll
-                    for (int h = 0; h < M::kValueParts; ++h) finite &= all_finite(v[d][h]);
-                if (!__all(finite))
-#pragma unroll
-                    for (int d = 0; d < W / 16; ++d)
-#pragma unroll
-                        for (int h = 0; h < M::kValueParts; ++h) {
-                            const Fragment spoiled = take_spoiled(v[d][h]);
-#pragma unroll
-                            for (int b = 0; b < NB; ++b) spoil<M>(spoiled, min(limit[b] - t + 1, end), h, g, x[b].o[d]);
-                        }
-            }
-#pragma unroll
-            for (int b = 0; b < NB; ++b) {
-                if (hides || end < kTile) hide<M>(score[b], min(limit[b] - t + 1, end), g);
-                float p[8];
-                x[b].take(score[b], q[b].factor, M::kTop, p);
-                typename M::Weights w;
-                M::weights(p, w);
-#pragma unroll
-                for (int h = 0; h < M::kValueParts; ++h)
-#pragma unroll
-                    for (int term = 0; term < M::kTerms; ++term)
-#pragma unroll
-                        for (int d = 0; d < W / 16; ++d) x[b].o[d] = M::weigh(v[d][h], w, h, term, x[b].o[d]);
-            }
-        }
-
-        // The waves' results joined, 16 pairs and up to 128 lanes at a time.
-        __syncthreads();
-#pragma unroll
-        for (int b = 0; b < NB; ++b) {
-            if (b >= blocks) continue;
-            const float sum = column_sum(x[b].l);
-            if (g == 0) {
-                stats[wave][c][0] = x[b].m;
-                stats[wave][c][1] = sum;
-            }
-#pragma unroll
-            for (int part = 0; part < (W + kPart - 1) / kPart; ++part) {
-#pragma unroll
-                for (int d = 0; d < kPart / 16; ++d) {
-                    const int of = part * (kPart / 16) + d;
-                    if (of < W / 16) *reinterpret_cast<f32x4*>(&joined[wave][c][16 * d + 4 * g]) = x[b].o[of < W / 16 ? of : 0];
-                }
-                __syncthreads();
-                const int pair = threadIdx.x >> 4;  // 16 threads a pair, four lanes each and turn
-                const Pair p = pair_of(a, item, 16 * b + pair);
-                if (p.is) {
-                    float top = -INFINITY, total = 0, weight[kNarrowWaves];
-#pragma unroll
-                    for (int w = 0; w < kNarrowWaves; ++w) top = fmaxf(top, stats[w][pair][0]);
-#pragma unroll
-                    for (int w = 0; w < kNarrowWaves; ++w) {
-                        weight[w] = __builtin_amdgcn_exp2f(stats[w][pair][0] - (top == -INFINITY ? 0.0f : top));
-                        total += weight[w] * stats[w][pair][1];
-                    }
-                    const int left = W - part * kPart < kPart ? W - part * kPart : kPart;
-                    for (int d = 4 * (threadIdx.x & 15); d < left; d += 64) {
-                        f32x4 o{0, 0, 0, 0};
-#pragma unroll
-                        for (int w = 0; w < kNarrowWaves; ++w)
-                            o = o + *reinterpret_cast<const f32x4*>(&joined[w][pair][d]) * weight[w];
-                        give<W>(a, item, p, part * kPart + d, o, total);
-                    }
-                    if (part == 0 && (threadIdx.x & 15) == 0) give_sums<W>(a, item, p, top, total);
-                }
-                __syncthreads();
-            }
-        }
-    }
-}
-
-// Many pairs: PG groups of 16 * NB pairs, one per wave, share the tiles, which pass through LDS (two buffers: while one is
-// attended, the next steps' bytes are on their way in registers); TG such sets of waves take tiles in turn and are joined
-// at the end. Rows of a tile are 16-byte pieces, put where the 16 lanes that read a column of them reach different banks:
-// piece p of row r lies at p ^ (r's bits that its place in a 256-byte line leaves open).
 template <int PIECES>
 __device__ __forceinline__ int piece_at(int row, int piece) {
     constexpr int kWhole = (PIECES & -PIECES) < 16 ? (PIECES & -PIECES) : 16;  // pieces that an XOR may permute
@@ -667,345 +526,440 @@ __device__ __forceinline__ int piece_at(int row, int piece) {
     return row * PIECES + (piece ^ ((row >> kShift) & (kWhole - 1)));
 }
 
-template <typename T, int W, int NB, int PG, int TG>
-struct Wide {
-    static constexpr int kThreads = 64 * PG * TG;
-    static constexpr int kPairs = 16 * NB * PG;
+template <typename T, int W>
+struct Shape {
+    // Blocks of 16 pairs of a wave, as its registers allow: with two waves a SIMD up to 128 lanes, with one past them.
+    static constexpr int kBlocks = (sizeof(T) == 2 && W <= 192) || W <= 64 ? 2 : 1;
+    static constexpr int kWavesPerSimd = W <= 128 ? 2 : 1;
+    static constexpr int kPairs = 16 * kBlocks * kWaves;
     static constexpr int kKeyPieces = W * sizeof(T) / 16, kValuePieces = kTile * sizeof(T) / 16;
     static constexpr int kKeys = kTile * kKeyPieces, kValues = W * kValuePieces;  // pieces of a tile
     static constexpr int kPieces = kKeys + kValues;
-    static constexpr int kPer = (kPieces * TG + kThreads - 1) / kThreads;         // pieces a thread moves per step
-    // Steps whose bytes are on their way while one is attended: two where the registers allow it.
-    static constexpr int kAhead = W * sizeof(T) <= 512 && W < 256 ? 2 : 1;
-    // Whether all threads' i-th pieces belong to one tile, and to its keys or its values.
+    static constexpr int kPer = (kPieces + kThreads - 1) / kThreads;             // pieces a thread moves
+    // Whether all threads' i-th pieces belong to the keys, or all to the values.
     static constexpr bool kEven = kKeys % kThreads == 0 && kValues % kThreads == 0;
-    static constexpr size_t kBuffers = size_t(2) * TG * kPieces * 16;
-    static constexpr size_t kJoin = size_t(TG - 1) * PG * NB * 16 * (W + 4 + 2) * sizeof(float);
-    static constexpr size_t kTiles = kBuffers > kJoin ? kBuffers : kJoin;
-    static constexpr size_t kLds = kTiles + size_t(2) * TG * W * sizeof(uint32_t);
+    static constexpr int kPart = W < 128 ? W : 128;                              // lanes of narrow results joined at once
+    static constexpr int kTiles = 2 * kPieces * 16, kJoin = kWaves * 16 * (kPart + 4 + 2) * 4;
+    // LDS: tiles or results, the pairs' rows, and a bit per token of every value lane (two buffers).
+    static constexpr int kRowsAt = kTiles > kJoin ? kTiles : kJoin, kSpoiledAt = kRowsAt + kPairs * 16;
+    static constexpr int kLds = kSpoiledAt + 2 * W * 4;
 };
 
-template <typename T, int W, int NB, int PG, int TG>
-__global__ __launch_bounds__(64 * PG * TG, 2) void cache_attention_wide_kernel(AttentionArgs a) {
+template <typename T, int W>
+__device__ __forceinline__ void attend_few(const AttentionArgs& a, const PlanItem& item, uint8_t* lds, int wave) {
     using M = Math<T, W>;
-    using S = Wide<T, W, NB, PG, TG>;
+    using S = Shape<T, W>;
     using Fragment = typename M::Fragment;
-    extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
-    const int count = reinterpret_cast<const PlanHeader*>(a.image)->wide;
-    const PlanItem* items = reinterpret_cast<const PlanItem*>(a.image + a.at.wide_at);
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int pg = wave / TG, tg = wave % TG;
-    uint32_t* spoiled = reinterpret_cast<uint32_t*>(lds + S::kTiles);  // [2][TG][W]
-    for (int u = blockIdx.x; u < count; u += gridDim.x) {
-        const PlanItem item = scalar_load(items + u);
-        const int thread = unknown(threadIdx.x), lane = thread & 63, c = lane & 15, g = lane >> 4;
-        const int head_dim = unknown_scalar(a.s.head_dim);
-        const Pages pages(a, item, static_cast<int64_t>(a.s.page_tokens) * W * sizeof(T));
-        const int tiles = (item.tokens + kTile - 1) / kTile, steps = (tiles + TG - 1) / TG;
-        const int blocks = min(NB, (item.pairs - 16 * NB * pg + 15) / 16);  // of this wave; none or less: it only carries
-
-        int of_set[TG];  // the pages of the step that is fetched next, read a step before
-        const auto look = [&](int step) {
+    constexpr int kPart = S::kPart;
+    constexpr int kKeyUnit = sizeof(T) == 2 ? 32 : 16;  // lanes a key fragment's step covers
+    constexpr int kGroupLanes = 16 / sizeof(T);         // elements of a fragment
+    const int thread = unknown(threadIdx.x), lane = thread & 63, c = lane & 15, g = lane >> 4;
+    const int head_dim = unknown_scalar(a.s.head_dim);
+    const Pages pages(a, item, static_cast<int64_t>(a.s.page_tokens) * W * sizeof(T));
+    Fragment k[2][M::kKeyParts], v[W / 16][M::kValueParts];
+    const auto load_keys = [&](int page, int t) {
+        const T* p = reinterpret_cast<const T*>(pages.keys(page)) + pages.within(t) * W + kGroupLanes * g;
 #pragma unroll
-            for (int k = 0; k < TG; ++k) of_set[k] = pages.page(min(step * TG + k, tiles - 1) * kTile);
-        };
-        const auto fetch = [&](int step, u32x4 (&moved)[S::kPer]) {
+        for (int h = 0; h < 2; ++h)
 #pragma unroll
-            for (int i = 0; i < S::kPer; ++i) {
-                const int n = thread + i * S::kThreads;
-                const int set = S::kEven ? i * S::kThreads / S::kPieces : n / S::kPieces;
-                const int piece = S::kEven ? thread + i * S::kThreads % S::kPieces : n % S::kPieces;
-                const int tile = step * TG + set;
-                if ((S::kPieces * TG % S::kThreads != 0 && n >= S::kPieces * TG) || tile >= tiles) continue;
-                int page = of_set[0];
+            for (int s = 0; s < M::kKeyParts; ++s)
+                k[h][s] = *(const SATORI_GLOBAL Fragment*)(p + M::key_token(h, c) * W + kKeyUnit * s);
+    };
+    const auto load_values = [&](int page, int t) {
+        const T* p = reinterpret_cast<const T*>(pages.values(page)) + pages.within(t) + c * pages.tokens + kGroupLanes * g;
 #pragma unroll
-                for (int k = 1; k < TG; ++k) page = set == k ? of_set[k] : page;
-                const uint8_t* from;
-                if (S::kEven ? i * S::kThreads % S::kPieces < S::kKeys : piece < S::kKeys) {
-                    from = pages.keys(page) + pages.within(tile * kTile) * (W * static_cast<int>(sizeof(T))) + piece * 16;
-                } else {
-                    const int row = (piece - S::kKeys) / S::kValuePieces, of = (piece - S::kKeys) % S::kValuePieces;
-                    from = pages.values(page) + (row * pages.tokens + pages.within(tile * kTile)) * static_cast<int>(sizeof(T)) + of * 16;
-                }
-                moved[i] = *(const SATORI_GLOBAL u32x4*)(from);
-            }
-        };
-        const auto put = [&](int step, const u32x4 (&moved)[S::kPer]) {
-            u32x4* buffer = reinterpret_cast<u32x4*>(lds) + (step & 1) * TG * S::kPieces;
+        for (int d = 0; d < W / 16; ++d)
 #pragma unroll
-            for (int i = 0; i < S::kPer; ++i) {
-                const int n = thread + i * S::kThreads;
-                const int set = S::kEven ? i * S::kThreads / S::kPieces : n / S::kPieces;
-                const int piece = S::kEven ? thread + i * S::kThreads % S::kPieces : n % S::kPieces;
-                if (S::kPieces * TG % S::kThreads != 0 && n >= S::kPieces * TG) continue;
-                if (S::kEven ? i * S::kThreads % S::kPieces < S::kKeys : piece < S::kKeys) {
-                    const int row = M::key_row(piece / S::kKeyPieces);
-                    buffer[set * S::kPieces + piece_at<S::kKeyPieces>(row, piece % S::kKeyPieces)] = moved[i];
-                } else {
-                    const int row = (piece - S::kKeys) / S::kValuePieces, of = (piece - S::kKeys) % S::kValuePieces;
-                    buffer[set * S::kPieces + S::kKeys + piece_at<S::kValuePieces>(row, of)] = moved[i];
-                }
-            }
-        };
-
-        u32x4 moved[S::kAhead][S::kPer];
-        if (tiles > 0) {
-            look(0);
-            fetch(0, moved[0]);
-            look(1);
-            if (S::kAhead > 1 && steps > 1) {
-                fetch(1, moved[S::kAhead - 1]);
-                look(2);
-            }
+            for (int h = 0; h < M::kValueParts; ++h)
+                v[d][h] = *(const SATORI_GLOBAL Fragment*)(p + 16 * d * pages.tokens + 16 * h);
+    };
+    int t = wave * kTile, page = 0;
+    if (t < item.tokens) {
+        page = pages.page(t);
+        load_keys(page, t);
+        load_values(page, t);
+        if (t + kWaves * kTile < item.tokens) page = pages.page(t + kWaves * kTile);
+    }
+    const Pair pair = pair_of(a, item, c);
+    PlanRow* row_of = reinterpret_cast<PlanRow*>(lds + S::kRowsAt);
+    if (thread < 16) row_of[thread] = pair.row;
+    typename M::Query q;
+    M::load_query(q, query_of(a, pair), pair.is, head_dim, a.quads, a.scale, g);
+    const int limit = pair.is ? pair.row.position - item.first : -1;
+    Softmax<W> x;
+    x.clear();
+    while (t < item.tokens) {
+        f32x4 score[2] = {f32x4{0, 0, 0, 0}, f32x4{0, 0, 0, 0}};
+#pragma unroll
+        for (int s = 0; s < M::kKeyParts; ++s)
+#pragma unroll
+            for (int term = 0; term < M::kTerms; ++term)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) score[h] = M::score(k[h][s], q, s, term, score[h]);
+        const int next = t + kWaves * kTile;
+        if (next < item.tokens) load_keys(page, next);
+        const int end = item.tokens - t;  // tokens of this tile that exist
+        const bool hides = item.first + t + kTile - 1 > item.limit;
+        if (end < kTile) {
+            // Values of tokens behind the end become zero (they are nobody's, and may hold anything).
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (M::token(g, i) >= end)
+#pragma unroll
+                    for (int d = 0; d < W / 16; ++d) v[d][i / kGroupLanes][i % kGroupLanes] = 0;
         }
-        typename M::Query q[NB];
-        Softmax<W> x[NB];
-        int limit[NB];
+        const int seen = min(limit - t + 1, end);
+        if (hides) {
+            bool finite = true;
 #pragma unroll
-        for (int b = 0; b < NB; ++b) {
-            x[b].clear();
-            limit[b] = -1;
-            const Pair p = pair_of(a, item, 16 * (NB * pg + b) + c);
-            if (p.is) limit[b] = p.row.position - item.first;
-            M::load_query(q[b], query_of(a, p), p.is, head_dim, a.quads, a.scale, g);
-        }
-        // Tiles that some pair does not see whole, once they are in LDS: values of tokens behind the item's end become zero
-        // (they are nobody's, and may hold anything), and so do values that are not finite, whose places are kept as a bit
-        // per token of every lane: 0 * infinity would spoil the sums of pairs that must not see them.
-        const auto partial = [&](int tile) {
-            return tile < tiles && (item.first + tile * kTile + kTile - 1 > item.limit || tile * kTile + kTile > item.tokens);
-        };
-        const auto settle = [&](int step) {
-            if (!partial(min(step * TG + TG, tiles) - 1)) return;  // (the later a tile, the more it hides)
-            __syncthreads();
-            constexpr int kOf = 16 / sizeof(T);
-#pragma unroll 1
-            for (int n = thread; n < TG * W; n += S::kThreads) {
-                const int set = n / W, row = n % W, tile = step * TG + set, left = item.tokens - tile * kTile;
-                if (!partial(tile)) continue;
-                Fragment* values = reinterpret_cast<Fragment*>(lds) + ((step & 1) * TG + set) * S::kPieces + S::kKeys;
-                uint32_t where = 0;
-#pragma unroll 1
-                for (int piece = 0; piece < S::kValuePieces; ++piece) {
-                    Fragment v = values[piece_at<S::kValuePieces>(row, piece)];
+            for (int d = 0; d < W / 16; ++d)
 #pragma unroll
-                    for (int j = 0; j < kOf; ++j) {
-                        const int token = piece * kOf + j;
-                        const bool fine = __builtin_isfinite(static_cast<float>(v[j]));
-                        if (!fine && token < left) where |= 1u << token;
-                        v[j] = fine && token < left ? v[j] : 0;
+                for (int h = 0; h < M::kValueParts; ++h) finite &= all_finite(v[d][h]);
+            if (!__all(finite))
+#pragma unroll
+                for (int d = 0; d < W / 16; ++d)
+#pragma unroll
+                    for (int h = 0; h < M::kValueParts; ++h) {
+                        const Fragment spoiled = take_spoiled(v[d][h]);
+                        spoil<M>(spoiled, seen, h, g, x.o[d]);
                     }
-                    values[piece_at<S::kValuePieces>(row, piece)] = v;
-                }
-                spoiled[((step & 1) * TG + set) * W + row] = where;
-            }
-        };
+        }
+        if (hides || end < kTile) hide<M>(score, seen, g);
+        float p[8];
+        x.take(score, q.factor, M::kTop, p);
+        typename M::Weights w;
+        M::weights(p, w);
+#pragma unroll
+        for (int h = 0; h < M::kValueParts; ++h)
+#pragma unroll
+            for (int term = 0; term < M::kTerms; ++term)
+#pragma unroll
+                for (int d = 0; d < W / 16; ++d) x.o[d] = M::weigh(v[d][h], w, h, term, x.o[d]);
+        if (next < item.tokens) {
+            load_values(page, next);
+            if (next + kWaves * kTile < item.tokens) page = pages.page(next + kWaves * kTile);
+        }
+        t = next;
+    }
 
-        if (tiles > 0) {
-            put(0, moved[0]);
-            settle(0);
+    // The waves' results joined, up to 128 lanes at a time: [wave][pair][kPart + 4], then (maximum, sum) of each.
+    float* joined = reinterpret_cast<float*>(lds);
+    float* stats = joined + kWaves * 16 * (kPart + 4);
+    const float sum = column_sum(x.l);
+    if (g == 0) {
+        stats[(wave * 16 + c) * 2] = x.m;
+        stats[(wave * 16 + c) * 2 + 1] = sum;
+    }
+    const int mine = thread >> 4;  // 16 threads a pair, four lanes each and turn
+#pragma unroll
+    for (int part = 0; part < (W + kPart - 1) / kPart; ++part) {
+        if (part > 0) __syncthreads();
+#pragma unroll
+        for (int d = 0; d < kPart / 16; ++d) {
+            const int of = part * (kPart / 16) + d;
+            if (of < W / 16) *reinterpret_cast<f32x4*>(joined + (wave * 16 + c) * (kPart + 4) + 16 * d + 4 * g) = x.o[of < W / 16 ? of : 0];
         }
         __syncthreads();
-        const auto attend = [&](int step, u32x4 (&free)[S::kPer], const u32x4 (&next)[S::kPer]) {
-            if (step + S::kAhead < steps) {
-                fetch(step + S::kAhead, free);
-                look(step + S::kAhead + 1);
+        if (mine >= item.pairs) continue;
+        const int group = a.s.heads / a.s.kv_heads;
+        const Pair to{row_of[mine], item.kv * group + (item.pair + mine) % group, true};
+        float top = -INFINITY, total = 0, weight[kWaves];
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) top = fmaxf(top, stats[(w * 16 + mine) * 2]);
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) {
+            weight[w] = __builtin_amdgcn_exp2f(stats[(w * 16 + mine) * 2] - (top == -INFINITY ? 0.0f : top));
+            total += weight[w] * stats[(w * 16 + mine) * 2 + 1];
+        }
+        const int left = W - part * kPart < kPart ? W - part * kPart : kPart;
+        for (int d = 4 * (thread & 15); d < left; d += 64) {
+            f32x4 o{0, 0, 0, 0};
+#pragma unroll
+            for (int w = 0; w < kWaves; ++w)
+                o = o + *reinterpret_cast<const f32x4*>(joined + (w * 16 + mine) * (kPart + 4) + d) * weight[w];
+            give<W>(a, item, to, part * kPart + d, o, total);
+        }
+        if (part == 0 && (thread & 15) == 0) give_sums<W>(a, item, to, top, total);
+    }
+}
+
+template <typename T, int W>
+__device__ __forceinline__ void attend_many(const AttentionArgs& a, const PlanItem& item, uint8_t* lds, int wave) {
+    using M = Math<T, W>;
+    using S = Shape<T, W>;
+    using Fragment = typename M::Fragment;
+    constexpr int NB = S::kBlocks;
+    const int thread = unknown(threadIdx.x), lane = thread & 63, c = lane & 15, g = lane >> 4;
+    const int head_dim = unknown_scalar(a.s.head_dim);
+    const Pages pages(a, item, static_cast<int64_t>(a.s.page_tokens) * W * sizeof(T));
+    const int tiles = (item.tokens + kTile - 1) / kTile;
+    const bool idle = 16 * NB * wave >= item.pairs;  // a wave without pairs only carries
+    uint32_t* spoiled = reinterpret_cast<uint32_t*>(lds + S::kSpoiledAt);  // [2][W]
+
+    const auto fetch = [&](int page, int tile, u32x4 (&moved)[S::kPer]) {
+        const int within = pages.within(tile * kTile);
+#pragma unroll
+        for (int i = 0; i < S::kPer; ++i) {
+            const int piece = thread + i * kThreads;
+            if (S::kPieces % kThreads != 0 && piece >= S::kPieces) continue;
+            const uint8_t* from;
+            if (S::kEven ? i * kThreads < S::kKeys : piece < S::kKeys) {
+                from = pages.keys(page) + within * (W * static_cast<int>(sizeof(T))) + piece * 16;
+            } else {
+                const int row = (piece - S::kKeys) / S::kValuePieces, of = (piece - S::kKeys) % S::kValuePieces;
+                from = pages.values(page) + (row * pages.tokens + within) * static_cast<int>(sizeof(T)) + of * 16;
             }
-            const int t = (step * TG + tg) * kTile;
-            if (t < item.tokens && blocks > 0) {
-                const Fragment* keys = reinterpret_cast<const Fragment*>(lds) + ((step & 1) * TG + tg) * S::kPieces;
-                const Fragment* values = keys + S::kKeys;
-                f32x4 score[NB][2];
+            moved[i] = *(const SATORI_GLOBAL u32x4*)(from);
+        }
+    };
+    const auto put = [&](int tile, const u32x4 (&moved)[S::kPer]) {
+        u32x4* buffer = reinterpret_cast<u32x4*>(lds) + (tile & 1) * S::kPieces;
 #pragma unroll
-                for (int b = 0; b < NB; ++b) score[b][0] = score[b][1] = f32x4{0, 0, 0, 0};
+        for (int i = 0; i < S::kPer; ++i) {
+            const int piece = thread + i * kThreads;
+            if (S::kPieces % kThreads != 0 && piece >= S::kPieces) continue;
+            if (S::kEven ? i * kThreads < S::kKeys : piece < S::kKeys) {
+                buffer[piece_at<S::kKeyPieces>(M::key_row(piece / S::kKeyPieces), piece % S::kKeyPieces)] = moved[i];
+            } else {
+                const int row = (piece - S::kKeys) / S::kValuePieces, of = (piece - S::kKeys) % S::kValuePieces;
+                buffer[S::kKeys + piece_at<S::kValuePieces>(row, of)] = moved[i];
+            }
+        }
+    };
+    // A tile that some pair does not see whole, once it is in LDS: values of tokens behind the item's end become zero (they
+    // are nobody's, and may hold anything), and so do values that are not finite, whose places are kept as a bit per token
+    // of every lane.
+    const auto settle = [&](int tile) {
+        const int left = item.tokens - tile * kTile;
+        if (item.first + tile * kTile + kTile - 1 <= item.limit && left >= kTile) return;
+        __syncthreads();
+        constexpr int kOf = 16 / sizeof(T);
+        Fragment* values = reinterpret_cast<Fragment*>(lds) + (tile & 1) * S::kPieces + S::kKeys;
+#pragma unroll 1
+        for (int row = thread; row < W; row += kThreads) {
+            uint32_t where = 0;
+#pragma unroll 1
+            for (int piece = 0; piece < S::kValuePieces; ++piece) {
+                Fragment v = values[piece_at<S::kValuePieces>(row, piece)];
 #pragma unroll
-                for (int s = 0; s < M::kKeyParts; ++s) {
-                    Fragment k[2];
+                for (int j = 0; j < kOf; ++j) {
+                    const int token = piece * kOf + j;
+                    const bool fine = __builtin_isfinite(static_cast<float>(v[j]));
+                    if (!fine && token < left) where |= 1u << token;
+                    v[j] = fine && token < left ? v[j] : 0;
+                }
+                values[piece_at<S::kValuePieces>(row, piece)] = v;
+            }
+            spoiled[(tile & 1) * W + row] = where;
+        }
+    };
+
+    u32x4 moved[2][S::kPer];
+    int page = 0;  // of the tile that is fetched next, read a tile before
+    const auto page_of = [&](int tile) { return pages.page(min(tile, tiles - 1) * kTile); };
+    if (tiles > 0) {
+        fetch(page_of(0), 0, moved[0]);
+        page = page_of(1);
+        if (tiles > 1) fetch(page, 1, moved[1]);
+        page = page_of(2);
+    }
+    typename M::Query q[NB];
+    Softmax<W> x[NB];
+    int limit[NB];
+    PlanRow* row_of = reinterpret_cast<PlanRow*>(lds + S::kRowsAt) + 16 * NB * wave;  // this wave's
 #pragma unroll
-                    for (int h = 0; h < 2; ++h) k[h] = keys[piece_at<S::kKeyPieces>(16 * h + c, 4 * s + g)];
+    for (int b = 0; b < NB; ++b) {
+        x[b].clear();
+        const Pair p = pair_of(a, item, 16 * (NB * wave + b) + c);
+        limit[b] = p.is ? p.row.position - item.first : -1;
+        if (g == 0) row_of[16 * b + c] = p.row;
+        M::load_query(q[b], query_of(a, p), p.is, head_dim, a.quads, a.scale, g);
+    }
+    if (tiles > 0) {
+        put(0, moved[0]);
+        settle(0);
+    }
+    __syncthreads();
+    const auto attend = [&](int tile, u32x4 (&free)[S::kPer], const u32x4 (&next)[S::kPer]) {
+        if (tile + 2 < tiles) {
+            fetch(page, tile + 2, free);
+            page = page_of(tile + 3);
+        }
+        if (!idle) {
+            const int t = tile * kTile;
+            const Fragment* keys = reinterpret_cast<const Fragment*>(lds) + (tile & 1) * S::kPieces;
+            const Fragment* values = keys + S::kKeys;
+            f32x4 score[NB][2];
+#pragma unroll
+            for (int b = 0; b < NB; ++b) score[b][0] = score[b][1] = f32x4{0, 0, 0, 0};
+#pragma unroll
+            for (int s = 0; s < M::kKeyParts; ++s) {
+                Fragment k[2];
+#pragma unroll
+                for (int h = 0; h < 2; ++h) k[h] = keys[piece_at<S::kKeyPieces>(16 * h + c, 4 * s + g)];
+#pragma unroll
+                for (int term = 0; term < M::kTerms; ++term)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h)
+#pragma unroll
+                        for (int b = 0; b < NB; ++b) score[b][h] = M::score(k[h], q[b], s, term, score[b][h]);
+            }
+            __builtin_amdgcn_sched_barrier(0);  // (the scheduler would hold both products' fragments at once, and spill)
+            const int end = item.tokens - t;
+            const bool hides = item.first + t + kTile - 1 > item.limit;
+            typename M::Weights w[NB];
+#pragma unroll
+            for (int b = 0; b < NB; ++b) {
+                const int seen = min(limit[b] - t + 1, end);
+                if (hides || end < kTile) hide<M>(score[b], seen, g);
+                float p[8];
+                x[b].take(score[b], q[b].factor, M::kTop, p);
+                M::weights(p, w[b]);
+                if (hides) {
+                    const uint32_t sees = seen <= 0 ? 0u : ~0u >> (kTile - min(seen, kTile));
+                    const u32x4* bits = reinterpret_cast<const u32x4*>(spoiled + (tile & 1) * W);
+#pragma unroll
+                    for (int d = 0; d < W / 16; ++d) {
+                        const u32x4 where = bits[4 * d + g];
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) x[b].o[d][j] = where[j] & sees ? NAN : x[b].o[d][j];
+                    }
+                }
+            }
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int h = 0; h < M::kValueParts; ++h)
+#pragma unroll
+                for (int d = 0; d < W / 16; ++d) {
+                    const Fragment v = values[piece_at<S::kValuePieces>(16 * d + c, 4 * h + g)];
 #pragma unroll
                     for (int term = 0; term < M::kTerms; ++term)
 #pragma unroll
-                        for (int h = 0; h < 2; ++h)
-#pragma unroll
-                            for (int b = 0; b < NB; ++b) score[b][h] = M::score(k[h], q[b], s, term, score[b][h]);
+                        for (int b = 0; b < NB; ++b) x[b].o[d] = M::weigh(v, w[b], h, term, x[b].o[d]);
                 }
-                __builtin_amdgcn_sched_barrier(0);  // (the scheduler would hold both products' fragments at once, and spill)
-                const int end = item.tokens - t;
-                const bool hides = item.first + t + kTile - 1 > item.limit;
-                const auto value = [&](int d, int h) { return values[piece_at<S::kValuePieces>(16 * d + c, 4 * h + g)]; };
-                typename M::Weights w[NB];
-#pragma unroll
-                for (int b = 0; b < NB; ++b) {
-                    if (hides || end < kTile) hide<M>(score[b], min(limit[b] - t + 1, end), g);
-                    float p[8];
-                    x[b].take(score[b], q[b].factor, M::kTop, p);
-                    M::weights(p, w[b]);
-                    if (hides) {
-                        const int seen = min(limit[b] - t + 1, kTile);
-                        const uint32_t sees = seen <= 0 ? 0u : ~0u >> (kTile - seen);
-                        const u32x4* bits = reinterpret_cast<const u32x4*>(spoiled + ((step & 1) * TG + tg) * W);
-#pragma unroll
-                        for (int d = 0; d < W / 16; ++d) {
-                            const u32x4 where = bits[4 * d + g];
-#pragma unroll
-                            for (int j = 0; j < 4; ++j) x[b].o[d][j] = where[j] & sees ? NAN : x[b].o[d][j];
-                        }
-                    }
-                }
-                __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-                for (int h = 0; h < M::kValueParts; ++h)
-#pragma unroll
-                    for (int d = 0; d < W / 16; ++d) {
-                        const Fragment v = value(d, h);
-#pragma unroll
-                        for (int term = 0; term < M::kTerms; ++term)
-#pragma unroll
-                            for (int b = 0; b < NB; ++b) x[b].o[d] = M::weigh(v, w[b], h, term, x[b].o[d]);
-                    }
-            }
-            if (step + 1 < steps) {
-                put(step + 1, next);
-                settle(step + 1);
-            }
-            __syncthreads();
-        };
-        for (int step = 0; step < steps; step += S::kAhead) {
-            attend(step, moved[0], moved[S::kAhead - 1]);
-            if (S::kAhead > 1 && step + 1 < steps) attend(step + 1, moved[S::kAhead - 1], moved[0]);
         }
+        if (tile + 1 < tiles) {
+            put(tile + 1, next);
+            settle(tile + 1);
+        }
+        __syncthreads();
+    };
+    for (int tile = 0; tile < tiles; tile += 2) {
+        attend(tile, moved[0], moved[1]);
+        if (tile + 1 < tiles) attend(tile + 1, moved[1], moved[0]);
+    }
 
-        // The sets joined by the first of each pair group, in order.
-        constexpr int kRow = W + 4 + 2;
-        float* joined = reinterpret_cast<float*>(lds);
+    if (idle) return;
+    const int group = a.s.heads / a.s.kv_heads;
 #pragma unroll
-        for (int b = 0; b < NB; ++b) x[b].l = column_sum(x[b].l);
-        if (TG > 1) {
-            if (tg > 0 && blocks > 0) {
+    for (int b = 0; b < NB; ++b) {
+        const float total = column_sum(x[b].l);
+        const int p = 16 * (NB * wave + b) + c;
+        if (p >= item.pairs) continue;
+        const Pair to{row_of[16 * b + c], item.kv * group + (item.pair + p) % group, true};
 #pragma unroll
-                for (int b = 0; b < NB; ++b) {
-                    float* to = joined + (((tg - 1) * PG + pg) * NB * 16 + 16 * b + c) * kRow;
-#pragma unroll
-                    for (int d = 0; d < W / 16; ++d)
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) to[16 * d + 4 * g + j] = x[b].o[d][j];
-                    if (g == 0) {
-                        to[W] = x[b].m;
-                        to[W + 1] = x[b].l;
-                    }
-                }
-            }
-            __syncthreads();
-        }
-        if (tg == 0 && blocks > 0) {
-#pragma unroll
-            for (int b = 0; b < NB; ++b) {
-                if (b >= blocks) continue;
-                float top = x[b].m;
-#pragma unroll
-                for (int k = 1; k < TG; ++k) top = fmaxf(top, joined[(((k - 1) * PG + pg) * NB * 16 + 16 * b + c) * kRow + W]);
-                const float from = top == -INFINITY ? 0.0f : top;
-                const float own = __builtin_amdgcn_exp2f(x[b].m - from);
-                float total = own * x[b].l;
-#pragma unroll
-                for (int d = 0; d < W / 16; ++d) x[b].o[d] = x[b].o[d] * own;
-#pragma unroll
-                for (int k = 1; k < TG; ++k) {
-                    const float* of = joined + (((k - 1) * PG + pg) * NB * 16 + 16 * b + c) * kRow;
-                    const float weight = __builtin_amdgcn_exp2f(of[W] - from);
-                    total += weight * of[W + 1];
-#pragma unroll
-                    for (int d = 0; d < W / 16; ++d)
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) x[b].o[d][j] += weight * of[16 * d + 4 * g + j];
-                }
-                const Pair p = pair_of(a, item, 16 * (NB * pg + b) + c);
-                if (p.is) {
-#pragma unroll
-                    for (int d = 0; d < W / 16; ++d) give<W>(a, item, p, 16 * d + 4 * g, x[b].o[d], total);
-                    if (g == 0) give_sums<W>(a, item, p, top, total);
-                }
-            }
-        }
-        __syncthreads();  // the next item's tiles go where the sets' results are
+        for (int d = 0; d < W / 16; ++d) give<W>(a, item, to, 16 * d + 4 * g, x[b].o[d], total);
+        if (g == 0) give_sums<W>(a, item, to, x[b].m, total);
     }
 }
 
-// The partial results of one (row, head), joined by a wave with weights 2^(m_i - m): lanes first take a part each for the
-// maximum and the sum, then four lanes of the head each, several parts at once.
+// Items of many pairs first, which take longest (one a CU, bound by arithmetic); those of few, bound by memory, run beside
+// them. Workgroup u is u % 8 of its eight, which keeps items that read the same tokens on one XCD.
+template <typename T, int W>
+__global__ __launch_bounds__(kThreads, (Shape<T, W>::kWavesPerSimd)) void cache_attention_kernel(AttentionArgs a) {
+    extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
+    const PlanHeader* h = reinterpret_cast<const PlanHeader*>(a.image);
+    const int wide = a.wide >= 0 ? a.wide : scalar_load(&h->wide), narrow = a.narrow >= 0 ? a.narrow : scalar_load(&h->narrow);
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    for (int u = blockIdx.x; u < wide + narrow; u += gridDim.x) {
+        const bool many = u < wide;
+        const int at = many ? a.at.wide_at : a.at.narrow_at;
+        const PlanItem item = scalar_load(reinterpret_cast<const PlanItem*>(a.image + at) + (many ? u : u - wide));
+        if (many)
+            attend_many<T, W>(a, item, lds, wave);
+        else
+            attend_few<T, W>(a, item, lds, wave);
+        if (u + static_cast<int>(gridDim.x) < wide + narrow) __syncthreads();  // the next item's tiles go where results lie
+    }
+}
+
+// The partial results of one (row, head), joined by a workgroup with weights 2^(m_i - m): every wave finds the maximum, then
+// groups of lanes read a part's values each, four lanes of the head a lane, and LDS joins the groups in order. Bound by the
+// latency of its chain of reads (the parts come from other XCDs), so all parts of common plans are read at once.
 __global__ __launch_bounds__(kThreads) void cache_join_kernel(AttentionArgs a) {
     const CacheShape& s = a.s;
+    const int count = a.rows >= 0 ? a.rows : scalar_load(&reinterpret_cast<const PlanHeader*>(a.image)->rows);
     const PlanRow* rows = reinterpret_cast<const PlanRow*>(a.image + a.at.rows_at);
-    const int lane = threadIdx.x & 63;
-    const int64_t units = static_cast<int64_t>(reinterpret_cast<const PlanHeader*>(a.image)->rows) * s.heads;
-    const int quads = s.width / 4;                          // 8 .. 64 lanes take a part's values
-    const int at_once = 64 / quads, mine = lane / quads;    // parts read at once by the wave
-    const int d = lane % quads * 4;
-    for (int64_t u = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6); u < units; u += gridDim.x * 4) {
-        const int head = static_cast<int>(u % s.heads);
-        const PlanRow row = rows[u / s.heads];
+    __shared__ f32x4 joined[kThreads];
+    __shared__ float sums_of[kThreads];
+    const int thread = threadIdx.x, lane = thread & 63;
+    const int quads = s.width / 4, groups = kThreads / quads;  // 8 .. 64 threads take a part's values
+    const int mine = thread / quads, d = thread % quads * 4;
+    const int units = count * s.heads;
+    for (int u = blockIdx.x; u < units; u += gridDim.x) {
+        const int head = u % s.heads;
+        const PlanRow row = scalar_load(rows + u / s.heads);
         if (row.slots <= 1) continue;
         const int64_t first = static_cast<int64_t>(row.slot) * s.heads + head;
+        const float* sums = a.partials.sums(s.width, first);
+        const float* values = a.partials.values(s.width, first) + d;
         float top = -INFINITY;
         for (int i = lane; i < row.slots; i += 64)
-            top = fmaxf(top, a.partials.sums(s.width, first + static_cast<int64_t>(i) * s.heads)[0]);
-#pragma unroll
-        for (int k = 32; k > 0; k >>= 1) top = fmaxf(top, __shfl_xor(top, k, 64));
-        const float from = top == -INFINITY ? 0.0f : top;
+            top = fmaxf(top, load_f32(sums + static_cast<int64_t>(i) * s.heads * 2));
         float total = 0;
         f32x4 o{0, 0, 0, 0};
-        if (mine < at_once) {
-#pragma unroll 4
-            for (int i = mine; i < row.slots; i += at_once) {
-                const int64_t index = first + static_cast<int64_t>(i) * s.heads;
-                const float* sums = a.partials.sums(s.width, index);
-                const float weight = __builtin_amdgcn_exp2f(sums[0] - from);
-                total += weight * sums[1];
-                o = o + *reinterpret_cast<const f32x4*>(a.partials.values(s.width, index) + d) * weight;
+        float from = 0;
+        for (int i0 = mine; i0 < row.slots || i0 == mine; i0 += 4 * groups) {
+            f32x4 v[4];
+            f32x2 part[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const int64_t i = min(i0 + k * groups, row.slots - 1);
+                part[k] = *(const SATORI_GLOBAL f32x2*)(sums + i * s.heads * 2);
+                v[k] = *(const SATORI_GLOBAL f32x4*)(values + i * s.heads * s.width);
+            }
+            if (i0 == mine) {
+#pragma unroll
+                for (int k = 32; k > 0; k >>= 1) top = fmaxf(top, __shfl_xor(top, k, 64));
+                from = top == -INFINITY ? 0.0f : top;
+            }
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                if (mine >= groups || i0 + k * groups >= row.slots) break;
+                const float weight = __builtin_amdgcn_exp2f(part[k][0] - from);
+                total += weight * part[k][1];
+                o = o + v[k] * weight;
             }
         }
-        // The groups of lanes added to the first, in order.
-        float all = 0;
-        f32x4 sum{0, 0, 0, 0};
-        for (int k = 0; k < at_once; ++k) {
-            all += __shfl(total, k * quads + lane % quads, 64);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) sum[j] += __shfl(o[j], k * quads + lane % quads, 64);
-        }
-        if (mine == 0)
+        joined[thread] = o;
+        sums_of[thread] = total;
+        __syncthreads();
+        if (thread < quads) {
+            for (int k = 1; k < groups; ++k) {
+                o = o + joined[k * quads + thread];
+                total += sums_of[k * quads + thread];
+            }
 #pragma unroll
             for (int j = 0; j < 4; ++j)
-                if (d + j < s.head_dim) store_f32(a.output + u * s.head_dim + d + j, sum[j] / all);
+                if (d + j < s.head_dim) store_f32(a.output + static_cast<int64_t>(u) * s.head_dim + d + j, o[j] / total);
+        }
+        __syncthreads();
     }
 }
 
-// The wide kernel of a type and width: its pair groups are as wide as a wave's registers allow with two waves a SIMD, its
-// sets of waves as many as LDS holds two buffers for.
-template <typename T, int W>
-using WideOf = Wide<T, W, sizeof(T) * W <= 256 ? 2 : 1, sizeof(T) * W <= 512 ? 4 : 8, sizeof(T) * W <= 256 ? 2 : 1>;
-constexpr int kNarrowBlocks = 1;
 constexpr int kMostGroups = 1024;  // workgroups of a launch whose work is only known when it is replayed
 
-template <typename T, int W, int NB, int PG, int TG>
-hipError_t launch_wide(Wide<T, W, NB, PG, TG>, int groups, const AttentionArgs& a, hipStream_t stream) {
-    using S = Wide<T, W, NB, PG, TG>;
-    const auto kernel = cache_attention_wide_kernel<T, W, NB, PG, TG>;
-    // (more than 64 KB of LDS; set for the current device, where it is a table lookup after the first time)
-    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize,
-                                             static_cast<int>(S::kLds));
-    if (e != hipSuccess) return e;
-    kernel<<<groups, S::kThreads, S::kLds, stream>>>(a);
-    return hipGetLastError();
-}
-
 template <typename T, int W>
-hipError_t attention_of_width(AttentionArgs a, const PlanHeader& now, bool all, hipStream_t stream) {
-    if (now.wide || all)
-        if (const hipError_t e = launch_wide(WideOf<T, W>{}, all ? kMostGroups : now.wide, a, stream); e != hipSuccess) return e;
-    if (now.narrow || all)
-        cache_attention_narrow_kernel<T, W, kNarrowBlocks>
-            <<<all ? kMostGroups : now.narrow, kNarrowWaves * 64, 0, stream>>>(a);
+hipError_t attention_of_width(const AttentionArgs& a, int groups, hipStream_t stream) {
+    using S = Shape<T, W>;
+    const auto kernel = cache_attention_kernel<T, W>;
+    // (more than 64 KB of LDS; set for the current device, where it is a table lookup after the first time)
+    if (S::kLds > 64 * 1024)
+        if (const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
+                                                     hipFuncAttributeMaxDynamicSharedMemorySize, S::kLds);
+            e != hipSuccess)
+            return e;
+    kernel<<<groups, kThreads, S::kLds, stream>>>(a);
     return hipGetLastError();
 }
 
@@ -1028,7 +982,7 @@ auto of_shape(int type, int width, F&& f) {
 }  // namespace
 
 int cache_wide_pairs(int type, int width) {
-    return of_shape(type, width, [](auto t, auto w) { return WideOf<decltype(t), decltype(w)::value>::kPairs; });
+    return of_shape(type, width, [](auto t, auto w) { return Shape<decltype(t), decltype(w)::value>::kPairs; });
 }
 
 hipError_t launch_plan_copy(const int* from, int* to, const PlanLayout& layout, const PlanLayout& used, hipStream_t stream) {
@@ -1086,14 +1040,25 @@ hipError_t launch_cache_attention(const CacheShape& shape, const int* image, con
     if (now.rows == 0 && !all) return hipSuccess;
     const int64_t room = static_cast<int64_t>(bytes / cache_partial_bytes(shape, 1)) * shape.heads;
     const float scale = static_cast<float>(static_cast<double>(kLog2e) / std::sqrt(static_cast<double>(shape.head_dim)));
-    const AttentionArgs a{shape, image, layout, layer, query, output, Partials{partials, room}, scale,
+    const AttentionArgs a{shape,
+                          image,
+                          layout,
+                          all ? -1 : now.wide,
+                          all ? -1 : now.narrow,
+                          all ? -1 : now.rows,
+                          layer,
+                          query,
+                          output,
+                          Partials{partials, room},
+                          scale,
                           shape.head_dim % 4 == 0 && reinterpret_cast<uintptr_t>(query) % 16 == 0};
+    const int groups = all ? kMostGroups : now.wide + now.narrow;
     const hipError_t e = of_shape(shape.type, shape.width, [&](auto t, auto w) {
-        return attention_of_width<decltype(t), decltype(w)::value>(a, now, all, stream);
+        return attention_of_width<decltype(t), decltype(w)::value>(a, groups, stream);
     });
     if (e != hipSuccess || (now.joined == 0 && !all)) return e;
-    const int64_t groups = (static_cast<int64_t>(now.rows) * shape.heads + 3) / 4;
-    cache_join_kernel<<<all ? kMostGroups : static_cast<int>(std::min<int64_t>(groups, 65536)), kThreads, 0, stream>>>(a);
+    const int64_t joins = static_cast<int64_t>(now.rows) * shape.heads;
+    cache_join_kernel<<<all ? kMostGroups : static_cast<int>(std::min<int64_t>(joins, 65536)), kThreads, 0, stream>>>(a);
     return hipGetLastError();
 }
 

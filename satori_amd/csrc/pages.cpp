@@ -336,7 +336,7 @@ PlanImage plan_batch(const PageTables& tables, const int* sequences, const int* 
         const int64_t c = (tokens / workgroups + step - 1) / step * step;
         return static_cast<int>(std::min<int64_t>(std::max<int64_t>(c, step), 1 << 20));
     };
-    const int narrow_chunk = chunk_for(narrow_tokens, 1024), wide_chunk = chunk_for(wide_tokens, 256);
+    const int narrow_chunk = chunk_for(narrow_tokens, 256), wide_chunk = chunk_for(wide_tokens, 256);
 
     std::vector<int>& page_list = image.pages;
     std::vector<int> row_list;

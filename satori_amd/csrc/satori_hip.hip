@@ -2474,6 +2474,8 @@ int satori_hip_cache_plan_set(satori_hip_cache_plan* p, satori_hip_pages* pages,
                 fail(SATORI_HIP_E_ARGUMENT, "The pages are not those of the plan's pool.");
             image = plan_batch(tables, sequences, new_tokens, count, p->plan);
         }
+        if (static_cast<int64_t>(image.header.rows) * p->shape.heads > INT32_MAX / 4)
+            fail(SATORI_HIP_E_OVERFLOW, "Arithmetic operation resulted in an overflow.");
         PlanLayout layout = p->layout;
         const PlanLayout used = image.least();
         if (layout.grow(used) && p->steps > 0) plan_held();
