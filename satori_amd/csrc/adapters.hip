@@ -15,164 +15,175 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kWaves = 4;
 constexpr int kMostSplits = 16;
+constexpr int64_t kBothBytes = 24 << 20;  // weights that one launch may read, tiles times the workgroups that read them
 constexpr int kSplitGroups = 256;  // workgroups that the first launch's splits make up
 constexpr int kStep = 32;  // columns a wave takes at once
 
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
 
-// Elements at .. at + N - 1 of a row of `length`, zero behind it; as FP32. `aligned`: the addresses of the row's groups of
-// N elements are multiples of their bytes (of 16 at most).
-template <typename T, int N>
-__device__ __forceinline__ void load_row(const T* row, int at, int length, bool aligned, float (&out)[N]) {
-    if (aligned && at + N <= length) {
-        if constexpr (sizeof(T) == 4) {
+// N elements of a row from `at` on, as FP32, in one read (two for eight of FP32) at any element's address.
+template <int N, typename T>
+__device__ __forceinline__ void load_inside(const T* row, int at, float (&out)[N]) {
+    constexpr int kGroup = N * sizeof(T) > 16 ? 16 / sizeof(T) : N;
+    typedef T pack __attribute__((ext_vector_type(kGroup), aligned(sizeof(T))));
 #pragma unroll
-            for (int i = 0; i < N; i += 4) {
-                const f32x4 v = *(const SATORI_GLOBAL f32x4*)(row + at + i);
+    for (int i = 0; i < N; i += kGroup) {
+        const pack v = *(const SATORI_GLOBAL pack*)(row + at + i);
 #pragma unroll
-                for (int j = 0; j < 4; ++j) out[i + j] = v[j];
-            }
-        } else if constexpr (N == 8) {
-            const f16x8 v = *(const SATORI_GLOBAL f16x8*)(row + at);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) out[j] = static_cast<float>(v[j]);
-        } else {
-            const f16x4 v = *(const SATORI_GLOBAL f16x4*)(row + at);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) out[j] = static_cast<float>(v[j]);
-        }
-        return;
+        for (int j = 0; j < kGroup; ++j) out[i + j] = static_cast<float>(v[j]);
     }
+}
+// The same where the row may end: zero from `end` on.
+template <int N, typename T>
+__device__ __forceinline__ void load_at_end(const T* row, int at, int end, float (&out)[N]) {
 #pragma unroll
-    for (int i = 0; i < N; ++i)
-        out[i] = at + i < length ? static_cast<float>(*(const SATORI_GLOBAL T*)(row + at + i)) : 0.0f;
+    for (int i = 0; i < N; ++i) {
+        const T v = *(const SATORI_GLOBAL T*)(row + min(at + i, end - 1));
+        out[i] = at + i < end ? static_cast<float>(v) : 0.0f;
+    }
 }
 
-constexpr int kRankTiles = 4;  // tiles of 16 ranks that share a workgroup's input rows
+// What a launch knows of a tile: its adapter and rows.
+struct Tile {
+    Adapter adapter;
+    int begin, count;
+    bool none;
+};
+__device__ __forceinline__ Tile tile_of(const AdapterShape& s, const AdapterTiles& tiles, int tile) {
+    Tile t;
+    t.begin = tiles.begin[tile];
+    t.count = tiles.begin[tile + 1] - t.begin;
+    t.none = tiles.adapter[tile] == kNoAdapter;
+    t.adapter = t.none ? Adapter{nullptr, nullptr, 0, 0.0f} : s.adapters[tiles.adapter[tile]];
+    return t;
+}
 
-// Workgroup (tile, 64 ranks, split): its waves take steps of 32 columns in turn; lane (c, g) holds columns 8 g .. 8 g + 7
-// of rank c's weights (of each tile of 16 ranks) and of row c's input.
+// A wave's part of 16 ranks of a tile's reduced vectors: steps of 32 columns from `first` on, `stride` apart, four of them
+// read at once; lane (c, g) holds columns 8 g .. 8 g + 7 of rank c's weights and of row c's input, and gets ranks
+// 4 g .. 4 g + 3 of row c. (Ranks past the last repeat the first, rows past the last the tile's first: nobody takes those.)
+template <typename T>
+__device__ __forceinline__ f32x4 reduce(const AdapterShape& s, const Tile& tile, const float* x, int rank0, int first, int stride,
+                                        int end) {
+    constexpr int kAtOnce = 4;
+    const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
+    const T* down = static_cast<const T*>(tile.adapter.down) +
+                    static_cast<int64_t>(rank0 + c < tile.adapter.rank ? rank0 + c : 0) * s.columns;
+    f32x4 sum{0, 0, 0, 0};
+    for (int at = first; at < end; at += kAtOnce * stride) {
+        float w[kAtOnce][8] = {}, v[kAtOnce][8] = {};
+#pragma unroll
+        for (int i = 0; i < kAtOnce; ++i) {
+            const int step = at + i * stride;
+            if (step + kStep <= end) {
+                load_inside(down, step + 8 * g, w[i]);
+                load_inside(x, step + 8 * g, v[i]);
+            } else if (step < end) {
+                load_at_end(down, step + 8 * g, end, w[i]);
+                load_at_end(x, step + 8 * g, end, v[i]);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < kAtOnce; ++i)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) sum = __builtin_amdgcn_mfma_f32_16x16x4f32(w[i][j], v[i][j], sum, 0, 0, 0);
+    }
+    return sum;
+}
+
+// Workgroup (tile, 16 ranks, split of the columns).
 template <typename T>
 __global__ __launch_bounds__(kThreads) void adapter_down_kernel(AdapterShape s, AdapterTiles tiles,
                                                                 const float* __restrict__ input,
-                                                                float* __restrict__ reduced, int split_columns,
-                                                                bool aligned) {
-    const int tile = blockIdx.x, rank0 = blockIdx.y * 16 * kRankTiles, split = blockIdx.z;
-    if (tiles.adapter[tile] == kNoAdapter) return;
-    const Adapter a = s.adapters[tiles.adapter[tile]];
-    if (rank0 >= a.rank) return;
+                                                                float* __restrict__ reduced, int split_columns) {
+    const Tile tile = tile_of(s, tiles, blockIdx.x);
+    const int rank0 = blockIdx.y * 16, split = blockIdx.z;
+    if (rank0 >= tile.adapter.rank) return;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = lane & 15, g = lane >> 4;
-    const int begin = tiles.begin[tile], count = tiles.begin[tile + 1] - begin;
-    const int rank_tiles = min(kRankTiles, (a.rank - rank0 + 15) / 16);
-    const int row = c < count ? tiles.order[begin + c] : 0;
-    const float* x = input + static_cast<int64_t>(row) * s.columns;
-    const T* down = static_cast<const T*>(a.down) + static_cast<int64_t>(rank0) * s.columns;
+    const int row = c < tile.count ? tiles.order[tile.begin + c] : 0;
     const int first = split * split_columns;
-    const int end = first + split_columns < s.columns ? first + split_columns : s.columns;
-    f32x4 sum[kRankTiles];
-#pragma unroll
-    for (int k = 0; k < kRankTiles; ++k) sum[k] = f32x4{0, 0, 0, 0};
-#pragma unroll 2
-    for (int at = first + wave * kStep + 8 * g; at - 8 * g < end; at += kWaves * kStep) {
-        float v[8];
-        load_row(x, at, c < count ? end : 0, aligned, v);
-#pragma unroll
-        for (int k = 0; k < kRankTiles; ++k) {
-            if (k >= rank_tiles) break;
-            const bool has_rank = rank0 + 16 * k + c < a.rank;
-            float w[8];
-            load_row(down + static_cast<int64_t>(has_rank ? 16 * k + c : 0) * s.columns, at, has_rank ? end : 0, aligned, w);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) sum[k] = __builtin_amdgcn_mfma_f32_16x16x4f32(w[j], v[j], sum[k], 0, 0, 0);
-        }
-    }
-    __shared__ f32x4 parts[kWaves][kRankTiles][64];
-#pragma unroll
-    for (int k = 0; k < kRankTiles; ++k)
-        if (k < rank_tiles) parts[wave][k][lane] = sum[k];
+    f32x4 sum = reduce<T>(s, tile, input + static_cast<int64_t>(row) * s.columns, rank0, first + wave * kStep,
+                                   kWaves * kStep, first + split_columns < s.columns ? first + split_columns : s.columns);
+    __shared__ f32x4 parts[kWaves][64];
+    parts[wave][lane] = sum;
     __syncthreads();
-    if (wave < rank_tiles && c < count) {  // wave k joins tile k of the ranks
-        f32x4 total = parts[0][wave][lane];
+    if (wave == 0 && c < tile.count) {
 #pragma unroll
-        for (int w = 1; w < kWaves; ++w) total = total + parts[w][wave][lane];
-        float* out = reduced + (static_cast<int64_t>(split) * tiles.positions + row) * s.rank_most + rank0 + 16 * wave + 4 * g;
-        *reinterpret_cast<f32x4*>(out) = total;
+        for (int w = 1; w < kWaves; ++w) sum = sum + parts[w][lane];
+        *reinterpret_cast<f32x4*>(reduced + (static_cast<int64_t>(split) * tiles.positions + row) * s.rank_most + rank0 + 4 * g) = sum;
     }
 }
 
-// Workgroup (tile, 256 output rows): the tile's reduced vectors summed over the splits into LDS (eight loads in flight),
-// then 64 output rows a wave; lane (c, g) holds ranks 4 g .. 4 g + 3 of a step of 16. `whole`: rows of the output and the
-// base start at multiples of 16 bytes.
-template <typename T>
-__global__ __launch_bounds__(kThreads) void adapter_up_kernel(AdapterShape s, AdapterTiles tiles,
-                                                              const float* __restrict__ reduced, const float* base,
-                                                              float* output, int splits, bool whole) {
-    extern __shared__ float t[];  // [16][rank_most + 4]
-    const int tile = blockIdx.x;
-    const int begin = tiles.begin[tile], count = tiles.begin[tile + 1] - begin;
-    const bool none = tiles.adapter[tile] == kNoAdapter;
-    const Adapter a = none ? Adapter{nullptr, nullptr, 0, 0.0f} : s.adapters[tiles.adapter[tile]];
-    const int ranks = (a.rank + 15) / 16 * 16, stride = s.rank_most + 4;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = lane & 15, g = lane >> 4;
-    const int n0 = blockIdx.y * 256 + wave * 64;
-    const bool has_row = c < count;
-    const int64_t row = static_cast<int64_t>(has_row ? tiles.order[begin + c] : 0) * s.rows;
-    f32x4 kept[4];  // the base, on its way while the rest is computed
+// 64 output rows from n0 on of a tile's rows, with its reduced vectors `t` [16][stride] in LDS; lane (c, g) holds ranks
+// 4 g .. 4 g + 3 of a step of 16 and gets output rows 4 g .. 4 g + 3 of each of four tiles, of row c. `whole`: rows of the
+// output and the base start at multiples of 16 bytes.
+struct Kept {
+    f32x4 v[4];
+};
+__device__ __forceinline__ Kept load_base(const AdapterShape& s, const float* base, int64_t row, bool has_row, int n0, bool whole) {
+    const int g = (threadIdx.x & 63) >> 4;
+    Kept kept;
 #pragma unroll
     for (int n = 0; n < 4; ++n) {
         const int at = n0 + 16 * n + 4 * g;
-        kept[n] = f32x4{0, 0, 0, 0};
+        kept.v[n] = f32x4{0, 0, 0, 0};
         if (!has_row) continue;
         if (whole && at + 4 <= s.rows) {
-            kept[n] = *(const SATORI_GLOBAL f32x4*)(base + row + at);
+            kept.v[n] = *(const SATORI_GLOBAL f32x4*)(base + row + at);
         } else {
 #pragma unroll
             for (int j = 0; j < 4; ++j)
-                if (at + j < s.rows) kept[n][j] = load_f32(base + row + at + j);
+                if (at + j < s.rows) kept.v[n][j] = load_f32(base + row + at + j);
         }
     }
-    const int64_t next = static_cast<int64_t>(tiles.positions) * s.rank_most;
-    for (int i = threadIdx.x; i < count * (ranks / 4); i += kThreads) {
-        const int r = i / (ranks / 4), k = i % (ranks / 4) * 4;
-        const float* from = reduced + static_cast<int64_t>(tiles.order[begin + r]) * s.rank_most + k;
-        f32x4 sum{0, 0, 0, 0};
-        for (int p0 = 0; p0 < splits; p0 += 8) {
-            f32x4 v[8];
+    return kept;
+}
+// The weights of four steps of 16 ranks: read before what they are multiplied with is there.
+template <typename T>
+struct UpWeights {
+    float w[4][4][4];
+    __device__ __forceinline__ void load(const AdapterShape& s, const Tile& tile, int n0, int k) {
+        const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4, rank = tile.adapter.rank;
 #pragma unroll
-            for (int p = 0; p < 8; ++p)
-                v[p] = p0 + p < splits ? *(const SATORI_GLOBAL f32x4*)(from + (p0 + p) * next) : f32x4{0, 0, 0, 0};
+        for (int i = 0; i < 4; ++i) {
+            const int step = k + 16 * i;
+            if (step >= rank) break;
 #pragma unroll
-            for (int p = 0; p < 8; ++p) sum = sum + v[p];
+            for (int n = 0; n < 4; ++n) {
+                const T* up = static_cast<const T*>(tile.adapter.up) + static_cast<int64_t>(min(n0 + 16 * n + c, s.rows - 1)) * rank;
+                if (step + 16 <= rank)
+                    load_inside(up, step + 4 * g, w[i][n]);
+                else
+                    load_at_end(up, step + 4 * g, rank, w[i][n]);
+            }
         }
-#pragma unroll
-        for (int j = 0; j < 4; ++j) t[r * stride + k + j] = k + j < a.rank ? sum[j] * a.scale : 0.0f;
     }
-    __syncthreads();
+};
+template <typename T>
+__device__ __forceinline__ void expand(const AdapterShape& s, const Tile& tile, UpWeights<T>& up, const float* t, int stride,
+                                       const Kept& kept, float* output, int64_t row, bool has_row, int n0, bool whole) {
+    const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4, rank = tile.adapter.rank;
     f32x4 sum[4];
 #pragma unroll
     for (int n = 0; n < 4; ++n) sum[n] = f32x4{0, 0, 0, 0};
-    const T* up = static_cast<const T*>(a.up);
-    const bool aligned = a.rank % 4 == 0 && reinterpret_cast<uintptr_t>(up) % 16 == 0;
-    for (int k = 4 * g; k - 4 * g < ranks; k += 16) {
-        float v[4], w[4][4];
+    for (int k = 0; k < rank; k += 64) {
+        if (k > 0) up.load(s, tile, n0, k);
 #pragma unroll
-        for (int n = 0; n < 4; ++n) {
-            const int at = n0 + 16 * n + c;
-            load_row(up + static_cast<int64_t>(at < s.rows ? at : 0) * a.rank, k, at < s.rows ? a.rank : 0, aligned, w[n]);
+        for (int i = 0; i < 4; ++i) {
+            if (k + 16 * i >= rank) break;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const float v = t[c * stride + k + 16 * i + 4 * g + j];  // (rows past the last: nobody takes those)
+#pragma unroll
+                for (int n = 0; n < 4; ++n) sum[n] = __builtin_amdgcn_mfma_f32_16x16x4f32(up.w[i][n][j], v, sum[n], 0, 0, 0);
+            }
         }
-#pragma unroll
-        for (int j = 0; j < 4; ++j) v[j] = has_row ? t[c * stride + k + j] : 0.0f;
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-#pragma unroll
-            for (int n = 0; n < 4; ++n) sum[n] = __builtin_amdgcn_mfma_f32_16x16x4f32(w[n][j], v[j], sum[n], 0, 0, 0);
     }
     if (!has_row) return;
 #pragma unroll
     for (int n = 0; n < 4; ++n) {
         const int at = n0 + 16 * n + 4 * g;
-        const f32x4 out = kept[n] + sum[n];
+        const f32x4 out = kept.v[n] + sum[n];
         if (whole && at + 4 <= s.rows) {
             *(SATORI_GLOBAL f32x4*)(output + row + at) = out;
         } else {
@@ -183,19 +194,107 @@ __global__ __launch_bounds__(kThreads) void adapter_up_kernel(AdapterShape s, Ad
     }
 }
 
+// Workgroup (tile, 256 output rows): the tile's reduced vectors summed over the splits into LDS, then 64 output rows a wave.
+template <typename T>
+__global__ __launch_bounds__(kThreads) void adapter_up_kernel(AdapterShape s, AdapterTiles tiles,
+                                                              const float* __restrict__ reduced, const float* base,
+                                                              float* output, int splits, bool whole) {
+    extern __shared__ float t[];  // [16][rank_most + 4]
+    const Tile tile = tile_of(s, tiles, blockIdx.x);
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = lane & 15;
+    const int n0 = blockIdx.y * 256 + wave * 64, stride = s.rank_most + 4;
+    const bool has_row = c < tile.count;
+    const int64_t row = static_cast<int64_t>(has_row ? tiles.order[tile.begin + c] : 0) * s.rows;
+    UpWeights<T> up;
+    up.load(s, tile, n0, 0);
+    const Kept kept = load_base(s, base, row, has_row, n0, whole);
+    const int quads = (tile.adapter.rank + 15) / 16 * 4;
+    const int64_t next = static_cast<int64_t>(tiles.positions) * s.rank_most;
+    for (int i = threadIdx.x; i < tile.count * quads; i += kThreads) {
+        const int r = i / quads, k = i % quads * 4;
+        const float* from = reduced + static_cast<int64_t>(tiles.order[tile.begin + r]) * s.rank_most + k;
+        f32x4 sum{0, 0, 0, 0};
+        for (int p0 = 0; p0 < splits; p0 += 4) {
+            f32x4 v[4];
+#pragma unroll
+            for (int p = 0; p < 4; ++p)
+                v[p] = p0 + p < splits ? *(const SATORI_GLOBAL f32x4*)(from + (p0 + p) * next) : f32x4{0, 0, 0, 0};
+#pragma unroll
+            for (int p = 0; p < 4; ++p) sum = sum + v[p];
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) t[r * stride + k + j] = k + j < tile.adapter.rank ? sum[j] * tile.adapter.scale : 0.0f;
+    }
+    __syncthreads();
+    expand<T>(s, tile, up, t, stride, kept, output, row, has_row, n0, whole);
+}
+
+// Both products in one launch, for small adapters and few tiles: workgroup (tile, 512 output rows or less) makes the tile's
+// whole reduced vectors for itself.
+constexpr int kBothWaves = 8;
+constexpr int kBothRanks = 4;  // tiles of 16 ranks
+
+template <typename T>
+__global__ __launch_bounds__(kBothWaves * 64) void adapter_both_kernel(AdapterShape s, AdapterTiles tiles,
+                                                                       const float* __restrict__ input, const float* base,
+                                                                       float* output, int rows_each, bool whole) {
+    __shared__ f32x4 parts[kBothWaves][64];
+    __shared__ float t[16][16 * kBothRanks + 4];
+    const Tile tile = tile_of(s, tiles, blockIdx.x);
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = lane & 15, g = lane >> 4;
+    const bool has_row = c < tile.count;
+    const int order = has_row ? tiles.order[tile.begin + c] : 0;
+    const int64_t row = static_cast<int64_t>(order) * s.rows;
+    const int n0 = blockIdx.y * rows_each + wave * 64;
+    const bool works = wave * 64 < rows_each && n0 < s.rows;
+    Kept kept{};
+    UpWeights<T> up;
+    if (works) {
+        up.load(s, tile, n0, 0);
+        kept = load_base(s, base, row, has_row, n0, whole);
+    }
+    for (int rank0 = 0; rank0 < tile.adapter.rank; rank0 += 16) {
+        const f32x4 sum = reduce<T>(s, tile, input + static_cast<int64_t>(order) * s.columns, rank0, wave * kStep,
+                                             kBothWaves * kStep, s.columns);
+        if (rank0) __syncthreads();
+        parts[wave][lane] = sum;
+        __syncthreads();
+        if (wave == 0) {
+            f32x4 total = sum;
+#pragma unroll
+            for (int w = 1; w < kBothWaves; ++w) total = total + parts[w][lane];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int k = rank0 + 4 * g + j;
+                t[c][k] = k < tile.adapter.rank ? total[j] * tile.adapter.scale : 0.0f;
+            }
+        }
+    }
+    __syncthreads();
+    if (works) expand<T>(s, tile, up, &t[0][0], 16 * kBothRanks + 4, kept, output, row, has_row, n0, whole);
+}
+
 template <typename T>
 void launch(const AdapterShape& s, const AdapterTiles& tiles, const float* input, const float* base, float* output,
             float* workspace, hipStream_t stream) {
-    const int ranks = (s.rank_most / 16 + kRankTiles - 1) / kRankTiles;
+    const bool whole = s.rows % 4 == 0 && reinterpret_cast<uintptr_t>(base) % 16 == 0 &&
+                       reinterpret_cast<uintptr_t>(output) % 16 == 0;
+    const int ranks = s.rank_most / 16;
+    const int64_t both_groups = static_cast<int64_t>(tiles.tiles) * ((s.rows + 511) / 512);
+    if (ranks <= kBothRanks && both_groups * ranks * 16 * s.columns * static_cast<int64_t>(sizeof(T)) <= kBothBytes) {
+        // 64 rows a wave and turn; fewer waves work on them where that lets more CUs share them.
+        int each = 512;
+        while (each > 64 && tiles.tiles * ((s.rows + each - 1) / each) < 128) each /= 2;
+        adapter_both_kernel<T><<<dim3(tiles.tiles, (s.rows + each - 1) / each), kBothWaves * 64, 0, stream>>>(
+            s, tiles, input, base, output, each, whole);
+        return;
+    }
     // Splits of whole steps of the four waves, for about one workgroup a CU.
     const int steps = (s.columns + kWaves * kStep - 1) / (kWaves * kStep);
     const int want = std::min({std::max(1, kSplitGroups / (tiles.tiles * ranks)), steps, kMostSplits});
     const int per = (steps + want - 1) / want, splits = (steps + per - 1) / per;
-    const bool aligned = s.aligned && reinterpret_cast<uintptr_t>(input) % 16 == 0;
-    const bool whole = s.rows % 4 == 0 && reinterpret_cast<uintptr_t>(base) % 16 == 0 &&
-                       reinterpret_cast<uintptr_t>(output) % 16 == 0;
-    adapter_down_kernel<T><<<dim3(tiles.tiles, ranks, splits), kThreads, 0, stream>>>(
-        s, tiles, input, workspace, per * kWaves * kStep, aligned);
+    adapter_down_kernel<T><<<dim3(tiles.tiles, ranks, splits), kThreads, 0, stream>>>(s, tiles, input, workspace,
+                                                                                               per * kWaves * kStep);
     adapter_up_kernel<T><<<dim3(tiles.tiles, (s.rows + 255) / 256), kThreads, 16 * (s.rank_most + 4) * sizeof(float),
                            stream>>>(s, tiles, workspace, base, output, splits, whole);
 }

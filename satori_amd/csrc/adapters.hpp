@@ -33,7 +33,6 @@ struct AdapterShape {
     int rows, columns;
     int rank_most;            // largest rank, rounded up to a multiple of 16
     int type;                 // Element (cache_ops.hpp): kF32 or kF16
-    bool aligned;             // the rows of every `down` (and of an aligned input) start at multiples of 16 bytes
 };
 
 // Bytes of `workspace` (the rows' reduced vectors, [splits][positions][rank_most]).

@@ -2568,7 +2568,6 @@ int satori_hip_adapters_create(satori_hip_context* c, int rows, int columns, int
         shape.columns = columns;
         shape.type = type;
         const uintptr_t unit = element_bytes(type);
-        shape.aligned = columns * unit % 16 == 0 && columns % 4 == 0;
         std::vector<Adapter> table(count);
         for (int i = 0; i < count; ++i) {
             require(down[i], "down");
@@ -2578,7 +2577,6 @@ int satori_hip_adapters_create(satori_hip_context* c, int rows, int columns, int
                 fail(SATORI_HIP_E_ARGUMENT, "Adapter weights must be aligned to their elements.");
             table[i] = Adapter{down[i], up[i], ranks[i], scales[i]};
             shape.rank_most = std::max(shape.rank_most, (ranks[i] + 15) / 16 * 16);
-            shape.aligned &= reinterpret_cast<uintptr_t>(down[i]) % 16 == 0;
         }
         set_device(c);
         auto* a = new satori_hip_adapters();
