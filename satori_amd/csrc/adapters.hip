@@ -114,34 +114,54 @@ __global__ __launch_bounds__(kThreads) void adapter_down_kernel(AdapterShape s, 
     }
 }
 
-// 64 output rows from n0 on of a tile's rows, with its reduced vectors `t` [16][stride] in LDS; lane (c, g) holds ranks
-// 4 g .. 4 g + 3 of a step of 16 and gets output rows 4 g .. 4 g + 3 of each of four tiles, of row c. `whole`: rows of the
+// 16 * N output rows from n0 on of a tile's rows, with its reduced vectors `t` [16][stride] in LDS; lane (c, g) holds ranks
+// 4 g .. 4 g + 3 of a step of 16 and gets output rows 4 g .. 4 g + 3 of each of N tiles, of row c. `whole`: rows of the
 // output and the base start at multiples of 16 bytes.
-struct Kept {
-    f32x4 v[4];
-};
-__device__ __forceinline__ Kept load_base(const AdapterShape& s, const float* base, int64_t row, bool has_row, int n0, bool whole) {
-    const int g = (threadIdx.x & 63) >> 4;
-    Kept kept;
+template <int N>
+struct Outputs {
+    f32x4 base[N];
+    int64_t row;  // of the tile's row c, in elements
+    bool is;      // there is such a row
+    __device__ __forceinline__ void load(const AdapterShape& s, const AdapterTiles& tiles, const Tile& tile, const float* from,
+                                         int first, int n0, bool whole) {
+        const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
+        is = first + c < tile.count;
+        row = static_cast<int64_t>(is ? tiles.order[tile.begin + first + c] : 0) * s.rows;
 #pragma unroll
-    for (int n = 0; n < 4; ++n) {
-        const int at = n0 + 16 * n + 4 * g;
-        kept.v[n] = f32x4{0, 0, 0, 0};
-        if (!has_row) continue;
-        if (whole && at + 4 <= s.rows) {
-            kept.v[n] = *(const SATORI_GLOBAL f32x4*)(base + row + at);
-        } else {
+        for (int n = 0; n < N; ++n) {
+            const int at = n0 + 16 * n + 4 * g;
+            base[n] = f32x4{0, 0, 0, 0};
+            if (!is) continue;
+            if (whole && at + 4 <= s.rows) {
+                base[n] = *(const SATORI_GLOBAL f32x4*)(from + row + at);
+            } else {
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-                if (at + j < s.rows) kept.v[n][j] = load_f32(base + row + at + j);
+                for (int j = 0; j < 4; ++j)
+                    if (at + j < s.rows) base[n][j] = load_f32(from + row + at + j);
+            }
         }
     }
-    return kept;
-}
+    __device__ __forceinline__ void store(const AdapterShape& s, float* to, const f32x4 (&sum)[N], int n0, bool whole) const {
+        const int g = (threadIdx.x & 63) >> 4;
+        if (!is) return;
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+            const int at = n0 + 16 * n + 4 * g;
+            const f32x4 out = base[n] + sum[n];
+            if (whole && at + 4 <= s.rows) {
+                *(SATORI_GLOBAL f32x4*)(to + row + at) = out;
+            } else {
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    if (at + j < s.rows) store_f32(to + row + at + j, out[j]);
+            }
+        }
+    }
+};
 // The weights of four steps of 16 ranks: read before what they are multiplied with is there.
-template <typename T>
+template <typename T, int N>
 struct UpWeights {
-    float w[4][4][4];
+    float w[4][N][4];
     __device__ __forceinline__ void load(const AdapterShape& s, const Tile& tile, int n0, int k) {
         const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4, rank = tile.adapter.rank;
 #pragma unroll
@@ -149,7 +169,7 @@ struct UpWeights {
             const int step = k + 16 * i;
             if (step >= rank) break;
 #pragma unroll
-            for (int n = 0; n < 4; ++n) {
+            for (int n = 0; n < N; ++n) {
                 const T* up = static_cast<const T*>(tile.adapter.up) + static_cast<int64_t>(min(n0 + 16 * n + c, s.rows - 1)) * rank;
                 if (step + 16 <= rank)
                     load_inside(up, step + 4 * g, w[i][n]);
@@ -158,56 +178,35 @@ struct UpWeights {
             }
         }
     }
-};
-template <typename T>
-__device__ __forceinline__ void expand(const AdapterShape& s, const Tile& tile, UpWeights<T>& up, const float* t, int stride,
-                                       const Kept& kept, float* output, int64_t row, bool has_row, int n0, bool whole) {
-    const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4, rank = tile.adapter.rank;
-    f32x4 sum[4];
-#pragma unroll
-    for (int n = 0; n < 4; ++n) sum[n] = f32x4{0, 0, 0, 0};
-    for (int k = 0; k < rank; k += 64) {
-        if (k > 0) up.load(s, tile, n0, k);
+    // Adds the product with those steps of t's rows.
+    __device__ __forceinline__ void expand(const Tile& tile, const float* t, int stride, int k, f32x4 (&sum)[N]) const {
+        const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            if (k + 16 * i >= rank) break;
+            if (k + 16 * i >= tile.adapter.rank) break;
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 const float v = t[c * stride + k + 16 * i + 4 * g + j];  // (rows past the last: nobody takes those)
 #pragma unroll
-                for (int n = 0; n < 4; ++n) sum[n] = __builtin_amdgcn_mfma_f32_16x16x4f32(up.w[i][n][j], v, sum[n], 0, 0, 0);
+                for (int n = 0; n < N; ++n) sum[n] = __builtin_amdgcn_mfma_f32_16x16x4f32(w[i][n][j], v, sum[n], 0, 0, 0);
             }
         }
     }
-    if (!has_row) return;
-#pragma unroll
-    for (int n = 0; n < 4; ++n) {
-        const int at = n0 + 16 * n + 4 * g;
-        const f32x4 out = kept.v[n] + sum[n];
-        if (whole && at + 4 <= s.rows) {
-            *(SATORI_GLOBAL f32x4*)(output + row + at) = out;
-        } else {
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-                if (at + j < s.rows) store_f32(output + row + at + j, out[j]);
-        }
-    }
-}
+};
 
-// Workgroup (tile, 256 output rows): the tile's reduced vectors summed over the splits into LDS, then 64 output rows a wave.
+// Workgroup (up to two tiles of one adapter, 128 output rows): the tiles' reduced vectors summed over the splits into LDS,
+// then 32 output rows a wave, whose weights serve all the tiles (read once per tile they took 10 of 18 us at 256 rows, rank
+// 64, 11008 output rows).
 template <typename T>
 __global__ __launch_bounds__(kThreads) void adapter_up_kernel(AdapterShape s, AdapterTiles tiles,
                                                               const float* __restrict__ reduced, const float* base,
                                                               float* output, int splits, bool whole) {
-    extern __shared__ float t[];  // [16][rank_most + 4]
-    const Tile tile = tile_of(s, tiles, blockIdx.x);
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = lane & 15;
-    const int n0 = blockIdx.y * 256 + wave * 64, stride = s.rank_most + 4;
-    const bool has_row = c < tile.count;
-    const int64_t row = static_cast<int64_t>(has_row ? tiles.order[tile.begin + c] : 0) * s.rows;
-    UpWeights<T> up;
+    extern __shared__ float t[];  // [16 * kGroupTiles][rank_most + 4]
+    Tile tile = tile_of(s, tiles, tiles.group[blockIdx.x]);
+    tile.count = tiles.begin[tiles.group[blockIdx.x + 1]] - tile.begin;
+    const int wave = threadIdx.x >> 6, n0 = blockIdx.y * 128 + wave * 32, stride = s.rank_most + 4;
+    UpWeights<T, 2> up;
     up.load(s, tile, n0, 0);
-    const Kept kept = load_base(s, base, row, has_row, n0, whole);
     const int quads = (tile.adapter.rank + 15) / 16 * 4;
     const int64_t next = static_cast<int64_t>(tiles.positions) * s.rank_most;
     for (int i = threadIdx.x; i < tile.count * quads; i += kThreads) {
@@ -225,8 +224,23 @@ __global__ __launch_bounds__(kThreads) void adapter_up_kernel(AdapterShape s, Ad
 #pragma unroll
         for (int j = 0; j < 4; ++j) t[r * stride + k + j] = k + j < tile.adapter.rank ? sum[j] * tile.adapter.scale : 0.0f;
     }
+    Outputs<2> out[kGroupTiles];
+#pragma unroll
+    for (int r = 0; r < kGroupTiles; ++r)
+        if (16 * r < tile.count) out[r].load(s, tiles, tile, base, 16 * r, n0, whole);
     __syncthreads();
-    expand<T>(s, tile, up, t, stride, kept, output, row, has_row, n0, whole);
+    f32x4 sum[kGroupTiles][2];
+#pragma unroll
+    for (int r = 0; r < kGroupTiles; ++r) sum[r][0] = sum[r][1] = f32x4{0, 0, 0, 0};
+    for (int k = 0; k < tile.adapter.rank; k += 64) {
+        if (k > 0) up.load(s, tile, n0, k);
+#pragma unroll
+        for (int r = 0; r < kGroupTiles; ++r)
+            if (16 * r < tile.count) up.expand(tile, t + 16 * r * stride, stride, k, sum[r]);
+    }
+#pragma unroll
+    for (int r = 0; r < kGroupTiles; ++r)
+        if (16 * r < tile.count) out[r].store(s, output, sum[r], n0, whole);
 }
 
 // Both products in one launch, for small adapters and few tiles: workgroup (tile, 512 output rows or less) makes the tile's
@@ -242,20 +256,17 @@ __global__ __launch_bounds__(kBothWaves * 64) void adapter_both_kernel(AdapterSh
     __shared__ float t[16][16 * kBothRanks + 4];
     const Tile tile = tile_of(s, tiles, blockIdx.x);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = lane & 15, g = lane >> 4;
-    const bool has_row = c < tile.count;
-    const int order = has_row ? tiles.order[tile.begin + c] : 0;
-    const int64_t row = static_cast<int64_t>(order) * s.rows;
     const int n0 = blockIdx.y * rows_each + wave * 64;
     const bool works = wave * 64 < rows_each && n0 < s.rows;
-    Kept kept{};
-    UpWeights<T> up;
+    UpWeights<T, 4> up;
+    Outputs<4> out;
     if (works) {
         up.load(s, tile, n0, 0);
-        kept = load_base(s, base, row, has_row, n0, whole);
+        out.load(s, tiles, tile, base, 0, n0, whole);
     }
+    const float* x = input + static_cast<int64_t>(tiles.order[tile.begin + (c < tile.count ? c : 0)]) * s.columns;
     for (int rank0 = 0; rank0 < tile.adapter.rank; rank0 += 16) {
-        const f32x4 sum = reduce<T>(s, tile, input + static_cast<int64_t>(order) * s.columns, rank0, wave * kStep,
-                                             kBothWaves * kStep, s.columns);
+        const f32x4 sum = reduce<T>(s, tile, x, rank0, wave * kStep, kBothWaves * kStep, s.columns);
         if (rank0) __syncthreads();
         parts[wave][lane] = sum;
         __syncthreads();
@@ -271,11 +282,16 @@ __global__ __launch_bounds__(kBothWaves * 64) void adapter_both_kernel(AdapterSh
         }
     }
     __syncthreads();
-    if (works) expand<T>(s, tile, up, &t[0][0], 16 * kBothRanks + 4, kept, output, row, has_row, n0, whole);
+    if (!works) return;
+    f32x4 sum[4];
+#pragma unroll
+    for (int n = 0; n < 4; ++n) sum[n] = f32x4{0, 0, 0, 0};
+    up.expand(tile, &t[0][0], 16 * kBothRanks + 4, 0, sum);
+    out.store(s, output, sum, n0, whole);
 }
 
 template <typename T>
-void launch(const AdapterShape& s, const AdapterTiles& tiles, const float* input, const float* base, float* output,
+hipError_t launch(const AdapterShape& s, const AdapterTiles& tiles, const float* input, const float* base, float* output,
             float* workspace, hipStream_t stream) {
     const bool whole = s.rows % 4 == 0 && reinterpret_cast<uintptr_t>(base) % 16 == 0 &&
                        reinterpret_cast<uintptr_t>(output) % 16 == 0;
@@ -287,7 +303,7 @@ void launch(const AdapterShape& s, const AdapterTiles& tiles, const float* input
         while (each > 64 && tiles.tiles * ((s.rows + each - 1) / each) < 128) each /= 2;
         adapter_both_kernel<T><<<dim3(tiles.tiles, (s.rows + each - 1) / each), kBothWaves * 64, 0, stream>>>(
             s, tiles, input, base, output, each, whole);
-        return;
+        return hipGetLastError();
     }
     // Splits of whole steps of the four waves, for about one workgroup a CU.
     const int steps = (s.columns + kWaves * kStep - 1) / (kWaves * kStep);
@@ -295,8 +311,15 @@ void launch(const AdapterShape& s, const AdapterTiles& tiles, const float* input
     const int per = (steps + want - 1) / want, splits = (steps + per - 1) / per;
     adapter_down_kernel<T><<<dim3(tiles.tiles, ranks, splits), kThreads, 0, stream>>>(s, tiles, input, workspace,
                                                                                                per * kWaves * kStep);
-    adapter_up_kernel<T><<<dim3(tiles.tiles, (s.rows + 255) / 256), kThreads, 16 * (s.rank_most + 4) * sizeof(float),
-                           stream>>>(s, tiles, workspace, base, output, splits, whole);
+    const int lds = 16 * kGroupTiles * (s.rank_most + 4) * static_cast<int>(sizeof(float));
+    if (lds > 64 * 1024)
+        if (const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(adapter_up_kernel<T>),
+                                                     hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+            e != hipSuccess)
+            return e;
+    adapter_up_kernel<T><<<dim3(tiles.groups, (s.rows + 127) / 128), kThreads, lds, stream>>>(s, tiles, workspace, base, output,
+                                                                                             splits, whole);
+    return hipGetLastError();
 }
 
 }  // namespace
@@ -308,8 +331,7 @@ size_t adapter_workspace_bytes(const AdapterShape& s) {
 hipError_t launch_adapters(const AdapterShape& s, const AdapterTiles& tiles, const float* input, const float* base,
                            float* output, float* workspace, hipStream_t stream) {
     if (tiles.tiles == 0) return hipSuccess;
-    (s.type == kF32 ? launch<float> : launch<_Float16>)(s, tiles, input, base, output, workspace, stream);
-    return hipGetLastError();
+    return (s.type == kF32 ? launch<float> : launch<_Float16>)(s, tiles, input, base, output, workspace, stream);
 }
 
 }  // namespace satori

@@ -17,15 +17,17 @@ struct Adapter {
 
 constexpr int kAdapterRows = 256;  // positions of one launch
 constexpr int kMaxAdapters = 65535;
-constexpr int kMaxRank = 512;     // a tile's reduced vectors lie in 33 KB of LDS then
+constexpr int kMaxRank = 512;     // a run of two tiles' reduced vectors lie in 66 KB of LDS then
 
 // The rows of a launch by adapter: tile i is rows order[begin[i]] .. order[begin[i + 1] - 1] (16 at most) of adapter[i],
 // kNoAdapter for rows without one. In the launch's arguments, so a captured launch keeps what it was called with.
 constexpr uint16_t kNoAdapter = 65535;
+constexpr int kGroupTiles = 2;
 struct AdapterTiles {
-    int tiles, positions;
+    int tiles, positions, groups;
     uint8_t order[kAdapterRows];
     uint16_t begin[kAdapterRows + 1], adapter[kAdapterRows];
+    uint16_t group[kAdapterRows + 1];  // runs of at most kGroupTiles tiles of one adapter: tiles group[i] .. group[i + 1] - 1
 };
 
 struct AdapterShape {

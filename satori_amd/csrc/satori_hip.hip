@@ -2555,7 +2555,7 @@ int satori_hip_adapters_create(satori_hip_context* c, int rows, int columns, int
         std::lock_guard<std::mutex> guard(c->lock);
         require_live(c);
         require_not_capturing(c);
-        if (rows <= 0 || rows > (1 << 23)) out_of_range("rows");
+        if (rows <= 0 || rows > (1 << 22)) out_of_range("rows");
         if (columns <= 0 || columns > (1 << 24)) out_of_range("columns");
         if (count <= 0 || count >= kMaxAdapters) out_of_range("count");
         element_type(type);
@@ -2652,6 +2652,12 @@ int satori_hip_adapters_apply(satori_hip_adapters* a, const int* selection, int 
                     tiles.begin[tiles.tiles++] = static_cast<uint16_t>(i);
                 }
                 tiles.begin[tiles.tiles] = static_cast<uint16_t>(i + 1);
+            }
+            for (int i = 0; i < tiles.tiles; ++i) {
+                const int first = tiles.groups ? tiles.group[tiles.groups - 1] : 0;
+                if (i == 0 || tiles.adapter[i] != tiles.adapter[i - 1] || i - first == kGroupTiles)
+                    tiles.group[tiles.groups++] = static_cast<uint16_t>(i);
+                tiles.group[tiles.groups] = static_cast<uint16_t>(i + 1);
             }
             const int64_t at = p0;
             check_hip(launch_adapters(s, tiles, input + at * s.columns, base + at * s.rows, output + at * s.rows,
