@@ -86,9 +86,9 @@ SIGNATURES = {
     "satori_hip_pages_extend": (I, [P, P, P, I, P, P, I, P]),
     "satori_hip_pages_truncate": (I, [P, I, I]),
     "satori_hip_pages_fork": (I, [P, I, I, P]),
-    "satori_hip_pages_copy": (I, [P, I, PI, P, P, I, PI]),
+    "satori_hip_pages_copy": (I, [P, I, PI, P, P, I, P]),
     "satori_hip_pages_free": (I, [P, P, I]),
-    "satori_hip_pages_compact": (I, [P, P, P, I, PI]),
+    "satori_hip_pages_compact": (I, [P, P, P, I, P]),
     "satori_hip_pages_free_count": (I, [P, PI]),
     "satori_hip_pages_sequence": (I, [P, I, P, P, I, P]),
     "satori_hip_cache_page_bytes": (I, [I, I, I, I, I, ctypes.POINTER(ctypes.c_int64)]),

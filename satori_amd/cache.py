@@ -9,6 +9,8 @@ from __future__ import annotations
 
 import ctypes
 import enum
+import threading
+from array import array
 from collections.abc import Sequence
 from dataclasses import dataclass
 
@@ -28,20 +30,46 @@ def _ints(values) -> np.ndarray:
     return np.array(values, dtype=np.int32).reshape(-1)
 
 
-def _at(array: np.ndarray) -> ctypes.c_void_p:
-    return ctypes.c_void_p(array.ctypes.data)
+def _array(values) -> array:
+    """Plain ints for a call: a tenth of the time that numpy takes to make and to locate a short array."""
+    return array("i", values.tolist() if isinstance(values, np.ndarray) else values)
+
+
+def _address(values: array) -> int:
+    return values.buffer_info()[0]
+
+
+def _at(values: np.ndarray) -> ctypes.c_void_p:
+    return ctypes.c_void_p(values.ctypes.data)
 
 
 def _pointer(address: int) -> ctypes.c_void_p:
     return ctypes.c_void_p(address or None)
 
 
+class _Moves:
+    """Page moves of one call: `count` of them, in the caller's arrays of `room` each."""
+
+    def __init__(self, room: int):
+        self.room, self.buffer = room, array("i", bytes(8 * room + 4))
+        self.sources = _address(self.buffer)
+        self.destinations, self.counted = self.sources + 4 * room, self.sources + 8 * room
+
+    @property
+    def count(self) -> int:
+        return self.buffer[2 * self.room]
+
+    def arrays(self) -> tuple[np.ndarray, np.ndarray]:
+        values, n = np.frombuffer(self.buffer, np.int32), self.count
+        return values[:n], values[self.room:self.room + n]
+
+
 class PageTable:
     """Page lists and reference counts of a cache of `page_count` pages (satori_hip_pages): host only. Calls that need
     page bytes to follow return them as moves, (sources, destinations)."""
 
-    # A table's read returns a few dozen page numbers and takes about a microsecond, most of it building ctypes arguments,
-    # so the small calls pass plain addresses of one array per call (of its own: threads may call at once).
+    # A table's read returns a few dozen page numbers and takes about a microsecond, most of it building ctypes arguments
+    # and results, so it passes plain addresses of one buffer, under a lock (threads may call at once).
 
     def __init__(self, page_count: int, page_tokens: int = 32):
         handle = ctypes.c_void_p()
@@ -50,8 +78,10 @@ class PageTable:
         self._handle = handle
         self.page_count, self.page_tokens = page_count, page_tokens
         self._read, self._address = lib.satori_hip_pages_sequence, handle.value
-        self._room = min(page_count, 256)
-        self._array = ctypes.c_int * (self._room + 1)  # and the count
+        self._room = min(page_count, 1024)
+        buffer = np.zeros(self._room + 1, np.int32)  # and the count
+        self._buffer, self._at, self._lock = memoryview(buffer), buffer.ctypes.data, threading.Lock()
+        self._count_at = self._at + 4 * self._room
 
     @property
     def handle(self) -> ctypes.c_void_p:
@@ -62,44 +92,49 @@ class PageTable:
         _check(_ffi.lib().satori_hip_pages_open(self._handle, ctypes.byref(sequence)))
         return sequence.value
 
-    def extend(self, sequences, tokens) -> tuple[np.ndarray, np.ndarray]:
-        ids, counts = _ints(sequences), _ints(tokens)
-        n = ids.size
-        if n != counts.size:
+    def _extend(self, sequences, tokens) -> _Moves:
+        ids, counts = _array(sequences), _array(tokens)
+        n = len(ids)
+        if n != len(counts):
             raise ArgumentException("Lengths differ.")
-        moves = np.empty(2 * n + 1, np.int32)
-        at = moves.ctypes.data
-        _check(_ffi.lib().satori_hip_pages_extend(self._handle, ids.ctypes.data, counts.ctypes.data, n, at, at + 4 * n, n,
-                                                  at + 8 * n))
-        made = int(moves[2 * n])
-        return moves[:made], moves[n:n + made]
+        moves = _Moves(n)
+        _check(_ffi.lib().satori_hip_pages_extend(self._address, _address(ids), _address(counts), n, moves.sources,
+                                                  moves.destinations, n, moves.counted))
+        return moves
+
+    def extend(self, sequences, tokens) -> tuple[np.ndarray, np.ndarray]:
+        return self._extend(sequences, tokens).arrays()
 
     def truncate(self, sequence: int, tokens: int) -> None:
-        _check(_ffi.lib().satori_hip_pages_truncate(self._handle, sequence, tokens))
+        _check(_ffi.lib().satori_hip_pages_truncate(self._address, sequence, tokens))
 
     def fork(self, sequence: int, count: int = 1) -> list[int]:
-        forks = np.empty(max(count, 1), np.int32)
-        _check(_ffi.lib().satori_hip_pages_fork(self._handle, sequence, count, forks.ctypes.data))
+        forks = array("i", bytes(4 * max(count, 1)))
+        _check(_ffi.lib().satori_hip_pages_fork(self._address, sequence, count, _address(forks)))
         return forks[:count].tolist()
 
+    def _copy(self, sequence: int) -> tuple[int, _Moves]:
+        moves, made = _Moves(self._describe(sequence)[1]), ctypes.c_int()
+        _check(_ffi.lib().satori_hip_pages_copy(self._address, sequence, ctypes.byref(made), moves.sources,
+                                                moves.destinations, moves.room, moves.counted))
+        return made.value, moves
+
     def copy(self, sequence: int) -> tuple[int, tuple[np.ndarray, np.ndarray]]:
-        most = self._describe(sequence)[1]
-        sources, destinations = np.empty(most, np.int32), np.empty(most, np.int32)
-        made, moves = ctypes.c_int(), ctypes.c_int()
-        _check(_ffi.lib().satori_hip_pages_copy(self._handle, sequence, ctypes.byref(made), _at(sources),
-                                                _at(destinations), most, ctypes.byref(moves)))
-        return made.value, (sources[:moves.value], destinations[:moves.value])
+        made, moves = self._copy(sequence)
+        return made, moves.arrays()
 
     def free(self, sequences) -> None:
-        ids = _ints(sequences)
-        _check(_ffi.lib().satori_hip_pages_free(self._handle, ids.ctypes.data, ids.size))
+        ids = _array(sequences)
+        _check(_ffi.lib().satori_hip_pages_free(self._address, _address(ids), len(ids)))
+
+    def _compact(self) -> _Moves:
+        moves = _Moves(self.page_count - self.free_pages)
+        _check(_ffi.lib().satori_hip_pages_compact(self._address, moves.sources, moves.destinations, moves.room,
+                                                   moves.counted))
+        return moves
 
     def compact(self) -> tuple[np.ndarray, np.ndarray]:
-        most = self.page_count - self.free_pages
-        sources, destinations, moves = np.empty(most, np.int32), np.empty(most, np.int32), ctypes.c_int()
-        _check(_ffi.lib().satori_hip_pages_compact(self._handle, _at(sources), _at(destinations), most,
-                                                   ctypes.byref(moves)))
-        return sources[:moves.value], destinations[:moves.value]
+        return self._compact().arrays()
 
     @property
     def free_pages(self) -> int:
@@ -117,16 +152,18 @@ class PageTable:
         return self._describe(sequence)[0]
 
     def pages(self, sequence: int) -> list[int]:
-        array, room = self._array(), self._room
-        at = ctypes.addressof(array)
-        status = self._read(self._address, sequence, None, at, room, at + 4 * room)
-        count = array[room]
-        if count > room:  # a long table: a call of its own size
-            array = (ctypes.c_int * count)()
-            status = self._read(self._address, sequence, None, ctypes.addressof(array), count, None)
-        if status:
+        buffer, room = self._buffer, self._room
+        with self._lock:
+            buffer[room] = 0
+            status = self._read(self._address, sequence, None, self._at, room, self._count_at)
+            count = buffer[room]
+            if not status:
+                return buffer[:count].tolist()
+        if count <= room:
             _check(status)
-        return array[:count]
+        table = np.empty(count, np.int32)  # a long table: a call of its own size
+        _check(self._read(self._address, sequence, None, table.ctypes.data, count, None))
+        return table.tolist()
 
     def dispose(self) -> None:
         _check(_ffi.lib().satori_hip_pages_destroy(self._handle))
@@ -150,8 +187,8 @@ class CacheLayout:
 
 
 class PagedCache:
-    """A pool of pages on the device with its page table: the calls of PageTable, with the page bytes moved on the
-    context stream. `pool` is a device pointer to page_count * layout.page_bytes bytes; 0: allocated here."""
+    """A pool of pages on the device with its page table: the calls of PageTable (open, tokens and pages are the table's
+    own), with the page bytes moved on the context stream. `pool` is a device pointer to page_count * layout.page_bytes bytes; 0: allocated here."""
 
     def __init__(self, context: HipContext, layout: CacheLayout, page_count: int, pool: int = 0):
         self.context, self.layout, self.page_count = context, layout, page_count
@@ -161,20 +198,20 @@ class PagedCache:
         if not pool:
             self._owned = pool = context.alloc(page_count * self.page_bytes)
         self.pool = pool
+        self.open, self.pages, self.tokens = self.table.open, self.table.pages, self.table.tokens
 
-    def _move(self, moves: tuple[np.ndarray, np.ndarray]) -> None:
-        sources, destinations = moves
-        if sources.size:
-            _check(_ffi.lib().satori_hip_cache_copy_pages(self.context.handle, self.pool, self.page_bytes, self.page_count,
-                                                          sources.ctypes.data, destinations.ctypes.data, sources.size,
-                                                          None))
+    def _move(self, moves: _Moves) -> None:
+        if moves.count:
+            self.copy_pages(moves.sources, moves.destinations, moves.count)
 
-    def open(self) -> int:
-        return self.table.open()
+    def copy_pages(self, sources: int, destinations: int, count: int) -> None:
+        """Pool page destinations[i] = pool page sources[i], from host arrays at these addresses."""
+        _check(_ffi.lib().satori_hip_cache_copy_pages(self.context.handle, self.pool, self.page_bytes, self.page_count,
+                                                      sources, destinations, count, None))
 
     def extend(self, sequences, tokens) -> None:
         """Makes room for tokens[i] more positions of sequences[i]."""
-        self._move(self.table.extend(sequences, tokens))
+        self._move(self.table._extend(sequences, tokens))
 
     def truncate(self, sequence: int, tokens: int) -> None:
         self.table.truncate(sequence, tokens)
@@ -183,7 +220,7 @@ class PagedCache:
         return self.table.fork(sequence, count)
 
     def copy(self, sequence: int) -> int:
-        made, moves = self.table.copy(sequence)
+        made, moves = self.table._copy(sequence)
         self._move(moves)
         return made
 
@@ -191,13 +228,7 @@ class PagedCache:
         self.table.free(sequences)
 
     def compact(self) -> None:
-        self._move(self.table.compact())
-
-    def tokens(self, sequence: int) -> int:
-        return self.table.tokens(sequence)
-
-    def pages(self, sequence: int) -> list[int]:
-        return self.table.pages(sequence)
+        self._move(self.table._compact())
 
     @property
     def free_pages(self) -> int:

@@ -375,6 +375,11 @@ def test_append_equals_the_single_sequence_operator(context, device, type_, head
 
 # ---- page copies ----
 
+def copy_pages(cache, sources, destinations):
+    s, d = np.array(sources, np.int32), np.array(destinations, np.int32)
+    cache.copy_pages(s.ctypes.data, d.ctypes.data, s.size)
+
+
 @pytest.mark.parametrize("layers,pages", [(1, 3), (5, 700)])
 def test_page_copies(context, device, layers, pages):
     layout = CacheLayout(layers, 1, 32, 32, F16)
@@ -385,7 +390,7 @@ def test_page_copies(context, device, layers, pages):
     order = g.permutation(pages)
     destinations = order[:pages // 2]
     sources = g.choice(order[pages // 2:], destinations.size)  # one page can go to several places
-    pool.cache._move((sources.astype(np.int32), destinations.astype(np.int32)))
+    copy_pages(pool.cache, sources, destinations)
     expected = pool.host.view(np.uint16).copy()
     expected[destinations] = expected[sources]
     assert np.array_equal(pool.download().host.view(np.uint16), expected)
@@ -564,10 +569,10 @@ def test_refusals(context, device):
     context.capture_end().dispose()
     for moves in (([0], [0]), ([0, 1], [2, 2]), ([0, 1], [1, 2])):
         with pytest.raises(S.ArgumentException):
-            c._move(tuple(np.array(m, np.int32) for m in moves))
+            copy_pages(c, *moves)
     for moves in (([8], [0]), ([0], [8]), ([-1], [0])):
         with pytest.raises(S.ArgumentOutOfRangeException):
-            c._move(tuple(np.array(m, np.int32) for m in moves))
+            copy_pages(c, *moves)
     with pytest.raises(S.ArgumentException):
         PagedCache(context, layout, 8, pool.at + 4).plan(4)
     for heads in (3, 0, -2):
