@@ -41,9 +41,10 @@ static_assert(SATORI_HIP_Q8_0 == satori::kQ8_0 && SATORI_HIP_Q4_0 == satori::kQ4
               "format codes");
 
 void check_hip(hipError_t e, const char* what) {
-    if (e != hipSuccess)
-        fail(e == hipErrorOutOfMemory ? SATORI_HIP_E_OUT_OF_MEMORY : SATORI_HIP_E_DEVICE,
-             std::string(what) + ": " + hipGetErrorString(e));
+    if (e == hipSuccess) return;
+    (void)hipGetLastError();  // told here: the next launch's check must not find it
+    fail(e == hipErrorOutOfMemory ? SATORI_HIP_E_OUT_OF_MEMORY : SATORI_HIP_E_DEVICE,
+         std::string(what) + ": " + hipGetErrorString(e));
 }
 
 // While it lives, this thread's allocations neither fail because of a stream capture in progress (another library's in
@@ -2346,7 +2347,6 @@ void free_plan(satori_hip_cache_plan* p) {
 
 // What the calls on a plan ask of it, and whether the launch becomes part of a captured step.
 bool note_plan(satori_hip_context* c, satori_hip_cache_plan* p, int layer, hipStream_t stream) {
-    if (!p->set) fail(SATORI_HIP_E_INVALID_OPERATION, "Set the plan's batch first.");
     if (layer < 0 || layer >= p->layers) out_of_range("layer");
     const bool captured = c->capturing && stream == c->stream;
     if (captured) c->captured_plans.push_back(p);
@@ -2480,6 +2480,7 @@ int satori_hip_cache_plan_set(satori_hip_cache_plan* p, satori_hip_pages* pages,
         const PlanLayout used = image.least();
         if (layout.grow(used) && p->steps > 0) plan_held();
         const size_t bytes = static_cast<size_t>(layout.words) * 4;
+        p->set = false;  // until the new batch is on its way: where memory cannot be had, the old one's may be gone
         reserve_for_plan(p, p->image, bytes);
         reserve_for_plan(p, p->partials, cache_partial_bytes(p->shape, image.header.slots));
         const int turn = p->turn;
@@ -2534,6 +2535,7 @@ int satori_hip_cache_attention(satori_hip_cache_plan* p, int layer, const float*
         require(output, "output");
         const CacheShape& s = p->shape;
         const hipStream_t st = op_stream(c, stream);
+        if (!p->set) fail(SATORI_HIP_E_INVALID_OPERATION, "Set the plan's batch first.");
         const int64_t bytes = static_cast<int64_t>(p->header.rows) * s.heads * s.head_dim * 4;
         const int64_t pool = s.page_bytes * p->page_count;
         if (bytes_overlap(query, bytes, output, bytes) || bytes_overlap(output, bytes, s.pool, pool))

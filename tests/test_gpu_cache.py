@@ -610,3 +610,26 @@ def test_a_step_keeps_its_plans_memory(context, device):
     step.dispose()
     plan.set(others, [1] * 3000)
     plan.dispose()
+
+
+def test_a_batch_whose_memory_cannot_be_had_leaves_no_plan(context, device):
+    # The partial results of 500,000 rows of 512 heads take 264 GB and half as much again; only page 0 is behind the pool, and
+    # nothing is launched on others.
+    layout = CacheLayout(1, 512, 256, 256, F16)
+    first = PagedCache(context, layout, 1)
+    cache = PagedCache(context, layout, 2100, first.pool)
+    small, large = cache.open(), cache.open()
+    cache.extend([small], [1])
+    cache.extend([large], [500000])
+    plan = cache.plan(512)
+    q, out = device(np.ones((1, 512 * 256), np.float32)), device(np.zeros((1, 512 * 256), np.float32))
+    plan.set([small], [1])
+    with pytest.raises(S.OutOfMemoryException):
+        plan.set([large], [500000])
+    for call in (lambda: plan.attention(0, q, out), lambda: plan.append(0, q, 0, out, q, 0, q, 0, 1e4, 256)):
+        with pytest.raises(S.InvalidOperationException):
+            call()
+    plan.set([small], [1])  # the plan can be set again
+    plan.dispose()
+    cache.dispose()
+    first.dispose()
