@@ -479,10 +479,13 @@ int satori_hip_cache_copy_pages(satori_hip_context* context, void* pool, int64_t
  * pages as they were when it was set: set it again after any change to its sequences and after a compaction. The copy to
  * the device is enqueued on `stream`, so the launches that read it must follow on that stream (or be ordered by the
  * caller); not while capturing. A captured step reads the plan when it is replayed: capture a step once, then extend, set
- * and replay it per token, with as many rows as its other launches were captured with. While steps read a plan, a batch
- * that needs more memory than the largest before fails with SATORI_HIP_E_INVALID_OPERATION. Each plan owns the workspace
- * of its attention, so calls on one plan must not overlap in time on different streams; different plans may. The pool must
- * be 16-byte aligned and outlive the plan; destroy plans before their context. */
+ * and replay it per token, with as many rows as its other launches were captured with (the buffers that the captured calls
+ * were given must hold every later batch's rows). While steps read a plan, a batch that needs more memory than the largest
+ * before fails with SATORI_HIP_E_INVALID_OPERATION, and so does one whose rows lie in shared pages if a step writes them; the
+ * plan stays as it was. After a call in another library's capture the plan is read by that graph until the plan is destroyed
+ * (which must come after the graph's end). Each plan owns the workspace of its attention, so calls on one plan must not
+ * overlap in time on different streams; different plans may. After a set that failed for memory or on the device, calls
+ * fail until one succeeds. The pool must be 16-byte aligned and outlive the plan; destroy plans before their context. */
 int satori_hip_cache_plan_create(satori_hip_context* context, void* pool, int page_count, int layers, int query_heads,
                                  int kv_heads, int head_dim, int page_tokens, int type, satori_hip_cache_plan** plan);
 int satori_hip_cache_plan_set(satori_hip_cache_plan* plan, satori_hip_pages* pages, const int* sequences,
@@ -502,9 +505,10 @@ int satori_hip_cache_append(satori_hip_cache_plan* plan, int layer, const float*
 /* GroupedAttention (src/Satori.Core/TransformerOps.cs:135-179) of every row over the positions of its sequence up to its
  * own. Pages that several sequences of the batch hold are read once for all of them: the tables are divided where they
  * part, each part is attended by the rows below it, and the partial results are joined. FP32 scores, maxima and sums
- * (the single-sequence attention's are FP64); of F16 pages every bit is used, and queries and probabilities keep 22. A row
- * that sees a key or value that is not finite gives outputs that are not finite (NaN where the definition may give an
- * infinity); what a row does not see never reaches it. query and output [rows][query_heads * head_dim], not overlapping. */
+ * (the single-sequence attention's are FP64); of F16 pages every bit is used, and queries and probabilities keep 22, down to
+ * 2^-36 of a row's largest probability. Where a row sees a key or value that is not finite, its outputs may be NaN where the
+ * definition gives an infinity or a weight of zero; what a row does not see never reaches it. query and output
+ * [rows][query_heads * head_dim], not overlapping. */
 int satori_hip_cache_attention(satori_hip_cache_plan* plan, int layer, const float* query, float* output, void* stream);
 
 /* ---- low-rank adapters of many requests beside one projection ----

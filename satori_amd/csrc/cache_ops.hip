@@ -177,12 +177,13 @@ __global__ __launch_bounds__(kThreads) void cache_append_kernel(CacheShape s, co
 // group g the tokens 8 g .. 8 g + 7; F32: row m of tile a is token 16 * a + m).
 //
 // F16 keys and values are exact in the matrix instructions; what they meet is not, so queries and probabilities go in as
-// two halves of 11 bits, x = hi + lo, both products summed in the same FP32 accumulator: 2^-22 of a value is lost. Their
-// scale is a power of two that puts the largest query lane of a pair at 2^14 and a probability of one between 2^6 and 2^14,
-// far from where halves lose bits. F32 caches use the FP32 matrix instructions.
+// two halves of 11 bits, x = hi + lo, both products summed in the same FP32 accumulator. A power of two puts the largest
+// query lane of a pair at 2^14 and its largest probability at 2^11 or more (2^15 at most), so that what is lost of either is
+// 2^-22 of the value, or 2^-39 of the largest lane and 2^-36 of the largest probability where that is more (half a step of
+// the smallest half). F32 caches use the FP32 matrix instructions.
 
 constexpr int kTile = 32;  // tokens that a wave attends at once
-constexpr float kSlack = 8.0f;
+constexpr float kSlack = 4.0f;
 constexpr float kLog2e = 1.44269504088896340736f;
 
 // Maximum and sum over the four lanes that hold one column (lane, lane ^ 16, lane ^ 32, lane ^ 48).
@@ -222,7 +223,7 @@ struct Math;
 
 template <int W>
 struct Math<_Float16, W> {
-    static constexpr float kTop = 6.0f;         // log2 of a probability of one, as the second product takes it
+    static constexpr float kTop = 11.0f;        // log2 of a probability of one, as the second product takes it
     static constexpr int kKeyParts = W / 32;    // fragments of a key tile's 16 rows, of a value tile's 16 lanes
     static constexpr int kValueParts = 1;
     typedef f16x8 Fragment;                     // 16 bytes: lanes 32 s + 8 g .. of a key, tokens 8 g .. of a value lane
@@ -337,7 +338,8 @@ struct Softmax {
                           fmaxf(fmaxf(score[1][0], score[1][1]), fmaxf(score[1][2], score[1][3])));
         top = column_max(top) * factor;
         // The maximum may fall behind by a factor of 2^kSlack before everything is scaled again (in the first tiles of random
-        // scores some pair of a wave has a new maximum almost every time).
+        // scores some pair of a wave has a new maximum almost every time; 2^8 gives no more than 2^4, and leaves small
+        // probabilities fewer bits).
         if (__any(top > m + kSlack)) {
             const float now = fmaxf(m, top);
             const float shrink = __builtin_amdgcn_exp2f(m - (now == -INFINITY ? 0.0f : now));
@@ -1021,7 +1023,7 @@ hipError_t launch_cache_append(const CacheShape& s, const int* image, const Plan
     const int64_t turns = static_cast<int64_t>(longest) * (s.heads + s.kv_heads) * (args.rotary / (packed ? 8 : 2));
     const int64_t values = (static_cast<int64_t>(longest) / kGroupTokens + 1) * s.kv_heads * s.head_dim;
     const int y = static_cast<int>(std::min<int64_t>((std::max(turns, values) + kThreads - 1) / kThreads, 1024));
-    const dim3 grid(all ? 256 : now.runs, y);
+    const dim3 grid(all ? 256 : std::min(now.runs, 1 << 16), y);
     const auto launch = [&](auto kernel) { kernel<<<grid, kThreads, 0, stream>>>(s, image, layout.runs_at, args); };
     if (s.type == kF32)
         packed ? launch(cache_append_kernel<float, 4>) : launch(cache_append_kernel<float, 1>);
@@ -1052,7 +1054,7 @@ hipError_t launch_cache_attention(const CacheShape& shape, const int* image, con
                           Partials{partials, room},
                           scale,
                           shape.head_dim % 4 == 0 && reinterpret_cast<uintptr_t>(query) % 16 == 0};
-    const int groups = all ? kMostGroups : now.wide + now.narrow;
+    const int groups = all ? kMostGroups : std::min(now.wide + now.narrow, 1 << 20);
     const hipError_t e = of_shape(shape.type, shape.width, [&](auto t, auto w) {
         return attention_of_width<decltype(t), decltype(w)::value>(a, groups, stream);
     });

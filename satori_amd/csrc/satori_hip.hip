@@ -203,6 +203,8 @@ struct satori_hip_cache_plan {
     hipEvent_t copied[2] = {nullptr, nullptr};
     int turn = 0;
     int steps = 0;                   // captured steps that read the plan
+    bool elsewhere = false;          // another library's graph may read it (until the plan is destroyed: its end is not told)
+    bool appended = false;           // by a captured launch
     bool live = true;
 };
 
@@ -1624,7 +1626,8 @@ int satori_hip_step_destroy(satori_hip_step* s) {
         }
         if (s->attention) c->attention_steps--;
         s->attention = false;
-        for (satori_hip_cache_plan* p : s->plans) p->steps--;
+        for (satori_hip_cache_plan* p : s->plans)
+            if (--p->steps == 0) p->appended = p->elsewhere && p->appended;
         for (satori_hip_adapters* a : s->adapters) a->steps--;
         s->plans.clear();
         s->adapters.clear();
@@ -2282,7 +2285,7 @@ CacheShape cache_shape(int layers, int query_heads, int kv_heads, int head_dim, 
     s.head_dim = head_dim;
     s.page_tokens = page_tokens;
     while (1 << s.page_shift < page_tokens) ++s.page_shift;
-    const int64_t row = static_cast<int64_t>(kv_heads) * s.width, head = static_cast<int64_t>(query_heads) * head_dim;
+    const int64_t row = static_cast<int64_t>(kv_heads) * s.width, head = static_cast<int64_t>(query_heads) * s.width;
     if (row > INT32_MAX / 512 || head > INT32_MAX / 512)
         fail(SATORI_HIP_E_OVERFLOW, "Arithmetic operation resulted in an overflow.");
     s.layer_bytes = 2 * row * page_tokens * element_bytes(type);
@@ -2327,11 +2330,13 @@ int plan_call(satori_hip_cache_plan* p, F&& body) {
          "before capturing.");
 }
 
-// Grows a buffer of the plan, unless a captured step reads it.
+bool held(const satori_hip_cache_plan* p) { return p->steps > 0 || p->elsewhere; }
+
+// Grows a buffer of the plan, unless a graph reads it. (Freeing the old one waits for the launches that read it, on any
+// stream.)
 void reserve_for_plan(satori_hip_cache_plan* p, DeviceBuffer& buffer, size_t need) {
     if (need <= buffer.bytes) return;
-    if (p->steps > 0) plan_held();
-    check_hip(hipDeviceSynchronize(), "device");  // earlier launches on any stream may read the old one
+    if (held(p)) plan_held();
     buffer.reserve(need + need / 2);
 }
 
@@ -2349,8 +2354,13 @@ void free_plan(satori_hip_cache_plan* p) {
 bool note_plan(satori_hip_context* c, satori_hip_cache_plan* p, int layer, hipStream_t stream) {
     if (layer < 0 || layer >= p->layers) out_of_range("layer");
     const bool captured = c->capturing && stream == c->stream;
-    if (captured) c->captured_plans.push_back(p);
-    return captured || captured_elsewhere(c, stream);
+    if (captured) {
+        c->captured_plans.push_back(p);
+        return true;
+    }
+    if (!captured_elsewhere(c, stream)) return false;
+    p->elsewhere = true;
+    return true;
 }
 
 }  // namespace
@@ -2369,7 +2379,8 @@ int satori_hip_cache_copy_pages(satori_hip_context* c, void* pool, int64_t page_
     return op_call(c, [&] {
         require_pool(pool);
         if (page_count <= 0) out_of_range("pageCount");
-        if (page_bytes <= 0 || page_bytes % 16 != 0 || page_bytes > (int64_t(1) << 40)) out_of_range("pageBytes");
+        if (page_bytes <= 0 || page_bytes % 16 != 0 || page_bytes > (int64_t(1) << 36)) out_of_range("pageBytes");
+        if (page_bytes > INT64_MAX / page_count) fail(SATORI_HIP_E_OVERFLOW, "Arithmetic operation resulted in an overflow.");
         if (count < 0 || count > page_count) out_of_range("count");
         if (count == 0) return;
         require(sources, "sources");
@@ -2476,10 +2487,16 @@ int satori_hip_cache_plan_set(satori_hip_cache_plan* p, satori_hip_pages* pages,
         }
         if (static_cast<int64_t>(image.header.rows) * p->shape.heads > INT32_MAX / 4)
             fail(SATORI_HIP_E_OVERFLOW, "Arithmetic operation resulted in an overflow.");
+        if (!image.writable && p->appended && held(p))
+            fail(SATORI_HIP_E_INVALID_OPERATION,
+                 "A captured step writes the rows, which lie in pages that other sequences hold: extend their sequences.");
         PlanLayout layout = p->layout;
         const PlanLayout used = image.least();
-        if (layout.grow(used) && p->steps > 0) plan_held();
+        if (layout.grow(used) && held(p)) plan_held();
         const size_t bytes = static_cast<size_t>(layout.words) * 4;
+        if (held(p) && (bytes > p->image.bytes || cache_partial_bytes(p->shape, image.header.slots) > p->partials.bytes))
+            plan_held();
+        const CaptureRelaxed relaxed;  // another stream may be in a capture that forbids allocations
         p->set = false;  // until the new batch is on its way: where memory cannot be had, the old one's may be gone
         reserve_for_plan(p, p->image, bytes);
         reserve_for_plan(p, p->partials, cache_partial_bytes(p->shape, image.header.slots));
@@ -2522,6 +2539,7 @@ int satori_hip_cache_append(satori_hip_cache_plan* p, int layer, const float* qu
             bytes_overlap(value, kb, s.pool, pool))
             fail(SATORI_HIP_E_ARGUMENT, "Partial overlap.");
         const bool captured = note_plan(c, p, layer, st);
+        p->appended |= captured;
         const AppendArgs args{query, query_bias, key, key_bias, value, value_bias, query_out, frequency_base,
                               rotary_dimensions, rope_table, rope_table ? rope_positions : 0, layer};
         check_hip(launch_cache_append(s, static_cast<const int*>(p->image.ptr), p->layout, p->header, captured, args, st),

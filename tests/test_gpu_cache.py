@@ -9,6 +9,8 @@ instruction: (T / 32 + 64) e, and 16 e for probabilities in two halves, exp2 and
 |o - exact| <= (2 (D + 8) e max A + 2 (T / 32 + 80) e) * sum p |v|, which the tests take times 1.01 (second order)."""
 from __future__ import annotations
 
+import ctypes
+
 import numpy as np
 import pytest
 
@@ -633,3 +635,183 @@ def test_a_batch_whose_memory_cannot_be_had_leaves_no_plan(context, device):
     plan.dispose()
     cache.dispose()
     first.dispose()
+
+
+@pytest.mark.parametrize("type_,heads,kv,D", [(F32, 16, 1, 128), (F16, 12, 2, 192), (F32, 3, 1, 200)])
+def test_the_largest_tiles_captured_first(type_, heads, kv, D):
+    # Kernels that take more than 64 KB of LDS, launched by a capture before any eager call of theirs (a context of its own;
+    # the process may have run them before), then replayed as the sequences grow, against eager calls on another plan.
+    g = rng(77)
+    context = S.HipContext(0)
+    device = Device(context)
+    pool = Pool(context, device, CacheLayout(1, kv, D, 64, type_), 40)
+    c = pool.cache
+    first = c.open()
+    c.extend([first], [300])
+    sequences = [first] + c.fork(first, 2)
+    c.extend(sequences, [9, 1, 3])
+    pool.write(g, sequences)
+    new = [9, 1, 3]
+    q, out, eager_out = (device(g.standard_normal((13, heads, D)).astype(np.float32)) for _ in range(3))
+    plan, other = c.plan(heads), c.plan(heads)
+    plan.set(sequences, new)
+    context.capture_begin()
+    plan.attention(0, q, out)
+    step = context.capture_end()
+    for turn in range(3):
+        step.execute()
+        got = context.download(np.zeros((13, heads, D), np.float32), out)
+        other.set(sequences, new)
+        other.attention(0, q, eager_out)
+        assert np.array_equal(got, context.download(np.zeros((13, heads, D), np.float32), eager_out)), turn
+        check_attention(pool, sequences, new, heads, context.download(np.zeros((13, heads, D), np.float32), q), got)
+        c.extend(sequences, [40, 70, 5])
+        pool.download().write(g, sequences)
+        plan.set(sequences, new)
+    step.dispose()
+    plan.dispose()
+    other.dispose()
+    device.close()
+    context.dispose()
+
+
+def test_another_librarys_capture(context, device):
+    # The plan cannot know when such a graph ends: its memory stays where it is from then on. While the capture lasts (in the
+    # global mode, which forbids allocations), another plan grows and runs on the context stream.
+    hip = ctypes.CDLL("libamdhip64.so")
+    P = ctypes.c_void_p
+    hip.hipStreamCreateWithFlags.argtypes = [ctypes.POINTER(P), ctypes.c_uint]
+    hip.hipStreamBeginCapture.argtypes = [P, ctypes.c_int]
+    hip.hipStreamEndCapture.argtypes = [P, ctypes.POINTER(P)]
+    hip.hipGraphInstantiate.argtypes = [ctypes.POINTER(P), P, P, P, ctypes.c_size_t]
+    hip.hipGraphLaunch.argtypes = [P, P]
+    hip.hipStreamSynchronize.argtypes = hip.hipStreamDestroy.argtypes = [P]
+    hip.hipGraphExecDestroy.argtypes = hip.hipGraphDestroy.argtypes = [P]
+    g = rng(78)
+    pool = Pool(context, device, CacheLayout(1, 1, 32, 32, F16), 4000)
+    c = pool.cache
+    s = c.open()
+    c.extend([s], [50])
+    others = [c.open() for _ in range(3000)]
+    c.extend(others, [1] * 3000)
+    pool.write(g, [s] + others)
+    plan, other = c.plan(4), c.plan(4)
+    plan.set([s], [1])
+    q, out = device(g.standard_normal((1, 4, 32)).astype(np.float32)), device(np.zeros((1, 4, 32), np.float32))
+    many = g.standard_normal((3000, 4, 32)).astype(np.float32)
+    q_many, out_many = device(many), device(np.zeros_like(many))
+    foreign, graph, exe = P(), P(), P()
+    context.synchronize()
+    assert hip.hipStreamCreateWithFlags(ctypes.byref(foreign), 1) == 0
+    try:
+        assert hip.hipStreamBeginCapture(foreign, 0) == 0  # global
+        try:
+            plan.attention(0, q, out, foreign.value)
+            other.set(others, [1] * 3000)
+            other.attention(0, q_many, out_many)
+        finally:
+            ended = hip.hipStreamEndCapture(foreign, ctypes.byref(graph))
+        assert ended == 0
+        check_attention(pool, others, [1] * 3000, 4, many, context.download(np.zeros_like(many), out_many))
+        assert hip.hipGraphInstantiate(ctypes.byref(exe), graph, None, None, 0) == 0
+        with pytest.raises(S.InvalidOperationException):
+            plan.set(others, [1] * 3000)
+        for replay in range(3):
+            context.upload(out, np.zeros((1, 4, 32), np.float32))
+            context.synchronize()
+            assert hip.hipGraphLaunch(exe, foreign) == 0
+            assert hip.hipStreamSynchronize(foreign) == 0
+            got = context.download(np.zeros((1, 4, 32), np.float32), out)
+            check_attention(pool, [s], [1], 4, context.download(np.zeros((1, 4, 32), np.float32), q), got, label=f"{replay}")
+            c.extend([s], [60])
+            pool.write(g, [s])
+            plan.set([s], [1])
+        hip.hipGraphExecDestroy(exe)
+        hip.hipGraphDestroy(graph)
+    finally:
+        hip.hipStreamDestroy(foreign)
+    plan.dispose()
+    other.dispose()
+
+
+def test_a_captured_write_keeps_to_pages_of_its_own(context, device):
+    pool = Pool(context, device, CacheLayout(1, 1, 32, 32, F16), 8)
+    c = pool.cache
+    s = c.open()
+    c.extend([s], [40])
+    plan = c.plan(1)
+    plan.set([s], [1])
+    q, out = device(np.zeros((1, 32), np.float32)), device(np.zeros((1, 32), np.float32))
+    context.capture_begin()
+    plan.append(0, q, 0, out, q, 0, q, 0, 1e4, 32)
+    step = context.capture_end()
+    other = c.fork(s)[0]
+    with pytest.raises(S.InvalidOperationException):  # the replay would write the page that both hold
+        plan.set([s, other], [1, 0])
+    c.extend([s], [1])
+    plan.set([s, other], [1, 0])
+    step.dispose()
+    context.capture_begin()
+    plan.attention(0, q, out)
+    step = context.capture_end()
+    plan.set([other], [1])
+    c.free([s])
+    s = c.fork(other)[0]
+    plan.set([s], [1])  # nothing is written
+    step.dispose()
+    plan.dispose()
+
+
+def test_sizes_that_overflow(context, device):
+    for heads, kv, D in ((1 << 20, 1, 8), (1 << 20, 1 << 20, 8)):
+        with pytest.raises(S.OverflowException):
+            PagedCache(context, CacheLayout(1, 1, D, 32, F16), 4, 16).plan(heads) if kv == 1 else \
+                CacheLayout(1, kv, D, 32, F16).page_bytes
+    lib = S._ffi.lib()
+    a = np.zeros(1, np.int32)
+    from satori_amd import _check
+    for page_bytes, pages in ((1 << 37, 1), (1 << 36, 1 << 30), (24, 4), (0, 4)):
+        with pytest.raises((S.OverflowException, S.ArgumentOutOfRangeException)):
+            _check(lib.satori_hip_cache_copy_pages(context.handle, 16, page_bytes, pages, a.ctypes.data, a.ctypes.data, 1, None))
+
+
+@pytest.mark.parametrize("type_", [F16, F32])
+@pytest.mark.parametrize("new", [1, 40])
+def test_small_weights_beside_one_that_takes_all(context, device, type_, new):
+    # One key has all the weight and a value of zero; the others' weights are 2^-22 of its, and make the output. Its score is
+    # one product of 1 and 122 (exact) over 8, off by less than 8 e 15.25 of the factor's and the subtraction's roundings; the
+    # others' as in the module's bound. Of F16 pages a weight in two halves is off by half a step of the smallest half, 2^-25,
+    # where the largest is at least 2^11: 2^-36 of it.
+    g = rng(41)
+    heads, D, tokens = 4, 64, 80
+    pool = Pool(context, device, CacheLayout(1, 1, D, 32, type_), 4)
+    s = pool.cache.open()
+    pool.cache.extend([s], [tokens])
+    pool.write(g, [s])
+    first = pool.cache.pages(s)[0]
+    pool.keys(0)[..., 0] = 0
+    pool.keys(0)[first, 0, 0] = 0
+    pool.keys(0)[first, 0, 0, 0] = 122
+    pool.values(0)[first, 0, :, 0] = 0
+    pool.upload()
+    q = (g.standard_normal((new, heads, D)) / 4).astype(np.float32)
+    q[..., 0] = 1
+    plan = pool.cache.plan(heads)
+    plan.set([s], [new])
+    out = device(np.zeros_like(q))
+    plan.attention(0, device(q), out)
+    got = context.download(np.zeros_like(q), out)
+    k, v = pool.of(s, 0)
+    for row in range(new):
+        n = tokens - new + row + 1
+        for h in range(heads):
+            scores = k[:n, 0] @ q[row, h].astype(np.float64) / 8
+            p = np.exp(scores - scores.max())
+            p /= p.sum()
+            a = (np.abs(k[1:n, 0]) @ np.abs(q[row, h].astype(np.float64))).max() / 8
+            bound = 1.01 * E * (2 * (8 * 15.25 + (D + 8) * a) + 2 * (n / 32 + 80)) * (p @ np.abs(v[:n, 0]))
+            if type_ == F16:
+                bound = bound + 1.01 * 2.0 ** -36 * np.abs(v[:n, 0]).sum(0)
+            err = np.abs(got[row, h] - p @ v[:n, 0])
+            assert np.all(err <= bound), (row, h, (err / bound).max())
+    plan.dispose()
