@@ -186,12 +186,15 @@ constexpr int kTile = 32;  // tokens that a wave attends at once
 constexpr float kSlack = 4.0f;
 constexpr float kLog2e = 1.44269504088896340736f;
 
+// The larger one, NaN where either is: one instruction for three numbers, where fmaxf first quiets each of them.
+__device__ __forceinline__ float larger(float a, float b) { return __builtin_elementwise_maximum(a, b); }
+
 // Maximum and sum over the four lanes that hold one column (lane, lane ^ 16, lane ^ 32, lane ^ 48).
 __device__ __forceinline__ float column_max(float v) {
     auto p = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-    v = fmaxf(__uint_as_float(p[0]), __uint_as_float(p[1]));
+    v = larger(__uint_as_float(p[0]), __uint_as_float(p[1]));
     p = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-    return fmaxf(__uint_as_float(p[0]), __uint_as_float(p[1]));
+    return larger(__uint_as_float(p[0]), __uint_as_float(p[1]));
 }
 __device__ __forceinline__ float column_sum(float v) {
     v += __shfl_xor(v, 16, 64);
@@ -215,6 +218,12 @@ __device__ __forceinline__ void load_lanes(const float* row, int d, int head_dim
             }
         }
     }
+}
+
+__device__ __forceinline__ float unknown_minus_one() {
+    float v = -1.0f;
+    __asm__("" : "+s"(v));
+    return v;
 }
 
 // The arithmetic of an element type: W lanes a head. Lane (c, g) = (lane % 16, lane / 16).
@@ -247,7 +256,7 @@ struct Math<_Float16, W> {
 #pragma unroll
         for (int s = 0; s < W / 32; ++s)
 #pragma unroll
-            for (int j = 0; j < 8; ++j) top = fmaxf(top, fabsf(x[s][j]));
+            for (int j = 0; j < 8; ++j) top = larger(top, fabsf(x[s][j]));
         top = column_max(top);
         const int exponent = static_cast<int>(__float_as_uint(top) >> 23) - 127;
         const int shift = top > 0 && exponent < 128 ? (14 - exponent < 100 ? 14 - exponent : 100) : 0;
@@ -266,13 +275,15 @@ struct Math<_Float16, W> {
         return __builtin_amdgcn_mfma_f32_16x16x32_f16(k, term ? q.lo[s] : q.hi[s], sum, 0, 0, 0);
     }
     static __device__ __forceinline__ void weights(const float (&p)[8], Weights& w) {
+        // High halves in pairs, as the conversion takes them; a low one is a single mixed multiply-add, (-1) hi + p rounded to
+        // a half (with a factor that the compiler knows it becomes three instructions).
+        const float minus = unknown_minus_one();
 #pragma unroll
-        for (int i = 0; i < 8; i += 2) {  // in pairs, as the conversion takes them; the difference is one mixed multiply-add
+        for (int i = 0; i < 8; i += 2) {
             const f16x2 hi = __builtin_convertvector((f32x2{p[i], p[i + 1]}), f16x2);
-            const f32x2 rest{__fmaf_rn(static_cast<float>(hi[0]), -1.0f, p[i]), __fmaf_rn(static_cast<float>(hi[1]), -1.0f, p[i + 1])};
-            const f16x2 lo = __builtin_convertvector(rest, f16x2);
             w.hi[i] = hi[0], w.hi[i + 1] = hi[1];
-            w.lo[i] = lo[0], w.lo[i + 1] = lo[1];
+            w.lo[i] = static_cast<_Float16>(__builtin_fmaf(static_cast<float>(hi[0]), minus, p[i]));
+            w.lo[i + 1] = static_cast<_Float16>(__builtin_fmaf(static_cast<float>(hi[1]), minus, p[i + 1]));
         }
     }
     static __device__ __forceinline__ f32x4 weigh(Fragment v, const Weights& w, int, int term, f32x4 sum) {
@@ -334,13 +345,14 @@ struct Softmax {
     }
     // Takes a tile's scores (as they leave the first product) and gives their weights.
     __device__ __forceinline__ void take(const f32x4 (&score)[2], float factor, float top_weight, float (&p)[8]) {
-        float top = fmaxf(fmaxf(fmaxf(score[0][0], score[0][1]), fmaxf(score[0][2], score[0][3])),
-                          fmaxf(fmaxf(score[1][0], score[1][1]), fmaxf(score[1][2], score[1][3])));
-        top = column_max(top) * factor;
+        float top = larger(larger(score[0][0], score[0][1]), score[0][2]);
+        top = larger(larger(top, score[0][3]), score[1][0]);
+        top = larger(larger(larger(top, score[1][1]), score[1][2]), score[1][3]) * factor;
         // The maximum may fall behind by a factor of 2^kSlack before everything is scaled again (in the first tiles of random
         // scores some pair of a wave has a new maximum almost every time; 2^8 gives no more than 2^4, and leaves small
         // probabilities fewer bits).
         if (__any(top > m + kSlack)) {
+            top = column_max(top);
             const float now = fmaxf(m, top);
             const float shrink = __builtin_amdgcn_exp2f(m - (now == -INFINITY ? 0.0f : now));
             m = now;
@@ -698,23 +710,28 @@ __device__ __forceinline__ void attend_many(const AttentionArgs& a, const PlanIt
     const bool idle = 16 * NB * wave >= item.pairs;  // a wave without pairs only carries
     uint32_t* spoiled = reinterpret_cast<uint32_t*>(lds + S::kSpoiledAt);  // [2][W]
 
+    // Where its pieces go and come from stays in a thread's registers from tile to tile if they are few.
+    const auto of_thread = [&] { return S::kPer > 8 ? unknown(thread) : thread; };
     const auto fetch = [&](int page, int tile, u32x4 (&moved)[S::kPer]) {
+        const int thread = of_thread();
         const int within = pages.within(tile * kTile);
+        const uint8_t* keys = pages.keys(page) + within * (W * static_cast<int>(sizeof(T)));
+        const uint8_t* values = pages.values(page) + within * static_cast<int>(sizeof(T));
 #pragma unroll
         for (int i = 0; i < S::kPer; ++i) {
             const int piece = thread + i * kThreads;
             if (S::kPieces % kThreads != 0 && piece >= S::kPieces) continue;
-            const uint8_t* from;
-            if (S::kEven ? i * kThreads < S::kKeys : piece < S::kKeys) {
-                from = pages.keys(page) + within * (W * static_cast<int>(sizeof(T))) + piece * 16;
-            } else {
-                const int row = (piece - S::kKeys) / S::kValuePieces, of = (piece - S::kKeys) % S::kValuePieces;
-                from = pages.values(page) + (row * pages.tokens + within) * static_cast<int>(sizeof(T)) + of * 16;
-            }
-            moved[i] = *(const SATORI_GLOBAL u32x4*)(from);
+            const uint32_t row = (piece - S::kKeys) / S::kValuePieces, of = (piece - S::kKeys) % S::kValuePieces;
+            const uint32_t value = row * pages.tokens * static_cast<uint32_t>(sizeof(T)) + of * 16;
+            if (S::kEven)  // (a scalar base and 32 bits that stay the same from tile to tile)
+                moved[i] = i * kThreads < S::kKeys ? *(const SATORI_GLOBAL u32x4*)(keys + static_cast<uint32_t>(piece) * 16)
+                                                   : *(const SATORI_GLOBAL u32x4*)(values + value);
+            else
+                moved[i] = *(const SATORI_GLOBAL u32x4*)(piece < S::kKeys ? keys + piece * 16 : values + value);
         }
     };
     const auto put = [&](int tile, const u32x4 (&moved)[S::kPer]) {
+        const int thread = of_thread();
         u32x4* buffer = reinterpret_cast<u32x4*>(lds) + (tile & 1) * S::kPieces;
 #pragma unroll
         for (int i = 0; i < S::kPer; ++i) {
@@ -756,8 +773,8 @@ __device__ __forceinline__ void attend_many(const AttentionArgs& a, const PlanIt
         }
     };
 
-    u32x4 moved[2][S::kPer];
-    int page = 0;  // of the tile that is fetched next, read a tile before
+    u32x4 moved[2][S::kPer];  // tile i in set i % 2
+    int page = 0;             // of the tile that is fetched next, read a tile before
     const auto page_of = [&](int tile) { return pages.page(min(tile, tiles - 1) * kTile); };
     if (tiles > 0) {
         fetch(page_of(0), 0, moved[0]);
@@ -779,34 +796,59 @@ __device__ __forceinline__ void attend_many(const AttentionArgs& a, const PlanIt
     }
     if (tiles > 0) {
         put(0, moved[0]);
+        if (tiles > 2) fetch(page, 2, moved[0]);
+        page = page_of(3);
         settle(0);
     }
     __syncthreads();
-    const auto attend = [&](int tile, u32x4 (&free)[S::kPer], const u32x4 (&next)[S::kPer]) {
-        if (tile + 2 < tiles) {
-            fetch(page, tile + 2, free);
-            page = page_of(tile + 3);
-        }
-        if (!idle) {
+    const auto attend = [&](int tile, u32x4 (&next)[S::kPer]) {
+        // The next tile's bytes, which came while the last two were attended, go into the other buffer (everyone has left it),
+        // and the one three ahead sets out.
+        const auto carry = [&] {
+            if (tile + 1 < tiles) put(tile + 1, next);
+            if (tile + 3 < tiles) {
+                fetch(page, tile + 3, next);
+                page = page_of(tile + 4);
+            }
+        };
+        if (idle) {
+            carry();
+        } else {
             const int t = tile * kTile;
             const Fragment* keys = reinterpret_cast<const Fragment*>(lds) + (tile & 1) * S::kPieces;
             const Fragment* values = keys + S::kKeys;
             f32x4 score[NB][2];
 #pragma unroll
             for (int b = 0; b < NB; ++b) score[b][0] = score[b][1] = f32x4{0, 0, 0, 0};
+            // Fragments are read ahead of the products that take them: a read takes as long as eight products, and a wave is
+            // alone on its SIMD. (The barriers keep the order: the compiler would read each right before its use.)
+            Fragment k[2][2];
+            const auto read_keys = [&](int s) {
+#pragma unroll
+                for (int h = 0; h < 2; ++h) k[s & 1][h] = keys[piece_at<S::kKeyPieces>(16 * h + c, 4 * s + g)];
+            };
+            read_keys(0);
 #pragma unroll
             for (int s = 0; s < M::kKeyParts; ++s) {
-                Fragment k[2];
-#pragma unroll
-                for (int h = 0; h < 2; ++h) k[h] = keys[piece_at<S::kKeyPieces>(16 * h + c, 4 * s + g)];
+                if (s + 1 < M::kKeyParts) read_keys(s + 1);
+                __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
                 for (int term = 0; term < M::kTerms; ++term)
 #pragma unroll
                     for (int h = 0; h < 2; ++h)
 #pragma unroll
-                        for (int b = 0; b < NB; ++b) score[b][h] = M::score(k[h], q[b], s, term, score[b][h]);
+                        for (int b = 0; b < NB; ++b) score[b][h] = M::score(k[s & 1][h], q[b], s, term, score[b][h]);
+                __builtin_amdgcn_sched_barrier(0);
             }
-            __builtin_amdgcn_sched_barrier(0);  // (the scheduler would hold both products' fragments at once, and spill)
+            constexpr int kAhead = W < 256 ? 4 : 2, kFragments = M::kValueParts * (W / 16);
+            Fragment v[kAhead];
+            const auto read_values = [&](int i) {
+                v[i % kAhead] = values[piece_at<S::kValuePieces>(16 * (i % (W / 16)) + c, 4 * (i / (W / 16)) + g)];
+            };
+            carry();
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int i = 0; i < kAhead; ++i) read_values(i);
             const int end = item.tokens - t;
             const bool hides = item.first + t + kTile - 1 > item.limit;
             typename M::Weights w[NB];
@@ -828,27 +870,23 @@ __device__ __forceinline__ void attend_many(const AttentionArgs& a, const PlanIt
                     }
                 }
             }
-            __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-            for (int h = 0; h < M::kValueParts; ++h)
+            for (int i = 0; i < kFragments; ++i) {
+                __builtin_amdgcn_sched_barrier(0);
+                const int d = i % (W / 16), h = i / (W / 16);
 #pragma unroll
-                for (int d = 0; d < W / 16; ++d) {
-                    const Fragment v = values[piece_at<S::kValuePieces>(16 * d + c, 4 * h + g)];
+                for (int term = 0; term < M::kTerms; ++term)
 #pragma unroll
-                    for (int term = 0; term < M::kTerms; ++term)
-#pragma unroll
-                        for (int b = 0; b < NB; ++b) x[b].o[d] = M::weigh(v, w[b], h, term, x[b].o[d]);
-                }
+                    for (int b = 0; b < NB; ++b) x[b].o[d] = M::weigh(v[i % kAhead], w[b], h, term, x[b].o[d]);
+                if (i + kAhead < kFragments) read_values(i + kAhead);
+            }
         }
-        if (tile + 1 < tiles) {
-            put(tile + 1, next);
-            settle(tile + 1);
-        }
+        if (tile + 1 < tiles) settle(tile + 1);
         __syncthreads();
     };
     for (int tile = 0; tile < tiles; tile += 2) {
-        attend(tile, moved[0], moved[1]);
-        if (tile + 1 < tiles) attend(tile + 1, moved[1], moved[0]);
+        attend(tile, moved[1]);
+        if (tile + 1 < tiles) attend(tile + 1, moved[0]);
     }
 
     if (idle) return;
