@@ -444,7 +444,12 @@ __device__ __forceinline__ int pair_place(const PlanItem& item, int p) { return 
 __device__ __forceinline__ Pair pair_of(const AttentionArgs& a, const PlanItem& item, int p) {
     const int group = a.s.heads / a.s.kv_heads, of = pair_place(item, p);
     Pair r;
-    r.row = reinterpret_cast<const PlanRow*>(a.image + a.at.list_at)[item.rows + of / group];
+    if (item.row_slots > 0) {
+        const int behind = of / group - item.pair / group;
+        r.row = PlanRow{item.limit + behind, item.row_slot + behind * item.row_slots, item.row_slots, item.row + behind};
+    } else {
+        r.row = reinterpret_cast<const PlanRow*>(a.image + a.at.list_at)[item.rows + of / group];
+    }
     r.head = item.kv * group + of % group;
     r.is = p < item.pairs;
     return r;
@@ -588,13 +593,13 @@ __device__ __forceinline__ void attend_few(const AttentionArgs& a, const PlanIte
                 v[d][h] = *(const SATORI_GLOBAL Fragment*)(p + 16 * d * pages.tokens + 16 * h);
     };
     int t = wave * kTile, page = 0;
+    const Pair pair = pair_of(a, item, c);
     if (t < item.tokens) {
-        page = pages.page(t);
+        page = wave == 0 ? item.tile[0] : wave == 1 ? item.tile[1] : wave == 2 ? item.tile[2] : item.tile[3];
         load_keys(page, t);
         load_values(page, t);
         if (t + kWaves * kTile < item.tokens) page = pages.page(t + kWaves * kTile);
     }
-    const Pair pair = pair_of(a, item, c);
     PlanRow* row_of = reinterpret_cast<PlanRow*>(lds + S::kRowsAt);
     if (thread < 16) row_of[thread] = pair.row;
     typename M::Query q;
@@ -777,10 +782,8 @@ __device__ __forceinline__ void attend_many(const AttentionArgs& a, const PlanIt
     int page = 0;             // of the tile that is fetched next, read a tile before
     const auto page_of = [&](int tile) { return pages.page(min(tile, tiles - 1) * kTile); };
     if (tiles > 0) {
-        fetch(page_of(0), 0, moved[0]);
-        page = page_of(1);
-        if (tiles > 1) fetch(page, 1, moved[1]);
-        page = page_of(2);
+        fetch(item.tile[0], 0, moved[0]);
+        if (tiles > 1) fetch(item.tile[1], 1, moved[1]);
     }
     typename M::Query q[NB];
     Softmax<W> x[NB];
@@ -796,7 +799,7 @@ __device__ __forceinline__ void attend_many(const AttentionArgs& a, const PlanIt
     }
     if (tiles > 0) {
         put(0, moved[0]);
-        if (tiles > 2) fetch(page, 2, moved[0]);
+        if (tiles > 2) fetch(item.tile[2], 2, moved[0]);
         page = page_of(3);
         settle(0);
     }

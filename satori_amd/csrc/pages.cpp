@@ -399,6 +399,14 @@ PlanImage plan_batch(const PageTables& tables, const int* sequences, const int* 
                     item.limit = least;
                     // Tokens behind all rows of the block are not read (an empty item still writes its partials).
                     item.tokens = std::max(0, std::min(item.tokens, most + 1 - item.first));
+                    for (int i = 0; i < 4; ++i)
+                        item.tile[i] = page_list[item.pages + (item.first % P + std::min(i * kTile, std::max(0, item.tokens - 1))) / P];
+                    if (n.members.size() == 1) {
+                        const PlanRow& row = rows[row_list[n.rows + item.pair / shape.group]];
+                        item.row = row.row;
+                        item.row_slot = row.slot;
+                        item.row_slots = row.slots;
+                    }
                     list.push_back(item);
                 }
     }

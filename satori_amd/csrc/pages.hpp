@@ -82,10 +82,15 @@ struct PlanRow {
 // (the first of them holds token `first`, a multiple of 32), for the (row, query head) pairs pair .. pair + pairs - 1 of
 // the rows listed from `rows` on (pair p: row p / group, head p % group of the key/value head). `slot` counts from the
 // rows' first slots; `limit` is the least position of the rows, so tokens up to it are seen by all of them.
+// What a workgroup would otherwise have to read before it can ask for its first keys and queries, each some 0.7 us behind the
+// item itself, is in the item: the pages of its first tokens (tile[i]: of tokens 32 i on, the last one's where it has fewer),
+// and its rows where they are one sequence's (row_slots > 0): row and position of pair p are then those of the item's first
+// pair, `row` and `limit`, and p's distance from it in rows, and its slots begin at row_slot + that distance * row_slots.
 struct PlanItem {
     int pages, first, tokens, rows;
     int pair, pairs, slot, kv;
-    int limit, pad[3];
+    int limit, row, row_slot, row_slots;
+    int tile[4];
 };
 
 // Consecutive rows of one sequence whose positions lie in one page: row .. row + tokens - 1, from `position` on, at `offset`

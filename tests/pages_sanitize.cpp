@@ -81,11 +81,16 @@ void check_plan(const PageTables& tables, const std::vector<int>& sequences, con
     expect(writable == image.writable, "whether the pages are the rows' own", round);
     // Items: (row, kv, head of the group) -> positions seen, and slots written.
     std::map<std::tuple<int, int, int>, std::pair<std::vector<int>, std::set<int>>> seen;
+    static int singles = 0;
     for (int wide = 0; wide < 2; ++wide)
         for (const PlanItem& item : section<PlanItem>(words, wide ? at.wide_at : at.narrow_at, wide ? h.wide : h.narrow, round)) {
             expect(item.first % 32 == 0 && item.tokens >= 0, "an item's tokens", round);
             expect(item.pairs > 0 && item.pairs <= (wide ? shape.wide_pairs : 16), "an item's pairs", round);
             expect(item.kv >= 0 && item.kv < shape.kv_heads, "an item's head", round);
+            for (int i = 0; i < 4; ++i) {
+                const int token = item.first % P + std::min(32 * i, std::max(0, item.tokens - 1));
+                expect(item.tile[i] == words.at(at.pages_at + item.pages + token / P), "the page of a first tile", round);
+            }
             int least = INT32_MAX;
             for (int p = item.pair; p < item.pair + item.pairs; ++p) {
                 const int entry = item.rows + p / shape.group;
@@ -93,6 +98,13 @@ void check_plan(const PageTables& tables, const std::vector<int>& sequences, con
                 PlanRow listed;
                 std::memcpy(&listed, words.data() + at.list_at + 4 * entry, sizeof listed);
                 const int r = listed.row;
+                if (item.row_slots > 0) {
+                    const int behind = p / shape.group - item.pair / shape.group;
+                    const PlanRow derived{item.limit + behind, item.row_slot + behind * item.row_slots, item.row_slots,
+                                          item.row + behind};
+                    expect(std::memcmp(&derived, &listed, sizeof derived) == 0, "rows of one sequence follow one another", round);
+                    singles++;
+                }
                 expect(std::memcmp(&listed, &rows.at(r), sizeof listed) == 0, "a listed row", round);
                 const auto [s, position] = of_row.at(r);
                 least = std::min(least, position);
