@@ -68,8 +68,9 @@ class PageTable:
     """Page lists and reference counts of a cache of `page_count` pages (satori_hip_pages): host only. Calls that need
     page bytes to follow return them as moves, (sources, destinations)."""
 
-    # A table's read returns a few dozen page numbers and takes about a microsecond, most of it building ctypes arguments
-    # and results, so it passes plain addresses of one buffer, under a lock (threads may call at once).
+    # A table's read returns a few dozen page numbers and takes less than a microsecond, half of it making ctypes arguments
+    # and results, so its arguments but one are made here and name one buffer, read under a lock (threads may call at once),
+    # and the call, which waits for nothing, keeps the interpreter.
 
     def __init__(self, page_count: int, page_tokens: int = 32):
         handle = ctypes.c_void_p()
@@ -77,11 +78,12 @@ class PageTable:
         _check(lib.satori_hip_pages_create(page_count, page_tokens, ctypes.byref(handle)))
         self._handle = handle
         self.page_count, self.page_tokens = page_count, page_tokens
-        self._read, self._address = lib.satori_hip_pages_sequence, handle.value
-        self._room = min(page_count, 1024)
+        self._address, self._room = handle.value, min(page_count, 1024)
         buffer = np.zeros(self._room + 1, np.int32)  # and the count
-        self._buffer, self._at, self._lock = memoryview(buffer), buffer.ctypes.data, threading.Lock()
-        self._count_at = self._at + 4 * self._room
+        self._buffer, self._lock = memoryview(buffer), threading.Lock()
+        at = buffer.ctypes.data
+        self._read = (ctypes.PyDLL(lib._name).satori_hip_pages_sequence, handle, ctypes.c_void_p(), ctypes.c_void_p(at),
+                      ctypes.c_int(self._room), ctypes.c_void_p(at + 4 * self._room))
 
     @property
     def handle(self) -> ctypes.c_void_p:
@@ -152,17 +154,14 @@ class PageTable:
         return self._describe(sequence)[0]
 
     def pages(self, sequence: int) -> list[int]:
-        buffer, room = self._buffer, self._room
+        read, handle, none, at, room, count = self._read
+        buffer = self._buffer
         with self._lock:
-            buffer[room] = 0
-            status = self._read(self._address, sequence, None, self._at, room, self._count_at)
-            count = buffer[room]
-            if not status:
-                return buffer[:count].tolist()
-        if count <= room:
-            _check(status)
+            if not read(handle, sequence, none, at, room, count):
+                return buffer[:buffer[-1]].tolist()
+        count = self._describe(sequence)[1]
         table = np.empty(count, np.int32)  # a long table: a call of its own size
-        _check(self._read(self._address, sequence, None, table.ctypes.data, count, None))
+        _check(_ffi.lib().satori_hip_pages_sequence(handle, sequence, None, table.ctypes.data, count, None))
         return table.tolist()
 
     def dispose(self) -> None:
