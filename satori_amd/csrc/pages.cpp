@@ -212,6 +212,7 @@ namespace {
 constexpr int kTile = 32;         // tokens a wave attends at once
 constexpr int kWaves = 4;         // of a workgroup, which take tiles in turn
 constexpr int kNarrowPairs = 16;  // pairs of a narrow workgroup
+constexpr int64_t kNarrowBytes = 128 << 20;
 
 // Tokens [begin, end) of the pages of `sequence`, seen by the rows of the sequences members[0 .. count).
 struct Node {
@@ -315,22 +316,30 @@ PlanImage plan_batch(const PageTables& tables, const int* sequences, const int* 
         for (auto it = parts.rbegin(); it != parts.rend(); ++it) open.push_back(std::move(*it));
     }
 
-    // Chunks of tokens: as many as give every CU work (kv heads and blocks of pairs count too), and no shorter than
-    // one tile per wave.
-    const auto blocks_of = [&](const Node& n) {
-        int64_t pairs = 0;
-        for (int m : n.members) pairs += static_cast<int64_t>(new_tokens[m]) * shape.group;
-        return pairs;
-    };
-    int64_t narrow_tokens = 0, wide_tokens = 0;
+    // Which nodes' items are wide. A wide workgroup reads a tile once for all its pairs but takes them through it in four
+    // waves; narrow ones, 16 pairs each, read it again for each of their blocks (from L2, mostly) but give every wave tokens of
+    // its own. So narrow items serve up to half a wide workgroup's pairs, and all of them while the blocks together read no
+    // more than kNarrowBytes. Wide against narrow, F16 heads of 128 lanes, 96 pairs over 4096, 16384 and 65536 tokens of 2
+    // key/value heads (25, 100 and 400 MB): 19.7 us and 13.5, 24.7 and 22.6, 38.7 and 46.9; 128 pairs of 8 heads over 4096 and
+    // 8192 (134 and 268 MB): 26.1 and 27.0, 31.0 and 37.4; FP32, 144 pairs of 2 heads over 4000 and 8192 (74 and 151 MB): 25.7
+    // and 23.1, 35.5 and 50.3; 4 x 128 rows, F16 of 96 lanes (171 MB): 37 and 18.
+    int64_t narrow_tokens = 0, wide_tokens = 0, again = 0;
     std::vector<int64_t> pairs_of(nodes.size());
     for (size_t i = 0; i < nodes.size(); ++i) {
         Node& n = nodes[i];
-        pairs_of[i] = blocks_of(n);
-        n.wide = pairs_of[i] > kNarrowPairs;
-        const int64_t blocks = n.wide ? (pairs_of[i] + shape.wide_pairs - 1) / shape.wide_pairs : 1;
+        for (int m : n.members) pairs_of[i] += static_cast<int64_t>(new_tokens[m]) * shape.group;
+        n.wide = pairs_of[i] > shape.wide_pairs / 2;
+        if (n.wide) again += (pairs_of[i] + kNarrowPairs - 1) / kNarrowPairs * shape.kv_heads * (n.end - n.begin);
+    }
+    const auto pairs_a_block = [&](const Node& n) { return n.wide ? shape.wide_pairs : kNarrowPairs; };
+    for (size_t i = 0; i < nodes.size(); ++i) {
+        Node& n = nodes[i];
+        n.wide &= again > kNarrowBytes / shape.token_bytes;
+        const int64_t blocks = (pairs_of[i] + pairs_a_block(n) - 1) / pairs_a_block(n);
         (n.wide ? wide_tokens : narrow_tokens) += blocks * shape.kv_heads * (n.end - n.begin);
     }
+    // Chunks of tokens: as many as give every CU work (kv heads and blocks of pairs count too), and no shorter than
+    // one tile per wave.
     const auto chunk_for = [&](int64_t tokens, int workgroups) {
         const int64_t step = kTile * kWaves;
         const int64_t c = (tokens / workgroups + step - 1) / step * step;
@@ -369,7 +378,7 @@ PlanImage plan_batch(const PageTables& tables, const int* sequences, const int* 
     for (size_t i = 0; i < nodes.size(); ++i) {
         const Node& n = nodes[i];
         // Blocks of pairs, as even as whole matrix tiles of 16 make them.
-        const int most = n.wide ? shape.wide_pairs : kNarrowPairs;
+        const int most = pairs_a_block(n);
         const int64_t least = (pairs_of[i] + most - 1) / most;
         const int step = static_cast<int>((pairs_of[i] + 16 * least - 1) / (16 * least) * 16);
         const int blocks = static_cast<int>((pairs_of[i] + step - 1) / step);

@@ -121,6 +121,7 @@ struct PlanLayout {
 struct PlanShape {
     int kv_heads, group;  // group: query heads of a key/value head
     int wide_pairs;       // pairs of a wide workgroup; a narrow one takes 16
+    int token_bytes;      // a position's key and value of one head
 };
 
 // A plan's arrays, and what its launches need to know.

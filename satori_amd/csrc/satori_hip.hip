@@ -2431,6 +2431,7 @@ int satori_hip_cache_plan_create(satori_hip_context* c, void* pool, int page_cou
         p->plan.kv_heads = kv_heads;
         p->plan.group = query_heads / kv_heads;
         p->plan.wide_pairs = cache_wide_pairs(type, shape.width);
+        p->plan.token_bytes = 2 * shape.width * element_bytes(type);
         try {
             for (hipEvent_t& e : p->copied) check_hip(hipEventCreateWithFlags(&e, hipEventDisableTiming), "hipEventCreate");
             p->layout = PlanLayout::first();

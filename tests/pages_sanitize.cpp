@@ -201,7 +201,7 @@ int main() {
                     batch.push_back(id);
                     fresh.push_back(std::min(tables.tokens(id), up_to(2) ? 1 : up_to(40)));
                 }
-            check_plan(tables, batch, fresh, PlanShape{1 + up_to(2), 1 + up_to(6), 16 << up_to(2)}, layout, round);
+            check_plan(tables, batch, fresh, PlanShape{1 + up_to(2), 1 + up_to(6), 16 << up_to(2), 1 << (round % 2 ? 22 : 9)}, layout, round);
         }
     }
     // Long sequences, many chunks.
@@ -221,7 +221,7 @@ int main() {
             if (fresh.back() > n) fresh.back() = n;
         }
         PlanLayout layout;
-        check_plan(tables, batch, fresh, PlanShape{2, 3, 64}, layout, round);
+        check_plan(tables, batch, fresh, PlanShape{2, 3, 64, 1 << (round % 2 ? 12 : 20)}, layout, round);
     }
     if (failures) return 1;
     std::puts("ok");

@@ -815,3 +815,52 @@ def test_small_weights_beside_one_that_takes_all(context, device, type_, new):
             err = np.abs(got[row, h] - p @ v[:n, 0])
             assert np.all(err <= bound), (row, h, (err / bound).max())
     plan.dispose()
+
+
+@pytest.mark.parametrize("type_,heads,kv_heads,head_dim,page_tokens", SHAPES)
+def test_many_rows_over_many_positions(context, device, type_, heads, kv_heads, head_dim, page_tokens):
+    # Enough positions that blocks of 16 (row, head) pairs would read 128 MiB and more: tiles then pass through LDS. Some rows
+    # against the definition; then a value that is infinite and a key that is NaN, each inside a tile that some rows see and
+    # some do not, change what sees them and no bit of anything else.
+    g = rng(heads + head_dim)
+    own = [300, 20, 61]
+    pool = Pool(context, device, CacheLayout(1, kv_heads, head_dim, page_tokens, type_), 1)
+    blocks = (sum(own) * (heads // kv_heads) + 15) // 16
+    prefix = (128 << 20) // (blocks * kv_heads * 2 * pool.width * (2 if type_ == F16 else 4)) + 200
+    pool.cache.dispose()
+    pool = Pool(context, device, pool.layout, prefix // page_tokens + 2 * 300 // page_tokens + 8)
+    batch = forked(pool, prefix, own)
+    pool.host[...] = g.standard_normal(pool.host.shape, np.float32).astype(pool.host.dtype)
+    for s in batch:
+        last, n = pool.cache.pages(s)[-1], pool.cache.tokens(s) % page_tokens
+        if n:
+            pool.keys(0)[last, :, n:] = np.nan
+            pool.values(0)[last, ..., n:] = np.inf
+    pool.upload()
+    q, got = attend(context, device, pool, batch, own, heads, g)
+    row = 0
+    for s, n in zip(batch, own):
+        k, v = pool.of(s, 0)
+        for r in sorted({0, 1, n // 2, n - 2, n - 1} | {int(i) for i in g.integers(0, n, 4)}):
+            expected, bound = exact_attention(q[row + r], k, v, len(k) - n + r)
+            err = np.abs(got[row + r].astype(np.float64) - expected)
+            assert np.all(err <= bound), f"row {r} of {n}: {(err / bound).max()}"
+        row += n
+    group, table = heads // kv_heads, pool.cache.pages(batch[0])
+    place = lambda i: (table[(prefix + i) // page_tokens], (prefix + i) % page_tokens)  # noqa: E731
+    page, at = place(100)
+    pool.values(0)[page, 0, 0, at] = np.inf
+    page, at = place(155)
+    pool.keys(0)[page, 0, at, 0] = np.nan
+    pool.upload()
+    plan, out = pool.cache.plan(heads), device(np.zeros_like(q))
+    plan.set(batch, own)
+    plan.attention(0, device(q), out)
+    spoiled = context.download(np.zeros_like(q), out)
+    plan.dispose()
+    want = got.copy()
+    want[100:300, :group, 0] = np.nan
+    want[155:300, :group] = np.nan
+    hit = np.isnan(want)
+    assert not np.isfinite(spoiled[hit]).any()
+    assert np.array_equal(spoiled[~hit], want[~hit])
