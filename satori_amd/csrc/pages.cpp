@@ -225,8 +225,15 @@ struct Node {
 };
 
 // Runs of pages that sequences share but that are shorter than this are read by each of them: one more partial result
-// per row and head (and its joining) costs about what reading so many tokens again does.
+// per row and head (and its joining) costs about what reading so many tokens again does (16 sequences of 12 heads and 300 to
+// 400 positions, shared against not, F16: 64 positions 11.6 us and 11.9, 256 12.0 and 12.0, 1024 12.3 and 13.3, 4096 13.6 and
+// 17.8; 20 of 32 heads and 100 to 200: 128 positions 14.9 and 14.1, 256 14.8 and 15.4, 512 13.8 and 20.6).
 constexpr int kLeastShared = 128;
+// The card holds so many workgroups at once (two a CU), each of some 7 us for the chain of its reads alone. Where the items of
+// the sequences' own fill that and those of a shared run would come behind them, the run is shared if that saves this much
+// reading: 64 sequences of 8 key/value heads and 100 to 200 positions, F16, over 256 shared ones (50 MB) 24.6 us shared and
+// 17.5 not, 512 (100 MB) 24.4 and 21.9, 1024 (201 MB) 27.5 and 32.0.
+constexpr int64_t kPlaces = 512, kRoundBytes = 128 << 20;
 
 }  // namespace
 
@@ -260,6 +267,22 @@ PlanImage plan_batch(const PageTables& tables, const int* sequences, const int* 
         }
     }
 
+    const auto blocks_of = [](int64_t pairs) { return (pairs + kNarrowPairs - 1) / kNarrowPairs; };
+    int64_t own = 0;  // items of the sequences by themselves, at least
+    for (int i = 0; i < count; ++i) own += blocks_of(static_cast<int64_t>(new_tokens[i]) * shape.group) * shape.kv_heads;
+    const auto worth_sharing = [&](const std::vector<int>& members, int64_t tokens) {
+        if (tokens < kLeastShared) return false;
+        int64_t pairs = 0, apart = 0;
+        for (int m : members) {
+            pairs += static_cast<int64_t>(new_tokens[m]) * shape.group;
+            apart += blocks_of(static_cast<int64_t>(new_tokens[m]) * shape.group);
+        }
+        const int64_t together = blocks_of(pairs);
+        const auto rounds = [](int64_t items) { return (items + kPlaces - 1) / kPlaces; };
+        return rounds(own + together * shape.kv_heads) == rounds(own) ||
+               (apart - together) * tokens * shape.kv_heads >= kRoundBytes / shape.token_bytes;
+    };
+
     // The trie of the tables: a node for every run of pages that the same sequences share.
     std::vector<Node> nodes;
     struct Open {
@@ -292,7 +315,7 @@ PlanImage plan_batch(const PageTables& tables, const int* sequences, const int* 
         }
         const int begin = o.page * P, end = std::min(static_cast<int>(common) * P, longest);
         int from = o.page, ancestors = o.ancestors;
-        if (end - begin >= kLeastShared) {
+        if (worth_sharing(o.members, end - begin)) {
             nodes.push_back({begin, end, o.members, o.ancestors});
             from = static_cast<int>(common);
             ancestors = static_cast<int>(nodes.size()) - 1;
@@ -329,7 +352,7 @@ PlanImage plan_batch(const PageTables& tables, const int* sequences, const int* 
         Node& n = nodes[i];
         for (int m : n.members) pairs_of[i] += static_cast<int64_t>(new_tokens[m]) * shape.group;
         n.wide = pairs_of[i] > shape.wide_pairs / 2;
-        if (n.wide) again += (pairs_of[i] + kNarrowPairs - 1) / kNarrowPairs * shape.kv_heads * (n.end - n.begin);
+        if (n.wide) again += blocks_of(pairs_of[i]) * shape.kv_heads * (n.end - n.begin);
     }
     const auto pairs_a_block = [&](const Node& n) { return n.wide ? shape.wide_pairs : kNarrowPairs; };
     for (size_t i = 0; i < nodes.size(); ++i) {
