@@ -15,8 +15,9 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kWaves = 4;
 constexpr int kMostSplits = 16;
-constexpr int64_t kBothBytes = 24 << 20;  // weights that one launch may read, tiles times the workgroups that read them
-constexpr int kSplitGroups = 256;  // workgroups that the first launch's splits make up
+// Workgroups that the first launch's splits make up (11008 x 4096, rank 64, 256 rows of 2 adapters and 64 rows of 16: 128
+// 33.4 and 33.0 us for both launches, 256 24.1 and 23.3, 512 24.4 and 22.7).
+constexpr int kSplitGroups = 256;
 constexpr int kStep = 32;  // columns a wave takes at once
 
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
@@ -243,17 +244,24 @@ __global__ __launch_bounds__(kThreads) void adapter_up_kernel(AdapterShape s, Ad
         if (16 * r < tile.count) out[r].store(s, output, sum[r], n0, whole);
 }
 
-// Both products in one launch, for small adapters and few tiles: workgroup (tile, 512 output rows or less) makes the tile's
-// whole reduced vectors for itself.
+// Both products in one launch, for adapters of one tile of ranks and short rows: workgroup (tile, 512 output rows or less)
+// makes the tile's whole reduced vectors for itself, 1024 columns a turn of its waves, which takes as long as the second
+// launch would from some columns on. One launch against two, 32 rows of 32 adapters of rank 16, 1536 output rows: F16 1024
+// columns 6.4 us and 9.1, 2048 8.2 and 8.9, 2560 10.0 and 9.0, 8192 21 and 11.7; FP32 1024 7.2 and 9.0, 1477 8.9 and 9.1, 2048
+// 10.1 and 9.3; rank 32, F16, 1024 columns 9.5 and 9.0. And for few workgroups, each of which reads a tile's weights and rows:
+// 1536 columns, adapters of one row, 64 over 1536 output rows (10.6 MB) 9.0 and 10.5, 128 (21 MB) 17.5 and 15.4, 32 over 4096
+// (14 MB) 8.8 and 10.1, over 8192 (28 MB) 17.2 and 15.1; 256 rows of one adapter over 4096 (19 MB) 13.2 and 11.8.
 constexpr int kBothWaves = 8;
-constexpr int kBothRanks = 4;  // tiles of 16 ranks
+constexpr int kBothRank = 16;
+constexpr int64_t kBothBytes = 16 << 20;
+constexpr int both_columns(int type) { return type == kF32 ? 1536 : 2048; }
 
 template <typename T>
 __global__ __launch_bounds__(kBothWaves * 64) void adapter_both_kernel(AdapterShape s, AdapterTiles tiles,
                                                                        const float* __restrict__ input, const float* base,
                                                                        float* output, int rows_each, bool whole) {
     __shared__ f32x4 parts[kBothWaves][64];
-    __shared__ float t[16][16 * kBothRanks + 4];
+    __shared__ float t[16][kBothRank + 4];
     const Tile tile = tile_of(s, tiles, blockIdx.x);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = lane & 15, g = lane >> 4;
     const int n0 = blockIdx.y * rows_each + wave * 64;
@@ -265,28 +273,21 @@ __global__ __launch_bounds__(kBothWaves * 64) void adapter_both_kernel(AdapterSh
         out.load(s, tiles, tile, base, 0, n0, whole);
     }
     const float* x = input + static_cast<int64_t>(tiles.order[tile.begin + (c < tile.count ? c : 0)]) * s.columns;
-    for (int rank0 = 0; rank0 < tile.adapter.rank; rank0 += 16) {
-        const f32x4 sum = reduce<T>(s, tile, x, rank0, wave * kStep, kBothWaves * kStep, s.columns);
-        if (rank0) __syncthreads();
-        parts[wave][lane] = sum;
-        __syncthreads();
-        if (wave == 0) {
-            f32x4 total = sum;
+    if (!tile.none) parts[wave][lane] = reduce<T>(s, tile, x, 0, wave * kStep, kBothWaves * kStep, s.columns);
+    __syncthreads();
+    if (wave == 0 && !tile.none) {
+        f32x4 total = parts[0][lane];
 #pragma unroll
-            for (int w = 1; w < kBothWaves; ++w) total = total + parts[w][lane];
+        for (int w = 1; w < kBothWaves; ++w) total = total + parts[w][lane];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const int k = rank0 + 4 * g + j;
-                t[c][k] = k < tile.adapter.rank ? total[j] * tile.adapter.scale : 0.0f;
-            }
-        }
+        for (int j = 0; j < 4; ++j) t[c][4 * g + j] = 4 * g + j < tile.adapter.rank ? total[j] * tile.adapter.scale : 0.0f;
     }
     __syncthreads();
     if (!works) return;
     f32x4 sum[4];
 #pragma unroll
     for (int n = 0; n < 4; ++n) sum[n] = f32x4{0, 0, 0, 0};
-    up.expand(tile, &t[0][0], 16 * kBothRanks + 4, 0, sum);
+    up.expand(tile, &t[0][0], kBothRank + 4, 0, sum);
     out.store(s, output, sum, n0, whole);
 }
 
@@ -296,8 +297,9 @@ hipError_t launch(const AdapterShape& s, const AdapterTiles& tiles, const float*
     const bool whole = s.rows % 4 == 0 && reinterpret_cast<uintptr_t>(base) % 16 == 0 &&
                        reinterpret_cast<uintptr_t>(output) % 16 == 0;
     const int ranks = s.rank_most / 16;
-    const int64_t both_groups = static_cast<int64_t>(tiles.tiles) * ((s.rows + 511) / 512);
-    if (ranks <= kBothRanks && both_groups * ranks * 16 * s.columns * static_cast<int64_t>(sizeof(T)) <= kBothBytes) {
+    const int64_t both_bytes = (static_cast<int64_t>(tiles.tiles) * kBothRank * sizeof(T) + tiles.positions * sizeof(float)) *
+                               s.columns * ((s.rows + 511) / 512);
+    if (s.rank_most <= kBothRank && s.columns <= both_columns(s.type) && both_bytes <= kBothBytes) {
         // 64 rows a wave and turn; fewer waves work on them where that lets more CUs share them.
         int each = 512;
         while (each > 64 && tiles.tiles * ((s.rows + each - 1) / each) < 128) each /= 2;
