@@ -19,7 +19,10 @@ constexpr int kThreads = 256;
 
 // ---- page copies ----
 
-// Each workgroup copies kCopyBytes of one page, 16 bytes a thread and access, four accesses in flight.
+// Each workgroup copies kCopyBytes of one page, 16 bytes a thread and access, four accesses in flight; a page of all layers is
+// one run of bytes, so one launch serves any number of moves. Bound by memory: 224 moves of 917,504 bytes take 73 us (5.6
+// TB/s read and written, the large copy's 4.9 being one of 2 GiB), 48 whose source is one page 10.9 us (the 44 MB written at
+// 4.0 TB/s, launch included).
 constexpr int kCopyBytes = kThreads * 16 * 4;
 
 __global__ __launch_bounds__(kThreads) void copy_pages_kernel(uint8_t* pool, int64_t page_bytes, PageMoves moves) {
@@ -85,7 +88,9 @@ constexpr int kGroupTokens = 8;  // positions whose values a thread stores at on
 // The rows of a run, spread over gridDim.y workgroups: N rotated lane pairs of a query or key head per thread and turn,
 // then the lanes behind the rotated ones and the keys' padding, then the values. A page's values lie [lane][position], so a
 // thread gathers one lane of up to eight positions (its neighbours the next lanes: the reads are whole lines) and stores
-// them together where they fill an aligned group.
+// them together where they fill an aligned group (one value a store took 93 us where this takes 9.8). Few rows are bound by
+// the launch and two dependent reads (16 rows of 12 + 2 heads of 128 lanes 4.6 us), many by memory: 8 x 61 rows of 32 + 8 heads
+// move 22.6 MB in 9.8 us (2.3 TB/s); the rotation's angles come from the table in 64 bits, as the single-sequence operator's.
 template <typename T, int N>
 __global__ __launch_bounds__(kThreads) void cache_append_kernel(CacheShape s, const int* __restrict__ image, int runs_at,
                                                                 AppendArgs a) {
@@ -530,12 +535,18 @@ struct Pages {
 // A workgroup of four waves attends one item, in one of two ways.
 //
 // Few pairs (16 at most): each wave takes tiles of its own in turn, keys and values straight from the cache into registers
-// (nobody else in the workgroup wants them), and the waves' results are joined through LDS.
+// (nobody else in the workgroup wants them), and the waves' results are joined through LDS. Bound by the chain of reads of one
+// item (the item 0.8 us, keys and queries 1.3 to 3.4, of FP32 the 64 + 64 matrix instructions of a tile 1.9, the join 1.3): 4
+// sequences of 20 to 120 positions 10.4 us in all, 9 x 5 rows over 1500 shared positions 12.7 with their join.
 //
 // Many pairs: each wave has 16 * kBlocks of them, and the tiles that all four want pass through LDS, in two buffers: while
-// one is attended, the bytes of the next two are on their way in registers. Rows of a tile are 16-byte pieces, put where the
-// 16 lanes that read a column of them reach different banks: piece p of row r lies at p ^ (r's bits that its place in a
-// 256-byte line leaves open).
+// one is attended, the bytes of the next three are on their way, the nearest two in registers. Rows of a tile are 16-byte
+// pieces, put where the 16 lanes that read a column of them reach different banks: piece p of row r lies at p ^ (r's bits that
+// its place in a 256-byte line leaves open). A tile of 128 F16 lanes takes a wave 1.4 us: its 64 matrix instructions are 0.48
+// of them, the softmax's and the tile's carrying's other instructions most of the rest, and a wave is alone on its SIMD (two
+// workgroups a CU do a tile each in 1.8, but their twice as many partial results take the join that time). 64 sequences of 32
+// heads over 16384 shared positions and 64 to 600 of their own: 65.6 us in all, 17.4 GFLOP of the definition and twice that in
+// matrix instructions at 0.53 PFLOP/s, 133 MB read.
 constexpr int kWaves = 4;
 
 template <int PIECES>
@@ -907,7 +918,8 @@ __device__ __forceinline__ void attend_many(const AttentionArgs& a, const PlanIt
 }
 
 // Items of many pairs first, which take longest (one a CU, bound by arithmetic); those of few, bound by memory, run beside
-// them. Workgroup u is u % 8 of its eight, which keeps items that read the same tokens on one XCD.
+// them (64 sequences as above, before later steps: two launches 64 + 27 us, one with the items in turn 92, with the many first
+// 76). Workgroup u is u % 8 of its eight, which keeps items that read the same tokens on one XCD.
 template <typename T, int W>
 __global__ __launch_bounds__(kThreads, (Shape<T, W>::kWavesPerSimd)) void cache_attention_kernel(AttentionArgs a) {
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
@@ -928,7 +940,8 @@ __global__ __launch_bounds__(kThreads, (Shape<T, W>::kWavesPerSimd)) void cache_
 
 // The partial results of one (row, head), joined by a workgroup with weights 2^(m_i - m): every wave finds the maximum, then
 // groups of lanes read a part's values each, four lanes of the head a lane, and LDS joins the groups in order. Bound by the
-// latency of its chain of reads (the parts come from other XCDs), so all parts of common plans are read at once.
+// latency of its chain of reads (the parts come from other XCDs), so all parts of common plans are read at once: 24 x 12 pairs
+// of up to 17 parts 3.9 us, 64 x 32 of 17 (18 MB) 7.2 us.
 __global__ __launch_bounds__(kThreads) void cache_join_kernel(AttentionArgs a) {
     const CacheShape& s = a.s;
     const int count = a.rows >= 0 ? a.rows : scalar_load(&reinterpret_cast<const PlanHeader*>(a.image)->rows);
