@@ -375,9 +375,10 @@ struct Softmax {
 // The scores of the tokens that a pair does not see become -infinity: those from `seen` on, of the tile.
 template <typename M>
 __device__ __forceinline__ void hide(f32x4 (&score)[2], int seen, int g) {
+    const int left = seen - M::token(g, 0);  // (a lane's tokens are its first one's plus numbers that all lanes share)
 #pragma unroll
     for (int i = 0; i < 8; ++i)
-        if (M::token(g, i) >= seen) score[i >> 2][i & 3] = -INFINITY;
+        if (M::token(0, i) >= left) score[i >> 2][i & 3] = -INFINITY;
 }
 
 // Values that are not finite. Where some pairs see a token and others must not, the second product would spoil the others'

@@ -2286,7 +2286,7 @@ CacheShape cache_shape(int layers, int query_heads, int kv_heads, int head_dim, 
     s.page_tokens = page_tokens;
     while (1 << s.page_shift < page_tokens) ++s.page_shift;
     const int64_t row = static_cast<int64_t>(kv_heads) * s.width, head = static_cast<int64_t>(query_heads) * s.width;
-    if (row > INT32_MAX / 512 || head > INT32_MAX / 512)
+    if (row > INT32_MAX / 1024 || head > INT32_MAX / 1024)
         fail(SATORI_HIP_E_OVERFLOW, "Arithmetic operation resulted in an overflow.");
     s.layer_bytes = 2 * row * page_tokens * element_bytes(type);
     if (s.layer_bytes > INT64_MAX / layers) fail(SATORI_HIP_E_OVERFLOW, "Arithmetic operation resulted in an overflow.");
