@@ -864,3 +864,49 @@ def test_many_rows_over_many_positions(context, device, type_, heads, kv_heads, 
     hit = np.isnan(want)
     assert not np.isfinite(spoiled[hit]).any()
     assert np.array_equal(spoiled[~hit], want[~hit])
+
+
+@pytest.mark.parametrize("type_,heads,kv_heads,head_dim", [(F16, 16, 2, 128), (F32, 12, 1, 128), (F16, 8, 1, 256)])
+def test_a_captured_step_follows_batches_of_other_kinds(context, device, type_, heads, kv_heads, head_dim):
+    # The same 200 rows as one prompt without a past, as ten forks of a short prefix and as a chunk behind a long one (whose
+    # tiles pass through LDS), each replay against an eager call on another plan.
+    g = rng(head_dim + heads)
+    rows, group = 200, heads // kv_heads
+    width, size = head_dim, 2 if type_ == F16 else 4
+    past = (128 << 20) // ((rows * group + 15) // 16 * kv_heads * 2 * width * size) + 100
+    pool = Pool(context, device, CacheLayout(1, kv_heads, head_dim, 32, type_), past // 32 + 60)
+    c = pool.cache
+    prompt, behind, short = c.open(), c.open(), c.open()
+    c.extend([prompt, behind, short], [rows, past + rows, 70])
+    forks = [short] + c.fork(short, 9)
+    c.extend(forks, [20] * 10)
+    pool.write(g, [prompt, behind] + forks)
+    batches = [([behind], [rows]), ([prompt], [rows]), (forks, [20] * 10)]
+    q = g.standard_normal((rows, heads, head_dim)).astype(np.float32)
+    dq, out, eager_out = device(q), device(np.zeros_like(q)), device(np.zeros_like(q))
+    plan, other = c.plan(heads), c.plan(heads)
+    plan.set(*batches[0])  # the largest, before the capture
+    plan.set(*batches[1])
+    context.capture_begin()
+    plan.attention(0, dq, out)
+    step = context.capture_end()
+    for turn, i in enumerate((1, 0, 2, 0, 1)):
+        context.upload(out, np.full_like(q, np.nan))
+        plan.set(*batches[i])
+        step.execute()
+        got = context.download(np.zeros_like(q), out)
+        other.set(*batches[i])
+        other.attention(0, dq, eager_out)
+        assert np.array_equal(got, context.download(np.zeros_like(q), eager_out)), (turn, i)
+        if turn < 3:
+            sequences, new = batches[i]
+            some = rng(turn).integers(0, rows, 6)
+            starts = np.cumsum([0] + new)
+            for r in some:
+                s = int(np.searchsorted(starts, r, side="right") - 1)
+                k, v = pool.of(sequences[s], 0)
+                expected, bound = exact_attention(q[r], k, v, len(k) - new[s] + int(r) - starts[s])
+                assert np.all(np.abs(got[r] - expected) <= bound), (turn, int(r))
+    step.dispose()
+    plan.dispose()
+    other.dispose()

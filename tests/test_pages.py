@@ -181,3 +181,38 @@ def test_page_bytes():
             layout.page_bytes
     with pytest.raises(S.OverflowException):
         CacheLayout(1, 2 ** 30, 256).page_bytes
+
+
+def test_threads_read_lists_at_once():
+    # Reads share one buffer: each thread gets its own sequence's list, while another thread forks and frees.
+    import threading
+
+    t = PageTable(4000)
+    sequences = [t.open() for _ in range(4)]
+    t.extend(sequences, [1, 32 * 40, 32 * 700, 32 * 1500])  # (the last is longer than the buffer)
+    expected = [t.pages(s) for s in sequences]
+    assert [len(e) for e in expected] == [1, 40, 700, 1500]
+    wrong, done = [], threading.Event()
+
+    def read(i):
+        for _ in range(300):
+            if t.pages(sequences[i]) != expected[i]:
+                wrong.append(i)
+
+    def churn():
+        while not done.is_set():
+            forks = t.fork(sequences[1], 3)
+            t.extend(forks, [1] * 3)
+            t.free(forks)
+
+    threads = [threading.Thread(target=read, args=(i % 4,)) for i in range(8)] + [threading.Thread(target=churn)]
+    for thread in threads:
+        thread.start()
+    for thread in threads[:-1]:
+        thread.join()
+    done.set()
+    threads[-1].join()
+    assert not wrong
+    t.dispose()
+    with pytest.raises(S.ObjectDisposedException):
+        t.pages(sequences[0])
