@@ -362,7 +362,9 @@ PlanImage plan_batch(const PageTables& tables, const int* sequences, const int* 
         (n.wide ? wide_tokens : narrow_tokens) += blocks * shape.kv_heads * (n.end - n.begin);
     }
     // Chunks of tokens: as many as give every CU work (kv heads and blocks of pairs count too), and no shorter than
-    // one tile per wave.
+    // one tile per wave. (Few pairs in 256, 512 and 1024 workgroups: 24 rows over 4000 positions, FP32, 23.0, 28.9 and 31.6 us, 64
+    // of 1000 to 2000, F16, 68, 78 and 80, 9 x 5 over 4000 16.9, 15.4 and 19.3. Many in 256 and 512: 64 rows over 8192, F16, 46
+    // and 58, over 32768 103 and 102, 24 over 8192, FP32, 35 and 31: the more chunks, the more partial results.)
     const auto chunk_for = [&](int64_t tokens, int workgroups) {
         const int64_t step = kTile * kWaves;
         const int64_t c = (tokens / workgroups + step - 1) / step * step;
