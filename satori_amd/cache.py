@@ -27,7 +27,7 @@ class ElementType(enum.IntEnum):
 def _ints(values) -> np.ndarray:
     if isinstance(values, np.ndarray) and values.dtype == np.int32 and values.flags.c_contiguous:
         return values.reshape(-1)
-    return np.array(values, dtype=np.int32).reshape(-1)
+    return np.array(_array(values), np.int32)  # (integers of 32 bits or an error: a cast of numpy's would wrap)
 
 
 def _array(values) -> array:
@@ -201,10 +201,16 @@ class PagedCache:
 
     def _move(self, moves: _Moves) -> None:
         if moves.count:
-            self.copy_pages(moves.sources, moves.destinations, moves.count)
+            self._copy_pages(moves.sources, moves.destinations, moves.count)
 
-    def copy_pages(self, sources: int, destinations: int, count: int) -> None:
-        """Pool page destinations[i] = pool page sources[i], from host arrays at these addresses."""
+    def copy_pages(self, sources, destinations) -> None:
+        """Pool page destinations[i] = pool page sources[i] (moves of a page table's own calls, for instance)."""
+        s, d = _array(sources), _array(destinations)
+        if len(s) != len(d):
+            raise ArgumentException("Lengths differ.")
+        self._copy_pages(_address(s), _address(d), len(s))
+
+    def _copy_pages(self, sources: int, destinations: int, count: int) -> None:
         _check(_ffi.lib().satori_hip_cache_copy_pages(self.context.handle, self.pool, self.page_bytes, self.page_count,
                                                       sources, destinations, count, None))
 

@@ -378,8 +378,7 @@ def test_append_equals_the_single_sequence_operator(context, device, type_, head
 # ---- page copies ----
 
 def copy_pages(cache, sources, destinations):
-    s, d = np.array(sources, np.int32), np.array(destinations, np.int32)
-    cache.copy_pages(s.ctypes.data, d.ctypes.data, s.size)
+    cache.copy_pages(sources, destinations)
 
 
 @pytest.mark.parametrize("layers,pages", [(1, 3), (5, 700)])
@@ -910,3 +909,22 @@ def test_a_captured_step_follows_batches_of_other_kinds(context, device, type_, 
     step.dispose()
     plan.dispose()
     other.dispose()
+
+
+def test_numbers_that_are_no_32_bit_integers(context, device):
+    pool = Pool(context, device, CacheLayout(1, 1, 32, 32, F16), 8)
+    c = pool.cache
+    s = c.open()
+    c.extend([s], [5])
+    plan = c.plan(1)
+    for bad in ([1 << 32], [1.5], np.array([1 << 32]), np.array([1.0])):
+        with pytest.raises((OverflowError, TypeError)):
+            plan.set([s], bad)
+        with pytest.raises((OverflowError, TypeError)):
+            c.extend([s], bad)
+        with pytest.raises((OverflowError, TypeError)):
+            c.copy_pages(bad, [2])
+    with pytest.raises(S.ArgumentException):
+        c.copy_pages([0, 1], [2])
+    plan.set(np.array([s]), np.array([1]))  # 64-bit numpy integers that fit
+    plan.dispose()
