@@ -12,6 +12,9 @@ Names, argument meaning and exceptions follow the reference (src/Satori.Core, sr
   HipQuantizedMatrix.execute                          IQuantizedMatrix.Execute (IQuantizedMatrix.cs:7)
   Q8KCodec.quantize_row                               Q8KCodec.cs:85-93 (on the device)
 
+Beyond the reference's one sequence: satori_amd.cache (a key/value cache whose pages sequences share, its batched write and
+attention) and satori_amd.adapters (low-rank adapters of a batch's requests).
+
 Every MatVec runs on the GPU through the library; there is no CPU fallback. Importing this package needs
 the built library (``python -m satori_amd.build``); creating a HipContext needs a gfx950 device.
 """

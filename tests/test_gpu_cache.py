@@ -5,7 +5,8 @@ Attention's bound. A score is a sum of D products in FP32 (any order) times a fa
 (D + 8) e A, A = sum |q k| / sqrt(D) (8: the factor's and the subtraction's roundings, the 2^-22 of a query kept in two
 halves, exp2's argument). A relative error x of exp enters the weights and their sum once each. The sums over tokens run over
 tiles of 32 (at most T / 32 tiles and the joining of four waves and of the parts) with up to 32 products a tile in one
-instruction: (T / 32 + 64) e, and 16 e for probabilities in two halves, exp2 and the division. So
+instruction: (T / 32 + 64) e, and 16 e for probabilities in two halves, exp2 and the division (of F16 pages a probability is off
+by up to 2^-36 of its row's largest where that is more: over T random values less than the 80 e below while T < 2^16). So
 |o - exact| <= (2 (D + 8) e max A + 2 (T / 32 + 80) e) * sum p |v|, which the tests take times 1.01 (second order)."""
 from __future__ import annotations
 
