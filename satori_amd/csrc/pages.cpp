@@ -389,12 +389,19 @@ PlanImage plan_batch(const PageTables& tables, const int* sequences, const int* 
             }
     }
     int64_t slots = 0;
-    for (PlanRow& r : rows) {
+    const auto number = [&](PlanRow& r) {
         if (slots + r.slots > INT32_MAX) fail(SATORI_HIP_E_OVERFLOW, "Arithmetic operation resulted in an overflow.");
         r.slot = static_cast<int>(slots);
         slots += r.slots;
-        image.header.joined += r.slots > 1;
-    }
+    };
+    for (PlanRow& r : rows)
+        if (r.slots > 1) {
+            number(r);
+            ++image.header.joined;
+        }
+    image.header.partials = static_cast<int>(slots);
+    for (PlanRow& r : rows)
+        if (r.slots == 1) number(r);
     image.header.slots = static_cast<int>(slots);
 
     // The workgroups. Consecutive workgroups run on different XCDs (eight, each with an L2 of its own), so the blocks of

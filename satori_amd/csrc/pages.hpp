@@ -100,10 +100,11 @@ struct PlanRun {
     int position, pad[3];
 };
 
-// At the start of the image.
+// At the start of the image. Rows of several slots are `joined`; their slots come first, `partials` of them, and only those
+// are memory: a row of one slot has a number behind them, and its result goes straight to the output.
 struct PlanHeader {
     int rows, narrow, wide, runs;
-    int joined, slots, longest_run, pad;  // joined: rows of several slots; slots: of all rows
+    int joined, slots, longest_run, partials;
 };
 
 // Where the arrays lie in the image (in 4-byte words from its start) and how many entries each has room for. Launches

@@ -2495,12 +2495,18 @@ int satori_hip_cache_plan_set(satori_hip_cache_plan* p, satori_hip_pages* pages,
         const PlanLayout used = image.least();
         if (layout.grow(used) && held(p)) plan_held();
         const size_t bytes = static_cast<size_t>(layout.words) * 4;
-        if (held(p) && (bytes > p->image.bytes || cache_partial_bytes(p->shape, image.header.slots) > p->partials.bytes))
-            plan_held();
+        const size_t partials = cache_partial_bytes(p->shape, image.header.partials);
+        if (held(p) && (bytes > p->image.bytes || partials > p->partials.bytes)) plan_held();
         const CaptureRelaxed relaxed;  // another stream may be in a capture that forbids allocations
         p->set = false;  // until the new batch is on its way: where memory cannot be had, the old one's may be gone
+        // The rows' queries and outputs, which the calls need beside it (asked of the device only where it could matter).
+        const double rows_bytes = 8.0 * image.header.rows * p->shape.heads * p->shape.head_dim;
+        size_t free_bytes = 0, all_bytes = 0;
+        if (rows_bytes > 0x1p36) check_hip(hipMemGetInfo(&free_bytes, &all_bytes), "hipMemGetInfo");
+        if (rows_bytes > 0x1p36 && rows_bytes > static_cast<double>(all_bytes))
+            fail(SATORI_HIP_E_OUT_OF_MEMORY, "The queries and outputs of the plan's rows exceed the device's memory.");
         reserve_for_plan(p, p->image, bytes);
-        reserve_for_plan(p, p->partials, cache_partial_bytes(p->shape, image.header.slots));
+        reserve_for_plan(p, p->partials, partials);
         const int turn = p->turn;
         check_hip(hipEventSynchronize(p->copied[turn]), "plan copy");  // (done at once where none was recorded)
         p->staging[turn].reserve(p->image.bytes);
