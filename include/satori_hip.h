@@ -480,9 +480,11 @@ int satori_hip_cache_copy_pages(satori_hip_context* context, void* pool, int64_t
  * the device is enqueued on `stream`, so the launches that read it must follow on that stream (or be ordered by the
  * caller); not while capturing. A captured step reads the plan when it is replayed: capture a step once, then extend, set
  * and replay it per token, with as many rows as its other launches were captured with (the buffers that the captured calls
- * were given must hold every later batch's rows). While steps read a plan, a batch that needs more memory than the largest
- * before fails with SATORI_HIP_E_INVALID_OPERATION, and so does one whose rows lie in shared pages if a step writes them; the
- * plan stays as it was. After a call in another library's capture the plan is read by that graph until the plan is destroyed
+ * were given must hold every later batch's rows). While steps read a plan, its memory stays what it is: every batch of no
+ * more rows, no more sequences that have any and no longer page lists (together, and the longest) than one that was set before
+ * the capture is taken, divided into fewer parts where the usual ones do not fit (unless the plan's own data would be larger than
+ * 256 MB); one that does not fit fails with SATORI_HIP_E_INVALID_OPERATION, and so does one whose rows lie in shared pages if a
+ * step writes them; the plan stays as it was. After a call in another library's capture the plan is read by that graph until the plan is destroyed
  * (which must come after the graph's end). Each plan owns the workspace of its attention, so calls on one plan must not
  * overlap in time on different streams; different plans may. A batch whose queries and outputs together exceed the device's
  * memory fails with SATORI_HIP_E_OUT_OF_MEMORY. After a set that failed for memory or on the device, calls fail until one

@@ -213,6 +213,9 @@ constexpr int kTile = 32;         // tokens a wave attends at once
 constexpr int kWaves = 4;         // of a workgroup, which take tiles in turn
 constexpr int kNarrowPairs = 16;  // pairs of a narrow workgroup
 constexpr int64_t kNarrowBytes = 128 << 20;
+constexpr int kMostTokens = 1 << 20;  // of an item
+// A layout larger than this is not made larger still for plain divisions to come.
+constexpr int64_t kMostPlainWords = 64 << 20;
 
 // Tokens [begin, end) of the pages of `sequence`, seen by the rows of the sequences members[0 .. count).
 struct Node {
@@ -238,7 +241,7 @@ constexpr int64_t kPlaces = 512, kRoundBytes = 128 << 20;
 }  // namespace
 
 PlanImage plan_batch(const PageTables& tables, const int* sequences, const int* new_tokens, int count,
-                     const PlanShape& shape) {
+                     const PlanShape& shape, const PlanDivision& division) {
     PlanImage image;
     const int P = tables.page_tokens();
     std::vector<int> sorted(sequences, sequences + count);
@@ -271,7 +274,7 @@ PlanImage plan_batch(const PageTables& tables, const int* sequences, const int* 
     int64_t own = 0;  // items of the sequences by themselves, at least
     for (int i = 0; i < count; ++i) own += blocks_of(static_cast<int64_t>(new_tokens[i]) * shape.group) * shape.kv_heads;
     const auto worth_sharing = [&](const std::vector<int>& members, int64_t tokens) {
-        if (tokens < kLeastShared) return false;
+        if (division.plain || tokens < kLeastShared) return false;
         int64_t pairs = 0, apart = 0;
         for (int m : members) {
             pairs += static_cast<int64_t>(new_tokens[m]) * shape.group;
@@ -357,7 +360,7 @@ PlanImage plan_batch(const PageTables& tables, const int* sequences, const int* 
     const auto pairs_a_block = [&](const Node& n) { return n.wide ? shape.wide_pairs : kNarrowPairs; };
     for (size_t i = 0; i < nodes.size(); ++i) {
         Node& n = nodes[i];
-        n.wide &= again > kNarrowBytes / shape.token_bytes;
+        n.wide &= division.plain || again > kNarrowBytes / shape.token_bytes;
         const int64_t blocks = (pairs_of[i] + pairs_a_block(n) - 1) / pairs_a_block(n);
         (n.wide ? wide_tokens : narrow_tokens) += blocks * shape.kv_heads * (n.end - n.begin);
     }
@@ -365,12 +368,13 @@ PlanImage plan_batch(const PageTables& tables, const int* sequences, const int* 
     // one tile per wave. (Few pairs in 256, 512 and 1024 workgroups: 24 rows over 4000 positions, FP32, 23.0, 28.9 and 31.6 us, 64
     // of 1000 to 2000, F16, 68, 78 and 80, 9 x 5 over 4000 16.9, 15.4 and 19.3. Many in 256 and 512: 64 rows over 8192, F16, 46
     // and 58, over 32768 103 and 102, 24 over 8192, FP32, 35 and 31: the more chunks, the more partial results.)
-    const auto chunk_for = [&](int64_t tokens, int workgroups) {
+    const auto chunk_for = [&](int64_t tokens) {
+        if (division.plain) return kMostTokens;
         const int64_t step = kTile * kWaves;
-        const int64_t c = (tokens / workgroups + step - 1) / step * step;
-        return static_cast<int>(std::min<int64_t>(std::max<int64_t>(c, step), 1 << 20));
+        const int64_t c = (tokens / division.workgroups + step - 1) / step * step;
+        return static_cast<int>(std::min<int64_t>(std::max<int64_t>(c, step), kMostTokens));
     };
-    const int narrow_chunk = chunk_for(narrow_tokens, 256), wide_chunk = chunk_for(wide_tokens, 256);
+    const int narrow_chunk = chunk_for(narrow_tokens), wide_chunk = chunk_for(wide_tokens);
 
     std::vector<int>& page_list = image.pages;
     std::vector<int> row_list;
@@ -459,7 +463,44 @@ PlanImage plan_batch(const PageTables& tables, const int* sequences, const int* 
     h.narrow = static_cast<int>(narrow.size());
     h.wide = static_cast<int>(wide.size());
     h.runs = static_cast<int>(runs.size());
+
+    // What plain divisions take at most: a sequence's pairs fill their blocks but for the last one, sequences of up to half a
+    // wide workgroup's pairs (no more than that many blocks each) are narrow, those of more (so many there can be) wide; a run
+    // ends at a page's end or the sequence's.
+    int64_t of_rows = 0, list_pages = 0, longest = 0;
+    for (int i = 0; i < count; ++i)
+        if (new_tokens[i] > 0) {
+            ++of_rows;
+            list_pages += static_cast<int64_t>(tables.table(sequences[i]).size());
+            longest = std::max<int64_t>(longest, tables.tokens(sequences[i]));
+        }
+    const int64_t all = static_cast<int64_t>(h.rows) * shape.group, chunks = (longest + kMostTokens - 1) / kMostTokens;
+    const int64_t units = chunks * shape.kv_heads;
+    const int64_t narrow_blocks = std::min(all / kNarrowPairs + of_rows, of_rows * blocks_of(shape.wide_pairs / 2));
+    const int64_t wide_blocks = all / shape.wide_pairs + std::min(of_rows, 2 * all / shape.wide_pairs);
+    const auto entries = [](int64_t n) { return static_cast<int>(std::min<int64_t>(n, INT32_MAX / 64)); };
+    image.plain.rows = image.plain.list = h.rows;
+    image.plain.runs = entries(std::min<int64_t>(h.rows, h.rows / P + 2 * of_rows));
+    image.plain.pages = entries(list_pages);
+    image.plain.narrow = entries(narrow_blocks * units);
+    image.plain.wide = entries(wide_blocks * units);
+    image.plain_partials = chunks > 1 ? h.rows * chunks : 0;
     return image;
+}
+
+bool plan_batch_within(const PageTables& tables, const int* sequences, const int* new_tokens, int count,
+                       const PlanShape& shape, const PlanLayout& room, int64_t partials, PlanImage& image) {
+    PlanDivision division;
+    for (;;) {
+        image = plan_batch(tables, sequences, new_tokens, count, shape, division);
+        if (room.holds(image.least()) && image.header.partials <= partials) return true;
+        if (division.plain || image.header.rows > room.rows) return false;
+        division.workgroups > 1 ? void(division.workgroups /= 2) : void(division = kPlainDivision);
+    }
+}
+
+bool PlanLayout::holds(const PlanLayout& l) const {
+    return l.rows <= rows && l.narrow <= narrow && l.wide <= wide && l.runs <= runs && l.pages <= pages && l.list <= list;
 }
 
 bool PlanLayout::grow(const PlanLayout& least) {
@@ -493,11 +534,18 @@ bool PlanLayout::grow(const PlanLayout& least) {
     return true;
 }
 
+void PlanLayout::grow_plain(const PlanLayout& plain) {
+    const int64_t most = 2 * (static_cast<int64_t>(plain.rows + int64_t(plain.list)) * (sizeof(PlanRow) / 4) +
+                              (plain.narrow + int64_t(plain.wide)) * (sizeof(PlanItem) / 4) +
+                              int64_t(plain.runs) * (sizeof(PlanRun) / 4) + plain.pages);
+    if (words + most <= kMostPlainWords) grow(plain);
+}
+
 PlanLayout PlanLayout::first() {
     PlanLayout least, layout;
     least.rows = least.runs = 256;
     least.narrow = least.wide = 1024;
-    least.pages = 16384;
+    least.pages = 32768;
     least.list = 1024;
     layout.grow(least);
     return layout;

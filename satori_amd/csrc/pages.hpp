@@ -114,6 +114,9 @@ struct PlanLayout {
     int rows = 0, narrow = 0, wide = 0, runs = 0, pages = 0, list = 0;
     // Room for at least these; whether anything moved.
     bool grow(const PlanLayout& least);
+    bool holds(const PlanLayout& least) const;
+    // Room for plain divisions as well (PlanImage::plain), unless the image would be very large.
+    void grow_plain(const PlanLayout& plain);
     // What a plan begins with: a batch of a few hundred rows over long sequences, so that a captured step has room to
     // follow it.
     static PlanLayout first();
@@ -134,12 +137,29 @@ struct PlanImage {
     std::vector<int> pages;
     bool writable = true;  // no page that the rows lie in is shared
     PlanLayout least() const;  // the room they take
+    // What kPlainDivision can take of any batch of no more rows, sequences with rows and pages in their lists, none of them
+    // longer: both grow with the batch, unlike what the usual division takes.
+    PlanLayout plain{};
+    int64_t plain_partials = 0;
     void write(const PlanLayout& layout, int* words) const;
 };
 
+// How a batch's attention is divided: chunks for about so many workgroups, and whether runs of pages are attended once for all
+// sequences that share them. Plain: every sequence by itself in one chunk (of kMostTokens), so that what it takes follows from the
+// numbers of rows, sequences and pages alone.
+struct PlanDivision {
+    int workgroups = 256;
+    bool plain = false;
+};
+constexpr PlanDivision kPlainDivision{1, true};
+
 // Rows: the last new_tokens[i] positions of sequences[i], in this order.
 PlanImage plan_batch(const PageTables& tables, const int* sequences, const int* new_tokens, int count,
-                     const PlanShape& shape);
+                     const PlanShape& shape, const PlanDivision& division = {});
+
+// The batch in the room that a plan has: in the usual division, or the first coarser one that fits. Whether one does.
+bool plan_batch_within(const PageTables& tables, const int* sequences, const int* new_tokens, int count,
+                       const PlanShape& shape, const PlanLayout& room, int64_t partials, PlanImage& image);
 
 // The tables behind a handle (satori_hip_pages_*).
 PageTables& page_tables(satori_hip_pages* handle);

@@ -2326,8 +2326,8 @@ int plan_call(satori_hip_cache_plan* p, F&& body) {
 
 [[noreturn]] void plan_held() {
     fail(SATORI_HIP_E_INVALID_OPERATION,
-         "The memory of this plan cannot grow while a captured step reads it: destroy the step, or set the largest batch "
-         "before capturing.");
+         "The memory of this plan cannot grow while a captured step reads it: destroy the step, or set a batch of as many "
+         "rows, sequences and pages before capturing.");
 }
 
 bool held(const satori_hip_cache_plan* p) { return p->steps > 0 || p->elsewhere; }
@@ -2484,7 +2484,12 @@ int satori_hip_cache_plan_set(satori_hip_cache_plan* p, satori_hip_pages* pages,
                 fail(SATORI_HIP_E_OBJECT_DISPOSED, "Cannot access a disposed object. Object name: 'satori_hip_pages'.");
             if (tables.pages() != p->page_count || tables.page_tokens() != p->shape.page_tokens)
                 fail(SATORI_HIP_E_ARGUMENT, "The pages are not those of the plan's pool.");
-            image = plan_batch(tables, sequences, new_tokens, count, p->plan);
+            if (held(p)) {
+                const int64_t room = static_cast<int64_t>(p->partials.bytes / cache_partial_bytes(p->shape, 1));
+                if (!plan_batch_within(tables, sequences, new_tokens, count, p->plan, p->layout, room, image)) plan_held();
+            } else {
+                image = plan_batch(tables, sequences, new_tokens, count, p->plan);
+            }
         }
         if (static_cast<int64_t>(image.header.rows) * p->shape.heads > INT32_MAX / 4)
             fail(SATORI_HIP_E_OVERFLOW, "Arithmetic operation resulted in an overflow.");
@@ -2493,10 +2498,13 @@ int satori_hip_cache_plan_set(satori_hip_cache_plan* p, satori_hip_pages* pages,
                  "A captured step writes the rows, which lie in pages that other sequences hold: extend their sequences.");
         PlanLayout layout = p->layout;
         const PlanLayout used = image.least();
-        if (layout.grow(used) && held(p)) plan_held();
+        size_t partials = cache_partial_bytes(p->shape, image.header.partials);
+        if (!held(p)) {
+            layout.grow(used);
+            layout.grow_plain(image.plain);
+            partials = std::max(partials, cache_partial_bytes(p->shape, image.plain_partials));
+        }
         const size_t bytes = static_cast<size_t>(layout.words) * 4;
-        const size_t partials = cache_partial_bytes(p->shape, image.header.partials);
-        if (held(p) && (bytes > p->image.bytes || partials > p->partials.bytes)) plan_held();
         const CaptureRelaxed relaxed;  // another stream may be in a capture that forbids allocations
         p->set = false;  // until the new batch is on its way: where memory cannot be had, the old one's may be gone
         // The rows' queries and outputs, which the calls need beside it (asked of the device only where it could matter).

@@ -38,3 +38,38 @@ def test_a_prompt_in_one_chunk_needs_no_partial_results(context, device):  # noq
     check_attention(pool, [s], [rows], heads, q, context.download(np.zeros_like(q), out))
     step.dispose()
     plan.dispose()
+
+
+def test_a_captured_step_goes_from_long_sequences_to_short_ones(context, device):  # noqa: F811
+    # 32 sequences over 2000 shared positions: with 10 positions of their own the usual division asks for more partial results
+    # than with 390, and than the plan has; the batch is divided into fewer parts.
+    g = rng(390)
+    heads, kv, D, count = 32, 8, 256, 32
+    pool = Pool(context, device, CacheLayout(1, kv, D, 32, F16), 63 + 32 * 14)
+    c = pool.cache
+    first = c.open()
+    c.extend([first], [2000])
+    sequences = [first] + c.fork(first, count - 1)
+    c.extend(sequences, [390] * count)
+    pool.write(g, sequences)
+    q = g.standard_normal((count, heads, D)).astype(np.float32)
+    dq, out = device(q), device(np.zeros_like(q))
+    plan, ones = c.plan(heads), [1] * count
+    plan.set(sequences, ones)
+    context.capture_begin()
+    plan.attention(0, dq, out)
+    step = context.capture_end()
+    some = [0, 1, 17, 31]
+    for own in (390, 10, 200, 1):
+        for s in sequences:
+            c.truncate(s, 2000 + own) if c.tokens(s) > 2000 + own else c.extend([s], [2000 + own - c.tokens(s)])
+        if own == 200:  # (positions that were given up hold whatever they held: written anew)
+            pool.write(g, sequences)
+        plan.set(sequences, ones)
+        context.upload(out, np.full_like(q, np.nan))
+        step.execute()
+        got = context.download(np.zeros_like(q), out)
+        check_attention(pool, [sequences[i] for i in some], [1] * 4, heads, q[some], got[some], label=str(own))
+        assert np.isfinite(got).all()
+    step.dispose()
+    plan.dispose()

@@ -34,3 +34,7 @@ def run(exe, what):
 
 def test_rows_of_one_part_ask_for_no_partial_results(harness):
     run(harness, "partials")
+
+
+def test_a_plan_has_room_for_every_smaller_batch(harness):
+    run(harness, "smaller")
