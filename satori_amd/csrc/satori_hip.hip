@@ -112,6 +112,18 @@ struct PinnedBuffer {
 }  // namespace
 }  // namespace satori
 
+namespace satori {
+namespace {
+
+// A plan that a captured launch reads, and whether one writes the plan's rows into their pages.
+struct PlanUse {
+    satori_hip_cache_plan* plan;
+    bool appends;
+};
+
+}  // namespace
+}  // namespace satori
+
 struct satori_hip_context {
     int device = 0;
     hipStream_t stream = nullptr;
@@ -147,7 +159,7 @@ struct satori_hip_context {
     int captured_last[2] = {-1, -1};                     // the two in turn now
     std::vector<satori_hip_matrix*> captured_matrices;
     std::vector<satori_hip_group*> captured_groups;
-    std::vector<satori_hip_cache_plan*> captured_plans;
+    std::vector<satori::PlanUse> captured_plans;
     std::vector<satori_hip_adapters*> captured_adapters;
     int plans = 0, adapters = 0;  // live ones
 };
@@ -203,8 +215,9 @@ struct satori_hip_cache_plan {
     hipEvent_t copied[2] = {nullptr, nullptr};
     int turn = 0;
     int steps = 0;                   // captured steps that read the plan
-    bool elsewhere = false;          // another library's graph may read it (until the plan is destroyed: its end is not told)
-    bool appended = false;           // by a captured launch
+    int appends = 0;                 // those of them that write its rows
+    // Another library's graph may read it, or write its rows (until the plan is destroyed: such a graph's end is not told).
+    bool elsewhere = false, appended_elsewhere = false;
     bool live = true;
 };
 
@@ -228,7 +241,7 @@ struct satori_hip_step {
     std::vector<satori_hip_matrix*> matrices;  // launched directly in a captured step (each counts it)
     std::vector<satori::DeviceBuffer> scratch; // partial sums of its Q8_0 / Q4_0 batches
     bool attention = false;                    // the graph uses the context's split-attention workspace
-    std::vector<satori_hip_cache_plan*> plans; // read by the graph, and what they and the adapters own
+    std::vector<satori::PlanUse> plans;        // read by the graph (each once), and what they and the adapters own
     std::vector<satori_hip_adapters*> adapters;
     hipGraph_t graph = nullptr;
     hipGraphExec_t exec = nullptr;
@@ -1626,8 +1639,10 @@ int satori_hip_step_destroy(satori_hip_step* s) {
         }
         if (s->attention) c->attention_steps--;
         s->attention = false;
-        for (satori_hip_cache_plan* p : s->plans)
-            if (--p->steps == 0) p->appended = p->elsewhere && p->appended;
+        for (const PlanUse& use : s->plans) {
+            use.plan->steps--;
+            use.plan->appends -= use.appends;
+        }
         for (satori_hip_adapters* a : s->adapters) a->steps--;
         s->plans.clear();
         s->adapters.clear();
@@ -1669,7 +1684,7 @@ int satori_hip_capture_end(satori_hip_context* c, satori_hip_step** step) {
         std::vector<satori_hip_group*> groups;
         matrices.swap(c->captured_matrices);
         groups.swap(c->captured_groups);
-        std::vector<satori_hip_cache_plan*> plans;
+        std::vector<PlanUse> plans;
         std::vector<satori_hip_adapters*> adapters;
         plans.swap(c->captured_plans);
         adapters.swap(c->captured_adapters);
@@ -1708,11 +1723,16 @@ int satori_hip_capture_end(satori_hip_context* c, satori_hip_step** step) {
                 m->steps++;
             }
         }
-        for (satori_hip_cache_plan* p : plans) {
-            if (std::find(st->plans.begin(), st->plans.end(), p) == st->plans.end()) {
-                st->plans.push_back(p);
-                p->steps++;
-            }
+        for (const PlanUse& use : plans) {
+            const auto at = std::find_if(st->plans.begin(), st->plans.end(), [&](const PlanUse& u) { return u.plan == use.plan; });
+            if (at == st->plans.end())
+                st->plans.push_back(use);
+            else
+                at->appends |= use.appends;
+        }
+        for (const PlanUse& use : st->plans) {
+            use.plan->steps++;
+            use.plan->appends += use.appends;
         }
         for (satori_hip_adapters* a : adapters) {
             if (std::find(st->adapters.begin(), st->adapters.end(), a) == st->adapters.end()) {
@@ -2350,16 +2370,17 @@ void free_plan(satori_hip_cache_plan* p) {
     }
 }
 
-// What the calls on a plan ask of it, and whether the launch becomes part of a captured step.
-bool note_plan(satori_hip_context* c, satori_hip_cache_plan* p, int layer, hipStream_t stream) {
+// What the calls on a plan ask of it, and whether the launch becomes part of a captured step. `appends`: it writes the rows.
+bool note_plan(satori_hip_context* c, satori_hip_cache_plan* p, int layer, hipStream_t stream, bool appends) {
     if (layer < 0 || layer >= p->layers) out_of_range("layer");
     const bool captured = c->capturing && stream == c->stream;
     if (captured) {
-        c->captured_plans.push_back(p);
+        c->captured_plans.push_back({p, appends});
         return true;
     }
     if (!captured_elsewhere(c, stream)) return false;
     p->elsewhere = true;
+    p->appended_elsewhere |= appends;
     return true;
 }
 
@@ -2493,7 +2514,7 @@ int satori_hip_cache_plan_set(satori_hip_cache_plan* p, satori_hip_pages* pages,
         }
         if (static_cast<int64_t>(image.header.rows) * p->shape.heads > INT32_MAX / 4)
             fail(SATORI_HIP_E_OVERFLOW, "Arithmetic operation resulted in an overflow.");
-        if (!image.writable && p->appended && held(p))
+        if (!image.writable && (p->appends > 0 || p->appended_elsewhere))
             fail(SATORI_HIP_E_INVALID_OPERATION,
                  "A captured step writes the rows, which lie in pages that other sequences hold: extend their sequences.");
         PlanLayout layout = p->layout;
@@ -2553,8 +2574,7 @@ int satori_hip_cache_append(satori_hip_cache_plan* p, int layer, const float* qu
             bytes_overlap(query_out, qb, s.pool, pool) || bytes_overlap(key, kb, s.pool, pool) ||
             bytes_overlap(value, kb, s.pool, pool))
             fail(SATORI_HIP_E_ARGUMENT, "Partial overlap.");
-        const bool captured = note_plan(c, p, layer, st);
-        p->appended |= captured;
+        const bool captured = note_plan(c, p, layer, st, true);
         const AppendArgs args{query, query_bias, key, key_bias, value, value_bias, query_out, frequency_base,
                               rotary_dimensions, rope_table, rope_table ? rope_positions : 0, layer};
         check_hip(launch_cache_append(s, static_cast<const int*>(p->image.ptr), p->layout, p->header, captured, args, st),
@@ -2573,7 +2593,7 @@ int satori_hip_cache_attention(satori_hip_cache_plan* p, int layer, const float*
         const int64_t pool = s.page_bytes * p->page_count;
         if (bytes_overlap(query, bytes, output, bytes) || bytes_overlap(output, bytes, s.pool, pool))
             fail(SATORI_HIP_E_ARGUMENT, "Attention output overlaps input.");
-        const bool captured = note_plan(c, p, layer, st);
+        const bool captured = note_plan(c, p, layer, st, false);
         check_hip(launch_cache_attention(s, static_cast<const int*>(p->image.ptr), p->layout, p->header, captured, layer, query,
                                          output, static_cast<float*>(p->partials.ptr), p->partials.bytes, st),
                   "cache attention launch");

@@ -73,3 +73,38 @@ def test_a_captured_step_goes_from_long_sequences_to_short_ones(context, device)
         assert np.isfinite(got).all()
     step.dispose()
     plan.dispose()
+
+
+def test_a_plan_is_written_by_the_steps_that_append(context, device):  # noqa: F811
+    # Two steps read a plan and the first of them writes its rows; once that one is gone, batches in shared pages are taken
+    # again, whatever the other does. A plan whose only append was captured in a step that is gone is written by nothing.
+    pool = Pool(context, device, CacheLayout(1, 1, 32, 32, F16), 8)
+    c = pool.cache
+    s = c.open()
+    c.extend([s], [40])
+    plan = c.plan(1)
+    plan.set([s], [1])
+    q, out = device(np.zeros((1, 32), np.float32)), device(np.zeros((1, 32), np.float32))
+
+    def captured(*calls):
+        context.capture_begin()
+        for call in calls:
+            call()
+        return context.capture_end()
+
+    append = lambda: plan.append(0, q, 0, out, q, 0, q, 0, 1e4, 32)  # noqa: E731
+    attend = lambda: plan.attention(0, q, out)  # noqa: E731
+    both, reads, again = captured(attend, append, attend, append), captured(attend), captured(append)
+    other = c.fork(s)[0]
+    for step in (both, again):
+        with pytest.raises(S.InvalidOperationException):
+            plan.set([s, other], [1, 0])
+        step.dispose()
+    plan.set([s, other], [1, 0])  # `reads` alone is left
+    reads.execute()
+    with pytest.raises(S.InvalidOperationException):
+        append()
+    context.synchronize()
+    reads.dispose()
+    plan.set([s, other], [1, 0])
+    plan.dispose()
