@@ -433,7 +433,9 @@ int satori_hip_matrix_decode_row(satori_hip_matrix* matrix, int row, float* outp
  * handle's calls exclude one another); the pages' bytes are the caller's pool on the device. Where a call says that page
  * bytes must follow, it gives moves (source page, destination page), which the caller hands to
  * satori_hip_cache_copy_pages before anything reads or writes the destinations. Sources and destinations of one call's
- * moves are different pages. A call that fails changes nothing. New pages and sequence numbers are the lowest free ones. */
+ * moves are different pages. A call that fails changes nothing. New pages and sequence numbers are the lowest free ones, so a
+ * page that a call gives up may be in the next sequence's list, and be written to, at once: launches that still read it must come
+ * before those that write it, on the same stream or ordered by the caller. */
 int satori_hip_pages_create(int page_count, int page_tokens, satori_hip_pages** pages);
 /* Idempotent: NULL is accepted. */
 int satori_hip_pages_destroy(satori_hip_pages* pages);

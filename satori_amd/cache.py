@@ -187,7 +187,10 @@ class CacheLayout:
 
 class PagedCache:
     """A pool of pages on the device with its page table: the calls of PageTable (open, tokens and pages are the table's
-    own), with the page bytes moved on the context stream. `pool` is a device pointer to page_count * layout.page_bytes bytes; 0: allocated here."""
+    own), with the page bytes moved on `stream` (0: the context stream), which is to be the one that the cache's plans run on
+    (or ordered with it): a move reads what they have written and comes before what they write next. The same holds for pages
+    that free, truncate and compact give up: the next sequence to get them may be written to while a plan on another stream
+    still reads them. `pool` is a device pointer to page_count * layout.page_bytes bytes; 0: allocated here."""
 
     def __init__(self, context: HipContext, layout: CacheLayout, page_count: int, pool: int = 0):
         self.context, self.layout, self.page_count = context, layout, page_count
@@ -199,24 +202,24 @@ class PagedCache:
         self.pool = pool
         self.open, self.pages, self.tokens = self.table.open, self.table.pages, self.table.tokens
 
-    def _move(self, moves: _Moves) -> None:
+    def _move(self, moves: _Moves, stream: int) -> None:
         if moves.count:
-            self._copy_pages(moves.sources, moves.destinations, moves.count)
+            self._copy_pages(moves.sources, moves.destinations, moves.count, stream)
 
-    def copy_pages(self, sources, destinations) -> None:
+    def copy_pages(self, sources, destinations, stream: int = 0) -> None:
         """Pool page destinations[i] = pool page sources[i] (moves of a page table's own calls, for instance)."""
         s, d = _array(sources), _array(destinations)
         if len(s) != len(d):
             raise ArgumentException("Lengths differ.")
-        self._copy_pages(_address(s), _address(d), len(s))
+        self._copy_pages(_address(s), _address(d), len(s), stream)
 
-    def _copy_pages(self, sources: int, destinations: int, count: int) -> None:
+    def _copy_pages(self, sources: int, destinations: int, count: int, stream: int) -> None:
         _check(_ffi.lib().satori_hip_cache_copy_pages(self.context.handle, self.pool, self.page_bytes, self.page_count,
-                                                      sources, destinations, count, None))
+                                                      sources, destinations, count, stream or None))
 
-    def extend(self, sequences, tokens) -> None:
+    def extend(self, sequences, tokens, stream: int = 0) -> None:
         """Makes room for tokens[i] more positions of sequences[i]."""
-        self._move(self.table._extend(sequences, tokens))
+        self._move(self.table._extend(sequences, tokens), stream)
 
     def truncate(self, sequence: int, tokens: int) -> None:
         self.table.truncate(sequence, tokens)
@@ -224,16 +227,16 @@ class PagedCache:
     def fork(self, sequence: int, count: int = 1) -> list[int]:
         return self.table.fork(sequence, count)
 
-    def copy(self, sequence: int) -> int:
+    def copy(self, sequence: int, stream: int = 0) -> int:
         made, moves = self.table._copy(sequence)
-        self._move(moves)
+        self._move(moves, stream)
         return made
 
     def free(self, sequences) -> None:
         self.table.free(sequences)
 
-    def compact(self) -> None:
-        self._move(self.table._compact())
+    def compact(self, stream: int = 0) -> None:
+        self._move(self.table._compact(), stream)
 
     @property
     def free_pages(self) -> int:

@@ -108,3 +108,36 @@ def test_a_plan_is_written_by_the_steps_that_append(context, device):  # noqa: F
     reads.dispose()
     plan.set([s, other], [1, 0])
     plan.dispose()
+
+
+def test_page_moves_on_a_plans_stream(context, device):  # noqa: F811
+    # A position is appended on another stream, behind page copies that keep it busy; a fork made after it on the same stream
+    # holds the position in a page of its own.
+    layout = CacheLayout(64, 2, 64, 32, F16)
+    pool = Pool(context, device, layout, 400)
+    c = pool.cache
+    pool.host[...] = 0
+    pool.upload()
+    s = c.open()
+    c.extend([s], [40])
+    kv = rng(5).standard_normal((1, 2 * 64)).astype(np.float32)
+    q, dkv, out = device(np.zeros((1, 2 * 64), np.float32)), device(kv), device(np.zeros((1, 2 * 64), np.float32))
+    plan = c.plan(2)
+    context.synchronize()
+    with S.HipContext(0) as elsewhere:
+        stream = elsewhere.stream
+        plan.set([s], [1], stream)
+        for _ in range(40):
+            c.copy_pages(range(10, 200), range(200, 390), stream)
+        plan.append(63, q, 0, out, dkv, 0, dkv, 0, 1e4, 2, stream=stream)
+        fork = c.fork(s)[0]
+        c.extend([fork], [1], stream)
+        twin = c.copy(s, stream)
+        c.free([s])
+        c.compact(stream)
+        elsewhere.synchronize()
+    pool.download()
+    assert len({c.pages(t)[1] for t in (fork, twin)}) == 2
+    for t in (fork, twin):
+        assert np.array_equal(pool.of(t, 63)[1][39], kv.reshape(2, 64).astype(np.float16).astype(np.float64)), t
+    plan.dispose()
