@@ -11,6 +11,7 @@ import ctypes
 import enum
 import threading
 from array import array
+from collections import deque
 from collections.abc import Sequence
 from dataclasses import dataclass
 
@@ -190,13 +191,15 @@ class PagedCache:
     own), with the page bytes moved on `stream` (0: the context stream), which is to be the one that the cache's plans run on
     (or ordered with it): a move reads what they have written and comes before what they write next. The same holds for pages
     that free, truncate and compact give up: the next sequence to get them may be written to while a plan on another stream
-    still reads them. `pool` is a device pointer to page_count * layout.page_bytes bytes; 0: allocated here."""
+    still reads them. Where the device takes no copy (an exception), `copy` leaves no sequence behind; after extend and compact
+    the table has changed, and the moves stay due: the next call that moves pages, or sets a plan, makes them first.
+    `pool` is a device pointer to page_count * layout.page_bytes bytes; 0: allocated here."""
 
     def __init__(self, context: HipContext, layout: CacheLayout, page_count: int, pool: int = 0):
         self.context, self.layout, self.page_count = context, layout, page_count
         self.page_bytes = layout.page_bytes
         self.table = PageTable(page_count, layout.page_tokens)
-        self._owned = 0
+        self._owned, self._due = 0, deque()
         if not pool:
             self._owned = pool = context.alloc(page_count * self.page_bytes)
         self.pool = pool
@@ -204,13 +207,22 @@ class PagedCache:
 
     def _move(self, moves: _Moves, stream: int) -> None:
         if moves.count:
+            self._due.append(moves)
+        if self._due:
+            self._settle(stream)
+
+    def _settle(self, stream: int) -> None:
+        while self._due:  # (what is copied twice, where a call failed behind its first launch, is the same)
+            moves = self._due[0]
             self._copy_pages(moves.sources, moves.destinations, moves.count, stream)
+            self._due.popleft()
 
     def copy_pages(self, sources, destinations, stream: int = 0) -> None:
         """Pool page destinations[i] = pool page sources[i] (moves of a page table's own calls, for instance)."""
         s, d = _array(sources), _array(destinations)
         if len(s) != len(d):
             raise ArgumentException("Lengths differ.")
+        self._settle(stream)
         self._copy_pages(_address(s), _address(d), len(s), stream)
 
     def _copy_pages(self, sources: int, destinations: int, count: int, stream: int) -> None:
@@ -228,8 +240,14 @@ class PagedCache:
         return self.table.fork(sequence, count)
 
     def copy(self, sequence: int, stream: int = 0) -> int:
+        self._settle(stream)
         made, moves = self.table._copy(sequence)
-        self._move(moves, stream)
+        try:
+            self._move(moves, stream)
+        except Exception:
+            self._due.clear()  # (its own: nothing else was due)
+            self.table.free([made])
+            raise
         return made
 
     def free(self, sequences) -> None:
@@ -272,6 +290,7 @@ class CachePlan:
         ids, counts = _ints(sequences), _ints(new_tokens)
         if ids.size != counts.size:
             raise ArgumentException("Lengths differ.")
+        self.cache._settle(stream)
         _check(_ffi.lib().satori_hip_cache_plan_set(self._handle, self.cache.table.handle, _at(ids), _at(counts),
                                                     ids.size, _pointer(stream)))
 

@@ -5,8 +5,10 @@ from __future__ import annotations
 import ctypes
 from types import SimpleNamespace
 
+import pytest
+
 import satori_amd as S
-from satori_amd.cache import CacheLayout, PagedCache
+from satori_amd.cache import CacheLayout, CachePlan, PagedCache
 
 
 class Copies:
@@ -45,3 +47,47 @@ def test_page_moves_take_a_stream(monkeypatch):
     other = c.fork(twin)[0]
     c.extend([other], [1])
     assert copies.calls[-1][2] is None  # the context stream
+
+
+def test_a_copy_that_fails_is_made_up_for(monkeypatch):
+    copies = Copies(monkeypatch)
+    c = host_only_cache(16)
+    s = c.open()
+    c.extend([s], [40])
+    f = c.fork(s)[0]
+    copies.failing = True
+    before = c.free_pages
+    for _ in range(2):  # (the second finds what is due, and makes nothing of its own)
+        with pytest.raises(S.InvalidOperationException):
+            c.extend([f], [1])
+        assert c.tokens(f) == 41
+        with pytest.raises(S.InvalidOperationException):
+            c.copy(s)
+        assert c.free_pages == before - 1, "a copy that failed leaves nothing"
+        c.truncate(f, 40)
+    c.free([s])
+    with pytest.raises(S.InvalidOperationException):
+        c.compact()
+    plan = object.__new__(CachePlan)
+    plan.cache, plan._handle = c, None
+    with pytest.raises(S.InvalidOperationException):
+        plan.set([f], [1])
+    copies.failing = False
+    c.extend([f], [1], 5)
+    assert c.pages(f) == [0, 1]
+    assert copies.calls == [([1], [2], 5), ([2], [1], 5)], "in their order, before what comes next"
+    c.extend([f], [1])
+    assert len(copies.calls) == 2
+
+
+def test_a_failed_copy_leaves_the_sequences_as_they_were(monkeypatch):
+    copies = Copies(monkeypatch)
+    c = host_only_cache(16)
+    s = c.open()
+    c.extend([s], [40])
+    copies.failing = True
+    with pytest.raises(S.InvalidOperationException):
+        c.copy(s)
+    assert c.free_pages == 14 and c.open() == 1, "no sequence is left behind"
+    copies.failing = False
+    assert c.copy(s) == 2 and copies.calls == [([0, 1], [2, 3], None)]
