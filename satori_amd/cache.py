@@ -79,6 +79,8 @@ class PageTable:
         _check(lib.satori_hip_pages_create(page_count, page_tokens, ctypes.byref(handle)))
         self._handle = handle
         self.page_count, self.page_tokens = page_count, page_tokens
+        # Held by what takes two calls, or a call and the copies that follow it, and by whatever could change pages between.
+        self.changes = threading.RLock()
         self._address, self._room = handle.value, min(page_count, 1024)
         buffer = np.zeros(self._room + 1, np.int32)  # and the count
         self._buffer, self._lock = memoryview(buffer), threading.Lock()
@@ -101,8 +103,9 @@ class PageTable:
         if n != len(counts):
             raise ArgumentException("Lengths differ.")
         moves = _Moves(n)
-        _check(_ffi.lib().satori_hip_pages_extend(self._address, _address(ids), _address(counts), n, moves.sources,
-                                                  moves.destinations, n, moves.counted))
+        with self.changes:
+            _check(_ffi.lib().satori_hip_pages_extend(self._address, _address(ids), _address(counts), n, moves.sources,
+                                                      moves.destinations, n, moves.counted))
         return moves
 
     def extend(self, sequences, tokens) -> tuple[np.ndarray, np.ndarray]:
@@ -117,9 +120,11 @@ class PageTable:
         return forks[:count].tolist()
 
     def _copy(self, sequence: int) -> tuple[int, _Moves]:
-        moves, made = _Moves(self._describe(sequence)[1]), ctypes.c_int()
-        _check(_ffi.lib().satori_hip_pages_copy(self._address, sequence, ctypes.byref(made), moves.sources,
-                                                moves.destinations, moves.room, moves.counted))
+        made = ctypes.c_int()
+        with self.changes:
+            moves = _Moves(self._describe(sequence)[1])
+            _check(_ffi.lib().satori_hip_pages_copy(self._address, sequence, ctypes.byref(made), moves.sources,
+                                                    moves.destinations, moves.room, moves.counted))
         return made.value, moves
 
     def copy(self, sequence: int) -> tuple[int, tuple[np.ndarray, np.ndarray]]:
@@ -131,9 +136,10 @@ class PageTable:
         _check(_ffi.lib().satori_hip_pages_free(self._address, _address(ids), len(ids)))
 
     def _compact(self) -> _Moves:
-        moves = _Moves(self.page_count - self.free_pages)
-        _check(_ffi.lib().satori_hip_pages_compact(self._address, moves.sources, moves.destinations, moves.room,
-                                                   moves.counted))
+        with self.changes:
+            moves = _Moves(self.page_count - self.free_pages)
+            _check(_ffi.lib().satori_hip_pages_compact(self._address, moves.sources, moves.destinations, moves.room,
+                                                       moves.counted))
         return moves
 
     def compact(self) -> tuple[np.ndarray, np.ndarray]:
@@ -160,10 +166,11 @@ class PageTable:
         with self._lock:
             if not read(handle, sequence, none, at, room, count):
                 return buffer[:buffer[-1]].tolist()
-        count = self._describe(sequence)[1]
-        table = np.empty(count, np.int32)  # a long table: a call of its own size
-        _check(_ffi.lib().satori_hip_pages_sequence(handle, sequence, None, table.ctypes.data, count, None))
-        return table.tolist()
+        table = np.empty(self.page_count, np.int32)  # a long table: a call with room for any (of which only its pages are touched)
+        length = ctypes.c_int()
+        _check(_ffi.lib().satori_hip_pages_sequence(handle, sequence, None, table.ctypes.data, self.page_count,
+                                                    ctypes.byref(length)))
+        return table[:length.value].tolist()
 
     def dispose(self) -> None:
         _check(_ffi.lib().satori_hip_pages_destroy(self._handle))
@@ -222,8 +229,9 @@ class PagedCache:
         s, d = _array(sources), _array(destinations)
         if len(s) != len(d):
             raise ArgumentException("Lengths differ.")
-        self._settle(stream)
-        self._copy_pages(_address(s), _address(d), len(s), stream)
+        with self.table.changes:
+            self._settle(stream)
+            self._copy_pages(_address(s), _address(d), len(s), stream)
 
     def _copy_pages(self, sources: int, destinations: int, count: int, stream: int) -> None:
         _check(_ffi.lib().satori_hip_cache_copy_pages(self.context.handle, self.pool, self.page_bytes, self.page_count,
@@ -231,7 +239,8 @@ class PagedCache:
 
     def extend(self, sequences, tokens, stream: int = 0) -> None:
         """Makes room for tokens[i] more positions of sequences[i]."""
-        self._move(self.table._extend(sequences, tokens), stream)
+        with self.table.changes:
+            self._move(self.table._extend(sequences, tokens), stream)
 
     def truncate(self, sequence: int, tokens: int) -> None:
         self.table.truncate(sequence, tokens)
@@ -240,21 +249,23 @@ class PagedCache:
         return self.table.fork(sequence, count)
 
     def copy(self, sequence: int, stream: int = 0) -> int:
-        self._settle(stream)
-        made, moves = self.table._copy(sequence)
-        try:
-            self._move(moves, stream)
-        except Exception:
-            self._due.clear()  # (its own: nothing else was due)
-            self.table.free([made])
-            raise
+        with self.table.changes:
+            self._settle(stream)
+            made, moves = self.table._copy(sequence)
+            try:
+                self._move(moves, stream)
+            except Exception:
+                self._due.clear()  # (its own: nothing else was due)
+                self.table.free([made])
+                raise
         return made
 
     def free(self, sequences) -> None:
         self.table.free(sequences)
 
     def compact(self, stream: int = 0) -> None:
-        self._move(self.table._compact(), stream)
+        with self.table.changes:
+            self._move(self.table._compact(), stream)
 
     @property
     def free_pages(self) -> int:
@@ -290,7 +301,9 @@ class CachePlan:
         ids, counts = _ints(sequences), _ints(new_tokens)
         if ids.size != counts.size:
             raise ArgumentException("Lengths differ.")
-        self.cache._settle(stream)
+        if self.cache._due:
+            with self.cache.table.changes:
+                self.cache._settle(stream)
         _check(_ffi.lib().satori_hip_cache_plan_set(self._handle, self.cache.table.handle, _at(ids), _at(counts),
                                                     ids.size, _pointer(stream)))
 
