@@ -430,12 +430,13 @@ int satori_hip_matrix_decode_row(satori_hip_matrix* matrix, int row, float* outp
  * keys and values in arrays of its own. A key/value cache here is a pool of pages of `page_tokens` positions (32, 64, 128
  * or 256), a page holding them for every layer; sequences list the pages they hold, and sequences forked from one another
  * hold the same ones. satori_hip_pages keeps the lists and reference counts on the host (no device call, no context; a
- * handle's calls exclude one another); the pages' bytes are the caller's pool on the device. Where a call says that page
- * bytes must follow, it gives moves (source page, destination page), which the caller hands to
- * satori_hip_cache_copy_pages before anything reads or writes the destinations. Sources and destinations of one call's
- * moves are different pages. A call that fails changes nothing. New pages and sequence numbers are the lowest free ones, so a
- * page that a call gives up may be in the next sequence's list, and be written to, at once: launches that still read it must come
- * before those that write it, on the same stream or ordered by the caller. */
+ * handle's calls wait for one another, but what only reads the lists, a plan's set among it, runs beside others of that
+ * kind); the pages' bytes are the caller's pool on the device. Where a call says that page bytes must follow, it gives moves
+ * (source page, destination page), which the caller hands to satori_hip_cache_copy_pages before anything reads or writes the
+ * destinations. Sources and destinations of one call's moves are different pages. A call that fails changes nothing. New pages
+ * and sequence numbers are the lowest free ones, so a page that a call gives up may be in the next sequence's list, and be
+ * written to, at once: launches that still read it must come before those that write it, on the same stream or ordered by the
+ * caller. */
 int satori_hip_pages_create(int page_count, int page_tokens, satori_hip_pages** pages);
 /* Idempotent: NULL is accepted. */
 int satori_hip_pages_destroy(satori_hip_pages* pages);

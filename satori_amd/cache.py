@@ -71,7 +71,8 @@ class PageTable:
 
     # A table's read returns a few dozen page numbers and takes less than a microsecond, half of it making ctypes arguments
     # and results, so its arguments but one are made here and name one buffer, read under a lock (threads may call at once),
-    # and the call, which waits for nothing, keeps the interpreter.
+    # and the call keeps the interpreter. It waits for no plan that is being made (both only read the tables), but for a call
+    # that changes them: some microseconds of another thread's, or a compaction's pass over all lists.
 
     def __init__(self, page_count: int, page_tokens: int = 32):
         handle = ctypes.c_void_p()

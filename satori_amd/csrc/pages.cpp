@@ -5,6 +5,7 @@
 #include <algorithm>
 #include <climits>
 #include <cstring>
+#include <mutex>
 #include <new>
 #include <string>
 #include <unordered_map>
@@ -613,11 +614,12 @@ void require_pointer(const void* p, const char* name) {
     if (!p) fail(SATORI_HIP_E_ARGUMENT_NULL, std::string("Value cannot be null. (Parameter '") + name + "')");
 }
 
-template <class F>
+// Lock: std::unique_lock, or std::shared_lock where the tables stay as they are.
+template <template <class> class Lock = std::unique_lock, class F>
 int pages_call(satori_hip_pages* handle, F&& body) {
     return host_call([&] {
         require_pointer(handle, "pages");
-        std::lock_guard<std::mutex> guard(handle->tables.lock);
+        const Lock<std::shared_mutex> guard(handle->tables.lock);
         if (!handle->tables.live())
             fail(SATORI_HIP_E_OBJECT_DISPOSED, "Cannot access a disposed object. Object name: 'satori_hip_pages'.");
         body(handle->tables);
@@ -662,7 +664,7 @@ int satori_hip_pages_create(int page_count, int page_tokens, satori_hip_pages** 
 int satori_hip_pages_destroy(satori_hip_pages* pages) {
     return host_call([&] {
         if (!pages) return;
-        std::lock_guard<std::mutex> guard(pages->tables.lock);
+        const std::unique_lock<std::shared_mutex> guard(pages->tables.lock);
         pages->tables.close();  // the handle stays valid as a tombstone so a second destroy is a no-op
     });
 }
@@ -738,7 +740,7 @@ int satori_hip_pages_compact(satori_hip_pages* pages, int* sources, int* destina
 }
 
 int satori_hip_pages_free_count(satori_hip_pages* pages, int* free_pages) {
-    return pages_call(pages, [&](PageTables& t) {
+    return pages_call<std::shared_lock>(pages, [&](PageTables& t) {
         require_pointer(free_pages, "freePages");
         *free_pages = t.free_pages();
     });
@@ -746,7 +748,7 @@ int satori_hip_pages_free_count(satori_hip_pages* pages, int* free_pages) {
 
 int satori_hip_pages_sequence(satori_hip_pages* pages, int sequence, int* tokens, int* table, int capacity,
                               int* count) {
-    return pages_call(pages, [&](PageTables& t) {
+    return pages_call<std::shared_lock>(pages, [&](PageTables& t) {
         const std::vector<int>& list = t.table(sequence);
         if (tokens) *tokens = t.tokens(sequence);
         if (count) *count = static_cast<int>(list.size());

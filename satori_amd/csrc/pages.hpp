@@ -4,7 +4,7 @@
 #pragma once
 
 #include <cstdint>
-#include <mutex>
+#include <shared_mutex>
 #include <vector>
 
 struct satori_hip_pages;
@@ -44,8 +44,9 @@ public:
     int tokens(int sequence) const { return at(sequence).tokens; }
     const std::vector<int>& table(int sequence) const { return at(sequence).table; }
 
-    // For the handle that holds it: calls are made under `lock`, and none but live() after close().
-    std::mutex lock;
+    // For the handle that holds it: calls are made under `lock` (shared: those that change nothing, so that a list can be
+    // read while a plan is being made), and none but live() after close().
+    std::shared_mutex lock;
     bool live() const { return live_; }
     void close();
 

@@ -11,6 +11,7 @@
 #include <cmath>
 #include <cstring>
 #include <mutex>
+#include <shared_mutex>
 #include <string>
 #include <vector>
 
@@ -2500,7 +2501,7 @@ int satori_hip_cache_plan_set(satori_hip_cache_plan* p, satori_hip_pages* pages,
         PlanImage image;
         {
             PageTables& tables = page_tables(pages);
-            std::lock_guard<std::mutex> tables_guard(tables.lock);
+            const std::shared_lock<std::shared_mutex> tables_guard(tables.lock);
             if (!tables.live())
                 fail(SATORI_HIP_E_OBJECT_DISPOSED, "Cannot access a disposed object. Object name: 'satori_hip_pages'.");
             if (tables.pages() != p->page_count || tables.page_tokens() != p->shape.page_tokens)

@@ -1,10 +1,14 @@
 // The memory that a batch's plan asks for and the ranges it counts in (plan_batch of satori_amd/csrc/pages.cpp), one check a
 // run, named by the argument; built with the sanitizers and run by tests/test_plan_memory.py.
 #include <algorithm>
+#include <chrono>
 #include <cstdio>
 #include <cstring>
+#include <future>
 #include <random>
+#include <shared_mutex>
 #include <string>
+#include <thread>
 #include <vector>
 
 #include "../include/satori_hip.h"
@@ -175,6 +179,32 @@ void smaller_batches() {
     expect(!plan_batch_within(tables, &s, &rows, 1, kShape, room.layout, room.partials, image), "more rows do not fit");
 }
 
+// A list is read while a plan is being made, which holds the tables without changing them.
+void readers() {
+    satori_hip_pages* pages = nullptr;
+    expect(satori_hip_pages_create(8, 32, &pages) == SATORI_HIP_OK, "create");
+    int sequence = -1, tokens = -1, count = -1, free_pages = -1;
+    expect(satori_hip_pages_open(pages, &sequence) == SATORI_HIP_OK, "open");
+    PageTables& tables = page_tables(pages);
+    std::promise<void> held, release;
+    std::thread plan([&] {
+        const std::shared_lock<std::shared_mutex> lock(tables.lock);
+        held.set_value();
+        release.get_future().wait();
+    });
+    held.get_future().wait();
+    auto read = std::async(std::launch::async, [&] {
+        return satori_hip_pages_sequence(pages, sequence, &tokens, nullptr, 0, &count) == SATORI_HIP_OK &&
+               satori_hip_pages_free_count(pages, &free_pages) == SATORI_HIP_OK;
+    });
+    const bool done = read.wait_for(std::chrono::seconds(20)) == std::future_status::ready;
+    expect(done, "a read beside a plan");
+    release.set_value();
+    plan.join();
+    expect(read.get() && tokens == 0 && count == 0 && free_pages == 8, "what it reads");
+    satori_hip_pages_destroy(pages);
+}
+
 }  // namespace
 
 int main(int count, char** arguments) {
@@ -183,6 +213,8 @@ int main(int count, char** arguments) {
         partials();
     else if (what == "smaller")
         smaller_batches();
+    else if (what == "readers")
+        readers();
     else
         expect(false, "no such check");
     if (failures) return 1;

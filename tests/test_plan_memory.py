@@ -18,7 +18,7 @@ def harness(tmp_path_factory):
     sources = [os.path.join(ROOT, "tests", "plan_memory.cpp"), os.path.join(ROOT, "satori_amd", "csrc", "pages.cpp")]
     build = subprocess.run(
         ["g++", "-std=c++17", "-O1", "-g", "-fno-omit-frame-pointer", "-fsanitize=address,undefined",
-         "-fno-sanitize-recover=all", "-static-libasan", "-static-libubsan", *sources, "-o", exe],
+         "-fno-sanitize-recover=all", "-static-libasan", "-static-libubsan", "-pthread", *sources, "-o", exe],
         capture_output=True, text=True, timeout=600)
     assert build.returncode == 0, build.stderr[-4000:]
     return exe
@@ -38,3 +38,7 @@ def test_rows_of_one_part_ask_for_no_partial_results(harness):
 
 def test_a_plan_has_room_for_every_smaller_batch(harness):
     run(harness, "smaller")
+
+
+def test_lists_are_read_beside_a_plan(harness):
+    run(harness, "readers")
