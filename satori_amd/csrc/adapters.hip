@@ -144,13 +144,15 @@ struct Outputs {
             }
         }
     }
-    __device__ __forceinline__ void store(const AdapterShape& s, float* to, const f32x4 (&sum)[N], int n0, bool whole) const {
+    // `none`: the base as it is (a zero of its own sign among it).
+    __device__ __forceinline__ void store(const AdapterShape& s, float* to, const f32x4 (&sum)[N], int n0, bool whole,
+                                          bool none) const {
         const int g = (threadIdx.x & 63) >> 4;
         if (!is) return;
 #pragma unroll
         for (int n = 0; n < N; ++n) {
             const int at = n0 + 16 * n + 4 * g;
-            const f32x4 out = base[n] + sum[n];
+            const f32x4 out = none ? base[n] : base[n] + sum[n];
             if (whole && at + 4 <= s.rows) {
                 *(SATORI_GLOBAL f32x4*)(to + row + at) = out;
             } else {
@@ -245,7 +247,7 @@ __global__ __launch_bounds__(kThreads) void adapter_up_kernel(AdapterShape s, Ad
     }
 #pragma unroll
     for (int r = 0; r < kGroupTiles; ++r)
-        if (16 * r < tile.count) out[r].store(s, output, sum[r], n0, whole);
+        if (16 * r < tile.count) out[r].store(s, output, sum[r], n0, whole, tile.none);
 }
 
 // Both products in one launch, for adapters of one tile of ranks and short rows: workgroup (tile, 512 output rows or less)
@@ -292,7 +294,7 @@ __global__ __launch_bounds__(kBothWaves * 64) void adapter_both_kernel(AdapterSh
 #pragma unroll
     for (int n = 0; n < 4; ++n) sum[n] = f32x4{0, 0, 0, 0};
     up.expand(tile, &t[0][0], kBothRank + 4, 0, sum);
-    out.store(s, output, sum, n0, whole);
+    out.store(s, output, sum, n0, whole, tile.none);
 }
 
 template <typename T>

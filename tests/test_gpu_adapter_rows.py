@@ -31,3 +31,16 @@ def test_a_single_row(context, device, type_, rows, columns, ranks):  # noqa: F8
         case.adapters.apply([adapter], device(x), db, db)
         assert np.array_equal(context.download(np.zeros_like(base), db), got)
     case.adapters.dispose()
+
+
+@pytest.mark.parametrize("rank", [8, 40])  # one launch, two
+def test_rows_without_an_adapter_keep_their_bits(context, device, rank):  # noqa: F811
+    case = Case(context, device, F16, 70, 300, [rank], rank)
+    x, base = case.inputs(5)
+    base[1:4, ::3], base[1, 1], base[3, 2] = -0.0, -np.inf, np.float32(1e-45)
+    dy = device(np.full_like(base, np.nan))
+    case.adapters.apply([0, -1, -1, -1, 0], device(x), device(base), dy)
+    got = context.download(np.zeros_like(base), dy)
+    assert np.array_equal(got[1:4].view(np.uint32), base[1:4].view(np.uint32))
+    case.check([0, 0], x[[0, 4]], base[[0, 4]], got[[0, 4]])
+    case.adapters.dispose()
