@@ -381,11 +381,11 @@ PlanImage plan_batch(const PageTables& tables, const int* sequences, const int* 
     std::vector<int> row_list;
     for (Node& n : nodes) {
         n.chunk = n.wide ? wide_chunk : narrow_chunk;
-        n.chunks = (n.end - n.begin + n.chunk - 1) / n.chunk;
+        n.chunks = (n.end - n.begin - 1) / n.chunk + 1;  // (a sum with the chunk could pass 32 bits)
         n.slot = n.ancestors < 0 ? 0 : nodes[n.ancestors].slot + nodes[n.ancestors].chunks;
         n.pages = static_cast<int>(page_list.size());
         const std::vector<int>& table = tables.table(sequences[n.members[0]]);
-        page_list.insert(page_list.end(), table.begin() + n.begin / P, table.begin() + (n.end + P - 1) / P);
+        page_list.insert(page_list.end(), table.begin() + n.begin / P, table.begin() + ((n.end - 1) / P + 1));
         n.rows = static_cast<int>(row_list.size());
         for (int m : n.members)
             for (int r = first_row[m]; r < first_row[m + 1]; ++r) {

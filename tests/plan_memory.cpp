@@ -2,6 +2,7 @@
 // run, named by the argument; built with the sanitizers and run by tests/test_plan_memory.py.
 #include <algorithm>
 #include <chrono>
+#include <climits>
 #include <cstdio>
 #include <cstring>
 #include <future>
@@ -78,7 +79,7 @@ void check_division(const PageTables& tables, const std::vector<int>& sequences,
                     expect(image.pages.at(item.pages + t / P - item.first / P) == tables.table(sequence_of[row.row]).at(t / P),
                            "the page of a position");
                     seen[at] += next - t;
-                    sums[at] += static_cast<int64_t>(t + next - 1) * (next - t) / 2;
+                    sums[at] += (static_cast<int64_t>(t) + next - 1) * (next - t) / 2;
                 }
             }
     for (size_t at = 0; at < seen.size(); ++at) {
@@ -179,6 +180,21 @@ void smaller_batches() {
     expect(!plan_batch_within(tables, &s, &rows, 1, kShape, room.layout, room.partials, image), "more rows do not fit");
 }
 
+// As many positions as a cache can count.
+void longest() {
+    const PlanShape shape{1, 1, 128, 128};
+    PageTables tables(INT32_MAX / 256, 256);
+    std::vector<PageMove> moves;
+    const int s = tables.open(), tokens = INT32_MAX / 256 * 256, one = 1;
+    tables.extend(&s, &tokens, 1, moves);
+    for (const bool plain : {false, true}) {
+        const PlanImage image = plan_batch(tables, &s, &one, 1, shape, plain ? kPlainDivision : PlanDivision{});
+        expect(image.rows[0].slots == 2048, "chunks of 2^20 positions");
+        expect(plain == false || image.plain_partials >= image.header.partials, "their partial results");
+        check_division(tables, {s}, {1}, shape, image);
+    }
+}
+
 // A list is read while a plan is being made, which holds the tables without changing them.
 void readers() {
     satori_hip_pages* pages = nullptr;
@@ -213,6 +229,8 @@ int main(int count, char** arguments) {
         partials();
     else if (what == "smaller")
         smaller_batches();
+    else if (what == "longest")
+        longest();
     else if (what == "readers")
         readers();
     else

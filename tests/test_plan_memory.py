@@ -42,3 +42,7 @@ def test_a_plan_has_room_for_every_smaller_batch(harness):
 
 def test_lists_are_read_beside_a_plan(harness):
     run(harness, "readers")
+
+
+def test_a_sequence_as_long_as_positions_are_counted(harness):
+    run(harness, "longest")
