@@ -466,7 +466,8 @@ int satori_hip_pages_sequence(satori_hip_pages* pages, int sequence, int* tokens
 /* Bytes of a page: [layers][keys, values], a layer's keys [kv_heads][page_tokens][width] and its values
  * [kv_heads][width][page_tokens] (transposed: the order in which the attention's matrix instructions take them), `width`
  * being head_dim rounded up to 32, 64, 96, 128, 192 or 256 (SATORI_HIP_E_NOT_SUPPORTED past that), of the satori_hip_element
- * `type`. */
+ * `type`. A key's lanes from head_dim on are zero (satori_hip_cache_append writes them so, and pages filled otherwise must hold
+ * them); a value's may hold anything. */
 int satori_hip_cache_page_bytes(int layers, int kv_heads, int head_dim, int page_tokens, int type, int64_t* bytes);
 /* Copies page sources[i] of the pool to page destinations[i], i < count, enqueued on `stream` (NULL: the context stream).
  * The arrays are on the host and read before the call returns (a captured call keeps what it was given). No page may be
@@ -511,8 +512,8 @@ int satori_hip_cache_append(satori_hip_cache_plan* plan, int layer, const float*
 /* GroupedAttention (src/Satori.Core/TransformerOps.cs:135-179) of every row over the positions of its sequence up to its
  * own. Pages that several sequences of the batch hold are read once for all of them: the tables are divided where they
  * part, each part is attended by the rows below it, and the partial results are joined. FP32 scores, maxima and sums
- * (the single-sequence attention's are FP64); of F16 pages every bit is used, and queries and probabilities keep 22, down to
- * 2^-36 of a row's largest probability. Where a row sees a key or value that is not finite, its outputs may be NaN where the
+ * (the single-sequence attention's are FP64); of F16 pages every bit is used, and queries and probabilities keep 22 (with F32
+ * pages 24), down to 2^-39 of a query's largest lane and 2^-36 of a row's largest probability. Where a row sees a key or value that is not finite, its outputs may be NaN where the
  * definition gives an infinity or a weight of zero; what a row does not see never reaches it. query and output
  * [rows][query_heads * head_dim], not overlapping. */
 int satori_hip_cache_attention(satori_hip_cache_plan* plan, int layer, const float* query, float* output, void* stream);
@@ -523,7 +524,8 @@ int satori_hip_cache_attention(satori_hip_cache_plan* plan, int layer, const flo
  * Adapter i: down[i] [ranks[i]][columns] and up[i] [rows][ranks[i]] on the device, row-major, of the satori_hip_element
  * `type`, which the caller keeps alive; ranks 1 .. 512. selection is on the host and read before the call returns (a
  * captured call keeps it). Sums in FP32. Applications of one handle share its workspace and must not overlap in time on
- * different streams. Destroy adapters before their context. */
+ * different streams. Destroy adapters before their context, and after any graph of another library's capture that applies them
+ * (whose end is not told). */
 int satori_hip_adapters_create(satori_hip_context* context, int rows, int columns, int type, int count,
                                const void* const* down, const void* const* up, const int* ranks, const float* scales,
                                satori_hip_adapters** adapters);

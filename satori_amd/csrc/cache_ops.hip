@@ -89,8 +89,9 @@ constexpr int kGroupTokens = 8;  // positions whose values a thread stores at on
 // then the lanes behind the rotated ones and the keys' padding, then the values. A page's values lie [lane][position], so a
 // thread gathers one lane of up to eight positions (its neighbours the next lanes: the reads are whole lines) and stores
 // them together where they fill an aligned group (one value a store took 93 us where this takes 9.8). Few rows are bound by
-// the launch and two dependent reads (16 rows of 12 + 2 heads of 128 lanes 4.6 us), many by memory: 8 x 61 rows of 32 + 8 heads
-// move 22.6 MB in 9.8 us (2.3 TB/s); the rotation's angles come from the table in 64 bits, as the single-sequence operator's.
+// the launch and two dependent reads (16 rows of 12 + 2 heads of 128 lanes 4.6 us), many by that and, half of the time, by memory: 8 x
+// 61 rows of 32 + 8 heads move 22.6 MB in 9.8 us (2.3 TB/s, where a large copy reaches 4.9); in a captured step, whose grid does
+// for any batch, 15.1. The rotation's angles come from the table in 64 bits, as the single-sequence operator's.
 template <typename T, int N>
 __global__ __launch_bounds__(kThreads) void cache_append_kernel(CacheShape s, const int* __restrict__ image, int runs_at,
                                                                 AppendArgs a) {
@@ -185,7 +186,11 @@ __global__ __launch_bounds__(kThreads) void cache_append_kernel(CacheShape s, co
 // two halves of 11 bits, x = hi + lo, both products summed in the same FP32 accumulator. A power of two puts the largest
 // query lane of a pair at 2^14 and its largest probability at 2^11 or more (2^15 at most), so that what is lost of either is
 // 2^-22 of the value, or 2^-39 of the largest lane and 2^-36 of the largest probability where that is more (half a step of
-// the smallest half). F32 caches use the FP32 matrix instructions.
+// the smallest half). FP32 would keep 2^-24 of each; the difference shows where a row's output comes from weights far below its
+// largest, whose value is near zero: with one token of value 0 and 1.5% of the weight on 16000 others about 5e-6 of the output, with
+// 0.1% on them 1e-4, where rounding keys and values to F16 costs up to 2^-11 of each. Low halves times 2^12 with sums of their own, added
+// to the others by the vector unit, would keep 2^-48 and cost 64 rows of one position over 16384 shared ones 73 us instead of 67,
+// of 256 lanes 208 instead of 154. F32 caches use the FP32 matrix instructions and lose neither.
 
 constexpr int kTile = 32;  // tokens that a wave attends at once
 constexpr float kSlack = 4.0f;

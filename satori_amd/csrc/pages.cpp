@@ -233,10 +233,12 @@ struct Node {
 // 400 positions, shared against not, F16: 64 positions 11.6 us and 11.9, 256 12.0 and 12.0, 1024 12.3 and 13.3, 4096 13.6 and
 // 17.8; 20 of 32 heads and 100 to 200: 128 positions 14.9 and 14.1, 256 14.8 and 15.4, 512 13.8 and 20.6).
 constexpr int kLeastShared = 128;
-// The card holds so many workgroups at once (two a CU), each of some 7 us for the chain of its reads alone. Where the items of
+// The card holds so many workgroups at once (two a CU, up to 128 lanes), each of some 7 us for the chain of its reads alone. Where the items of
 // the sequences' own fill that and those of a shared run would come behind them, the run is shared if that saves this much
 // reading: 64 sequences of 8 key/value heads and 100 to 200 positions, F16, over 256 shared ones (50 MB) 24.6 us shared and
-// 17.5 not, 512 (100 MB) 24.4 and 21.9, 1024 (201 MB) 27.5 and 32.0.
+// 17.5 not, 512 (100 MB) 24.4 and 21.9, 1024 (201 MB) 27.5 and 32.0. Heads of 192 and 256 lanes fit one workgroup a CU, but half
+// the number serves them no better: F16, 256 lanes, 32 + 8 heads over 256 shared positions, 30 sequences take 31.1 us with 512
+// here and 38.8 with 256, 32 take 30.8 and 23.7, 40 take 32.5 with either; FP32, 30 sequences, 45.4 and 73.7.
 constexpr int64_t kPlaces = 512, kRoundBytes = 128 << 20;
 
 }  // namespace
@@ -349,7 +351,10 @@ PlanImage plan_batch(const PageTables& tables, const int* sequences, const int* 
     // more than kNarrowBytes. Wide against narrow, F16 heads of 128 lanes, 96 pairs over 4096, 16384 and 65536 tokens of 2
     // key/value heads (25, 100 and 400 MB): 19.7 us and 13.5, 24.7 and 22.6, 38.7 and 46.9; 128 pairs of 8 heads over 4096 and
     // 8192 (134 and 268 MB): 26.1 and 27.0, 31.0 and 37.4; FP32, 144 pairs of 2 heads over 4000 and 8192 (74 and 151 MB): 25.7
-    // and 23.1, 35.5 and 50.3; 4 x 128 rows, F16 of 96 lanes (171 MB): 37 and 18.
+    // and 23.1, 35.5 and 50.3. One number for all types and widths leaves prompts on the slower side just behind it: 4 x 128
+    // rows of 14 + 2 heads of 80 F16 lanes over 1128 positions (194 MB) take 38.9 wide and 20.0 narrow, 512 rows of 32 + 8 heads
+    // of 128 over themselves (268 MB) 49.9 and 28.3 (over 4512, 2.4 GB, 121 and 187); FP32 turns earlier, 128 rows of 12 + 2 heads
+    // of 128 lanes over 1128 (111 MB) taking 27.4 and 44.9.
     int64_t narrow_tokens = 0, wide_tokens = 0, again = 0;
     std::vector<int64_t> pairs_of(nodes.size());
     for (size_t i = 0; i < nodes.size(); ++i) {
@@ -367,7 +372,7 @@ PlanImage plan_batch(const PageTables& tables, const int* sequences, const int* 
     }
     // Chunks of tokens: as many as give every CU work (kv heads and blocks of pairs count too), and no shorter than
     // one tile per wave. (Few pairs in 256, 512 and 1024 workgroups: 24 rows over 4000 positions, FP32, 23.0, 28.9 and 31.6 us, 64
-    // of 1000 to 2000, F16, 68, 78 and 80, 9 x 5 over 4000 16.9, 15.4 and 19.3. Many in 256 and 512: 64 rows over 8192, F16, 46
+    // of 32 + 8 heads and 1000 to 2000 each, F16, 68, 78 and 80, 9 x 5 over 4000 16.9, 15.4 and 19.3. Many in 256 and 512: 64 rows over 8192, F16, 46
     // and 58, over 32768 103 and 102, 24 over 8192, FP32, 35 and 31: the more chunks, the more partial results.)
     const auto chunk_for = [&](int64_t tokens) {
         if (division.plain) return kMostTokens;
