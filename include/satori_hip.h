@@ -488,11 +488,12 @@ int satori_hip_cache_copy_pages(satori_hip_context* context, void* pool, int64_t
  * more rows, no more sequences that have any and no longer page lists (together, and the longest) than one that was set before
  * the capture is taken, divided into fewer parts where the usual ones do not fit (unless the plan's own data would be larger than
  * 256 MB); one that does not fit fails with SATORI_HIP_E_INVALID_OPERATION, and so does one whose rows lie in shared pages if a
- * step writes them; the plan stays as it was. After a call in another library's capture the plan is read by that graph until the plan is destroyed
- * (which must come after the graph's end). Each plan owns the workspace of its attention, so calls on one plan must not
- * overlap in time on different streams; different plans may. A batch whose queries and outputs together exceed the device's
- * memory fails with SATORI_HIP_E_OUT_OF_MEMORY. After a set that failed for memory or on the device, calls fail until one
- * succeeds. The pool must be 16-byte aligned and outlive the plan; destroy plans before their context. */
+ * step writes them; the plan stays as it was. After a call in another library's capture the plan is read by that graph
+ * until the plan is destroyed (which must come after the graph's end). Each plan owns the workspace of its attention, so
+ * calls on one plan, and replays of steps that read it, must not overlap in time on different streams; different plans may.
+ * A batch whose queries and outputs together exceed the device's memory fails with SATORI_HIP_E_OUT_OF_MEMORY. After a set
+ * that failed for memory or on the device, calls fail until one succeeds. The pool must be 16-byte aligned and outlive the
+ * plan; destroy plans before their context. */
 int satori_hip_cache_plan_create(satori_hip_context* context, void* pool, int page_count, int layers, int query_heads,
                                  int kv_heads, int head_dim, int page_tokens, int type, satori_hip_cache_plan** plan);
 int satori_hip_cache_plan_set(satori_hip_cache_plan* plan, satori_hip_pages* pages, const int* sequences,

@@ -167,11 +167,13 @@ class PageTable:
         with self._lock:
             if not read(handle, sequence, none, at, room, count):
                 return buffer[:buffer[-1]].tolist()
-        table = np.empty(self.page_count, np.int32)  # a long table: a call with room for any (of which only its pages are touched)
         length = ctypes.c_int()
-        _check(_ffi.lib().satori_hip_pages_sequence(handle, sequence, None, table.ctypes.data, self.page_count,
-                                                    ctypes.byref(length)))
-        return table[:length.value].tolist()
+        with self.changes:  # a long table: a call of its own size
+            count = self._describe(sequence)[1]
+            table = np.empty(count, np.int32)
+            _check(_ffi.lib().satori_hip_pages_sequence(handle, sequence, None, table.ctypes.data, count,
+                                                        ctypes.byref(length)))
+        return table[:length.value].tolist()  # (another thread may have shortened it)
 
     def dispose(self) -> None:
         _check(_ffi.lib().satori_hip_pages_destroy(self._handle))
