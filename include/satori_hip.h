@@ -38,6 +38,8 @@ typedef struct satori_hip_gguf satori_hip_gguf;
 typedef struct satori_hip_pages satori_hip_pages;
 typedef struct satori_hip_cache_plan satori_hip_cache_plan;
 typedef struct satori_hip_adapters satori_hip_adapters;
+typedef struct satori_hip_rotation satori_hip_rotation;
+typedef struct satori_hip_logit_rules satori_hip_logit_rules;
 
 typedef enum satori_hip_status {
     SATORI_HIP_OK = 0,
@@ -498,6 +500,17 @@ int satori_hip_cache_plan_create(satori_hip_context* context, void* pool, int pa
                                  int kv_heads, int head_dim, int page_tokens, int type, satori_hip_cache_plan** plan);
 int satori_hip_cache_plan_set(satori_hip_cache_plan* plan, satori_hip_pages* pages, const int* sequences,
                               const int* new_tokens, int count, void* stream);
+/* satori_hip_cache_plan_set for drafts to verify: the new rows of a sequence are a tree of tokens that may follow its context (its
+ * positions before them). parents, one number for every row in order: the row of the same sequence that it follows, counted
+ * from the sequence's first new one and before it, or -1 for the context (several rows may have it); anything else fails with
+ * SATORI_HIP_E_ARGUMENT_OUT_OF_RANGE. Row j lies at the j-th new position; its rotation is that of the position that it stands for,
+ * the context's length plus its depth, and its attention sees the context, the rows that it follows and itself. Rows that follow
+ * one another in order are no tree and may be any number, those of a tree 1024 of a sequence (SATORI_HIP_E_NOT_SUPPORTED).
+ * All that is said of satori_hip_cache_plan_set holds. A plan that has held a tree is launched with kernels that look for one:
+ * for a captured step to take trees, set one before the capture, of no fewer rows times the positions from its context's last
+ * multiple of 32 on (else SATORI_HIP_E_INVALID_OPERATION). */
+int satori_hip_cache_plan_set_tree(satori_hip_cache_plan* plan, satori_hip_pages* pages, const int* sequences,
+                                   const int* new_tokens, const int* parents, int count, void* stream);
 /* Fails with SATORI_HIP_E_ARGUMENT while a step reads the plan. */
 int satori_hip_cache_plan_destroy(satori_hip_cache_plan* plan);
 /* The attention inputs of every row (satori_hip_attention_inputs, with the same values): bias adds (biases may be NULL),
@@ -510,8 +523,20 @@ int satori_hip_cache_append(satori_hip_cache_plan* plan, int layer, const float*
                             float* query_out, const float* key, const float* key_bias, const float* value,
                             const float* value_bias, double frequency_base, int rotary_dimensions,
                             const double* rope_table, int rope_positions, void* stream);
+/* satori_hip_cache_append with a rotation's layout, dimensions and frequencies (satori_hip_rotation_create) in place of
+ * RopeHalf's: the values of satori_hip_rotation_apply over the biased rows. */
+int satori_hip_cache_append_rotated(satori_hip_cache_plan* plan, int layer, const float* query, const float* query_bias,
+                                    float* query_out, const float* key, const float* key_bias, const float* value,
+                                    const float* value_bias, satori_hip_rotation* rotation, void* stream);
+/* After drafts were verified: moves the keys and values of some of the plan's rows, in all layers, to the places right behind
+ * their sequences' contexts, so that satori_hip_pages_truncate to the context and the number kept leaves those alone. Sequence i
+ * of the plan (as it was set, count of them) keeps the next counts[i] rows of `kept`, its own by number, in ascending order
+ * (SATORI_HIP_E_ARGUMENT_OUT_OF_RANGE); a branch's rows stand for the positions that they move to, so nothing is rotated again.
+ * The places of the rows that are not kept hold anything afterwards. The arrays are on the host and read before the call returns;
+ * not while capturing. The plan shows the old rows: set it again before it is used. */
+int satori_hip_cache_keep(satori_hip_cache_plan* plan, const int* kept, const int* counts, int count, void* stream);
 /* GroupedAttention (src/Satori.Core/TransformerOps.cs:135-179) of every row over the positions of its sequence up to its
- * own. Pages that several sequences of the batch hold are read once for all of them: the tables are divided where they
+ * own (of a row of a tree: over its context, the rows that it follows and itself). Pages that several sequences of the batch hold are read once for all of them: the tables are divided where they
  * part, each part is attended by the rows below it, and the partial results are joined. FP32 scores, maxima and sums
  * (the single-sequence attention's are FP64); of F16 pages every bit is used, and queries and probabilities keep 22 (with F32
  * pages 24), down to 2^-39 of a query's largest lane and 2^-36 of a row's largest probability. Where a row sees a key or value that is not finite, its outputs may be NaN where the
@@ -534,6 +559,88 @@ int satori_hip_adapters_apply(satori_hip_adapters* adapters, const int* selectio
                               const float* base, float* output, void* stream);
 /* Fails with SATORI_HIP_E_ARGUMENT while a step applies the adapters. */
 int satori_hip_adapters_destroy(satori_hip_adapters* adapters);
+
+/* ---- rotary positions of rows ----
+ * The reference rotates one vector by one position with plain frequencies (satori_hip_rope, satori_hip_rope_half); this is the
+ * form for batches, and for models whose frequencies are scaled for long contexts. Pair k of a head's first `rotary_dimensions`
+ * lanes is turned by position * frequencies[k] and made longer by a magnitude, in FP64 with one rounding of each lane; the
+ * lanes behind are copied. */
+#define SATORI_HIP_ROTARY_HALF 0        /* pair k: lanes k and k + rotary_dimensions / 2, as RopeHalf */
+#define SATORI_HIP_ROTARY_INTERLEAVED 1 /* lanes 2 k and 2 k + 1, as Rope */
+/* Frequencies (rotary_dimensions / 2 of them) and magnitude, on the host. Plain ones are f_k = base^(-2 k / rotary_dimensions)
+ * with magnitude 1; `factor` >= 1 is how much longer the context is to be than `original_positions`:
+ *  SATORI_HIP_SCALING_LINEAR      f_k / factor;
+ *  SATORI_HIP_SCALING_NTK         the base times factor^(r / (r - 2)), r = rotary_dimensions (> 2): the slowest pair scaled in
+ *                                 full, the fastest not at all;
+ *  SATORI_HIP_SCALING_YARN        (Peng et al., 2023) f_k (1 - s + s / factor), s rising from 0 to 1 between the pairs that turn `high`
+ *                                 times and `low` times over original_positions, k = r ln(original_positions / (2 pi turns)) /
+ *                                 (2 ln base), rounded down and up (32 and 1 usually; base > 1); magnitude 1 + 0.1 ln(factor);
+ *  SATORI_HIP_SCALING_WAVELENGTH  f_k (s + (1 - s) / factor), s = (turns - low) / (high - low) within 0 .. 1, turns =
+ *                                 original_positions f_k / (2 pi) (4 and 1 usually).
+ * What a kind does not name is ignored. 0 < low < high. */
+#define SATORI_HIP_SCALING_NONE 0
+#define SATORI_HIP_SCALING_LINEAR 1
+#define SATORI_HIP_SCALING_NTK 2
+#define SATORI_HIP_SCALING_YARN 3
+#define SATORI_HIP_SCALING_WAVELENGTH 4
+int satori_hip_rotary_frequencies(int rotary_dimensions, double frequency_base, int scaling, double factor,
+                                  int original_positions, double low, double high, double* frequencies, double* magnitude);
+/* A rotation: frequencies (on the host, read before the call returns) and the sines and cosines of positions
+ * 0 .. positions - 1 (rotary_dimensions * 8 bytes each; 0: none), which other positions compute in the launch, to the same
+ * bits. */
+int satori_hip_rotation_create(satori_hip_context* context, int layout, int rotary_dimensions, const double* frequencies,
+                               double magnitude, int positions, satori_hip_rotation** rotation);
+/* Row r, `heads` heads of head_dim lanes from input + r * input_stride (elements of the satori_hip_element `type`, strides no less than
+ * a row), turned by positions[r] (on the device; negative ones turn back), to output + r * output_stride; what lies
+ * between rows stays as it is. output may be input, with the same stride; they must not overlap otherwise, as a whole. */
+int satori_hip_rotation_apply(satori_hip_rotation* rotation, int type, const void* input, int64_t input_stride, void* output,
+                              int64_t output_stride, int rows, int heads, int head_dim, const int* positions, void* stream);
+/* Fails with SATORI_HIP_E_ARGUMENT while a step uses the rotation; comes after any graph of another library's capture that uses it
+ * (whose end is not told), and before its context's. */
+int satori_hip_rotation_destroy(satori_hip_rotation* rotation);
+
+/* ---- logits of a batch ----
+ * No counterpart in the reference, whose samplers take logits as they are. For every row, in this order: a token that the row has
+ * had n > 0 times becomes l > 0 ? l / repetition : l * repetition, then l - (presence + frequency * n); the row's biases are added;
+ * what its mask does not allow becomes -infinity, whatever it was. FP32, every operation rounded; a token that nothing of
+ * this concerns keeps its bits. A row has had the tokens of its history and, where it is a draft, its own and those of the rows
+ * that it follows. The best token is the lowest of the greatest logits (zeros of either sign are equal), -1 where none is greater
+ * than -infinity; NaN is never greater. All arrays lie on the device and are read when the launches run, so a captured call
+ * follows what they then hold. */
+typedef struct satori_hip_logit_row {
+    float repetition, presence, frequency; /* 1, 0 and 0: no penalties */
+    int history;                           /* -1: none */
+    int parent;                            /* the row of the batch, before this one, that it follows; -1: none */
+    int token;                             /* the row's own; -1: none */
+    int biases;                            /* set; -1: none */
+    int mask;                              /* -1: none */
+} satori_hip_logit_row;
+/* Strides are in elements. History h: the first lengths[h] (at most history_stride) tokens from history + h * history_stride. A mask
+ * has a bit for each token, 32 a word from the lowest on (set: allowed). Tokens outside the vocabulary, and numbers of
+ * histories, sets, masks or parents that do not exist, are as if they were not there. */
+typedef struct satori_hip_logit_batch {
+    const satori_hip_logit_row* rows;
+    const float* logits;
+    float* output;                         /* may be logits, with the same stride; NULL: only the best tokens */
+    int* best;                             /* NULL: only the logits */
+    const int* history;
+    const int* lengths;
+    const uint32_t* masks;
+    int64_t logits_stride, output_stride, history_stride, mask_stride;
+    int count, histories, mask_count;      /* rows, histories (0: none) and masks (0: none) */
+} satori_hip_logit_batch;
+/* Room for bias_sets sets of at most bias_entries tokens each, all empty, and the workspace of the calls. */
+int satori_hip_logit_rules_create(satori_hip_context* context, int vocabulary, int bias_sets, int bias_entries,
+                                  satori_hip_logit_rules** rules);
+/* A set's tokens, in any order, each once, and their values (no NaN; -infinity bans a token that is not +infinity), on the host. The
+ * copy is ordered on `stream` and waited for; not while capturing. */
+int satori_hip_logit_rules_set_biases(satori_hip_logit_rules* rules, int set, const int* tokens, const float* values, int count,
+                                      void* stream);
+/* The batch struct is read before the call returns. Calls with one handle share its workspace and must not overlap in time on
+ * different streams (their best tokens are undefined then; later calls are not affected). */
+int satori_hip_logit_rules_apply(satori_hip_logit_rules* rules, const satori_hip_logit_batch* batch, void* stream);
+/* As satori_hip_rotation_destroy. */
+int satori_hip_logit_rules_destroy(satori_hip_logit_rules* rules);
 
 /* ---- GGUF containers (src/Satori.Formats.Gguf) ----
  * A GGUF v3 file mapped read-only and its catalogue parsed strictly, with the reference's limits and

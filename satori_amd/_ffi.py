@@ -101,6 +101,17 @@ SIGNATURES = {
     "satori_hip_adapters_create": (I, [P, I, I, I, I, P, P, P, P, PP]),
     "satori_hip_adapters_apply": (I, [P, P, I, P, P, P, P]),
     "satori_hip_adapters_destroy": (I, [P]),
+    "satori_hip_cache_plan_set_tree": (I, [P, P, P, P, P, I, P]),
+    "satori_hip_cache_append_rotated": (I, [P, I, P, P, P, P, P, P, P, P, P]),
+    "satori_hip_cache_keep": (I, [P, P, P, I, P]),
+    "satori_hip_rotary_frequencies": (I, [I, ctypes.c_double, I, ctypes.c_double, I, ctypes.c_double, ctypes.c_double, P, P]),
+    "satori_hip_rotation_create": (I, [P, I, I, P, ctypes.c_double, I, PP]),
+    "satori_hip_rotation_apply": (I, [P, I, P, ctypes.c_int64, P, ctypes.c_int64, I, I, I, P, P]),
+    "satori_hip_rotation_destroy": (I, [P]),
+    "satori_hip_logit_rules_create": (I, [P, I, I, I, PP]),
+    "satori_hip_logit_rules_set_biases": (I, [P, I, P, P, I, P]),
+    "satori_hip_logit_rules_apply": (I, [P, P, P]),
+    "satori_hip_logit_rules_destroy": (I, [P]),
     "satori_hip_gguf_open": (I, [ctypes.c_char_p, PP]),
     "satori_hip_gguf_close": (I, [P]),
     "satori_hip_gguf_data_offset": (I, [P, ctypes.POINTER(ctypes.c_int64)]),

@@ -310,6 +310,21 @@ class CachePlan:
         _check(_ffi.lib().satori_hip_cache_plan_set(self._handle, self.cache.table.handle, _at(ids), _at(counts),
                                                     ids.size, _pointer(stream)))
 
+    def set_tree(self, sequences: Sequence[int], parents: Sequence[Sequence[int]], stream: int = 0) -> None:
+        """The batch's rows as trees of drafts: the last len(parents[i]) positions of sequences[i], each after the row of the
+        same sequence that its number says, or after the context (-1)."""
+        ids, counts = _ints(sequences), _ints([len(p) for p in parents])
+        if ids.size != counts.size:
+            raise ArgumentException("Lengths differ.")
+        follows = array("i")
+        for p in parents:
+            follows.extend(_array(p))
+        if self.cache._due:
+            with self.cache.table.changes:
+                self.cache._settle(stream)
+        _check(_ffi.lib().satori_hip_cache_plan_set_tree(self._handle, self.cache.table.handle, _at(ids), _at(counts),
+                                                         _address(follows) or _at(counts), ids.size, _pointer(stream)))
+
     def append(self, layer: int, q: int, q_bias: int, q_out: int, k: int, k_bias: int, v: int, v_bias: int, base: float,
                rotary: int, rope_table: int = 0, rope_positions: int = 0, stream: int = 0) -> None:
         """Bias, rotation and cache write of every row (biases and rope_table may be 0); q_out may be q."""
@@ -317,6 +332,23 @@ class CachePlan:
                                                   _pointer(k), _pointer(k_bias), _pointer(v), _pointer(v_bias),
                                                   float(base), rotary, _pointer(rope_table), rope_positions,
                                                   _pointer(stream)))
+
+    def append_rotated(self, layer: int, q: int, q_bias: int, q_out: int, k: int, k_bias: int, v: int, v_bias: int,
+                       rotation, stream: int = 0) -> None:
+        """`append` with a Rotation (satori_amd.rotary)."""
+        _check(_ffi.lib().satori_hip_cache_append_rotated(self._handle, layer, _pointer(q), _pointer(q_bias),
+                                                          _pointer(q_out), _pointer(k), _pointer(k_bias), _pointer(v),
+                                                          _pointer(v_bias), rotation.handle, _pointer(stream)))
+
+    def keep(self, rows: Sequence[Sequence[int]], stream: int = 0) -> None:
+        """Moves the keys and values of rows[i], some of the plan's rows of its i-th sequence in ascending order, to follow that
+        sequence's context, in all layers. Truncate the sequence to its context and len(rows[i]) then, and set the plan
+        again before it is used."""
+        counts, kept = array("i", [len(r) for r in rows]), array("i")
+        for r in rows:
+            kept.extend(_array(r))
+        _check(_ffi.lib().satori_hip_cache_keep(self._handle, _address(kept) or None, _address(counts) or None, len(counts),
+                                                _pointer(stream)))
 
     def attention(self, layer: int, q: int, out: int, stream: int = 0) -> None:
         """Grouped attention of every row over the positions of its sequence up to its own."""

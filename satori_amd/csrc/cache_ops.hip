@@ -7,6 +7,7 @@
 #include "cache_ops.hpp"
 #include "device_common.hpp"
 #include "rope_device.hpp"
+#include "rotation_device.hpp"
 
 namespace satori {
 namespace {
@@ -40,7 +41,7 @@ __global__ __launch_bounds__(kThreads) void copy_pages_kernel(uint8_t* pool, int
 
 // ---- a plan's copy ----
 
-constexpr int kPlanParts = 7;
+constexpr int kPlanParts = 8;
 struct PlanParts {
     int at[kPlanParts], end[kPlanParts];  // 16-byte units; end: of the parts up to this one, counted through
 };
@@ -92,10 +93,13 @@ constexpr int kGroupTokens = 8;  // positions whose values a thread stores at on
 // the launch and two dependent reads (16 rows of 12 + 2 heads of 128 lanes 4.6 us), many by that and, half of the time, by memory: 8 x
 // 61 rows of 32 + 8 heads move 22.6 MB in 9.8 us (2.3 TB/s, where a large copy reaches 4.9); in a captured step, whose grid does
 // for any batch, 15.1. The rotation's angles come from the table in 64 bits, as the single-sequence operator's.
-template <typename T, int N>
-__global__ __launch_bounds__(kThreads) void cache_append_kernel(CacheShape s, const int* __restrict__ image, int runs_at,
+enum class Turn { kPlain, kTree, kInterleaved };  // pairs half a head apart, rows no tree's; also a tree's; neighbouring lanes
+template <typename T, int N, Turn TURN>
+__global__ __launch_bounds__(kThreads) void cache_append_kernel(CacheShape s, const int* __restrict__ image, int runs_at, int trees_at,
                                                                 AppendArgs a) {
+    constexpr bool kInterleaved = TURN == Turn::kInterleaved;
     const int count = reinterpret_cast<const PlanHeader*>(image)->runs;
+    const int tree_stride = TURN == Turn::kPlain ? 0 : reinterpret_cast<const PlanHeader*>(image)->tree_stride;
     const PlanRun* runs = reinterpret_cast<const PlanRun*>(image + runs_at);
     const int pairs = a.rotary / 2, D = s.head_dim, both = s.heads + s.kv_heads;
     const int64_t head_size = static_cast<int64_t>(s.page_tokens) * s.width;
@@ -108,13 +112,14 @@ __global__ __launch_bounds__(kThreads) void cache_append_kernel(CacheShape s, co
         const int packs = pairs / N;
         for (int i = start; i < run.tokens * both * packs; i += stride) {
             const int kk = i % packs * N, rest = i / packs, head = rest % both, t = rest / both;
-            const int position = position0 + t;
+            const int position = tree_stride ? image[trees_at + (run.row + t) * tree_stride] : position0 + t;
             const bool is_query = head < s.heads;
-            const int lane = (is_query ? head : head - s.heads) * D + kk;
+            const int first = (is_query ? head : head - s.heads) * D;
+            const int lane = first + (kInterleaved ? 2 * kk : kk), beside = kInterleaved ? N : pairs;
             const int64_t at = static_cast<int64_t>(run.row + t) * (is_query ? s.heads : s.kv_heads) * D;
             float x[N], y[N];
             load_biased(is_query ? a.query : a.key, is_query ? a.query_bias : a.key_bias, at, lane, x);
-            load_biased(is_query ? a.query : a.key, is_query ? a.query_bias : a.key_bias, at, lane + pairs, y);
+            load_biased(is_query ? a.query : a.key, is_query ? a.query_bias : a.key_bias, at, lane + beside, y);
             const bool listed = a.rope && position < a.rope_positions;
             const double* angles = a.rope + static_cast<int64_t>(position) * a.rotary + kk;
 #pragma unroll
@@ -123,18 +128,20 @@ __global__ __launch_bounds__(kThreads) void cache_append_kernel(CacheShape s, co
                 if (listed) {
                     sn = angles[j];
                     cs = angles[pairs + j];
+                } else if (a.frequencies) {
+                    rotation_angle(kk + j, position, a.frequencies, a.magnitude, sn, cs);
                 } else {
                     rope_angle(kk + j, position, a.base, a.rotary, sn, cs);
                 }
-                rope_apply(x[j], y[j], sn, cs, x[j], y[j]);
+                rotate_pair<kInterleaved>(x, y, j, sn, cs);
             }
             if (is_query) {
                 store_as(a.query_out + at + lane, x);
-                store_as(a.query_out + at + lane + pairs, y);
+                store_as(a.query_out + at + lane + beside, y);
             } else {
-                T* out = keys + (head - s.heads) * head_size + static_cast<int64_t>(run.offset + t) * s.width + kk;
+                T* out = keys + (head - s.heads) * head_size + static_cast<int64_t>(run.offset + t) * s.width + lane - first;
                 store_as(out, x);
-                store_as(out + pairs, y);
+                store_as(out + beside, y);
             }
         }
         const int behind = s.width - a.rotary;
@@ -174,6 +181,51 @@ __global__ __launch_bounds__(kThreads) void cache_append_kernel(CacheShape s, co
     }
 }
 
+// ---- positions that a sequence keeps ----
+
+// Moves the keys and values of a sequence's kept rows to the places behind its context, in all layers. A place that is
+// written may be read by an earlier move and by no later one (rows go in ascending order, none behind where it was), so a
+// thread makes all moves of its own bytes, eight at a time, each eight read before they are written: 16 bytes of a key, or
+// one lane of a value, whose positions lie side by side.
+template <typename V, typename At>
+__device__ __forceinline__ void keep_moves(const KeepMoves& moves, int begin, int end, const At& at) {
+    for (int i0 = begin; i0 < end; i0 += 8) {
+        V v[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = *(const SATORI_GLOBAL V*)(at(moves.source[min(i0 + j, end - 1)]));
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            if (i0 + j < end) *(SATORI_GLOBAL V*)(at(moves.destination[i0 + j])) = v[j];
+    }
+}
+
+template <typename T>
+__global__ __launch_bounds__(kThreads) void cache_keep_kernel(CacheShape s, int layers, KeepMoves moves) {
+    const int begin = moves.begin[blockIdx.y], end = moves.begin[blockIdx.y + 1];
+    const int pieces = s.width * static_cast<int>(sizeof(T)) / 16, heads = layers * s.kv_heads;
+    const int64_t head_bytes = static_cast<int64_t>(s.page_tokens) * s.width * sizeof(T);
+    const int mask = s.page_tokens - 1;
+    const int64_t units = static_cast<int64_t>(heads) * (pieces + s.head_dim);
+    for (int64_t u = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x; u < units;
+         u += static_cast<int64_t>(gridDim.x) * kThreads) {
+        const bool key = u < static_cast<int64_t>(heads) * pieces;
+        const uint32_t of = static_cast<uint32_t>(key ? u : u - static_cast<int64_t>(heads) * pieces);
+        const uint32_t head = of / (key ? pieces : s.head_dim), part = of % (key ? pieces : s.head_dim);
+        uint8_t* base = s.pool + head / s.kv_heads * s.layer_bytes + head % s.kv_heads * head_bytes;
+        if (key) {
+            base += part * 16;
+            keep_moves<u32x4>(moves, begin, end, [&](int place) {
+                return base + (place >> s.page_shift) * s.page_bytes + (place & mask) * (s.width * static_cast<int>(sizeof(T)));
+            });
+        } else {
+            base += s.kv_heads * head_bytes + static_cast<int64_t>(part) * s.page_tokens * sizeof(T);
+            keep_moves<T>(moves, begin, end, [&](int place) {
+                return base + (place >> s.page_shift) * s.page_bytes + (place & mask) * static_cast<int>(sizeof(T));
+            });
+        }
+    }
+}
+
 // ---- attention ----
 //
 // With S^T = K Q^T and O^T = V^T P^T, both computed by 16 x 16 matrix tiles, a column of either product is a (row, query
@@ -192,7 +244,7 @@ __global__ __launch_bounds__(kThreads) void cache_append_kernel(CacheShape s, co
 // to the others by the vector unit, would keep 2^-48 and cost 64 rows of one position over 16384 shared ones 73 us instead of 67,
 // of 256 lanes 208 instead of 154. F32 caches use the FP32 matrix instructions and lose neither.
 
-constexpr int kTile = 32;  // tokens that a wave attends at once
+constexpr int kTileShift = 5, kTile = 1 << kTileShift;  // tokens that a wave attends at once
 constexpr float kSlack = 4.0f;
 constexpr float kLog2e = 1.44269504088896340736f;
 
@@ -386,6 +438,19 @@ __device__ __forceinline__ void hide(f32x4 (&score)[2], int seen, int g) {
         if (M::token(0, i) >= left) score[i >> 2][i & 3] = -INFINITY;
 }
 
+// The same where a bit of `sees` says of each of the tile's tokens whether the pair sees it.
+template <typename M>
+__device__ __forceinline__ void hide(f32x4 (&score)[2], uint32_t sees, int g) {
+    const uint32_t mine = sees >> M::token(g, 0);
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+        if (!(mine >> M::token(0, i) & 1)) score[i >> 2][i & 3] = -INFINITY;
+}
+
+// Of a token's number and what a pair sees of the tile, in either form: whether it sees the token.
+__device__ __forceinline__ bool is_seen(int token, int seen) { return token < seen; }
+__device__ __forceinline__ bool is_seen(int token, uint32_t sees) { return sees >> token & 1; }
+
 // Values that are not finite. Where some pairs see a token and others must not, the second product would spoil the others'
 // sums (0 * infinity), so such a tile's values get zeros in those places, and the sum of each (pair, lane) that sees one
 // becomes NaN: here, with values in registers, a product tells which.
@@ -407,11 +472,11 @@ __device__ __forceinline__ F take_spoiled(F& v) {
     }
     return spoiled;
 }
-template <typename M>
-__device__ __forceinline__ void spoil(typename M::Fragment spoiled, int seen, int part, int g, f32x4& o) {
+template <typename M, typename Seen>
+__device__ __forceinline__ void spoil(typename M::Fragment spoiled, Seen seen, int part, int g, f32x4& o) {
     float one[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) one[i] = M::token(g, i) < seen ? 1.0f : 0.0f;
+    for (int i = 0; i < 8; ++i) one[i] = is_seen(M::token(g, i), seen) ? 1.0f : 0.0f;
     typename M::Weights w;
     M::weights(one, w);
     f32x4 hit{0, 0, 0, 0};
@@ -441,6 +506,7 @@ struct AttentionArgs {
     Partials partials;
     float scale;
     bool quads;  // heads of a query start at multiples of 16 bytes and are whole 16-byte pieces
+    int tree_stride;  // of the plan, as `wide` is
 };
 
 // A (row, query head) pair of an item, by its number; those past the item's last are the first, and not `is`.
@@ -452,12 +518,16 @@ struct Pair {
 
 __device__ __forceinline__ int pair_place(const PlanItem& item, int p) { return item.pair + (p < item.pairs ? p : 0); }
 
+template <bool TREES>
 __device__ __forceinline__ Pair pair_of(const AttentionArgs& a, const PlanItem& item, int p) {
     const int group = a.s.heads / a.s.kv_heads, of = pair_place(item, p);
     Pair r;
     if (item.row_slots > 0) {
         const int behind = of / group - item.pair / group;
         r.row = PlanRow{item.limit + behind, item.row_slot + behind * item.row_slots, item.row_slots, item.row + behind};
+    } else if (TREES && item.row_slots < 0) {
+        const int behind = of / group - item.pair / group;
+        r.row = PlanRow{-2 - item.limit, item.row_slot - behind * item.row_slots, -item.row_slots, item.row + behind};
     } else {
         r.row = reinterpret_cast<const PlanRow*>(a.image + a.at.list_at)[item.rows + of / group];
     }
@@ -469,6 +539,46 @@ __device__ __forceinline__ Pair pair_of(const AttentionArgs& a, const PlanItem& 
 __device__ __forceinline__ const float* query_of(const AttentionArgs& a, const Pair& p) {
     return a.query + (static_cast<int64_t>(p.row.row) * a.s.heads + p.head) * a.s.head_dim;
 }
+
+// What a pair sees of an item's tiles that its rows do not all see whole: the tokens before its row's position and that one.
+template <bool TREES>
+struct Sight {
+    typedef int Seen;  // the first so many
+    int limit;
+    __device__ __forceinline__ Sight() = default;
+    __device__ __forceinline__ Sight(const AttentionArgs&, const PlanItem& item, const Pair& p, int)
+        : limit(p.is ? p.row.position - item.first : -1) {}
+    __device__ __forceinline__ Seen of(const AttentionArgs&, const PlanItem&, int t, int end, int) const {
+        return min(limit - t + 1, end);
+    }
+    static __device__ __forceinline__ uint32_t bits(Seen seen) {
+        return seen <= 0 ? 0u : ~0u >> (kTile - min(seen, kTile));
+    }
+};
+
+// The same where rows may be a tree's: a bit per token of the tile, which the plan has ready (a row sees what lies before
+// its context's last multiple of 32, and nothing behind its own number's tile).
+template <>
+struct Sight<true> {
+    typedef uint32_t Seen;
+    int limit;  // relative to the item; of a tree's row its context's last position
+    int words;  // of the row, -1 for others
+    __device__ __forceinline__ Sight() = default;
+    __device__ __forceinline__ Sight(const AttentionArgs& a, const PlanItem& item, const Pair& p, int stride) {
+        const bool tree = p.is && p.row.position < 0;
+        limit = !p.is ? -1 : (tree ? -2 - p.row.position : p.row.position) - item.first;
+        words = tree ? a.at.trees_at + p.row.row * stride + 1 : -1;
+    }
+    __device__ __forceinline__ Seen of(const AttentionArgs& a, const PlanItem& item, int t, int end, int stride) const {
+        const int seen = min(words < 0 ? limit - t + 1 : kTile, end);
+        uint32_t sees = seen <= 0 ? 0u : ~0u >> (kTile - min(seen, kTile));
+        if (words < 0) return sees;
+        const int k = ((item.first + t) >> kTileShift) - ((item.first + limit + 1) >> kTileShift);
+        if (k >= 0) sees &= k < stride - 1 ? static_cast<uint32_t>(a.image[words + k]) : 0u;
+        return sees;
+    }
+    static __device__ __forceinline__ uint32_t bits(Seen sees) { return sees; }
+};
 
 // One joined result of a pair, four lanes from `d` on: the output where it is the row's only one.
 template <int W>
@@ -581,8 +691,8 @@ struct Shape {
     static constexpr int kLds = kSpoiledAt + 2 * W * 4;
 };
 
-template <typename T, int W>
-__device__ __forceinline__ void attend_few(const AttentionArgs& a, const PlanItem& item, uint8_t* lds, int wave) {
+template <typename T, int W, bool TREES>
+__device__ __forceinline__ void attend_few(const AttentionArgs& a, const PlanItem& item, uint8_t* lds, int wave, int stride) {
     using M = Math<T, W>;
     using S = Shape<T, W>;
     using Fragment = typename M::Fragment;
@@ -610,7 +720,7 @@ __device__ __forceinline__ void attend_few(const AttentionArgs& a, const PlanIte
                 v[d][h] = *(const SATORI_GLOBAL Fragment*)(p + 16 * d * pages.tokens + 16 * h);
     };
     int t = wave * kTile, page = 0;
-    const Pair pair = pair_of(a, item, c);
+    const Pair pair = pair_of<TREES>(a, item, c);
     if (t < item.tokens) {
         page = wave == 0 ? item.tile[0] : wave == 1 ? item.tile[1] : wave == 2 ? item.tile[2] : item.tile[3];
         load_keys(page, t);
@@ -621,7 +731,11 @@ __device__ __forceinline__ void attend_few(const AttentionArgs& a, const PlanIte
     if (thread < 16) row_of[thread] = pair.row;
     typename M::Query q;
     M::load_query(q, query_of(a, pair), pair.is, head_dim, a.quads, a.scale, g);
-    const int limit = pair.is ? pair.row.position - item.first : -1;
+    const Sight<TREES> sight(a, item, pair, stride);
+    const auto hidden = [&](int t) { return item.first + t + kTile - 1 > item.limit; };
+    const auto in_part = [&](int t) { return hidden(t) || item.tokens - t < kTile; };
+    typename Sight<TREES>::Seen ahead{};  // of the next tile that is not seen whole, read a tile before
+    if (t < item.tokens && in_part(t)) ahead = sight.of(a, item, t, item.tokens - t, stride);
     Softmax<W> x;
     x.clear();
     while (t < item.tokens) {
@@ -635,7 +749,9 @@ __device__ __forceinline__ void attend_few(const AttentionArgs& a, const PlanIte
         const int next = t + kWaves * kTile;
         if (next < item.tokens) load_keys(page, next);
         const int end = item.tokens - t;  // tokens of this tile that exist
-        const bool hides = item.first + t + kTile - 1 > item.limit;
+        const bool hides = hidden(t);
+        const auto seen = ahead;
+        if (next < item.tokens && in_part(next)) ahead = sight.of(a, item, next, item.tokens - next, stride);
         if (end < kTile) {
             // Values of tokens behind the end become zero (they are nobody's, and may hold anything).
 #pragma unroll
@@ -644,7 +760,6 @@ __device__ __forceinline__ void attend_few(const AttentionArgs& a, const PlanIte
 #pragma unroll
                     for (int d = 0; d < W / 16; ++d) v[d][i / kGroupLanes][i % kGroupLanes] = 0;
         }
-        const int seen = min(limit - t + 1, end);
         if (hides) {
             bool finite = true;
 #pragma unroll
@@ -719,8 +834,8 @@ __device__ __forceinline__ void attend_few(const AttentionArgs& a, const PlanIte
     }
 }
 
-template <typename T, int W>
-__device__ __forceinline__ void attend_many(const AttentionArgs& a, const PlanItem& item, uint8_t* lds, int wave) {
+template <typename T, int W, bool TREES>
+__device__ __forceinline__ void attend_many(const AttentionArgs& a, const PlanItem& item, uint8_t* lds, int wave, int stride) {
     using M = Math<T, W>;
     using S = Shape<T, W>;
     using Fragment = typename M::Fragment;
@@ -804,13 +919,13 @@ __device__ __forceinline__ void attend_many(const AttentionArgs& a, const PlanIt
     }
     typename M::Query q[NB];
     Softmax<W> x[NB];
-    int limit[NB];
+    Sight<TREES> sight[NB];
     PlanRow* row_of = reinterpret_cast<PlanRow*>(lds + S::kRowsAt) + 16 * NB * wave;  // this wave's
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
         x[b].clear();
-        const Pair p = pair_of(a, item, 16 * (NB * wave + b) + c);
-        limit[b] = p.is ? p.row.position - item.first : -1;
+        const Pair p = pair_of<TREES>(a, item, 16 * (NB * wave + b) + c);
+        sight[b] = Sight<TREES>(a, item, p, stride);
         if (g == 0) row_of[16 * b + c] = p.row;
         M::load_query(q[b], query_of(a, p), p.is, head_dim, a.quads, a.scale, g);
     }
@@ -834,7 +949,12 @@ __device__ __forceinline__ void attend_many(const AttentionArgs& a, const PlanIt
         if (idle) {
             carry();
         } else {
-            const int t = tile * kTile;
+            const int t = tile * kTile, end = item.tokens - t;
+            const bool hides = item.first + t + kTile - 1 > item.limit;
+            typename Sight<TREES>::Seen seen[NB] = {};
+            if (hides || end < kTile)
+#pragma unroll
+                for (int b = 0; b < NB; ++b) seen[b] = sight[b].of(a, item, t, end, stride);
             const Fragment* keys = reinterpret_cast<const Fragment*>(lds) + (tile & 1) * S::kPieces;
             const Fragment* values = keys + S::kKeys;
             f32x4 score[NB][2];
@@ -869,18 +989,15 @@ __device__ __forceinline__ void attend_many(const AttentionArgs& a, const PlanIt
             __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int i = 0; i < kAhead; ++i) read_values(i);
-            const int end = item.tokens - t;
-            const bool hides = item.first + t + kTile - 1 > item.limit;
             typename M::Weights w[NB];
 #pragma unroll
             for (int b = 0; b < NB; ++b) {
-                const int seen = min(limit[b] - t + 1, end);
-                if (hides || end < kTile) hide<M>(score[b], seen, g);
+                if (hides || end < kTile) hide<M>(score[b], seen[b], g);
                 float p[8];
                 x[b].take(score[b], q[b].factor, M::kTop, p);
                 M::weights(p, w[b]);
                 if (hides) {
-                    const uint32_t sees = seen <= 0 ? 0u : ~0u >> (kTile - min(seen, kTile));
+                    const uint32_t sees = Sight<TREES>::bits(seen[b]);
                     const u32x4* bits = reinterpret_cast<const u32x4*>(spoiled + (tile & 1) * W);
 #pragma unroll
                     for (int d = 0; d < W / 16; ++d) {
@@ -926,20 +1043,21 @@ __device__ __forceinline__ void attend_many(const AttentionArgs& a, const PlanIt
 // Items of many pairs first, which take longest (one a CU, bound by arithmetic); those of few, bound by memory, run beside
 // them (64 sequences as above, before later steps: two launches 64 + 27 us, one with the items in turn 92, with the many first
 // 76). Workgroup u is u % 8 of its eight, which keeps items that read the same tokens on one XCD.
-template <typename T, int W>
+template <typename T, int W, bool TREES>
 __global__ __launch_bounds__(kThreads, (Shape<T, W>::kWavesPerSimd)) void cache_attention_kernel(AttentionArgs a) {
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
     const PlanHeader* h = reinterpret_cast<const PlanHeader*>(a.image);
     const int wide = a.wide >= 0 ? a.wide : scalar_load(&h->wide), narrow = a.narrow >= 0 ? a.narrow : scalar_load(&h->narrow);
+    const int stride = !TREES ? 0 : a.wide >= 0 ? a.tree_stride : scalar_load(&h->tree_stride);
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     for (int u = blockIdx.x; u < wide + narrow; u += gridDim.x) {
         const bool many = u < wide;
         const int at = many ? a.at.wide_at : a.at.narrow_at;
         const PlanItem item = scalar_load(reinterpret_cast<const PlanItem*>(a.image + at) + (many ? u : u - wide));
         if (many)
-            attend_many<T, W>(a, item, lds, wave);
+            attend_many<T, W, TREES>(a, item, lds, wave, stride);
         else
-            attend_few<T, W>(a, item, lds, wave);
+            attend_few<T, W, TREES>(a, item, lds, wave, stride);
         if (u + static_cast<int>(gridDim.x) < wide + narrow) __syncthreads();  // the next item's tiles go where results lie
     }
 }
@@ -1012,9 +1130,9 @@ __global__ __launch_bounds__(kThreads) void cache_join_kernel(AttentionArgs a) {
 constexpr int kMostGroups = 1024;  // workgroups of a launch whose work is only known when it is replayed
 
 template <typename T, int W>
-hipError_t attention_of_width(const AttentionArgs& a, int groups, hipStream_t stream) {
+hipError_t attention_of_width(const AttentionArgs& a, int groups, bool trees, hipStream_t stream) {
     using S = Shape<T, W>;
-    const auto kernel = cache_attention_kernel<T, W>;
+    const auto kernel = trees ? cache_attention_kernel<T, W, true> : cache_attention_kernel<T, W, false>;
     // (more than 64 KB of LDS; set for the current device, where it is a table lookup after the first time)
     if (S::kLds > 64 * 1024)
         if (const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
@@ -1049,10 +1167,11 @@ int cache_wide_pairs(int type, int width) {
 
 hipError_t launch_plan_copy(const int* from, int* to, const PlanLayout& layout, const PlanLayout& used, hipStream_t stream) {
     const int at[kPlanParts] = {0, layout.rows_at, layout.narrow_at, layout.wide_at, layout.runs_at, layout.pages_at,
-                                layout.list_at};
+                                layout.list_at, layout.trees_at};
     const size_t words[kPlanParts] = {sizeof(PlanHeader) / 4, used.rows * sizeof(PlanRow) / 4, used.narrow * sizeof(PlanItem) / 4,
                                       used.wide * sizeof(PlanItem) / 4, used.runs * sizeof(PlanRun) / 4,
-                                      static_cast<size_t>(used.pages), used.list * sizeof(PlanRow) / 4};
+                                      static_cast<size_t>(used.pages), used.list * sizeof(PlanRow) / 4,
+                                      static_cast<size_t>(used.trees)};
     PlanParts parts;
     int end = 0;
     for (int i = 0; i < kPlanParts; ++i) {
@@ -1072,7 +1191,7 @@ hipError_t launch_copy_pages(uint8_t* pool, int64_t page_bytes, const PageMoves&
 }
 
 hipError_t launch_cache_append(const CacheShape& s, const int* image, const PlanLayout& layout, const PlanHeader& now,
-                               bool all, const AppendArgs& args, hipStream_t stream) {
+                               bool all, bool trees, const AppendArgs& args, hipStream_t stream) {
     if (now.runs == 0 && !all) return hipSuccess;
     // Four lane pairs a thread and access where every row allows it.
     const auto whole = [](const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; };
@@ -1084,11 +1203,33 @@ hipError_t launch_cache_append(const CacheShape& s, const int* image, const Plan
     const int64_t values = (static_cast<int64_t>(longest) / kGroupTokens + 1) * s.kv_heads * s.head_dim;
     const int y = static_cast<int>(std::min<int64_t>((std::max(turns, values) + kThreads - 1) / kThreads, 1024));
     const dim3 grid(all ? 256 : std::min(now.runs, 1 << 16), y);
-    const auto launch = [&](auto kernel) { kernel<<<grid, kThreads, 0, stream>>>(s, image, layout.runs_at, args); };
-    if (s.type == kF32)
-        packed ? launch(cache_append_kernel<float, 4>) : launch(cache_append_kernel<float, 1>);
+    const auto launch = [&](auto kernel) {
+        kernel<<<grid, kThreads, 0, stream>>>(s, image, layout.runs_at, layout.trees_at, args);
+    };
+    const auto of_turn = [&](auto turn) {
+        constexpr Turn kTurn = decltype(turn)::value;
+        if (s.type == kF32)
+            packed ? launch(cache_append_kernel<float, 4, kTurn>) : launch(cache_append_kernel<float, 1, kTurn>);
+        else
+            packed ? launch(cache_append_kernel<_Float16, 4, kTurn>) : launch(cache_append_kernel<_Float16, 1, kTurn>);
+    };
+    if (args.interleaved)
+        of_turn(std::integral_constant<Turn, Turn::kInterleaved>{});
+    else if (trees || args.frequencies)
+        of_turn(std::integral_constant<Turn, Turn::kTree>{});
     else
-        packed ? launch(cache_append_kernel<_Float16, 4>) : launch(cache_append_kernel<_Float16, 1>);
+        of_turn(std::integral_constant<Turn, Turn::kPlain>{});
+    return hipGetLastError();
+}
+
+hipError_t launch_cache_keep(const CacheShape& s, int layers, const KeepMoves& moves, hipStream_t stream) {
+    if (moves.sequences == 0) return hipSuccess;
+    const int64_t units = static_cast<int64_t>(layers) * s.kv_heads * (s.width * element_bytes(s.type) / 16 + s.head_dim);
+    const dim3 grid(static_cast<unsigned>(std::min<int64_t>((units + kThreads - 1) / kThreads, 1 << 16)), moves.sequences);
+    if (s.type == kF32)
+        cache_keep_kernel<float><<<grid, kThreads, 0, stream>>>(s, layers, moves);
+    else
+        cache_keep_kernel<_Float16><<<grid, kThreads, 0, stream>>>(s, layers, moves);
     return hipGetLastError();
 }
 
@@ -1097,8 +1238,8 @@ size_t cache_partial_bytes(const CacheShape& shape, int64_t slots) {
 }
 
 hipError_t launch_cache_attention(const CacheShape& shape, const int* image, const PlanLayout& layout, const PlanHeader& now,
-                                  bool all, int layer, const float* query, float* output, float* partials, size_t bytes,
-                                  hipStream_t stream) {
+                                  bool all, bool trees, int layer, const float* query, float* output, float* partials,
+                                  size_t bytes, hipStream_t stream) {
     if (now.rows == 0 && !all) return hipSuccess;
     const int64_t room = static_cast<int64_t>(bytes / cache_partial_bytes(shape, 1)) * shape.heads;
     const float scale = static_cast<float>(static_cast<double>(kLog2e) / std::sqrt(static_cast<double>(shape.head_dim)));
@@ -1113,10 +1254,11 @@ hipError_t launch_cache_attention(const CacheShape& shape, const int* image, con
                           output,
                           Partials{partials, room},
                           scale,
-                          shape.head_dim % 4 == 0 && reinterpret_cast<uintptr_t>(query) % 16 == 0};
+                          shape.head_dim % 4 == 0 && reinterpret_cast<uintptr_t>(query) % 16 == 0,
+                          now.tree_stride};
     const int groups = all ? kMostGroups : std::min(now.wide + now.narrow, 1 << 20);
     const hipError_t e = of_shape(shape.type, shape.width, [&](auto t, auto w) {
-        return attention_of_width<decltype(t), decltype(w)::value>(a, groups, stream);
+        return attention_of_width<decltype(t), decltype(w)::value>(a, groups, trees, stream);
     });
     if (e != hipSuccess || (now.joined == 0 && !all)) return e;
     const int64_t joins = static_cast<int64_t>(now.rows) * shape.heads;

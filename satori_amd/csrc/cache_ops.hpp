@@ -56,16 +56,30 @@ struct AppendArgs {
     const double* rope;   // table of rope_positions rows, or null
     int rope_positions;
     int layer;
+    // A rotation's own (rotation.hpp), in place of base: null without one.
+    const double* frequencies;
+    double magnitude;
+    bool interleaved;
 };
 // `image`: a plan's on the device, `now` its header. `all`: the launch is captured and replays may read any plan, so its
-// grid must do for any.
+// grid must do for any. `trees`: the plan may hold trees.
 hipError_t launch_cache_append(const CacheShape& shape, const int* image, const PlanLayout& layout, const PlanHeader& now,
-                               bool all, const AppendArgs& args, hipStream_t stream);
+                               bool all, bool trees, const AppendArgs& args, hipStream_t stream);
 
 // `partials`: at least cache_partial_bytes for the plan's slots. Launches with no work now are left out unless `all`.
 size_t cache_partial_bytes(const CacheShape& shape, int64_t slots);
 hipError_t launch_cache_attention(const CacheShape& shape, const int* image, const PlanLayout& layout, const PlanHeader& now,
-                                  bool all, int layer, const float* query, float* output, float* partials, size_t bytes,
-                                  hipStream_t stream);
+                                  bool all, bool trees, int layer, const float* query, float* output, float* partials,
+                                  size_t bytes, hipStream_t stream);
+
+// Positions to move within their sequences: pool place destination[i] = source[i] (page times page_tokens and the place in
+// it), in this order; begin: where a sequence's moves start. In the launch's arguments.
+constexpr int kKeepsPerLaunch = 256, kKeptSequences = 256;
+struct KeepMoves {
+    int sequences;
+    int source[kKeepsPerLaunch], destination[kKeepsPerLaunch];
+    uint16_t begin[kKeptSequences + 1];
+};
+hipError_t launch_cache_keep(const CacheShape& shape, int layers, const KeepMoves& moves, hipStream_t stream);
 
 }  // namespace satori

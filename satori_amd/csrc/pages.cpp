@@ -243,8 +243,57 @@ constexpr int64_t kPlaces = 512, kRoundBytes = 128 << 20;
 
 }  // namespace
 
+namespace {
+
+// The numbers of every row of a batch whose rows follow `parents` (PlanHeader::tree_stride of them each), and the context of
+// every sequence that is a tree; -1 for the others. Nothing where none is.
+void plan_trees(const PageTables& tables, const int* sequences, const int* new_tokens, int count, const int* parents,
+                PlanImage& image, std::vector<int>& contexts) {
+    int64_t stride = 0, first = 0;
+    for (int i = 0; i < count; first += new_tokens[i++]) {
+        const int rows = new_tokens[i], context = tables.tokens(sequences[i]) - rows;
+        bool tree = false;
+        for (int j = 0; j < rows; ++j) {
+            if (parents[first + j] < -1 || parents[first + j] >= j)
+                fail(SATORI_HIP_E_ARGUMENT_OUT_OF_RANGE, "A row of a tree follows one before it, or its context (-1).");
+            tree |= parents[first + j] != j - 1;
+        }
+        if (!tree) continue;
+        if (rows > kMostTree)
+            fail(SATORI_HIP_E_NOT_SUPPORTED, "Trees of more than " + std::to_string(kMostTree) + " rows are not supported.");
+        contexts[i] = context;
+        stride = std::max<int64_t>(stride, 1 + (context % kTile + rows + kTile - 1) / kTile);
+    }
+    if (stride == 0) return;
+    if (first * stride > INT32_MAX / 64) fail(SATORI_HIP_E_OVERFLOW, "Arithmetic operation resulted in an overflow.");
+    image.header.tree_stride = static_cast<int>(stride);
+    image.trees.resize(first * stride);
+    int* row = image.trees.data();
+    first = 0;
+    for (int i = 0; i < count; first += new_tokens[i++]) {
+        const int context = tables.tokens(sequences[i]) - new_tokens[i];
+        const int* const root = row;
+        for (int j = 0; j < new_tokens[i]; ++j, row += stride) {
+            const int parent = parents[first + j];
+            if (parent < 0) {
+                row[0] = context;
+                if (contexts[i] >= 0) row[1] = static_cast<int>((1u << context % kTile) - 1);
+            } else {
+                const int* of = root + parent * stride;
+                std::copy(of, of + (contexts[i] >= 0 ? stride : 1), row);
+                ++row[0];
+            }
+            if (contexts[i] < 0) continue;
+            const int bit = context % kTile + j;
+            row[1 + bit / kTile] = static_cast<int>(static_cast<unsigned>(row[1 + bit / kTile]) | 1u << bit % kTile);
+        }
+    }
+}
+
+}  // namespace
+
 PlanImage plan_batch(const PageTables& tables, const int* sequences, const int* new_tokens, int count,
-                     const PlanShape& shape, const PlanDivision& division) {
+                     const PlanShape& shape, const PlanDivision& division, const int* parents) {
     PlanImage image;
     const int P = tables.page_tokens();
     std::vector<int> sorted(sequences, sequences + count);
@@ -272,6 +321,11 @@ PlanImage plan_batch(const PageTables& tables, const int* sequences, const int* 
             rows.push_back({p, 0, 0, static_cast<int>(rows.size())});
         }
     }
+    // Of a tree's rows the context, which all of them see, and -1 of the others: by sequence, then by row.
+    std::vector<int> contexts(count, -1), context_of;
+    if (parents) plan_trees(tables, sequences, new_tokens, count, parents, image, contexts);
+    if (image.header.tree_stride > 0)
+        for (int i = 0; i < count; ++i) context_of.insert(context_of.end(), new_tokens[i], contexts[i]);
 
     const auto blocks_of = [](int64_t pairs) { return (pairs + kNarrowPairs - 1) / kNarrowPairs; };
     int64_t own = 0;  // items of the sequences by themselves, at least
@@ -443,8 +497,9 @@ PlanImage plan_batch(const PageTables& tables, const int* sequences, const int* 
                     item.kv = static_cast<int>(u % shape.kv_heads);
                     int least = INT_MAX, most = 0;
                     for (int r = item.pair / shape.group; r <= (item.pair + item.pairs - 1) / shape.group; ++r) {
-                        const int position = rows[row_list[n.rows + r]].position;
-                        least = std::min(least, position);
+                        const int of = row_list[n.rows + r], position = rows[of].position;
+                        const bool tree = !context_of.empty() && context_of[of] >= 0;
+                        least = std::min(least, tree ? context_of[of] - 1 : position);
                         most = std::max(most, position);
                     }
                     item.limit = least;
@@ -456,12 +511,14 @@ PlanImage plan_batch(const PageTables& tables, const int* sequences, const int* 
                         const PlanRow& row = rows[row_list[n.rows + item.pair / shape.group]];
                         item.row = row.row;
                         item.row_slot = row.slot;
-                        item.row_slots = row.slots;
+                        item.row_slots = contexts[n.members[0]] >= 0 ? -row.slots : row.slots;
                     }
                     list.push_back(item);
                 }
     }
 
+    for (size_t r = 0; r < context_of.size(); ++r)
+        if (context_of[r] >= 0) rows[r].position = -1 - context_of[r];
     image.list.reserve(row_list.size());
     for (int r : row_list) image.list.push_back(rows[r]);
     PlanHeader& h = image.header;
@@ -488,6 +545,7 @@ PlanImage plan_batch(const PageTables& tables, const int* sequences, const int* 
     image.plain.rows = image.plain.list = h.rows;
     image.plain.runs = entries(std::min<int64_t>(h.rows, h.rows / P + 2 * of_rows));
     image.plain.pages = entries(list_pages);
+    image.plain.trees = static_cast<int>(image.trees.size());
     image.plain.narrow = entries(narrow_blocks * units);
     image.plain.wide = entries(wide_blocks * units);
     image.plain_partials = chunks > 1 ? h.rows * chunks : 0;
@@ -495,18 +553,20 @@ PlanImage plan_batch(const PageTables& tables, const int* sequences, const int* 
 }
 
 bool plan_batch_within(const PageTables& tables, const int* sequences, const int* new_tokens, int count,
-                       const PlanShape& shape, const PlanLayout& room, int64_t partials, PlanImage& image) {
+                       const PlanShape& shape, const PlanLayout& room, int64_t partials, PlanImage& image,
+                       const int* parents) {
     PlanDivision division;
     for (;;) {
-        image = plan_batch(tables, sequences, new_tokens, count, shape, division);
+        image = plan_batch(tables, sequences, new_tokens, count, shape, division, parents);
         if (room.holds(image.least()) && image.header.partials <= partials) return true;
-        if (division.plain || image.header.rows > room.rows) return false;
+        if (division.plain || image.header.rows > room.rows || static_cast<int>(image.trees.size()) > room.trees) return false;
         division.workgroups > 1 ? void(division.workgroups /= 2) : void(division = kPlainDivision);
     }
 }
 
 bool PlanLayout::holds(const PlanLayout& l) const {
-    return l.rows <= rows && l.narrow <= narrow && l.wide <= wide && l.runs <= runs && l.pages <= pages && l.list <= list;
+    return l.rows <= rows && l.narrow <= narrow && l.wide <= wide && l.runs <= runs && l.pages <= pages && l.list <= list &&
+           l.trees <= trees;
 }
 
 bool PlanLayout::grow(const PlanLayout& least) {
@@ -523,6 +583,7 @@ bool PlanLayout::grow(const PlanLayout& least) {
     room(runs, least.runs);
     room(pages, least.pages);
     room(list, least.list);
+    room(trees, least.trees);
     if (!moved) return false;
     int64_t at = sizeof(PlanHeader) / 4;
     const auto place = [&](int& where, int64_t entries, size_t size) {
@@ -536,6 +597,7 @@ bool PlanLayout::grow(const PlanLayout& least) {
     place(runs_at, runs, sizeof(PlanRun));
     place(pages_at, pages, sizeof(int));
     place(list_at, list, sizeof(PlanRow));
+    place(trees_at, trees, sizeof(int));
     words = static_cast<int>(at);
     return true;
 }
@@ -543,7 +605,7 @@ bool PlanLayout::grow(const PlanLayout& least) {
 void PlanLayout::grow_plain(const PlanLayout& plain) {
     const int64_t most = 2 * (static_cast<int64_t>(plain.rows + int64_t(plain.list)) * (sizeof(PlanRow) / 4) +
                               (plain.narrow + int64_t(plain.wide)) * (sizeof(PlanItem) / 4) +
-                              int64_t(plain.runs) * (sizeof(PlanRun) / 4) + plain.pages);
+                              int64_t(plain.runs) * (sizeof(PlanRun) / 4) + plain.pages + plain.trees);
     if (words + most <= kMostPlainWords) grow(plain);
 }
 
@@ -565,6 +627,7 @@ PlanLayout PlanImage::least() const {
     l.runs = static_cast<int>(runs.size());
     l.pages = static_cast<int>(pages.size());
     l.list = static_cast<int>(list.size());
+    l.trees = static_cast<int>(trees.size());
     return l;
 }
 
@@ -582,6 +645,7 @@ void PlanImage::write(const PlanLayout& layout, int* words) const {
     put(layout.runs_at, runs);
     put(layout.pages_at, pages);
     put(layout.list_at, list);
+    put(layout.trees_at, trees);
 }
 
 }  // namespace satori

@@ -73,7 +73,8 @@ private:
 
 // ---- the plan of a batch ----
 
-// One query row: attends positions 0 .. position of its sequence. Its attention is the joined result of `slots` partial
+// One query row: attends positions 0 .. position of its sequence, or, as a row of a tree (position < 0), the first
+// -1 - position ones, its context, and what its words name (PlanTrees). Its attention is the joined result of `slots` partial
 // ones, slot .. slot + slots - 1 (one: written as the output by the workgroup that computes it).
 struct PlanRow {
     int position, slot, slots, row;
@@ -85,8 +86,9 @@ struct PlanRow {
 // rows' first slots; `limit` is the least position of the rows, so tokens up to it are seen by all of them.
 // What a workgroup would otherwise have to read before it can ask for its first keys and queries, each some 0.7 us behind the
 // item itself, is in the item: the pages of its first tokens (tile[i]: of tokens 32 i on, the last one's where it has fewer),
-// and its rows where they are one sequence's (row_slots > 0): row and position of pair p are then those of the item's first
+// and its rows where they are one sequence's (row_slots != 0): row and position of pair p are then those of the item's first
 // pair, `row` and `limit`, and p's distance from it in rows, and its slots begin at row_slot + that distance * row_slots.
+// Rows of a tree have -row_slots, and all of them the context 0 .. limit.
 struct PlanItem {
     int pages, first, tokens, rows;
     int pair, pairs, slot, kv;
@@ -106,13 +108,20 @@ struct PlanRun {
 struct PlanHeader {
     int rows, narrow, wide, runs;
     int joined, slots, longest_run, partials;
+    int tree_stride, pad[3];
 };
+
+// Where a batch has trees, tree_stride numbers for every row: the position that it stands for (its context and its depth in
+// the tree; where rows are no tree's, the one it lies at), and for a row of a tree a bit for each position from its context's
+// last multiple of 32 on, 32 a number: whether the row sees it. Bits in the order of positions, so that a tile of 32 has
+// one number; a row's own is its last one.
+constexpr int kMostTree = 1024;  // rows of a tree (33 numbers each)
 
 // Where the arrays lie in the image (in 4-byte words from its start) and how many entries each has room for. Launches
 // take it by value, so that a launch finds an array without reading where it is; room only grows.
 struct PlanLayout {
-    int rows_at = 0, narrow_at = 0, wide_at = 0, runs_at = 0, pages_at = 0, list_at = 0, words = 0;
-    int rows = 0, narrow = 0, wide = 0, runs = 0, pages = 0, list = 0;
+    int rows_at = 0, narrow_at = 0, wide_at = 0, runs_at = 0, pages_at = 0, list_at = 0, trees_at = 0, words = 0;
+    int rows = 0, narrow = 0, wide = 0, runs = 0, pages = 0, list = 0, trees = 0;
     // Room for at least these; whether anything moved.
     bool grow(const PlanLayout& least);
     bool holds(const PlanLayout& least) const;
@@ -135,7 +144,7 @@ struct PlanImage {
     std::vector<PlanRow> rows, list;  // list: the rows of every item's part of the tree
     std::vector<PlanItem> narrow, wide;
     std::vector<PlanRun> runs;
-    std::vector<int> pages;
+    std::vector<int> pages, trees;
     bool writable = true;  // no page that the rows lie in is shared
     PlanLayout least() const;  // the room they take
     // What kPlainDivision can take of any batch of no more rows, sequences with rows and pages in their lists, none of them
@@ -154,13 +163,16 @@ struct PlanDivision {
 };
 constexpr PlanDivision kPlainDivision{1, true};
 
-// Rows: the last new_tokens[i] positions of sequences[i], in this order.
+// Rows: the last new_tokens[i] positions of sequences[i], in this order. `parents`: of every row the one of the same sequence
+// that it follows, by its number among those, or -1 for the context; null: each the one before it. (Rows that follow one
+// another so are no tree, whether said or not.)
 PlanImage plan_batch(const PageTables& tables, const int* sequences, const int* new_tokens, int count,
-                     const PlanShape& shape, const PlanDivision& division = {});
+                     const PlanShape& shape, const PlanDivision& division = {}, const int* parents = nullptr);
 
 // The batch in the room that a plan has: in the usual division, or the first coarser one that fits. Whether one does.
 bool plan_batch_within(const PageTables& tables, const int* sequences, const int* new_tokens, int count,
-                       const PlanShape& shape, const PlanLayout& room, int64_t partials, PlanImage& image);
+                       const PlanShape& shape, const PlanLayout& room, int64_t partials, PlanImage& image,
+                       const int* parents = nullptr);
 
 // The tables behind a handle (satori_hip_pages_*).
 PageTables& page_tables(satori_hip_pages* handle);

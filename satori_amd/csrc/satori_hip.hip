@@ -21,6 +21,8 @@
 #include "gguf.hpp"
 #include "host_shapes.hpp"
 #include "kernels.hpp"
+#include "logits.hpp"
+#include "rotation.hpp"
 
 namespace satori {
 namespace {
@@ -162,7 +164,8 @@ struct satori_hip_context {
     std::vector<satori_hip_group*> captured_groups;
     std::vector<satori::PlanUse> captured_plans;
     std::vector<satori_hip_adapters*> captured_adapters;
-    int plans = 0, adapters = 0;  // live ones
+    std::vector<int*> captured_counts;  // `steps` of the rotations and logit rules (handles stay when they are destroyed)
+    int plans = 0, adapters = 0, handles = 0;  // live ones; handles: rotations and logit rules
 };
 
 struct satori_hip_matrix {
@@ -217,6 +220,9 @@ struct satori_hip_cache_plan {
     int turn = 0;
     int steps = 0;                   // captured steps that read the plan
     int appends = 0;                 // those of them that write its rows
+    // Whether it has held a tree: its launches then look for one (and captured ones take batches with and without).
+    bool trees = false;
+    std::vector<int> first_row, places;  // of the batch: every sequence's rows, and where each lies (KeepMoves)
     // Another library's graph may read it, or write its rows (until the plan is destroyed: such a graph's end is not told).
     bool elsewhere = false, appended_elsewhere = false;
     bool live = true;
@@ -227,6 +233,24 @@ struct satori_hip_adapters {
     satori::AdapterShape shape{};
     int count = 0;
     satori::DeviceBuffer table, workspace;
+    int steps = 0;
+    bool live = true;
+};
+
+struct satori_hip_rotation {
+    satori_hip_context* context = nullptr;
+    satori::RotationShape shape{};
+    satori::DeviceBuffer memory;  // frequencies, then the table
+    int steps = 0;
+    bool live = true;
+};
+
+struct satori_hip_logit_rules {
+    satori_hip_context* context = nullptr;
+    int vocabulary = 0;
+    satori::LogitBiases biases{};
+    satori::DeviceBuffer sets, found;
+    satori::PinnedBuffer staging;
     int steps = 0;
     bool live = true;
 };
@@ -244,6 +268,7 @@ struct satori_hip_step {
     bool attention = false;                    // the graph uses the context's split-attention workspace
     std::vector<satori::PlanUse> plans;        // read by the graph (each once), and what they and the adapters own
     std::vector<satori_hip_adapters*> adapters;
+    std::vector<int*> counts;                  // of the rotations and logit rules it launches with
     hipGraph_t graph = nullptr;
     hipGraphExec_t exec = nullptr;
     bool live = true;
@@ -966,8 +991,8 @@ int satori_hip_context_destroy(satori_hip_context* c) {
         if (!c->live) return;
         if (c->matrices > 0)
             fail(SATORI_HIP_E_ARGUMENT, "Matrices created on the context must be destroyed first.");
-        if (c->plans > 0 || c->adapters > 0)
-            fail(SATORI_HIP_E_ARGUMENT, "Cache plans and adapters created on the context must be destroyed first.");
+        if (c->plans > 0 || c->adapters > 0 || c->handles > 0)
+            fail(SATORI_HIP_E_ARGUMENT, "Cache plans, adapters, rotations and logit rules created on the context must be destroyed first.");
         (void)hipSetDevice(c->device);
         (void)hipStreamSynchronize(c->stream);
         c->x.release();
@@ -1645,6 +1670,8 @@ int satori_hip_step_destroy(satori_hip_step* s) {
             use.plan->appends -= use.appends;
         }
         for (satori_hip_adapters* a : s->adapters) a->steps--;
+        for (int* n : s->counts) --*n;
+        s->counts.clear();
         s->plans.clear();
         s->adapters.clear();
         s->groups.clear();
@@ -1668,6 +1695,7 @@ int satori_hip_capture_begin(satori_hip_context* c) {
         c->captured_groups.clear();
         c->captured_plans.clear();
         c->captured_adapters.clear();
+        c->captured_counts.clear();
         c->captured_attention = false;
     });
 }
@@ -1689,6 +1717,8 @@ int satori_hip_capture_end(satori_hip_context* c, satori_hip_step** step) {
         std::vector<satori_hip_adapters*> adapters;
         plans.swap(c->captured_plans);
         adapters.swap(c->captured_adapters);
+        std::vector<int*> counts;
+        counts.swap(c->captured_counts);
         struct Scratch {  // freed unless a step takes it
             std::vector<DeviceBuffer> buffers;
             ~Scratch() {
@@ -1741,6 +1771,8 @@ int satori_hip_capture_end(satori_hip_context* c, satori_hip_step** step) {
                 a->steps++;
             }
         }
+        st->counts.swap(counts);
+        for (int* n : st->counts) ++*n;
         st->attention = c->captured_attention;
         if (st->attention) c->attention_steps++;
         c->captured_attention = false;
@@ -2385,6 +2417,120 @@ bool note_plan(satori_hip_context* c, satori_hip_cache_plan* p, int layer, hipSt
     return true;
 }
 
+// A live rotation of the context for heads of head_dim lanes.
+void require_rotation(const satori_hip_rotation* r, const satori_hip_context* c, int head_dim) {
+    require(r, "rotation");
+    if (!r->live) fail(SATORI_HIP_E_OBJECT_DISPOSED, "Cannot access a disposed object. Object name: 'satori_hip_rotation'.");
+    if (r->context != c) fail(SATORI_HIP_E_ARGUMENT, "The rotation belongs to another context.");
+    if (2 * r->shape.pairs > head_dim) out_of_range("rotaryDimensions");
+}
+
+// The plan's next batch (satori_hip_cache_plan_set, and of trees where `parents` is given).
+void set_plan(satori_hip_context* c, satori_hip_cache_plan* p, satori_hip_pages* pages, const int* sequences,
+              const int* new_tokens, int count, const int* parents, void* stream) {
+    require(pages, "pages");
+    if (count < 0) out_of_range("count");
+    if (count > 0) {
+        require(sequences, "sequences");
+        require(new_tokens, "newTokens");
+    }
+    const hipStream_t st = op_stream(c, stream);
+    require_not_capturing(c);
+    if (captured_elsewhere(c, st))
+        fail(SATORI_HIP_E_INVALID_OPERATION, "A plan cannot be set while its stream is being captured.");
+    PlanImage image;
+    {
+        PageTables& tables = page_tables(pages);
+        const std::shared_lock<std::shared_mutex> tables_guard(tables.lock);
+        if (!tables.live())
+            fail(SATORI_HIP_E_OBJECT_DISPOSED, "Cannot access a disposed object. Object name: 'satori_hip_pages'.");
+        if (tables.pages() != p->page_count || tables.page_tokens() != p->shape.page_tokens)
+            fail(SATORI_HIP_E_ARGUMENT, "The pages are not those of the plan's pool.");
+        if (held(p)) {
+            const int64_t room = static_cast<int64_t>(p->partials.bytes / cache_partial_bytes(p->shape, 1));
+            if (!plan_batch_within(tables, sequences, new_tokens, count, p->plan, p->layout, room, image,
+                                   parents))
+                plan_held();
+        } else {
+            image = plan_batch(tables, sequences, new_tokens, count, p->plan, {}, parents);
+        }
+    }
+    if (static_cast<int64_t>(image.header.rows) * p->shape.heads > INT32_MAX / 4)
+        fail(SATORI_HIP_E_OVERFLOW, "Arithmetic operation resulted in an overflow.");
+    if (!image.writable && (p->appends > 0 || p->appended_elsewhere))
+        fail(SATORI_HIP_E_INVALID_OPERATION,
+             "A captured step writes the rows, which lie in pages that other sequences hold: extend their sequences.");
+    PlanLayout layout = p->layout;
+    const PlanLayout used = image.least();
+    size_t partials = cache_partial_bytes(p->shape, image.header.partials);
+    if (!held(p)) {
+        layout.grow(used);
+        layout.grow_plain(image.plain);
+        partials = std::max(partials, cache_partial_bytes(p->shape, image.plain_partials));
+    }
+    const size_t bytes = static_cast<size_t>(layout.words) * 4;
+    std::vector<int> first_row(count + 1), places(image.header.rows);
+    for (int i = 0; i < count; ++i) first_row[i + 1] = first_row[i] + new_tokens[i];
+    for (const PlanRun& run : image.runs)
+        for (int i = 0; i < run.tokens; ++i) places[run.row + i] = run.page * p->shape.page_tokens + run.offset + i;
+    const CaptureRelaxed relaxed;  // another stream may be in a capture that forbids allocations
+    p->set = false;  // until the new batch is on its way: where memory cannot be had, the old one's may be gone
+    // The rows' queries and outputs, which the calls need beside it (asked of the device only where it could matter).
+    const double rows_bytes = 8.0 * image.header.rows * p->shape.heads * p->shape.head_dim;
+    size_t free_bytes = 0, all_bytes = 0;
+    if (rows_bytes > 0x1p36) check_hip(hipMemGetInfo(&free_bytes, &all_bytes), "hipMemGetInfo");
+    if (rows_bytes > 0x1p36 && rows_bytes > static_cast<double>(all_bytes))
+        fail(SATORI_HIP_E_OUT_OF_MEMORY, "The queries and outputs of the plan's rows exceed the device's memory.");
+    reserve_for_plan(p, p->image, bytes);
+    reserve_for_plan(p, p->partials, partials);
+    const int turn = p->turn;
+    check_hip(hipEventSynchronize(p->copied[turn]), "plan copy");  // (done at once where none was recorded)
+    p->staging[turn].reserve(p->image.bytes);
+    int* staging = static_cast<int*>(p->staging[turn].ptr);
+    image.write(layout, staging);
+    check_hip(launch_plan_copy(staging, static_cast<int*>(p->image.ptr), layout, used, st), "plan copy");
+    check_hip(hipEventRecord(p->copied[turn], st), "plan copy");
+    p->turn ^= 1;
+    p->layout = layout;
+    p->header = image.header;
+    p->writable = image.writable;
+    p->trees |= image.header.tree_stride > 0;
+    p->first_row.swap(first_row);
+    p->places.swap(places);
+    p->set = true;
+}
+
+// The attention inputs of every row of the plan into its pages: by satori_hip_cache_append's arguments, or a rotation.
+void append_plan(satori_hip_context* c, satori_hip_cache_plan* p, AppendArgs args, void* stream) {
+    require(args.query, "query");
+    require(args.query_out, "queryOut");
+    require(args.key, "key");
+    require(args.value, "value");
+    const CacheShape& s = p->shape;
+    const hipStream_t st = op_stream(c, stream);
+    if (!p->set) fail(SATORI_HIP_E_INVALID_OPERATION, "Set the plan's batch first.");
+    if (!p->writable)
+        fail(SATORI_HIP_E_INVALID_OPERATION, "The rows lie in pages that other sequences hold: extend their sequences.");
+    const int64_t rows = p->header.rows, qb = rows * s.heads * s.head_dim * 4, kb = rows * s.kv_heads * s.head_dim * 4;
+    const int64_t pool = s.page_bytes * p->page_count;
+    if ((bytes_overlap(args.query, qb, args.query_out, qb) && args.query != args.query_out) ||
+        bytes_overlap(args.key, kb, args.query_out, qb) || bytes_overlap(args.value, kb, args.query_out, qb) ||
+        bytes_overlap(args.query, qb, s.pool, pool) || bytes_overlap(args.query_out, qb, s.pool, pool) ||
+        bytes_overlap(args.key, kb, s.pool, pool) || bytes_overlap(args.value, kb, s.pool, pool))
+        fail(SATORI_HIP_E_ARGUMENT, "Partial overlap.");
+    const bool captured = note_plan(c, p, args.layer, st, true);
+    check_hip(launch_cache_append(s, static_cast<const int*>(p->image.ptr), p->layout, p->header, captured, p->trees, args, st),
+              "cache append launch");
+}
+
+// A launch with a rotation or logit rules becomes part of the context's captured step.
+template <class H>
+void note_handle(satori_hip_context* c, H* handle, hipStream_t stream) {
+    if (!c->capturing || stream != c->stream) return;
+    if (std::find(c->captured_counts.begin(), c->captured_counts.end(), &handle->steps) == c->captured_counts.end())
+        c->captured_counts.push_back(&handle->steps);
+}
+
 }  // namespace
 
 extern "C" {
@@ -2487,68 +2633,14 @@ int satori_hip_cache_plan_destroy(satori_hip_cache_plan* p) {
 
 int satori_hip_cache_plan_set(satori_hip_cache_plan* p, satori_hip_pages* pages, const int* sequences,
                               const int* new_tokens, int count, void* stream) {
+    return plan_call(p, [&](satori_hip_context* c) { set_plan(c, p, pages, sequences, new_tokens, count, nullptr, stream); });
+}
+
+int satori_hip_cache_plan_set_tree(satori_hip_cache_plan* p, satori_hip_pages* pages, const int* sequences,
+                                   const int* new_tokens, const int* parents, int count, void* stream) {
     return plan_call(p, [&](satori_hip_context* c) {
-        require(pages, "pages");
-        if (count < 0) out_of_range("count");
-        if (count > 0) {
-            require(sequences, "sequences");
-            require(new_tokens, "newTokens");
-        }
-        const hipStream_t st = op_stream(c, stream);
-        require_not_capturing(c);
-        if (captured_elsewhere(c, st))
-            fail(SATORI_HIP_E_INVALID_OPERATION, "A plan cannot be set while its stream is being captured.");
-        PlanImage image;
-        {
-            PageTables& tables = page_tables(pages);
-            const std::shared_lock<std::shared_mutex> tables_guard(tables.lock);
-            if (!tables.live())
-                fail(SATORI_HIP_E_OBJECT_DISPOSED, "Cannot access a disposed object. Object name: 'satori_hip_pages'.");
-            if (tables.pages() != p->page_count || tables.page_tokens() != p->shape.page_tokens)
-                fail(SATORI_HIP_E_ARGUMENT, "The pages are not those of the plan's pool.");
-            if (held(p)) {
-                const int64_t room = static_cast<int64_t>(p->partials.bytes / cache_partial_bytes(p->shape, 1));
-                if (!plan_batch_within(tables, sequences, new_tokens, count, p->plan, p->layout, room, image)) plan_held();
-            } else {
-                image = plan_batch(tables, sequences, new_tokens, count, p->plan);
-            }
-        }
-        if (static_cast<int64_t>(image.header.rows) * p->shape.heads > INT32_MAX / 4)
-            fail(SATORI_HIP_E_OVERFLOW, "Arithmetic operation resulted in an overflow.");
-        if (!image.writable && (p->appends > 0 || p->appended_elsewhere))
-            fail(SATORI_HIP_E_INVALID_OPERATION,
-                 "A captured step writes the rows, which lie in pages that other sequences hold: extend their sequences.");
-        PlanLayout layout = p->layout;
-        const PlanLayout used = image.least();
-        size_t partials = cache_partial_bytes(p->shape, image.header.partials);
-        if (!held(p)) {
-            layout.grow(used);
-            layout.grow_plain(image.plain);
-            partials = std::max(partials, cache_partial_bytes(p->shape, image.plain_partials));
-        }
-        const size_t bytes = static_cast<size_t>(layout.words) * 4;
-        const CaptureRelaxed relaxed;  // another stream may be in a capture that forbids allocations
-        p->set = false;  // until the new batch is on its way: where memory cannot be had, the old one's may be gone
-        // The rows' queries and outputs, which the calls need beside it (asked of the device only where it could matter).
-        const double rows_bytes = 8.0 * image.header.rows * p->shape.heads * p->shape.head_dim;
-        size_t free_bytes = 0, all_bytes = 0;
-        if (rows_bytes > 0x1p36) check_hip(hipMemGetInfo(&free_bytes, &all_bytes), "hipMemGetInfo");
-        if (rows_bytes > 0x1p36 && rows_bytes > static_cast<double>(all_bytes))
-            fail(SATORI_HIP_E_OUT_OF_MEMORY, "The queries and outputs of the plan's rows exceed the device's memory.");
-        reserve_for_plan(p, p->image, bytes);
-        reserve_for_plan(p, p->partials, partials);
-        const int turn = p->turn;
-        check_hip(hipEventSynchronize(p->copied[turn]), "plan copy");  // (done at once where none was recorded)
-        p->staging[turn].reserve(p->image.bytes);
-        int* staging = static_cast<int*>(p->staging[turn].ptr);
-        image.write(layout, staging);
-        check_hip(launch_plan_copy(staging, static_cast<int*>(p->image.ptr), layout, used, st), "plan copy");
-        check_hip(hipEventRecord(p->copied[turn], st), "plan copy");
-        p->turn ^= 1;
-        p->layout = layout;
-        p->header = image.header;
-        p->writable = image.writable;
-        p->set = true;
+        if (count > 0) require(parents, "parents");
+        set_plan(c, p, pages, sequences, new_tokens, count, parents, stream);
     });
 }
 
@@ -2557,29 +2649,75 @@ int satori_hip_cache_append(satori_hip_cache_plan* p, int layer, const float* qu
                             const float* value_bias, double frequency_base, int rotary_dimensions,
                             const double* rope_table, int rope_positions, void* stream) {
     return plan_call(p, [&](satori_hip_context* c) {
-        require(query, "query");
-        require(query_out, "queryOut");
-        require(key, "key");
-        require(value, "value");
-        const CacheShape& s = p->shape;
-        check_rotation(s.head_dim, frequency_base, rotary_dimensions);
+        check_rotation(p->shape.head_dim, frequency_base, rotary_dimensions);
         if (rope_positions < 0) out_of_range("ropePositions");
+        append_plan(c, p,
+                    AppendArgs{query, query_bias, key, key_bias, value, value_bias, query_out, frequency_base,
+                               rotary_dimensions, rope_table, rope_table ? rope_positions : 0, layer, nullptr, 1.0, false},
+                    stream);
+    });
+}
+
+int satori_hip_cache_append_rotated(satori_hip_cache_plan* p, int layer, const float* query, const float* query_bias,
+                                    float* query_out, const float* key, const float* key_bias, const float* value,
+                                    const float* value_bias, satori_hip_rotation* rotation, void* stream) {
+    return plan_call(p, [&](satori_hip_context* c) {
+        require_rotation(rotation, c, p->shape.head_dim);
+        const RotationShape& r = rotation->shape;
+        append_plan(c, p,
+                    AppendArgs{query, query_bias, key, key_bias, value, value_bias, query_out, 1.0, 2 * r.pairs, r.table,
+                               r.positions, layer, r.frequencies, r.magnitude, r.interleaved},
+                    stream);
+        note_handle(c, rotation, op_stream(c, stream));
+    });
+}
+
+int satori_hip_cache_keep(satori_hip_cache_plan* p, const int* kept, const int* counts, int count, void* stream) {
+    return plan_call(p, [&](satori_hip_context* c) {
         const hipStream_t st = op_stream(c, stream);
+        require_not_capturing(c);
+        if (captured_elsewhere(c, st))
+            fail(SATORI_HIP_E_INVALID_OPERATION, "Rows cannot be kept while the stream is being captured.");
         if (!p->set) fail(SATORI_HIP_E_INVALID_OPERATION, "Set the plan's batch first.");
         if (!p->writable)
             fail(SATORI_HIP_E_INVALID_OPERATION, "The rows lie in pages that other sequences hold: extend their sequences.");
-        const int64_t rows = p->header.rows, qb = rows * s.heads * s.head_dim * 4, kb = rows * s.kv_heads * s.head_dim * 4;
-        const int64_t pool = s.page_bytes * p->page_count;
-        if ((bytes_overlap(query, qb, query_out, qb) && query != query_out) || bytes_overlap(key, kb, query_out, qb) ||
-            bytes_overlap(value, kb, query_out, qb) || bytes_overlap(query, qb, s.pool, pool) ||
-            bytes_overlap(query_out, qb, s.pool, pool) || bytes_overlap(key, kb, s.pool, pool) ||
-            bytes_overlap(value, kb, s.pool, pool))
-            fail(SATORI_HIP_E_ARGUMENT, "Partial overlap.");
-        const bool captured = note_plan(c, p, layer, st, true);
-        const AppendArgs args{query, query_bias, key, key_bias, value, value_bias, query_out, frequency_base,
-                              rotary_dimensions, rope_table, rope_table ? rope_positions : 0, layer};
-        check_hip(launch_cache_append(s, static_cast<const int*>(p->image.ptr), p->layout, p->header, captured, args, st),
-                  "cache append launch");
+        if (count != static_cast<int>(p->first_row.size()) - 1)
+            fail(SATORI_HIP_E_ARGUMENT, "A number of kept rows for every sequence of the plan.");
+        if (count > 0) require(counts, "counts");
+        int64_t total = 0;
+        for (int i = 0; i < count; ++i) {
+            if (counts[i] < 0 || counts[i] > p->first_row[i + 1] - p->first_row[i]) out_of_range("counts");
+            total += counts[i];
+        }
+        if (total > 0) require(kept, "kept");
+        const int* rows = kept;
+        for (int i = 0; i < count; rows += counts[i++])
+            for (int j = 0; j < counts[i]; ++j)
+                if (rows[j] < 0 || rows[j] >= p->first_row[i + 1] - p->first_row[i] || (j > 0 && rows[j] <= rows[j - 1]))
+                    fail(SATORI_HIP_E_ARGUMENT_OUT_OF_RANGE, "Kept rows are a sequence's own, in ascending order.");
+        KeepMoves moves{};
+        int made = 0;
+        const auto flush = [&] {
+            check_hip(launch_cache_keep(p->shape, p->layers, moves, st), "cache keep launch");
+            moves.sequences = made = 0;
+        };
+        rows = kept;
+        for (int i = 0; i < count; rows += counts[i++]) {
+            bool opened = false;  // in this launch
+            for (int j = 0; j < counts[i]; ++j) {
+                if (rows[j] == j) continue;
+                if (made == kKeepsPerLaunch || (!opened && moves.sequences == kKeptSequences)) {
+                    flush();
+                    opened = false;
+                }
+                if (!opened) ++moves.sequences;
+                opened = true;
+                moves.source[made] = p->places[p->first_row[i] + rows[j]];
+                moves.destination[made] = p->places[p->first_row[i] + j];
+                moves.begin[moves.sequences] = static_cast<uint16_t>(++made);
+            }
+        }
+        flush();
     });
 }
 
@@ -2595,8 +2733,8 @@ int satori_hip_cache_attention(satori_hip_cache_plan* p, int layer, const float*
         if (bytes_overlap(query, bytes, output, bytes) || bytes_overlap(output, bytes, s.pool, pool))
             fail(SATORI_HIP_E_ARGUMENT, "Attention output overlaps input.");
         const bool captured = note_plan(c, p, layer, st, false);
-        check_hip(launch_cache_attention(s, static_cast<const int*>(p->image.ptr), p->layout, p->header, captured, layer, query,
-                                         output, static_cast<float*>(p->partials.ptr), p->partials.bytes, st),
+        check_hip(launch_cache_attention(s, static_cast<const int*>(p->image.ptr), p->layout, p->header, captured, p->trees,
+                                         layer, query, output, static_cast<float*>(p->partials.ptr), p->partials.bytes, st),
                   "cache attention launch");
     });
 }
@@ -2720,6 +2858,244 @@ int satori_hip_adapters_apply(satori_hip_adapters* a, const int* selection, int 
                                       static_cast<float*>(a->workspace.ptr), st),
                       "adapters launch");
         }
+    });
+}
+
+int satori_hip_rotation_create(satori_hip_context* c, int layout, int rotary_dimensions, const double* frequencies,
+                               double magnitude, int positions, satori_hip_rotation** rotation) {
+    return guarded([&] {
+        require(rotation, "rotation");
+        *rotation = nullptr;
+        require_live(c);
+        std::lock_guard<std::mutex> guard(c->lock);
+        require_live(c);
+        require_not_capturing(c);
+        require(frequencies, "frequencies");
+        if (layout != SATORI_HIP_ROTARY_HALF && layout != SATORI_HIP_ROTARY_INTERLEAVED) out_of_range("layout");
+        if (rotary_dimensions <= 0 || rotary_dimensions % 2 != 0 || rotary_dimensions > (1 << 16)) out_of_range("rotaryDimensions");
+        if (!std::isfinite(magnitude)) out_of_range("magnitude");
+        if (positions < 0) out_of_range("positions");
+        const int pairs = rotary_dimensions / 2;
+        for (int k = 0; k < pairs; ++k)
+            if (!std::isfinite(frequencies[k])) out_of_range("frequencies");
+        set_device(c);
+        const CaptureRelaxed relaxed;  // another stream may be in a capture that forbids allocations
+        auto* r = new satori_hip_rotation();
+        r->context = c;
+        const size_t head = (static_cast<size_t>(pairs) + 1) / 2 * 2;  // the table starts at a multiple of 16 bytes
+        try {
+            r->memory.reserve((head + static_cast<size_t>(positions) * rotary_dimensions) * sizeof(double));
+            double* at = static_cast<double*>(r->memory.ptr);
+            r->shape = RotationShape{at, at + head, positions, pairs, magnitude, layout == SATORI_HIP_ROTARY_INTERLEAVED};
+            check_hip(hipMemcpyAsync(at, frequencies, pairs * sizeof(double), hipMemcpyHostToDevice, c->stream), "rotation copy");
+            check_hip(launch_rotation_table(r->shape, at + head, c->stream), "rotation table launch");
+            check_hip(hipStreamSynchronize(c->stream), "stream");
+        } catch (...) {
+            r->memory.release();
+            delete r;
+            throw;
+        }
+        c->handles++;
+        *rotation = r;
+    });
+}
+
+int satori_hip_rotation_destroy(satori_hip_rotation* r) {
+    return guarded([&] {
+        if (!r) return;
+        satori_hip_context* c = r->context;
+        std::lock_guard<std::mutex> guard(c->lock);
+        require_not_capturing(c);
+        if (!r->live) return;
+        if (r->steps > 0) fail(SATORI_HIP_E_ARGUMENT, "Steps that use the rotation must be destroyed first.");
+        (void)hipSetDevice(c->device);
+        (void)hipStreamSynchronize(c->stream);
+        r->memory.release();
+        r->live = false;
+        c->handles--;
+    });
+}
+
+int satori_hip_rotation_apply(satori_hip_rotation* r, int type, const void* input, int64_t input_stride, void* output,
+                              int64_t output_stride, int rows, int heads, int head_dim, const int* positions, void* stream) {
+    return handle_call(r, "rotation", "satori_hip_rotation", [&](satori_hip_context* c) {
+        require(input, "input");
+        require(output, "output");
+        require(positions, "positions");
+        element_type(type);
+        if (rows < 0) out_of_range("rows");
+        if (heads <= 0 || head_dim <= 0 || head_dim > INT32_MAX / 64 / heads) out_of_range("heads");
+        if (2 * r->shape.pairs > head_dim) out_of_range("rotaryDimensions");
+        if (rows == 0) return;
+        const int64_t width = static_cast<int64_t>(heads) * head_dim, size = element_bytes(type);
+        const int64_t most = INT64_MAX / 16 / rows;
+        if (input_stride < width || input_stride > most) out_of_range("inputStride");
+        if (output_stride < width || output_stride > most) out_of_range("outputStride");
+        if (reinterpret_cast<uintptr_t>(input) % size != 0 || reinterpret_cast<uintptr_t>(output) % size != 0 ||
+            reinterpret_cast<uintptr_t>(positions) % 4 != 0)
+            fail(SATORI_HIP_E_ARGUMENT, "Rows and positions must be aligned to their elements.");
+        const int64_t in = ((rows - 1) * input_stride + width) * size, out = ((rows - 1) * output_stride + width) * size;
+        if ((bytes_overlap(input, in, output, out) && !(input == output && input_stride == output_stride)) ||
+            bytes_overlap(positions, static_cast<int64_t>(rows) * 4, output, out))
+            fail(SATORI_HIP_E_ARGUMENT, "Partial overlap.");
+        const hipStream_t st = op_stream(c, stream);
+        check_hip(launch_rotate(r->shape, type, RotateArgs{input, output, input_stride, output_stride, positions, rows, heads, head_dim}, st),
+                  "rotation launch");
+        note_handle(c, r, st);
+    });
+}
+
+int satori_hip_logit_rules_create(satori_hip_context* c, int vocabulary, int bias_sets, int bias_entries,
+                                  satori_hip_logit_rules** rules) {
+    return guarded([&] {
+        require(rules, "rules");
+        *rules = nullptr;
+        require_live(c);
+        std::lock_guard<std::mutex> guard(c->lock);
+        require_live(c);
+        require_not_capturing(c);
+        if (vocabulary <= 0 || vocabulary > (1 << 28)) out_of_range("vocabulary");
+        if (bias_sets < 0) out_of_range("biasSets");
+        if (bias_entries < 0 || bias_entries > vocabulary) out_of_range("biasEntries");
+        const int64_t words = logit_bias_words(vocabulary, bias_entries);
+        if (words > INT32_MAX) fail(SATORI_HIP_E_OVERFLOW, "Arithmetic operation resulted in an overflow.");
+        set_device(c);
+        const CaptureRelaxed relaxed;  // another stream may be in a capture that forbids allocations
+        auto* r = new satori_hip_logit_rules();
+        r->context = c;
+        r->vocabulary = vocabulary;
+        try {
+            const size_t set_bytes = static_cast<size_t>(words) * 4, found = kLogitRows * sizeof(LogitBest);
+            r->sets.reserve(std::max<size_t>(set_bytes * bias_sets, 16));
+            r->found.reserve(found);
+            r->staging.reserve(set_bytes);
+            check_hip(hipMemsetAsync(r->sets.ptr, 0, r->sets.bytes, c->stream), "logit rules");  // (all sets empty)
+            check_hip(hipMemsetAsync(r->found.ptr, 0, found, c->stream), "logit rules");
+            check_hip(hipStreamSynchronize(c->stream), "stream");
+        } catch (...) {
+            r->sets.release();
+            r->found.release();
+            r->staging.release();
+            delete r;
+            throw;
+        }
+        r->biases = LogitBiases{static_cast<const int*>(r->sets.ptr), bias_sets, bias_entries, static_cast<int>(words)};
+        c->handles++;
+        *rules = r;
+    });
+}
+
+int satori_hip_logit_rules_destroy(satori_hip_logit_rules* r) {
+    return guarded([&] {
+        if (!r) return;
+        satori_hip_context* c = r->context;
+        std::lock_guard<std::mutex> guard(c->lock);
+        require_not_capturing(c);
+        if (!r->live) return;
+        if (r->steps > 0) fail(SATORI_HIP_E_ARGUMENT, "Steps that use the logit rules must be destroyed first.");
+        (void)hipSetDevice(c->device);
+        (void)hipStreamSynchronize(c->stream);
+        r->sets.release();
+        r->found.release();
+        r->staging.release();
+        r->live = false;
+        c->handles--;
+    });
+}
+
+int satori_hip_logit_rules_set_biases(satori_hip_logit_rules* r, int set, const int* tokens, const float* values, int count,
+                                      void* stream) {
+    return handle_call(r, "rules", "satori_hip_logit_rules", [&](satori_hip_context* c) {
+        const hipStream_t st = op_stream(c, stream);
+        require_not_capturing(c);
+        if (captured_elsewhere(c, st))
+            fail(SATORI_HIP_E_INVALID_OPERATION, "Biases cannot be set while the stream is being captured.");
+        if (set < 0 || set >= r->biases.count) out_of_range("set");
+        if (count < 0 || count > r->biases.entries) out_of_range("count");
+        if (count > 0) {
+            require(tokens, "tokens");
+            require(values, "values");
+        }
+        std::vector<int> order(count);
+        for (int i = 0; i < count; ++i) {
+            if (tokens[i] < 0 || tokens[i] >= r->vocabulary) out_of_range("tokens");
+            if (std::isnan(values[i])) out_of_range("values");
+            order[i] = i;
+        }
+        std::sort(order.begin(), order.end(), [&](int a, int b) { return tokens[a] < tokens[b]; });
+        for (int i = 1; i < count; ++i)
+            if (tokens[order[i]] == tokens[order[i - 1]]) fail(SATORI_HIP_E_ARGUMENT, "A token is listed twice.");
+        const int slices = logit_slices(r->vocabulary);
+        int* starts = static_cast<int*>(r->staging.ptr);
+        int* sorted = starts + slices + 1;
+        float* of = reinterpret_cast<float*>(sorted + r->biases.entries);
+        std::fill(starts, starts + slices + 1, 0);
+        for (int i = 0; i < count; ++i) {
+            sorted[i] = tokens[order[i]];
+            of[i] = values[order[i]];
+            ++starts[sorted[i] / kLogitSlice + 1];
+        }
+        for (int i = 0; i < slices; ++i) starts[i + 1] += starts[i];
+        int* to = static_cast<int*>(r->sets.ptr) + static_cast<int64_t>(set) * r->biases.words;
+        check_hip(hipMemcpyAsync(to, starts, static_cast<size_t>(r->biases.words) * 4, hipMemcpyHostToDevice, st), "bias copy");
+        check_hip(hipStreamSynchronize(st), "stream");
+    });
+}
+
+int satori_hip_logit_rules_apply(satori_hip_logit_rules* r, const satori_hip_logit_batch* b, void* stream) {
+    return handle_call(r, "rules", "satori_hip_logit_rules", [&](satori_hip_context* c) {
+        require(b, "batch");
+        if (b->count < 0) out_of_range("count");
+        if (b->histories < 0) out_of_range("histories");
+        if (b->mask_count < 0) out_of_range("maskCount");
+        if (b->count == 0) return;
+        require(b->rows, "rows");
+        require(b->logits, "logits");
+        if (!b->output && !b->best) fail(SATORI_HIP_E_ARGUMENT, "Neither logits nor best tokens are asked for.");
+        const int64_t rows = b->count, v = r->vocabulary, words = (v + 31) / 32;
+        const auto check_stride = [](int64_t stride, int64_t least, int64_t lines, const char* name) {
+            if (stride < least || stride > INT64_MAX / 16 / lines) out_of_range(name);
+        };
+        check_stride(b->logits_stride, v, rows, "logitsStride");
+        if (b->output) check_stride(b->output_stride, v, rows, "outputStride");
+        if (b->histories > 0) {
+            require(b->history, "history");
+            require(b->lengths, "lengths");
+            check_stride(b->history_stride, 0, b->histories, "historyStride");
+        }
+        if (b->mask_count > 0) {
+            require(b->masks, "masks");
+            check_stride(b->mask_stride, words, b->mask_count, "maskStride");
+        }
+        for (const void* p : {static_cast<const void*>(b->rows), static_cast<const void*>(b->logits), static_cast<const void*>(b->output),
+                              static_cast<const void*>(b->best), static_cast<const void*>(b->history),
+                              static_cast<const void*>(b->lengths), static_cast<const void*>(b->masks)})
+            if (reinterpret_cast<uintptr_t>(p) % 4 != 0) fail(SATORI_HIP_E_ARGUMENT, "Arrays must be aligned to their elements.");
+        // What the launches write against all that they read, and against each other.
+        struct Range {
+            const void* at;
+            int64_t bytes;
+        };
+        const int64_t in = ((rows - 1) * b->logits_stride + v) * 4, out = ((rows - 1) * b->output_stride + v) * 4;
+        const Range logits{b->logits, in}, output{b->output, b->output ? out : 0}, best{b->best, rows * 4};
+        const Range others[] = {{b->rows, rows * static_cast<int64_t>(sizeof(LogitRow))},
+                                {b->history, b->histories * b->history_stride * 4},
+                                {b->lengths, b->histories * int64_t(4)},
+                                {b->masks, b->mask_count > 0 ? ((b->mask_count - 1) * b->mask_stride + words) * 4 : 0}};
+        const auto overlap = [](const Range& x, const Range& y) { return bytes_overlap(x.at, x.bytes, y.at, y.bytes); };
+        bool clash = overlap(best, logits) || overlap(best, output) ||
+                     (overlap(logits, output) && !(b->logits == b->output && b->logits_stride == b->output_stride));
+        for (const Range& o : others) clash |= overlap(o, output) || overlap(o, best);
+        if (clash) fail(SATORI_HIP_E_ARGUMENT, "Partial overlap.");
+        const hipStream_t st = op_stream(c, stream);
+        for (int first = 0; first < b->count; first += kLogitRows) {
+            const LogitArgs args{reinterpret_cast<const LogitRow*>(b->rows), first, std::min(kLogitRows, b->count - first),
+                                 r->vocabulary, b->logits, b->output, b->best, b->logits_stride, b->output_stride, b->history,
+                                 b->lengths, b->history_stride, b->histories, b->mask_count, b->masks, b->mask_stride, r->biases,
+                                 static_cast<LogitBest*>(r->found.ptr)};
+            check_hip(launch_logits(args, st), "logits launch");
+        }
+        note_handle(c, r, st);
     });
 }
 
