@@ -2,6 +2,7 @@
 // and the best token.
 #include "logits.hpp"
 
+#include <algorithm>
 #include <cmath>
 
 #include "device_common.hpp"
@@ -10,9 +11,13 @@ namespace satori {
 namespace {
 
 constexpr int kThreads = 256;
+constexpr int kPlaces = 1024;  // workgroups at once: four a CU, by their LDS and registers
+constexpr int kListed = 2048;  // (where a row has had more of a slice's tokens, each thread looks at its own)
 constexpr int kPacks = kLogitSlice / kThreads / 4;  // of four logits a thread
 
 typedef float f32x4_a4 __attribute__((ext_vector_type(4), aligned(4)));
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+typedef int i32x4_a4 __attribute__((ext_vector_type(4), aligned(4)));
 
 // A number that orders keys as their values do, values of zero alike.
 __device__ __forceinline__ uint32_t ordered(float v) {
@@ -22,134 +27,264 @@ __device__ __forceinline__ uint32_t ordered(float v) {
 
 __device__ __forceinline__ unsigned long long greater(unsigned long long a, unsigned long long b) { return a > b ? a : b; }
 
-// One slice of a row's tokens: how often the row has had each (its history and, where it is a draft, its branch) is counted
-// in LDS, the biases put beside, then all of it meets the logits, which set out first. A row's slices meet in one atomic
-// maximum each; the last to arrive, which sees them all (each waits for its maximum before it counts itself in), gives the
-// best token. Sums and quotients in FP32, each rounded, in the order of the definition.
-__global__ __launch_bounds__(kThreads) void logits_kernel(LogitArgs a) {
-    __shared__ int counts[kLogitSlice];
-    __shared__ float biases[kLogitSlice];
-    __shared__ unsigned long long top[kThreads / 64];
-    const int thread = threadIdx.x, slice = blockIdx.x, local = blockIdx.y, row = a.first + local;
-    const int begin = slice * kLogitSlice, end = min(a.vocabulary - begin, kLogitSlice);
-    const LogitRow r = a.rows[row];
-    const float* in = a.logits + row * a.logits_stride + begin;
-
+// What a thread has of one row's slice.
+struct Slice {
     f32x4 x[kPacks];
-#pragma unroll
-    for (int i = 0; i < kPacks; ++i) {
-        const int at = i * kThreads * 4 + thread * 4;
-        x[i] = f32x4{0, 0, 0, 0};
-        if (at + 4 <= end) {
-            x[i] = *(const SATORI_GLOBAL f32x4_a4*)(in + at);
-        } else {
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-                if (at + j < end) x[i][j] = load_f32(in + at + j);
-        }
-    }
+    uint32_t allowed[kPacks];  // bit j of 4: of lane j of the pack
+};
 
-    const bool penalises = r.repetition != 1.0f || r.presence != 0.0f || r.frequency != 0.0f;
-    const bool biased = r.biases >= 0 && r.biases < a.biases.count;
-    if (penalises)
-        for (int i = thread; i < kLogitSlice; i += kThreads) counts[i] = 0;
-    if (biased)
-        for (int i = thread; i < kLogitSlice; i += kThreads) biases[i] = 0;
-    __syncthreads();
-    const auto count = [&](int token) {
-        const uint32_t at = static_cast<uint32_t>(token) - static_cast<uint32_t>(begin);
-        if (at < static_cast<uint32_t>(end)) atomicAdd(counts + at, 1);
+// One slice of the tokens of up to kLogitGroup rows, one row after another. How often a row has had each token (its history
+// and, where it is a draft, its branch) is counted in LDS, with a list of the tokens that it has had. Rows of one history follow
+// one another (a tree's, a request's), so the counts stay and only the branches change. What is listed, and what has a bias, is
+// changed in LDS, one token a thread (each thread at its own tokens would divide for whole waves, 16 times a row); a row's
+// logits and mask set out while the row before is at work. A row's slices meet in one atomic maximum each; the last to
+// arrive, which sees them all (each waits for its maximum before it counts itself in), gives the best token. Sums and
+// quotients in FP32, each rounded, in the order of the definition.
+__global__ __launch_bounds__(kThreads, 4) void logits_kernel(LogitArgs a) {
+    __shared__ __attribute__((aligned(16))) int counts[kLogitSlice];
+    __shared__ __attribute__((aligned(16))) float values[kLogitSlice];
+    __shared__ uint16_t listed[kListed];
+    __shared__ int list_length;
+    __shared__ unsigned long long branches[kLogitGroup];
+    __shared__ unsigned long long top[kLogitGroup][kThreads / 64];
+    __shared__ LogitRow params[kLogitGroup];
+    const int thread = threadIdx.x, slice = blockIdx.x, local = blockIdx.y * a.group, first = a.first + local;
+    const int rows = min(a.group, a.first + a.count - first);
+    const int begin = slice * kLogitSlice, end = min(a.vocabulary - begin, kLogitSlice);
+
+    const auto load = [&](int i, Slice& to) {
+        const float* in = a.logits + (first + i) * a.logits_stride + begin;
+#pragma unroll
+        for (int k = 0; k < kPacks; ++k) {
+            const int at = k * kThreads * 4 + thread * 4;
+            to.x[k] = f32x4{0, 0, 0, 0};
+            if (at + 4 <= end) {
+                to.x[k] = *(const SATORI_GLOBAL f32x4_a4*)(in + at);
+            } else {
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    if (at + j < end) to.x[k][j] = load_f32(in + at + j);
+            }
+        }
     };
-    if (penalises) {
-        if (r.history >= 0 && r.history < a.histories) {
-            const int* history = a.history + r.history * a.history_stride;
-            const int length = static_cast<int>(min(static_cast<int64_t>(max(a.lengths[r.history], 0)), a.history_stride));
-            for (int i = thread; i < length; i += kThreads) count(history[i]);
+    const auto load_mask = [&](int i, Slice& to) {
+        const int mask = __builtin_amdgcn_readfirstlane(params[i].mask);
+        const bool is = mask >= 0 && mask < a.mask_count;
+        const uint32_t* words = a.masks + (is ? mask : 0) * a.mask_stride + begin / 32;
+#pragma unroll
+        for (int k = 0; k < kPacks; ++k) {
+            const int at = k * kThreads * 4 + thread * 4;
+            to.allowed[k] = is && at < end ? words[at / 32] >> at % 32 : ~0u;
         }
-        if (thread < 64) {
-            // Up the branch: the rows of a window of 64 lie in the lanes.
-            int at = row, base = row + 1, parent = -1, token = -1;
-            while (at >= 0) {
-                if (at < base) {
-                    base = max(0, at - 63);
-                    const int mine = min(base + thread, row);
-                    parent = a.rows[mine].parent;
-                    token = a.rows[mine].token;
-                }
-                const int of = __builtin_amdgcn_readfirstlane(at - base);
-                if (thread == 0) count(__builtin_amdgcn_readlane(token, of));
-                const int up = __builtin_amdgcn_readlane(parent, of);
-                at = up < at ? up : -1;
-            }
-        }
-    }
-    if (biased) {
-        const int* set = a.biases.sets + static_cast<int64_t>(r.biases) * a.biases.words;
-        const int* tokens = set + gridDim.x + 1;
-        const float* values = reinterpret_cast<const float*>(tokens + a.biases.entries);
-        for (int i = set[slice] + thread; i < set[slice + 1]; i += kThreads) biases[tokens[i] - begin] = values[i];
-    }
+    };
+    Slice now, next;
+    load(0, now);
+    if (thread < rows * static_cast<int>(sizeof(LogitRow) / 4))
+        reinterpret_cast<int*>(params)[thread] = reinterpret_cast<const int*>(a.rows + first)[thread];
+    // The branches' rows: those of a window of 64 lie in the lanes of a wave, at first the last 64 up to the group's end.
+    const int lane = thread & 63, latest = max(0, first + rows - 64);
+    int base = latest, parent = -1, token = -1;
+    const auto look = [&](int from) {
+        base = from;
+        const int mine = min(base + lane, first + rows - 1);
+        parent = a.rows[mine].parent;
+        token = a.rows[mine].token;
+    };
+    look(latest);
     __syncthreads();
+    load_mask(0, now);
+    // A bit for every row of that window that a row's branch has, or none where it goes back further.
+    for (int i = __builtin_amdgcn_readfirstlane(thread / 64); i < rows; i += kThreads / 64) {
+        unsigned long long has = 0;
+        for (int at = first + i; at >= 0;) {
+            if (at < base) {
+                has = 0;
+                break;
+            }
+            has |= 1ull << (at - base);
+            const int up = __builtin_amdgcn_readlane(parent, at - base);
+            at = up < at ? up : -1;
+        }
+        if (lane == 0) branches[i] = has;
+    }
 
-    const bool masked = r.mask >= 0 && r.mask < a.mask_count;
-    const uint32_t* mask = masked ? a.masks + r.mask * a.mask_stride + begin / 32 : nullptr;
-    unsigned long long key = 0;
+    const auto count = [&](int of, int by) {
+        const uint32_t at = static_cast<uint32_t>(of) - static_cast<uint32_t>(begin);
+        if (at >= static_cast<uint32_t>(end) || atomicAdd(counts + at, by) != 0 || by < 0) return;
+        const int place = atomicAdd(&list_length, 1);
+        if (place < kListed) listed[place] = static_cast<uint16_t>(at);
+    };
+    // Counts a row's branch (the first wave): the rows that it has, at once, or window after window.
+    const auto count_branch = [&](int row, int by) {
+        const unsigned long long has = branches[row - first];
+        if (has) {
+            if (has >> lane & 1) count(token, by);
+            return;
+        }
+        for (int at = row; at >= 0;) {
+            if (at < base || at > base + 63) look(at > base ? latest : max(0, at - 63));
+            const int of = __builtin_amdgcn_readfirstlane(at - base);
+            if (lane == of) count(token, by);
+            const int up = __builtin_amdgcn_readlane(parent, of);
+            at = up < at ? up : -1;
+        }
+        look(latest);
+    };
+    // A bias set's entries of the slice: a thread's first one stays with it.
+    int put = -1, bias_end = 0, bias_from = 0, bias_at = 0;
+    float bias_by = 0;
+    const auto take_biases = [&](int set) {
+        const int* starts = a.biases.sets + static_cast<int64_t>(set) * a.biases.words;
+        put = set;
+        bias_from = starts[slice] + thread;
+        bias_end = starts[slice + 1];
+        if (bias_from < bias_end) {
+            bias_at = starts[gridDim.x + 1 + bias_from] - begin;
+            bias_by = reinterpret_cast<const float*>(starts)[gridDim.x + 1 + a.biases.entries + bias_from];
+        }
+    };
+    int counted = -2, of_history = 0, walked = -1;  // the history that LDS holds, its part of the list, and the branch
+    const auto pass = [&](int i, const Slice& now, Slice& next) {
+        const int row = first + i;
+        if (i + 1 < rows) {
+            load(i + 1, next);
+            load_mask(i + 1, next);
+        }
+        const LogitRow r = params[i];
+        const bool penalises = r.repetition != 1.0f || r.presence != 0.0f || r.frequency != 0.0f;
+        const int set = r.biases >= 0 && r.biases < a.biases.count ? r.biases : -1;
+        const int history = r.history >= 0 && r.history < a.histories ? r.history : -1;
+        if (penalises && history != counted) {
+            for (int k = thread; k < kLogitSlice / 4; k += kThreads) reinterpret_cast<u32x4*>(counts)[k] = u32x4{0, 0, 0, 0};
+            if (thread == 0) list_length = 0;
+            __syncthreads();
+            counted = history;
+            walked = -1;
+            if (history >= 0) {
+                const int* tokens = a.history + history * a.history_stride;
+                const int length = static_cast<int>(min(static_cast<int64_t>(max(a.lengths[history], 0)), a.history_stride));
+                // Sixteen tokens a thread and turn, all on their way at once.
+                for (int k0 = 0; k0 < length; k0 += kThreads * 16) {
+                    i32x4_a4 had[4];
 #pragma unroll
-    for (int i = 0; i < kPacks; ++i) {
-        const int at = i * kThreads * 4 + thread * 4;
-        if (at >= end) break;
-        const uint32_t allowed = masked ? mask[at / 32] >> at % 32 : ~0u;
+                    for (int k = 0; k < 4; ++k) {
+                        const int at = k0 + (k * kThreads + thread) * 4;
+                        if (at + 4 <= length) {
+                            had[k] = *(const SATORI_GLOBAL i32x4_a4*)(tokens + at);
+                        } else {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            float v = x[i][j];
-            if (penalises) {
-                const int n = counts[at + j];
-                if (n > 0) {
-                    v = v > 0 ? v / r.repetition : v * r.repetition;
-                    v = v - (r.presence + r.frequency * static_cast<float>(n));
+                            for (int j = 0; j < 4; ++j) had[k][j] = at + j < length ? tokens[at + j] : -1;
+                        }
+                    }
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) count(had[k][j], 1);
                 }
             }
-            if (biased) {
-                const float b = biases[at + j];
-                v = b != 0 ? v + b : v;
+            __syncthreads();
+            of_history = list_length;  // (the first wave's own is what counts)
+        }
+        if (penalises && thread < 64) {
+            if (walked >= 0) {
+                count_branch(walked, -1);
+                if (thread == 0) list_length = of_history;
             }
-            v = allowed >> j & 1 ? v : -INFINITY;
-            x[i][j] = v;
-            if (at + j < end && v > -INFINITY)
-                key = greater(key, static_cast<unsigned long long>(ordered(v)) << 32 | ~static_cast<uint32_t>(begin + at + j));
+            count_branch(row, 1);
         }
-        if (!a.output) continue;
-        float* out = a.output + row * a.output_stride + begin + at;
-        if (at + 4 <= end) {
-            *(SATORI_GLOBAL f32x4_a4*)(out) = x[i];
-        } else {
+        if (penalises) walked = row;
+        if (set >= 0 && set != put) take_biases(set);
+        Slice mine = now;
+        if (penalises || set >= 0) {
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-                if (at + j < end) store_f32(out + j, x[i][j]);
+            for (int k = 0; k < kPacks; ++k) *reinterpret_cast<f32x4*>(values + k * kThreads * 4 + thread * 4) = now.x[k];
+            __syncthreads();
+            if (penalises) {
+                const auto penalise = [&](int at) {
+                    const float x = values[at];
+                    const float v = x > 0 ? x / r.repetition : x * r.repetition;
+                    values[at] = v - (r.presence + r.frequency * static_cast<float>(counts[at]));
+                };
+                const int length = list_length;
+                if (length <= kListed)
+                    for (int k = thread; k < length; k += kThreads) penalise(listed[k]);
+                else
+                    for (int at = thread; at < end; at += kThreads)
+                        if (counts[at] > 0) penalise(at);
+            }
+            if (set >= 0) {
+                if (penalises) __syncthreads();
+                const auto add = [&](int at, float by) {
+                    if (by != 0) values[at] = values[at] + by;
+                };
+                if (bias_from < bias_end) add(bias_at, bias_by);
+                const int* tokens = a.biases.sets + static_cast<int64_t>(set) * a.biases.words + gridDim.x + 1;
+                for (int k = bias_from + kThreads; k < bias_end; k += kThreads)
+                    add(tokens[k] - begin, reinterpret_cast<const float*>(tokens)[a.biases.entries + k]);
+            }
+            __syncthreads();
+#pragma unroll
+            for (int k = 0; k < kPacks; ++k) mine.x[k] = *reinterpret_cast<const f32x4*>(values + k * kThreads * 4 + thread * 4);
         }
+
+        float best = -INFINITY;
+        int best_at = -1;  // a thread's tokens go up, so an equal one is a higher one
+#pragma unroll
+        for (int k = 0; k < kPacks; ++k) {
+            const int at = k * kThreads * 4 + thread * 4;
+            if (at >= end) break;
+            f32x4 x = mine.x[k];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                x[j] = now.allowed[k] >> j & 1 ? x[j] : -INFINITY;
+                if (x[j] > best && at + j < end) {
+                    best = x[j];
+                    best_at = at + j;
+                }
+            }
+            if (!a.output) continue;
+            float* out = a.output + row * a.output_stride + begin + at;
+            if (at + 4 <= end) {
+                *(SATORI_GLOBAL f32x4_a4*)(out) = x;
+            } else {
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    if (at + j < end) store_f32(out + j, x[j]);
+            }
+        }
+        if (a.best) {
+            const uint32_t value = best_at < 0 ? 0 : ordered(best), most = wave_extreme_u32<true>(value);
+            const uint32_t place = wave_extreme_u32<false>(value == most ? static_cast<uint32_t>(begin + best_at) : ~0u);
+            if (lane == 0) top[i][thread / 64] = most ? static_cast<unsigned long long>(most) << 32 | ~place : 0;
+        }
+    };
+    for (int i = 0; i < rows; i += 2) {
+        pass(i, now, next);
+        if (i + 1 < rows) pass(i + 1, next, now);
     }
-    if (!a.best) return;
-#pragma unroll
-    for (int k = 32; k > 0; k >>= 1) key = greater(key, __shfl_xor(key, k, 64));
-    if (thread % 64 == 0) top[thread / 64] = key;
     __syncthreads();
-    if (thread != 0) return;
+    if (!a.best || thread >= rows) return;
+    unsigned long long key = top[thread][0];
 #pragma unroll
-    for (int i = 1; i < kThreads / 64; ++i) key = greater(key, top[i]);
-    LogitBest* found = a.found + local;
+    for (int k = 1; k < kThreads / 64; ++k) key = greater(key, top[thread][k]);
+    LogitBest* found = a.found + local + thread;
     __hip_atomic_fetch_max(&found->key, key, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     __asm__ volatile("s_waitcnt vmcnt(0)" ::: "memory");
     const unsigned long long seen = __hip_atomic_fetch_add(&found->arrived, 1ull, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     if ((seen + 1) % gridDim.x != 0) return;
     key = __hip_atomic_exchange(&found->key, 0ull, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    a.best[row] = key ? static_cast<int>(~static_cast<uint32_t>(key)) : -1;
+    a.best[first + thread] = key ? static_cast<int>(~static_cast<uint32_t>(key)) : -1;
 }
 
 }  // namespace
 
-hipError_t launch_logits(const LogitArgs& args, hipStream_t stream) {
+hipError_t launch_logits(LogitArgs args, hipStream_t stream) {
     if (args.count <= 0) return hipSuccess;
-    logits_kernel<<<dim3(logit_slices(args.vocabulary), args.count), kThreads, 0, stream>>>(args);
+    // Rows of a workgroup: four rounds of the workgroups that the card holds (four a CU), as the last one is not full.
+    const int64_t units = static_cast<int64_t>(logit_slices(args.vocabulary)) * args.count;
+    args.group = static_cast<int>(std::min<int64_t>(kLogitGroup, std::max<int64_t>(1, units / (4 * kPlaces))));
+    const dim3 grid(logit_slices(args.vocabulary), (args.count + args.group - 1) / args.group);
+    logits_kernel<<<grid, kThreads, 0, stream>>>(args);
     return hipGetLastError();
 }
 

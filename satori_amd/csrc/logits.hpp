@@ -9,6 +9,7 @@
 namespace satori {
 
 constexpr int kLogitSlice = 4096;  // tokens of a workgroup
+constexpr int kLogitGroup = 16;    // rows of a workgroup, at most
 constexpr int kLogitRows = 1024;   // rows of a launch, for each of which the workspace has a LogitBest
 inline int logit_slices(int vocabulary) { return (vocabulary + kLogitSlice - 1) / kLogitSlice; }
 
@@ -49,7 +50,8 @@ struct LogitArgs {
     int64_t mask_stride;   // words
     LogitBiases biases;
     LogitBest* found;      // of the launch's rows
+    int group;             // rows of a workgroup (launch_logits says)
 };
-hipError_t launch_logits(const LogitArgs& args, hipStream_t stream);
+hipError_t launch_logits(LogitArgs args, hipStream_t stream);
 
 }  // namespace satori

@@ -3092,7 +3092,7 @@ int satori_hip_logit_rules_apply(satori_hip_logit_rules* r, const satori_hip_log
             const LogitArgs args{reinterpret_cast<const LogitRow*>(b->rows), first, std::min(kLogitRows, b->count - first),
                                  r->vocabulary, b->logits, b->output, b->best, b->logits_stride, b->output_stride, b->history,
                                  b->lengths, b->history_stride, b->histories, b->mask_count, b->masks, b->mask_stride, r->biases,
-                                 static_cast<LogitBest*>(r->found.ptr)};
+                                 static_cast<LogitBest*>(r->found.ptr), 1};
             check_hip(launch_logits(args, st), "logits launch");
         }
         note_handle(c, r, st);
