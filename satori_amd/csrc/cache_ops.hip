@@ -1127,6 +1127,46 @@ __global__ __launch_bounds__(kThreads) void cache_join_kernel(AttentionArgs a) {
     }
 }
 
+// The same where rows have few parts: four lanes of a (row, head) a thread, all parts at once, added in the same order (the
+// groups above would have one part each, and those without one add zeros).
+constexpr int kFewParts = 8;
+__global__ __launch_bounds__(kThreads) void cache_join_few_kernel(AttentionArgs a) {
+    const CacheShape& s = a.s;
+    const uint32_t quads = s.width / 4, thread = blockIdx.x * kThreads + threadIdx.x, u = thread / quads;
+    const int d = thread % quads * 4, head = u % s.heads;
+    if (u / s.heads >= static_cast<uint32_t>(a.rows)) return;
+    const PlanRow row = reinterpret_cast<const PlanRow*>(a.image + a.at.rows_at)[u / s.heads];
+    if (row.slots <= 1) return;
+    const int64_t first = static_cast<int64_t>(row.slot) * s.heads + head;
+    const float* sums = a.partials.sums(s.width, first);
+    const float* values = a.partials.values(s.width, first) + d;
+    f32x2 part[kFewParts];
+    f32x4 v[kFewParts];
+#pragma unroll
+    for (int i = 0; i < kFewParts; ++i) {
+        const int64_t of = min(i, row.slots - 1);
+        part[i] = *(const SATORI_GLOBAL f32x2*)(sums + of * s.heads * 2);
+        v[i] = *(const SATORI_GLOBAL f32x4*)(values + of * s.heads * s.width);
+    }
+    float top = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < kFewParts; ++i) top = fmaxf(top, part[i][0]);
+    const float from = top == -INFINITY ? 0.0f : top;
+    f32x4 o{0, 0, 0, 0};
+    float total = 0;
+#pragma unroll
+    for (int i = 0; i < kFewParts; ++i)
+        if (i < row.slots) {
+            const float weight = __builtin_amdgcn_exp2f(part[i][0] - from);
+            total += weight * part[i][1];
+            o = o + v[i] * weight;
+        }
+    o = o + f32x4{0, 0, 0, 0};
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+        if (d + j < s.head_dim) store_f32(a.output + static_cast<int64_t>(u) * s.head_dim + d + j, o[j] / total);
+}
+
 constexpr int kMostGroups = 1024;  // workgroups of a launch whose work is only known when it is replayed
 
 template <typename T, int W>
@@ -1262,6 +1302,11 @@ hipError_t launch_cache_attention(const CacheShape& shape, const int* image, con
     });
     if (e != hipSuccess || (now.joined == 0 && !all)) return e;
     const int64_t joins = static_cast<int64_t>(now.rows) * shape.heads;
+    const int quads = shape.width / 4;
+    if (!all && now.most_slots <= std::min(kFewParts, kThreads / quads) && joins * quads < INT32_MAX) {
+        cache_join_few_kernel<<<static_cast<unsigned>((joins * quads + kThreads - 1) / kThreads), kThreads, 0, stream>>>(a);
+        return hipGetLastError();
+    }
     cache_join_kernel<<<all ? kMostGroups : static_cast<int>(std::min<int64_t>(joins, 65536)), kThreads, 0, stream>>>(a);
     return hipGetLastError();
 }

@@ -239,6 +239,7 @@ constexpr int kLeastShared = 128;
 // 17.5 not, 512 (100 MB) 24.4 and 21.9, 1024 (201 MB) 27.5 and 32.0. Heads of 192 and 256 lanes fit one workgroup a CU, but half
 // the number serves them no better: F16, 256 lanes, 32 + 8 heads over 256 shared positions, 30 sequences take 31.1 us with 512
 // here and 38.8 with 256, 32 take 30.8 and 23.7, 40 take 32.5 with either; FP32, 30 sequences, 45.4 and 73.7.
+constexpr int64_t kWideTokenTime = 62, kNarrowTokenTime = 26;
 constexpr int64_t kPlaces = 512, kRoundBytes = 128 << 20;
 
 }  // namespace
@@ -327,6 +328,7 @@ PlanImage plan_batch(const PageTables& tables, const int* sequences, const int* 
     if (image.header.tree_stride > 0)
         for (int i = 0; i < count; ++i) context_of.insert(context_of.end(), new_tokens[i], contexts[i]);
 
+    const bool trees = image.header.tree_stride > 0 && !division.plain;
     const auto blocks_of = [](int64_t pairs) { return (pairs + kNarrowPairs - 1) / kNarrowPairs; };
     int64_t own = 0;  // items of the sequences by themselves, at least
     for (int i = 0; i < count; ++i) own += blocks_of(static_cast<int64_t>(new_tokens[i]) * shape.group) * shape.kv_heads;
@@ -338,6 +340,15 @@ PlanImage plan_batch(const PageTables& tables, const int* sequences, const int* 
             apart += blocks_of(static_cast<int64_t>(new_tokens[m]) * shape.group);
         }
         const int64_t together = blocks_of(pairs);
+        if (trees) {
+            const auto cost = [&](int64_t of) {
+                return of > shape.wide_pairs / 4 ? (of + shape.wide_pairs - 1) / shape.wide_pairs * kWideTokenTime
+                                                 : blocks_of(of) * kNarrowTokenTime;
+            };
+            int64_t saved = -cost(pairs);
+            for (int m : members) saved += cost(static_cast<int64_t>(new_tokens[m]) * shape.group);
+            if (saved * tokens * shape.kv_heads / shape.places > 2000 + pairs * shape.kv_heads / 4) return true;
+        }
         const auto rounds = [](int64_t items) { return (items + kPlaces - 1) / kPlaces; };
         return rounds(own + together * shape.kv_heads) == rounds(own) ||
                (apart - together) * tokens * shape.kv_heads >= kRoundBytes / shape.token_bytes;
@@ -414,7 +425,7 @@ PlanImage plan_batch(const PageTables& tables, const int* sequences, const int* 
     for (size_t i = 0; i < nodes.size(); ++i) {
         Node& n = nodes[i];
         for (int m : n.members) pairs_of[i] += static_cast<int64_t>(new_tokens[m]) * shape.group;
-        n.wide = pairs_of[i] > shape.wide_pairs / 2;
+        n.wide = pairs_of[i] > shape.wide_pairs / (trees ? 4 : 2);
         if (n.wide) again += blocks_of(pairs_of[i]) * shape.kv_heads * (n.end - n.begin);
     }
     const auto pairs_a_block = [&](const Node& n) { return n.wide ? shape.wide_pairs : kNarrowPairs; };
@@ -434,12 +445,34 @@ PlanImage plan_batch(const PageTables& tables, const int* sequences, const int* 
         const int64_t c = (tokens / division.workgroups + step - 1) / step * step;
         return static_cast<int>(std::min<int64_t>(std::max<int64_t>(c, step), kMostTokens));
     };
-    const int narrow_chunk = chunk_for(narrow_tokens), wide_chunk = chunk_for(wide_tokens);
+    int narrow_chunk = chunk_for(narrow_tokens), wide_chunk = chunk_for(wide_tokens);
+    if (trees) {
+        const int64_t step = kTile * kWaves, places = static_cast<int64_t>(shape.places) * division.workgroups / 256;
+        const auto items_of = [&](int64_t chunk) {
+            int64_t items = 0;
+            for (size_t i = 0; i < nodes.size(); ++i) {
+                const Node& n = nodes[i];
+                const int64_t blocks = (pairs_of[i] + pairs_a_block(n) - 1) / pairs_a_block(n);
+                items += (n.end - n.begin + chunk - 1) / chunk * blocks * shape.kv_heads;
+            }
+            return items;
+        };
+        int64_t low = 1, high = kMostTokens / step;  // the shortest chunk, in steps, whose items have places
+        while (low < high) {
+            const int64_t middle = (low + high) / 2;
+            items_of(middle * step) <= places ? high = middle : low = middle + 1;
+        }
+        narrow_chunk = wide_chunk = static_cast<int>(low * step);
+    }
 
     std::vector<int>& page_list = image.pages;
     std::vector<int> row_list;
     for (Node& n : nodes) {
         n.chunk = n.wide ? wide_chunk : narrow_chunk;
+        if (trees) {  // as even as whole steps make them
+            const int64_t step = kTile * kWaves, length = n.end - n.begin, chunks = (length - 1) / n.chunk + 1;
+            n.chunk = static_cast<int>(((length + chunks - 1) / chunks + step - 1) / step * step);
+        }
         n.chunks = (n.end - n.begin - 1) / n.chunk + 1;  // (a sum with the chunk could pass 32 bits)
         n.slot = n.ancestors < 0 ? 0 : nodes[n.ancestors].slot + nodes[n.ancestors].chunks;
         n.pages = static_cast<int>(page_list.size());
@@ -522,6 +555,7 @@ PlanImage plan_batch(const PageTables& tables, const int* sequences, const int* 
     image.list.reserve(row_list.size());
     for (int r : row_list) image.list.push_back(rows[r]);
     PlanHeader& h = image.header;
+    for (const PlanRow& r : rows) h.most_slots = std::max(h.most_slots, r.slots);
     h.rows = static_cast<int>(rows.size());
     h.narrow = static_cast<int>(narrow.size());
     h.wide = static_cast<int>(wide.size());

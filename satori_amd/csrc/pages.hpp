@@ -108,7 +108,7 @@ struct PlanRun {
 struct PlanHeader {
     int rows, narrow, wide, runs;
     int joined, slots, longest_run, partials;
-    int tree_stride, pad[3];
+    int tree_stride, most_slots, pad[2];  // most_slots: of a row
 };
 
 // Where a batch has trees, tree_stride numbers for every row: the position that it stands for (its context and its depth in
@@ -136,6 +136,7 @@ struct PlanShape {
     int kv_heads, group;  // group: query heads of a key/value head
     int wide_pairs;       // pairs of a wide workgroup; a narrow one takes 16
     int token_bytes;      // a position's key and value of one head
+    int places = 512;     // workgroups that the card holds at once
 };
 
 // A plan's arrays, and what its launches need to know.
