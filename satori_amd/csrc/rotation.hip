@@ -41,98 +41,136 @@ __device__ __forceinline__ void store_pack(T* p, const float (&v)[N]) {
     *(SATORI_GLOBAL pack*)(p) = x;
 }
 
-// A thread turns N pairs of one row in kHeads heads, whose angles it reads once: both lanes' 16 bytes a head and access.
-// Behind the last whole N pairs of a head single ones, and packs for the lanes behind the rotated ones, which are copied
-// unless the output is the input.
-template <typename T, bool INTERLEAVED, int HEADS>
-__global__ __launch_bounds__(kThreads) void rotate_kernel(RotationShape s, RotateArgs a, int units, int packs, int groups) {
+// A workgroup turns some pairs (kThreads at most, all rows together) of some rows: its threads read, or compute, the sine and
+// cosine of one pair of one row each and leave them in LDS, while what they turn first is on its way: N pairs of kHeads heads a
+// thread and turn, 16 bytes a head and access. Behind the last whole N pairs single ones; the lanes behind the rotated ones are
+// copied, unless the output is the input.
+constexpr int kHeads = 4;
+
+// Where a pair's angle lies: a pack's 128 bytes start at other banks than the next one's.
+__device__ __forceinline__ int angle_at(int i) { return i + (i >> 3); }
+
+template <typename T, bool INTERLEAVED>
+__global__ __launch_bounds__(kThreads) void rotate_kernel(RotationShape s, RotateArgs a, int group_rows, int group_pairs) {
     constexpr int N = 16 / sizeof(T);
-    const uint32_t i = blockIdx.x * kThreads + threadIdx.x;
-    const uint32_t unit = i % units, rest = i / units, group = rest % groups, row = rest / groups;
-    if (row >= static_cast<uint32_t>(a.rows)) return;
-    const int first = group * HEADS, heads = min(HEADS, a.heads - first), D = a.head_dim;
-    const T* in = static_cast<const T*>(a.input) + row * a.input_stride + static_cast<int64_t>(first) * D;
-    T* out = static_cast<T*>(a.output) + row * a.output_stride + static_cast<int64_t>(first) * D;
-    if (static_cast<int>(unit) >= packs) {
-        const int lane = 2 * s.pairs + (unit - packs) * N;
-        for (int h = 0; h < heads; ++h) {
-            if (lane + N <= D) {
-                float v[N];
-                load_pack<T, N>(in + h * D + lane, v);
-                store_pack<T, N>(out + h * D + lane, v);
-            } else {
-                for (int j = lane; j < D; ++j) out[h * D + j] = in[h * D + j];
+    typedef double f64x2 __attribute__((ext_vector_type(2)));
+    __shared__ f64x2 angles[kThreads + kThreads / 8];
+    const int thread = threadIdx.x, row0 = blockIdx.x * group_rows, k0 = blockIdx.y * group_pairs, D = a.head_dim;
+    const int rows = min(group_rows, a.rows - row0), pairs = min(group_pairs, s.pairs - k0);
+    const int packs = (pairs + N - 1) / N, groups = (a.heads + kHeads - 1) / kHeads;
+    const bool copies = a.output != a.input && blockIdx.y + 1 == gridDim.y;
+    const int units = packs + (copies ? (D - 2 * s.pairs + N - 1) / N : 0), row_units = units * groups;
+
+    struct Unit {
+        int row, k, heads;  // k: the first pair of the workgroup's; past its pairs: a pack to copy
+        const T* in;
+        T* out;
+    };
+    const auto locate = [&](int u) {
+        Unit r;
+        r.row = u / row_units;
+        const int rest = u % row_units, first = rest / units * kHeads;
+        r.k = rest % units * N;
+        r.heads = min(kHeads, a.heads - first);
+        r.in = static_cast<const T*>(a.input) + (row0 + r.row) * a.input_stride + static_cast<int64_t>(first) * D;
+        r.out = static_cast<T*>(a.output) + (row0 + r.row) * a.output_stride + static_cast<int64_t>(first) * D;
+        return r;
+    };
+    float x[kHeads][N], y[kHeads][N];
+    const auto load = [&](const Unit& r) {
+        if (r.k + N > pairs) return;
+        const int at = INTERLEAVED ? 2 * (k0 + r.k) : k0 + r.k, beside = INTERLEAVED ? N : s.pairs;
+#pragma unroll
+        for (int h = 0; h < kHeads; ++h)
+            if (h < r.heads) {
+                load_pack<T, N>(r.in + h * D + at, x[h]);
+                load_pack<T, N>(r.in + h * D + at + beside, y[h]);
             }
-        }
-        return;
-    }
-    const int k = unit * N, position = a.positions[row], left = min(N, s.pairs - k);
-    const bool listed = position >= 0 && position < s.positions;
-    const double* angles = s.table + static_cast<int64_t>(listed ? position : 0) * 2 * s.pairs + k;
-    const auto angle = [&](int j, double& sn, double& cs) {
-        if (listed) {
-            sn = angles[j];
-            cs = angles[s.pairs + j];
+    };
+    const auto turn = [&](const Unit& r) {
+        if (r.k >= packs * N) {
+            const int lane = 2 * s.pairs + r.k - packs * N;
+            for (int h = 0; h < r.heads; ++h) {
+                if (lane + N <= D) {
+                    float v[N];
+                    load_pack<T, N>(r.in + h * D + lane, v);
+                    store_pack<T, N>(r.out + h * D + lane, v);
+                } else {
+                    for (int j = lane; j < D; ++j) r.out[h * D + j] = r.in[h * D + j];
+                }
+            }
+        } else if (r.k + N > pairs) {
+            for (int k = r.k; k < pairs; ++k) {
+                const f64x2 angle = angles[angle_at(r.row * pairs + k)];
+                const int at = INTERLEAVED ? 2 * (k0 + k) : k0 + k, beside = INTERLEAVED ? 1 : s.pairs;
+                for (int h = 0; h < r.heads; ++h) {
+                    float u, v;
+                    rope_apply(static_cast<float>(r.in[h * D + at]), static_cast<float>(r.in[h * D + at + beside]), angle[0],
+                               angle[1], u, v);
+                    r.out[h * D + at] = static_cast<T>(u);
+                    r.out[h * D + at + beside] = static_cast<T>(v);
+                }
+            }
         } else {
-            rotation_angle(k + j, position, s.frequencies, s.magnitude, sn, cs);
+#pragma unroll
+            for (int j = 0; j < N; ++j) {
+                const f64x2 angle = angles[angle_at(r.row * pairs + r.k + j)];
+#pragma unroll
+                for (int h = 0; h < kHeads; ++h) rotate_pair<INTERLEAVED>(x[h], y[h], j, angle[0], angle[1]);
+            }
+            const int at = INTERLEAVED ? 2 * (k0 + r.k) : k0 + r.k, beside = INTERLEAVED ? N : s.pairs;
+#pragma unroll
+            for (int h = 0; h < kHeads; ++h)
+                if (h < r.heads) {
+                    store_pack<T, N>(r.out + h * D + at, x[h]);
+                    store_pack<T, N>(r.out + h * D + at + beside, y[h]);
+                }
         }
     };
-    const int at = INTERLEAVED ? 2 * k : k, beside = INTERLEAVED ? N : s.pairs;
-    if (left < N) {
-        for (int j = 0; j < left; ++j) {
+
+    const int all = rows * row_units;
+    Unit now{};
+    if (thread < all) {
+        now = locate(thread);
+        load(now);
+    }
+    if (thread < rows * pairs) {
+        const int position = a.positions[row0 + thread / pairs], k = k0 + thread % pairs;
+        f64x2 angle;
+        if (position >= 0 && position < s.positions) {
+            const double* row = s.table + static_cast<int64_t>(position) * 2 * s.pairs;
+            angle[0] = row[k];
+            angle[1] = row[s.pairs + k];
+        } else {
             double sn, cs;
-            angle(j, sn, cs);
-            const int x = INTERLEAVED ? at + 2 * j : at + j, y = INTERLEAVED ? x + 1 : x + s.pairs;
-            for (int h = 0; h < heads; ++h) {
-                float u, v;
-                rope_apply(static_cast<float>(in[h * D + x]), static_cast<float>(in[h * D + y]), sn, cs, u, v);
-                out[h * D + x] = static_cast<T>(u);
-                out[h * D + y] = static_cast<T>(v);
-            }
+            rotation_angle(k, position, s.frequencies, s.magnitude, sn, cs);
+            angle[0] = sn;
+            angle[1] = cs;
         }
-        return;
+        angles[angle_at(thread)] = angle;
     }
-    float x[HEADS][N], y[HEADS][N];
-#pragma unroll
-    for (int h = 0; h < HEADS; ++h)
-        if (h < heads) {
-            load_pack<T, N>(in + h * D + at, x[h]);
-            load_pack<T, N>(in + h * D + at + beside, y[h]);
+    __syncthreads();
+    for (int u = thread; u < all; u += kThreads) {
+        if (u != thread) {
+            now = locate(u);
+            load(now);
         }
-#pragma unroll
-    for (int j = 0; j < N; ++j) {
-        double sn, cs;
-        angle(j, sn, cs);
-#pragma unroll
-        for (int h = 0; h < HEADS; ++h)
-            if (h < heads) rotate_pair<INTERLEAVED>(x[h], y[h], j, sn, cs);
+        turn(now);
     }
-#pragma unroll
-    for (int h = 0; h < HEADS; ++h)
-        if (h < heads) {
-            store_pack<T, N>(out + h * D + at, x[h]);
-            store_pack<T, N>(out + h * D + at + beside, y[h]);
-        }
 }
 
 template <typename T, bool INTERLEAVED>
 hipError_t rotate_of(const RotationShape& s, const RotateArgs& a, hipStream_t stream) {
-    constexpr int N = 16 / sizeof(T);
-    const int packs = (s.pairs + N - 1) / N, behind = a.output == a.input ? 0 : (a.head_dim - 2 * s.pairs + N - 1) / N;
-    const int units = packs + behind;
-    constexpr int kHeads = 4;
-    const int groups = (a.heads + kHeads - 1) / kHeads;
-    const int64_t row_units = static_cast<int64_t>(units) * groups;
-    // (a launch's threads are counted in 32 bits)
-    const int most = static_cast<int>(std::max<int64_t>(1, (int64_t(1) << 30) / row_units));
-    for (int row = 0; row < a.rows; row += most) {
+    const int pairs = std::min(s.pairs, kThreads), parts = (s.pairs + pairs - 1) / pairs;
+    const int rows = std::min(16, kThreads / pairs);
+    constexpr int kMost = 1 << 22;  // (a launch's threads are counted in 32 bits)
+    for (int64_t row = 0; row < a.rows; row += kMost) {
         RotateArgs part = a;
-        part.rows = std::min(most, a.rows - row);
+        part.rows = static_cast<int>(std::min<int64_t>(kMost, a.rows - row));
         part.input = static_cast<const T*>(a.input) + row * a.input_stride;
         part.output = static_cast<T*>(a.output) + row * a.output_stride;
         part.positions = a.positions + row;
-        const unsigned blocks = static_cast<unsigned>((part.rows * row_units + kThreads - 1) / kThreads);
-        rotate_kernel<T, INTERLEAVED, kHeads><<<blocks, kThreads, 0, stream>>>(s, part, units, packs, groups);
+        rotate_kernel<T, INTERLEAVED><<<dim3((part.rows + rows - 1) / rows, parts), kThreads, 0, stream>>>(s, part, rows, pairs);
         if (const hipError_t e = hipGetLastError(); e != hipSuccess) return e;
     }
     return hipSuccess;
