@@ -14,6 +14,7 @@ from array import array
 from collections import deque
 from collections.abc import Sequence
 from dataclasses import dataclass
+from itertools import chain
 
 import numpy as np
 
@@ -316,9 +317,7 @@ class CachePlan:
         ids, counts = _ints(sequences), _ints([len(p) for p in parents])
         if ids.size != counts.size:
             raise ArgumentException("Lengths differ.")
-        follows = array("i")
-        for p in parents:
-            follows.extend(_array(p))
+        follows = array("i", chain.from_iterable(parents))
         if self.cache._due:
             with self.cache.table.changes:
                 self.cache._settle(stream)
@@ -344,9 +343,7 @@ class CachePlan:
         """Moves the keys and values of rows[i], some of the plan's rows of its i-th sequence in ascending order, to follow that
         sequence's context, in all layers. Truncate the sequence to its context and len(rows[i]) then, and set the plan
         again before it is used."""
-        counts, kept = array("i", [len(r) for r in rows]), array("i")
-        for r in rows:
-            kept.extend(_array(r))
+        counts, kept = array("i", map(len, rows)), array("i", chain.from_iterable(rows))
         _check(_ffi.lib().satori_hip_cache_keep(self._handle, _address(kept) or None, _address(counts) or None, len(counts),
                                                 _pointer(stream)))
 

@@ -94,7 +94,7 @@ constexpr int kGroupTokens = 8;  // positions whose values a thread stores at on
 // 61 rows of 32 + 8 heads move 22.6 MB in 9.8 us (2.3 TB/s, where a large copy reaches 4.9); in a captured step, whose grid does
 // for any batch, 15.1. The rotation's angles come from the table in 64 bits, as the single-sequence operator's.
 enum class Turn { kPlain, kTree, kInterleaved };  // pairs half a head apart, rows no tree's; also a tree's; neighbouring lanes
-template <typename T, int N, Turn TURN>
+template <typename T, int N, Turn TURN, bool LISTED>  // LISTED: the table has every position
 __global__ __launch_bounds__(kThreads) void cache_append_kernel(CacheShape s, const int* __restrict__ image, int runs_at, int trees_at,
                                                                 AppendArgs a) {
     constexpr bool kInterleaved = TURN == Turn::kInterleaved;
@@ -120,12 +120,12 @@ __global__ __launch_bounds__(kThreads) void cache_append_kernel(CacheShape s, co
             float x[N], y[N];
             load_biased(is_query ? a.query : a.key, is_query ? a.query_bias : a.key_bias, at, lane, x);
             load_biased(is_query ? a.query : a.key, is_query ? a.query_bias : a.key_bias, at, lane + beside, y);
-            const bool listed = a.rope && position < a.rope_positions;
+            const bool listed = LISTED || (a.rope && position < a.rope_positions);
             const double* angles = a.rope + static_cast<int64_t>(position) * a.rotary + kk;
 #pragma unroll
             for (int j = 0; j < N; ++j) {
                 double sn, cs;
-                if (listed) {
+                if (LISTED || listed) {
                     sn = angles[j];
                     cs = angles[pairs + j];
                 } else if (a.frequencies) {
@@ -144,18 +144,20 @@ __global__ __launch_bounds__(kThreads) void cache_append_kernel(CacheShape s, co
                 store_as(out + beside, y);
             }
         }
-        const int behind = s.width - a.rotary;
+        // N lanes at once, as the rotated ones: a whole number of those, of heads and of what lies behind.
+        const int behind = (s.width - a.rotary) / N;
         if (behind > 0)
             for (int i = start; i < run.tokens * both * behind; i += stride) {
-                const int lane = a.rotary + i % behind, head = i / behind % both, t = i / behind / both;
+                const int lane = a.rotary + i % behind * N, head = i / behind % both, t = i / behind / both;
                 const int64_t row = run.row + t;
+                float v[N] = {};
                 if (head < s.heads) {
-                    if (lane < D)
-                        store_f32(a.query_out + row * s.heads * D + head * D + lane,
-                                  biased(a.query + row * s.heads * D, a.query_bias, head * D + lane));
+                    if (lane >= D) continue;
+                    load_biased(a.query, a.query_bias, row * s.heads * D, head * D + lane, v);
+                    store_as(a.query_out + row * s.heads * D + head * D + lane, v);
                 } else {
                     const int kh = head - s.heads;
-                    const float v[1] = {lane < D ? biased(a.key + row * s.kv_heads * D, a.key_bias, kh * D + lane) : 0.0f};
+                    if (lane < D) load_biased(a.key, a.key_bias, row * s.kv_heads * D, kh * D + lane, v);
                     store_as(keys + kh * head_size + static_cast<int64_t>(run.offset + t) * s.width + lane, v);
                 }
             }
@@ -1246,19 +1248,26 @@ hipError_t launch_cache_append(const CacheShape& s, const int* image, const Plan
     const auto launch = [&](auto kernel) {
         kernel<<<grid, kThreads, 0, stream>>>(s, image, layout.runs_at, layout.trees_at, args);
     };
-    const auto of_turn = [&](auto turn) {
+    const auto of_turn = [&](auto turn, auto listed) {
         constexpr Turn kTurn = decltype(turn)::value;
+        constexpr bool kListed = decltype(listed)::value;
         if (s.type == kF32)
-            packed ? launch(cache_append_kernel<float, 4, kTurn>) : launch(cache_append_kernel<float, 1, kTurn>);
+            packed ? launch(cache_append_kernel<float, 4, kTurn, kListed>) : launch(cache_append_kernel<float, 1, kTurn, kListed>);
         else
-            packed ? launch(cache_append_kernel<_Float16, 4, kTurn>) : launch(cache_append_kernel<_Float16, 1, kTurn>);
+            packed ? launch(cache_append_kernel<_Float16, 4, kTurn, kListed>)
+                   : launch(cache_append_kernel<_Float16, 1, kTurn, kListed>);
+    };
+    // Without the code that computes angles a wave takes half the registers. (A captured launch may meet any position.)
+    const bool listed = !all && args.rope && now.most_position < args.rope_positions;
+    const auto with = [&](auto turn) {
+        listed ? of_turn(turn, std::true_type{}) : of_turn(turn, std::false_type{});
     };
     if (args.interleaved)
-        of_turn(std::integral_constant<Turn, Turn::kInterleaved>{});
+        with(std::integral_constant<Turn, Turn::kInterleaved>{});
     else if (trees || args.frequencies)
-        of_turn(std::integral_constant<Turn, Turn::kTree>{});
+        with(std::integral_constant<Turn, Turn::kTree>{});
     else
-        of_turn(std::integral_constant<Turn, Turn::kPlain>{});
+        with(std::integral_constant<Turn, Turn::kPlain>{});
     return hipGetLastError();
 }
 

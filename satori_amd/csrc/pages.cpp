@@ -555,7 +555,10 @@ PlanImage plan_batch(const PageTables& tables, const int* sequences, const int* 
     image.list.reserve(row_list.size());
     for (int r : row_list) image.list.push_back(rows[r]);
     PlanHeader& h = image.header;
-    for (const PlanRow& r : rows) h.most_slots = std::max(h.most_slots, r.slots);
+    for (const PlanRow& r : rows) {
+        h.most_slots = std::max(h.most_slots, r.slots);
+        h.most_position = std::max(h.most_position, h.tree_stride ? image.trees[static_cast<size_t>(r.row) * h.tree_stride] : r.position);
+    }
     h.rows = static_cast<int>(rows.size());
     h.narrow = static_cast<int>(narrow.size());
     h.wide = static_cast<int>(wide.size());

@@ -108,7 +108,7 @@ struct PlanRun {
 struct PlanHeader {
     int rows, narrow, wide, runs;
     int joined, slots, longest_run, partials;
-    int tree_stride, most_slots, pad[2];  // most_slots: of a row
+    int tree_stride, most_slots, most_position, pad;  // most_slots: of a row; most_position: that a row stands for
 };
 
 // Where a batch has trees, tree_stride numbers for every row: the position that it stands for (its context and its depth in
