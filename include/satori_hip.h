@@ -615,8 +615,8 @@ typedef struct satori_hip_logit_row {
     int biases;                            /* set; -1: none */
     int mask;                              /* -1: none */
 } satori_hip_logit_row;
-/* Strides are in elements. History h: the first lengths[h] (at most history_stride) tokens from history + h * history_stride. A mask
- * has a bit for each token, 32 a word from the lowest on (set: allowed). Tokens outside the vocabulary, and numbers of
+/* Strides are in elements. history is [histories][history_stride]; a history is the first lengths[h] (at most history_stride) tokens of its
+ * line. A mask has a bit for each token, 32 a word from the lowest on (set: allowed). Tokens outside the vocabulary, and numbers of
  * histories, sets, masks or parents that do not exist, are as if they were not there. */
 typedef struct satori_hip_logit_batch {
     const satori_hip_logit_row* rows;
@@ -633,7 +633,8 @@ typedef struct satori_hip_logit_batch {
 int satori_hip_logit_rules_create(satori_hip_context* context, int vocabulary, int bias_sets, int bias_entries,
                                   satori_hip_logit_rules** rules);
 /* A set's tokens, in any order, each once, and their values (no NaN; -infinity bans a token that is not +infinity), on the host. The
- * copy is ordered on `stream` and waited for; not while capturing. */
+ * copy is ordered on `stream` and waited for (calls on other streams that read the set are the caller's to order); not while
+ * capturing. */
 int satori_hip_logit_rules_set_biases(satori_hip_logit_rules* rules, int set, const int* tokens, const float* values, int count,
                                       void* stream);
 /* The batch struct is read before the call returns. Calls with one handle share its workspace and must not overlap in time on

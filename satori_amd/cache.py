@@ -335,17 +335,15 @@ class CachePlan:
     def append_rotated(self, layer: int, q: int, q_bias: int, q_out: int, k: int, k_bias: int, v: int, v_bias: int,
                        rotation, stream: int = 0) -> None:
         """`append` with a Rotation (satori_amd.rotary)."""
-        _check(_ffi.lib().satori_hip_cache_append_rotated(self._handle, layer, _pointer(q), _pointer(q_bias),
-                                                          _pointer(q_out), _pointer(k), _pointer(k_bias), _pointer(v),
-                                                          _pointer(v_bias), rotation.handle, _pointer(stream)))
+        _check(_ffi.lib().satori_hip_cache_append_rotated(self._handle, layer, q, q_bias, q_out, k, k_bias, v, v_bias,
+                                                          rotation.handle, stream))
 
     def keep(self, rows: Sequence[Sequence[int]], stream: int = 0) -> None:
         """Moves the keys and values of rows[i], some of the plan's rows of its i-th sequence in ascending order, to follow that
         sequence's context, in all layers. Truncate the sequence to its context and len(rows[i]) then, and set the plan
         again before it is used."""
         counts, kept = array("i", map(len, rows)), array("i", chain.from_iterable(rows))
-        _check(_ffi.lib().satori_hip_cache_keep(self._handle, _address(kept) or None, _address(counts) or None, len(counts),
-                                                _pointer(stream)))
+        _check(_ffi.lib().satori_hip_cache_keep(self._handle, _address(kept), _address(counts), len(counts), stream))
 
     def attention(self, layer: int, q: int, out: int, stream: int = 0) -> None:
         """Grouped attention of every row over the positions of its sequence up to its own."""

@@ -267,6 +267,10 @@ __global__ __launch_bounds__(kThreads, 4) void logits_kernel(LogitArgs a) {
     unsigned long long key = top[thread][0];
 #pragma unroll
     for (int k = 1; k < kThreads / 64; ++k) key = greater(key, top[thread][k]);
+    if (gridDim.x == 1) {
+        a.best[first + thread] = key ? static_cast<int>(~static_cast<uint32_t>(key)) : -1;
+        return;
+    }
     LogitBest* found = a.found + local + thread;
     __hip_atomic_fetch_max(&found->key, key, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     __asm__ volatile("s_waitcnt vmcnt(0)" ::: "memory");

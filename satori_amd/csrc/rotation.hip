@@ -13,11 +13,12 @@ namespace {
 constexpr int kThreads = 256;
 
 __global__ __launch_bounds__(kThreads) void rotation_table_kernel(RotationShape s, double* table) {
-    const int64_t i = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x;
-    if (i >= static_cast<int64_t>(s.positions) * s.pairs) return;
-    const int p = static_cast<int>(i / s.pairs), k = static_cast<int>(i % s.pairs);
-    double* row = table + static_cast<int64_t>(p) * 2 * s.pairs;
-    rotation_angle(k, p, s.frequencies, s.magnitude, row[k], row[s.pairs + k]);
+    const int64_t all = static_cast<int64_t>(s.positions) * s.pairs, stride = static_cast<int64_t>(gridDim.x) * kThreads;
+    for (int64_t i = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x; i < all; i += stride) {
+        const int p = static_cast<int>(i / s.pairs), k = static_cast<int>(i % s.pairs);
+        double* row = table + static_cast<int64_t>(p) * 2 * s.pairs;
+        rotation_angle(k, p, s.frequencies, s.magnitude, row[k], row[s.pairs + k]);
+    }
 }
 
 // N elements at any place of theirs, one access.
@@ -181,7 +182,8 @@ hipError_t rotate_of(const RotationShape& s, const RotateArgs& a, hipStream_t st
 hipError_t launch_rotation_table(const RotationShape& shape, double* table, hipStream_t stream) {
     const int64_t n = static_cast<int64_t>(shape.positions) * shape.pairs;
     if (n <= 0) return hipSuccess;
-    rotation_table_kernel<<<static_cast<unsigned>((n + kThreads - 1) / kThreads), kThreads, 0, stream>>>(shape, table);
+    const int64_t groups = std::min<int64_t>((n + kThreads - 1) / kThreads, 1 << 20);  // (a launch's threads are counted in 32 bits)
+    rotation_table_kernel<<<static_cast<unsigned>(groups), kThreads, 0, stream>>>(shape, table);
     return hipGetLastError();
 }
 

@@ -7,7 +7,7 @@ import ctypes
 import numpy as np
 
 from . import ArgumentException, HipContext, _check, _ffi
-from .cache import _address, _array, _at, _pointer
+from .cache import _address, _array, _at
 
 # A row's parameters, as they lie on the device (satori_hip_logit_row).
 LOGIT_ROW = np.dtype([("repetition", "<f4"), ("presence", "<f4"), ("frequency", "<f4"), ("history", "<i4"), ("parent", "<i4"),
@@ -37,11 +37,11 @@ class LogitRules:
         listed, added = _array(tokens), np.ascontiguousarray(values, np.float32).reshape(-1)
         if len(listed) != added.size:
             raise ArgumentException("Lengths differ.")
-        _check(_ffi.lib().satori_hip_logit_rules_set_biases(self._handle, index, _address(listed) or None, _at(added),
-                                                            len(listed), _pointer(stream)))
+        _check(_ffi.lib().satori_hip_logit_rules_set_biases(self._handle, index, _address(listed), _at(added),
+                                                            len(listed), stream))
 
     def apply(self, batch: LogitBatch, stream: int = 0) -> None:
-        _check(_ffi.lib().satori_hip_logit_rules_apply(self._handle, ctypes.byref(batch), _pointer(stream)))
+        _check(_ffi.lib().satori_hip_logit_rules_apply(self._handle, ctypes.byref(batch), stream))
 
     def dispose(self) -> None:
         _check(_ffi.lib().satori_hip_logit_rules_destroy(self._handle))

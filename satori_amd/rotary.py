@@ -7,7 +7,7 @@ import enum
 import numpy as np
 
 from . import HipContext, _check, _ffi
-from .cache import ElementType, _at, _pointer
+from .cache import ElementType, _at
 
 
 class RotaryLayout(enum.IntEnum):
@@ -55,9 +55,8 @@ class Rotation:
         width = heads * head_dim
         if not out:
             out, out_stride = x, out_stride or stride
-        _check(_ffi.lib().satori_hip_rotation_apply(self._handle, int(type), _pointer(x), stride or width, _pointer(out),
-                                                    out_stride or width, rows, heads, head_dim, _pointer(positions),
-                                                    _pointer(stream)))
+        _check(_ffi.lib().satori_hip_rotation_apply(self._handle, type, x, stride or width, out, out_stride or width, rows, heads,
+                                                    head_dim, positions, stream))
 
     def dispose(self) -> None:
         _check(_ffi.lib().satori_hip_rotation_destroy(self._handle))

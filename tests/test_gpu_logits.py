@@ -291,6 +291,27 @@ def test_lengths_that_say_too_much(context, device):
     rules.dispose()
 
 
+def test_rows_behind_the_fourth_gibibyte(context, device):
+    v, n, stride = 500, 3, 1_600_000_001
+    g = rng(14)
+    logits = g.standard_normal((n, v)).astype(np.float32)
+    p, best = context.alloc(((n - 1) * stride + v) * 4), device(np.zeros(n, np.int32))
+    for i in range(n):
+        context.upload(p + i * stride * 4, logits[i])
+    history = [[1, 1, 2, 499]]
+    rows = [row(1.5, 0.25, 0.5, 0), row(), row(1.0, 1.0, 0.0, 0, parent=1, token=7)]
+    rules = make_rules(context, v, [])
+    rules.apply(LogitBatch(rows=device(np.array(rows, LOGIT_ROW)), count=n, logits=p, logits_stride=stride, output=p, output_stride=stride,
+                           best=best, history=device(np.array(history, np.int32)), history_stride=4, histories=1,
+                           lengths=device(np.array([4], np.int32))))
+    got = np.stack([context.download(np.zeros(v, np.float32), p + i * stride * 4) for i in range(n)])
+    chosen = context.download(np.zeros(n, np.int32), best)
+    context.free(p)
+    want, expected_best = expected(logits, rows, history, [], [])
+    assert same(got, want) and np.array_equal(chosen, expected_best)
+    rules.dispose()
+
+
 def test_refused_calls(context, device):
     for bad in ((0, 0, 0), (-1, 0, 0), (10, -1, 0), (10, 1, -1), (10, 1, 11), (2 ** 28 + 1, 0, 0)):
         with pytest.raises(S.ArgumentOutOfRangeException):
