@@ -43,27 +43,26 @@ __device__ __forceinline__ void store_pack(T* p, const float (&v)[N]) {
 }
 
 // A workgroup turns some pairs (kThreads at most, all rows together) of some rows: its threads read, or compute, the sine and
-// cosine of one pair of one row each and leave them in LDS, while what they turn first is on its way: N pairs of kHeads heads a
-// thread and turn, 16 bytes a head and access. Behind the last whole N pairs single ones; the lanes behind the rotated ones are
-// copied, unless the output is the input.
-constexpr int kHeads = 4;
+// cosine of one pair of one row each and leave them in LDS, while what they turn first is on its way: four accesses of 16 bytes
+// a thread and turn, each half a head apart its pairs' other one (two heads), or with whole pairs (four heads). Behind the
+// last whole pack of a head single pairs; the lanes behind the rotated ones are copied, unless the output is the input.
 
 // Where a pair's angle lies: a pack's 128 bytes start at other banks than the next one's.
 __device__ __forceinline__ int angle_at(int i) { return i + (i >> 3); }
 
 template <typename T, bool INTERLEAVED>
 __global__ __launch_bounds__(kThreads) void rotate_kernel(RotationShape s, RotateArgs a, int group_rows, int group_pairs) {
-    constexpr int N = 16 / sizeof(T);
+    constexpr int N = 16 / sizeof(T), kHeads = INTERLEAVED ? 4 : 2, kPairs = INTERLEAVED ? N / 2 : N;  // pairs of a pack
     typedef double f64x2 __attribute__((ext_vector_type(2)));
     __shared__ f64x2 angles[kThreads + kThreads / 8];
     const int thread = threadIdx.x, row0 = blockIdx.x * group_rows, k0 = blockIdx.y * group_pairs, D = a.head_dim;
     const int rows = min(group_rows, a.rows - row0), pairs = min(group_pairs, s.pairs - k0);
-    const int packs = (pairs + N - 1) / N, groups = (a.heads + kHeads - 1) / kHeads;
+    const int packs = (pairs + kPairs - 1) / kPairs, groups = (a.heads + kHeads - 1) / kHeads;
     const bool copies = a.output != a.input && blockIdx.y + 1 == gridDim.y;
     const int units = packs + (copies ? (D - 2 * s.pairs + N - 1) / N : 0), row_units = units * groups;
 
     struct Unit {
-        int row, k, heads;  // k: the first pair of the workgroup's; past its pairs: a pack to copy
+        int row, pack, heads;  // past the pairs' packs: one to copy
         const T* in;
         T* out;
     };
@@ -71,26 +70,28 @@ __global__ __launch_bounds__(kThreads) void rotate_kernel(RotationShape s, Rotat
         Unit r;
         r.row = u / row_units;
         const int rest = u % row_units, first = rest / units * kHeads;
-        r.k = rest % units * N;
+        r.pack = rest % units;
         r.heads = min(kHeads, a.heads - first);
         r.in = static_cast<const T*>(a.input) + (row0 + r.row) * a.input_stride + static_cast<int64_t>(first) * D;
         r.out = static_cast<T*>(a.output) + (row0 + r.row) * a.output_stride + static_cast<int64_t>(first) * D;
         return r;
     };
-    float x[kHeads][N], y[kHeads][N];
+    float x[kHeads][N], y[INTERLEAVED ? 1 : kHeads][N];
     const auto load = [&](const Unit& r) {
-        if (r.k + N > pairs) return;
-        const int at = INTERLEAVED ? 2 * (k0 + r.k) : k0 + r.k, beside = INTERLEAVED ? N : s.pairs;
+        const int k = r.pack * kPairs;
+        if (k + kPairs > pairs) return;
+        const int at = INTERLEAVED ? 2 * (k0 + k) : k0 + k;
 #pragma unroll
         for (int h = 0; h < kHeads; ++h)
             if (h < r.heads) {
                 load_pack<T, N>(r.in + h * D + at, x[h]);
-                load_pack<T, N>(r.in + h * D + at + beside, y[h]);
+                if constexpr (!INTERLEAVED) load_pack<T, N>(r.in + h * D + at + s.pairs, y[h]);
             }
     };
     const auto turn = [&](const Unit& r) {
-        if (r.k >= packs * N) {
-            const int lane = 2 * s.pairs + r.k - packs * N;
+        const int k = r.pack * kPairs;
+        if (r.pack >= packs) {
+            const int lane = 2 * s.pairs + (r.pack - packs) * N;
             for (int h = 0; h < r.heads; ++h) {
                 if (lane + N <= D) {
                     float v[N];
@@ -100,10 +101,10 @@ __global__ __launch_bounds__(kThreads) void rotate_kernel(RotationShape s, Rotat
                     for (int j = lane; j < D; ++j) r.out[h * D + j] = r.in[h * D + j];
                 }
             }
-        } else if (r.k + N > pairs) {
-            for (int k = r.k; k < pairs; ++k) {
-                const f64x2 angle = angles[angle_at(r.row * pairs + k)];
-                const int at = INTERLEAVED ? 2 * (k0 + k) : k0 + k, beside = INTERLEAVED ? 1 : s.pairs;
+        } else if (k + kPairs > pairs) {
+            for (int i = k; i < pairs; ++i) {
+                const f64x2 angle = angles[angle_at(r.row * pairs + i)];
+                const int at = INTERLEAVED ? 2 * (k0 + i) : k0 + i, beside = INTERLEAVED ? 1 : s.pairs;
                 for (int h = 0; h < r.heads; ++h) {
                     float u, v;
                     rope_apply(static_cast<float>(r.in[h * D + at]), static_cast<float>(r.in[h * D + at + beside]), angle[0],
@@ -114,17 +115,20 @@ __global__ __launch_bounds__(kThreads) void rotate_kernel(RotationShape s, Rotat
             }
         } else {
 #pragma unroll
-            for (int j = 0; j < N; ++j) {
-                const f64x2 angle = angles[angle_at(r.row * pairs + r.k + j)];
+            for (int j = 0; j < kPairs; ++j) {
+                const f64x2 angle = angles[angle_at(r.row * pairs + k + j)];
 #pragma unroll
-                for (int h = 0; h < kHeads; ++h) rotate_pair<INTERLEAVED>(x[h], y[h], j, angle[0], angle[1]);
+                for (int h = 0; h < kHeads; ++h) {
+                    float &u = INTERLEAVED ? x[h][2 * j] : x[h][j], &v = INTERLEAVED ? x[h][2 * j + 1] : y[INTERLEAVED ? 0 : h][j];
+                    rope_apply(u, v, angle[0], angle[1], u, v);
+                }
             }
-            const int at = INTERLEAVED ? 2 * (k0 + r.k) : k0 + r.k, beside = INTERLEAVED ? N : s.pairs;
+            const int at = INTERLEAVED ? 2 * (k0 + k) : k0 + k;
 #pragma unroll
             for (int h = 0; h < kHeads; ++h)
                 if (h < r.heads) {
                     store_pack<T, N>(r.out + h * D + at, x[h]);
-                    store_pack<T, N>(r.out + h * D + at + beside, y[h]);
+                    if constexpr (!INTERLEAVED) store_pack<T, N>(r.out + h * D + at + s.pairs, y[h]);
                 }
         }
     };
