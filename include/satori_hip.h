@@ -66,7 +66,7 @@ typedef enum satori_hip_format {
     SATORI_HIP_TERNARY2 = 16
 } satori_hip_format;
 
-/* Element types of key/value pages and adapters. */
+/* Element types of key/value pages, adapters and rotated rows. */
 typedef enum satori_hip_element {
     SATORI_HIP_F32 = 0,
     SATORI_HIP_F16 = 1
@@ -507,8 +507,8 @@ int satori_hip_cache_plan_set(satori_hip_cache_plan* plan, satori_hip_pages* pag
  * the context's length plus its depth, and its attention sees the context, the rows that it follows and itself. Rows that follow
  * one another in order are no tree and may be any number, those of a tree 1024 of a sequence (SATORI_HIP_E_NOT_SUPPORTED).
  * All that is said of satori_hip_cache_plan_set holds. A plan that has held a tree is launched with kernels that look for one:
- * for a captured step to take trees, set one before the capture, of no fewer rows times the positions from its context's last
- * multiple of 32 on (else SATORI_HIP_E_INVALID_OPERATION). */
+ * for a captured step to take trees, set a batch of as many rows with as large a tree before the capture (else
+ * SATORI_HIP_E_INVALID_OPERATION). */
 int satori_hip_cache_plan_set_tree(satori_hip_cache_plan* plan, satori_hip_pages* pages, const int* sequences,
                                    const int* new_tokens, const int* parents, int count, void* stream);
 /* Fails with SATORI_HIP_E_ARGUMENT while a step reads the plan. */

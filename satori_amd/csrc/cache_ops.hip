@@ -92,7 +92,10 @@ constexpr int kGroupTokens = 8;  // positions whose values a thread stores at on
 // them together where they fill an aligned group (one value a store took 93 us where this takes 9.8). Few rows are bound by
 // the launch and two dependent reads (16 rows of 12 + 2 heads of 128 lanes 4.6 us), many by that and, half of the time, by memory: 8 x
 // 61 rows of 32 + 8 heads move 22.6 MB in 9.8 us (2.3 TB/s, where a large copy reaches 4.9); in a captured step, whose grid does
-// for any batch, 15.1. The rotation's angles come from the table in 64 bits, as the single-sequence operator's.
+// for any batch, 15.1. The rotation's angles come from the table in 64 bits, as the single-sequence operator's; where the host knows
+// that the table has them all, the launch leaves out the code that computes them, and a wave takes 60 registers instead of 127:
+// with that and the lanes behind the rotated ones in fours, 16 x 61 rows of a tree, 64 of 128 lanes rotated, 12.0 us instead of
+// 21.4 (44 MB, a floor of 8.5).
 enum class Turn { kPlain, kTree, kInterleaved };  // pairs half a head apart, rows no tree's; also a tree's; neighbouring lanes
 template <typename T, int N, Turn TURN, bool LISTED>  // LISTED: the table has every position
 __global__ __launch_bounds__(kThreads) void cache_append_kernel(CacheShape s, const int* __restrict__ image, int runs_at, int trees_at,
@@ -188,7 +191,10 @@ __global__ __launch_bounds__(kThreads) void cache_append_kernel(CacheShape s, co
 // Moves the keys and values of a sequence's kept rows to the places behind its context, in all layers. A place that is
 // written may be read by an earlier move and by no later one (rows go in ascending order, none behind where it was), so a
 // thread makes all moves of its own bytes, eight at a time, each eight read before they are written: 16 bytes of a key, or
-// one lane of a value, whose positions lie side by side.
+// one lane of a value, whose positions lie side by side. Few moves are bound by the launch (one sequence, 4 layers 2.9 us), many
+// by the lines that hold the values, of which a move wants 2 bytes each: 245 moves of 64 sequences, 28 layers of 2 heads of 128
+// lanes, F16, move 14 MB through some 85 in 24 us. (A wave for each sequence and head, eight lanes a value row: 31 us; that with
+// whole 64 bytes written through LDS 23, but 3.8 for one sequence.)
 template <typename V, typename At>
 __device__ __forceinline__ void keep_moves(const KeepMoves& moves, int begin, int end, const At& at) {
     for (int i0 = begin; i0 < end; i0 += 8) {
@@ -559,7 +565,9 @@ struct Sight {
 };
 
 // The same where rows may be a tree's: a bit per token of the tile, which the plan has ready (a row sees what lies before
-// its context's last multiple of 32, and nothing behind its own number's tile).
+// its context's last multiple of 32, and nothing behind its own number's tile). One number a pair and tile, read a tile ahead
+// (few pairs) or before the first product (many); tiles that all rows see whole, all but the last few, read none, and kernels
+// of plans that never held a tree know of none.
 template <>
 struct Sight<true> {
     typedef uint32_t Seen;
@@ -1130,7 +1138,8 @@ __global__ __launch_bounds__(kThreads) void cache_join_kernel(AttentionArgs a) {
 }
 
 // The same where rows have few parts: four lanes of a (row, head) a thread, all parts at once, added in the same order (the
-// groups above would have one part each, and those without one add zeros).
+// groups above would have one part each, and those without one add zeros). 512 x 32 pairs of 2 to 7 parts 10 us, where the
+// workgroup a pair took 27; 1024 x 32 of 1 to 3 8 us instead of 34.
 constexpr int kFewParts = 8;
 __global__ __launch_bounds__(kThreads) void cache_join_few_kernel(AttentionArgs a) {
     const CacheShape& s = a.s;

@@ -239,6 +239,10 @@ constexpr int kLeastShared = 128;
 // 17.5 not, 512 (100 MB) 24.4 and 21.9, 1024 (201 MB) 27.5 and 32.0. Heads of 192 and 256 lanes fit one workgroup a CU, but half
 // the number serves them no better: F16, 256 lanes, 32 + 8 heads over 256 shared positions, 30 sequences take 31.1 us with 512
 // here and 38.8 with 256, 32 take 30.8 and 23.7, 40 take 32.5 with either; FP32, 30 sequences, 45.4 and 73.7.
+// Of batches with trees, whose sequences have many rows each: what a token costs a wide workgroup and one of 16 pairs (ns, two
+// workgroups a CU). A node is wide from a quarter of a wide workgroup's pairs on, where two narrow ones cost less than it
+// (32 sequences of 16 rows and 64 pairs over 4096 and 100 to 1000 positions: from half 198 us, from a quarter 151), and a run is
+// also shared where that saves more of this time than its partial results take (the same: 101).
 constexpr int64_t kWideTokenTime = 62, kNarrowTokenTime = 26;
 constexpr int64_t kPlaces = 512, kRoundBytes = 128 << 20;
 
@@ -247,10 +251,11 @@ constexpr int64_t kPlaces = 512, kRoundBytes = 128 << 20;
 namespace {
 
 // The numbers of every row of a batch whose rows follow `parents` (PlanHeader::tree_stride of them each), and the context of
-// every sequence that is a tree; -1 for the others. Nothing where none is.
+// every sequence that is a tree; -1 for the others. Nothing where none is. Room for as many rows and as large a tree behind
+// any context goes with what plain divisions take.
 void plan_trees(const PageTables& tables, const int* sequences, const int* new_tokens, int count, const int* parents,
                 PlanImage& image, std::vector<int>& contexts) {
-    int64_t stride = 0, first = 0;
+    int64_t stride = 0, first = 0, largest = 0;
     for (int i = 0; i < count; first += new_tokens[i++]) {
         const int rows = new_tokens[i], context = tables.tokens(sequences[i]) - rows;
         bool tree = false;
@@ -263,11 +268,14 @@ void plan_trees(const PageTables& tables, const int* sequences, const int* new_t
         if (rows > kMostTree)
             fail(SATORI_HIP_E_NOT_SUPPORTED, "Trees of more than " + std::to_string(kMostTree) + " rows are not supported.");
         contexts[i] = context;
+        largest = std::max<int64_t>(largest, rows);
         stride = std::max<int64_t>(stride, 1 + (context % kTile + rows + kTile - 1) / kTile);
     }
     if (stride == 0) return;
-    if (first * stride > INT32_MAX / 64) fail(SATORI_HIP_E_OVERFLOW, "Arithmetic operation resulted in an overflow.");
+    const int64_t most = first * (1 + (largest + 2 * (kTile - 1)) / kTile);
+    if (most > INT32_MAX / 64) fail(SATORI_HIP_E_OVERFLOW, "Arithmetic operation resulted in an overflow.");
     image.header.tree_stride = static_cast<int>(stride);
+    image.plain.trees = static_cast<int>(most);
     image.trees.resize(first * stride);
     int* row = image.trees.data();
     first = 0;
@@ -447,6 +455,10 @@ PlanImage plan_batch(const PageTables& tables, const int* sequences, const int* 
     };
     int narrow_chunk = chunk_for(narrow_tokens), wide_chunk = chunk_for(wide_tokens);
     if (trees) {
+        // The shortest chunk whose items all have a place at once: sequences of different lengths leave chunks of one length for so
+        // many workgroups with remainders that some places wait for. (8 trees of 64 rows over 4000 to 16384 positions, F16, 32 + 8
+        // heads, 247 us in chunks for 256 workgroups, 196 for 512, 234 so for 256 places, 186 for 512; 16 over 500 to 4000 135, 146,
+        // 168, 120; FP32, 12 + 2 heads, 8 over 2000 to 8000 232, 140, 188, 141.)
         const int64_t step = kTile * kWaves, places = static_cast<int64_t>(shape.places) * division.workgroups / 256;
         const auto items_of = [&](int64_t chunk) {
             int64_t items = 0;
@@ -582,7 +594,6 @@ PlanImage plan_batch(const PageTables& tables, const int* sequences, const int* 
     image.plain.rows = image.plain.list = h.rows;
     image.plain.runs = entries(std::min<int64_t>(h.rows, h.rows / P + 2 * of_rows));
     image.plain.pages = entries(list_pages);
-    image.plain.trees = static_cast<int>(image.trees.size());
     image.plain.narrow = entries(narrow_blocks * units);
     image.plain.wide = entries(wide_blocks * units);
     image.plain_partials = chunks > 1 ? h.rows * chunks : 0;

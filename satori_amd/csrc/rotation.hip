@@ -46,6 +46,8 @@ __device__ __forceinline__ void store_pack(T* p, const float (&v)[N]) {
 // cosine of one pair of one row each and leave them in LDS, while what they turn first is on its way: four accesses of 16 bytes
 // a thread and turn, each half a head apart its pairs' other one (two heads), or with whole pairs (four heads). Behind the
 // last whole pack of a head single pairs; the lanes behind the rotated ones are copied, unless the output is the input.
+// Bound by the launch (8 rows of 12 heads 3.2 us) or by memory: 4096 rows of 32 heads of 128 F16 lanes 13.0 us, 67 MB at 5.2 TB/s
+// (two accesses a thread 14.4, eight 13.8; angles read by every thread, 64 bytes a pack, 18).
 
 // Where a pair's angle lies: a pack's 128 bytes start at other banks than the next one's.
 __device__ __forceinline__ int angle_at(int i) { return i + (i >> 3); }

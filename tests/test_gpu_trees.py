@@ -470,6 +470,32 @@ def test_a_captured_step_follows_trees(context, device, type_, heads, kv_heads, 
     eager.dispose()
 
 
+def test_a_captured_step_takes_a_tree_behind_any_context(context, device):
+    # Where a tree's context ends within 32 positions changes what the plan keeps for it.
+    g = rng(15)
+    pool = Pool(context, device, CacheLayout(1, 1, 32, 32, F32), 30)
+    s, other = pool.cache.open(), pool.cache.open()
+    pool.cache.extend([s, other], [320 + 61, 40])
+    pool.write(g, [s, other])
+    q = g.standard_normal((65, 2, 32)).astype(np.float32)
+    dq, out = device(q), device(np.zeros_like(q))
+    plan = pool.cache.plan(2)
+    plan.set_tree([s], [mixed(40, 1)])  # (leaves some room, not enough)
+    plan.set_tree([s, other], [mixed(61, 1), star(4)])
+    context.capture_begin()
+    plan.attention(0, dq, out)
+    step = context.capture_end()
+    for more in (0, 1, 3, 26, 1, 1, 17):
+        pool.cache.extend([s], [more])
+        pool.write(g, [s, other])
+        trees = [mixed(61, more), star(4)]
+        plan.set_tree([s, other], trees)
+        step.execute()
+        check_tree(pool, [s, other], trees, 2, q, context.download(np.zeros_like(q), out))
+    step.dispose()
+    plan.dispose()
+
+
 def test_a_step_captured_without_trees_takes_none(context, device):
     g = rng(4)
     pool = Pool(context, device, CacheLayout(1, 2, 64, 32, F16), 40)
