@@ -18,6 +18,12 @@ typedef float f32x2 __attribute__((ext_vector_type(2)));
 
 constexpr int kThreads = 256;
 
+// The same value, of which the compiler knows nothing.
+__device__ __forceinline__ int unknown_scalar(int v) {
+    __asm__ volatile("" : "+s"(v));
+    return v;
+}
+
 // ---- page copies ----
 
 // Each workgroup copies kCopyBytes of one page, 16 bytes a thread and access, four accesses in flight; a page of all layers is
@@ -189,48 +195,70 @@ __global__ __launch_bounds__(kThreads) void cache_append_kernel(CacheShape s, co
 // ---- positions that a sequence keeps ----
 
 // Moves the keys and values of a sequence's kept rows to the places behind its context, in all layers. A place that is
-// written may be read by an earlier move and by no later one (rows go in ascending order, none behind where it was), so a
-// thread makes all moves of its own bytes, eight at a time, each eight read before they are written: 16 bytes of a key, or
-// one lane of a value, whose positions lie side by side. Few moves are bound by the launch (one sequence, 4 layers 2.9 us), many
-// by the lines that hold the values, of which a move wants 2 bytes each: 245 moves of 64 sequences, 28 layers of 2 heads of 128
-// lanes, F16, move 14 MB through some 85 in 24 us. (A wave for each sequence and head, eight lanes a value row: 31 us; that with
-// whole 64 bytes written through LDS 23, but 3.8 for one sequence.)
-template <typename V, typename At>
-__device__ __forceinline__ void keep_moves(const KeepMoves& moves, int begin, int end, const At& at) {
-    for (int i0 = begin; i0 < end; i0 += 8) {
-        V v[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = *(const SATORI_GLOBAL V*)(at(moves.source[min(i0 + j, end - 1)]));
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-            if (i0 + j < end) *(SATORI_GLOBAL V*)(at(moves.destination[i0 + j])) = v[j];
-    }
-}
-
+// written may be read by an earlier move and by no later one (rows go in ascending order, none behind where it was), so eight
+// moves are read before they are written, and the next eight come behind them in the same wave. Of keys a thread takes 16 bytes
+// through all moves. Of values, whose positions lie side by side, eight threads take a move each of one lane of the head, so
+// that the destinations, which follow one another, are one access; a wave takes 32 lanes of a head. Few moves are bound by
+// the launch (one sequence, 4 layers 3.1 us), many by the lines that hold the values, of which a move wants 2 bytes each: 245
+// moves of 64 sequences, 28 layers of 2 heads of 128 lanes, F16, 14 MB, in 20 us. (A thread through all moves of a lane asks for
+// 1.8 million writes instead of 0.5 and takes 25; a wave for all lanes of a head 31, the same with whole 64 bytes written through
+// LDS 23.)
 template <typename T>
 __global__ __launch_bounds__(kThreads) void cache_keep_kernel(CacheShape s, int layers, KeepMoves moves) {
-    const int begin = moves.begin[blockIdx.y], end = moves.begin[blockIdx.y + 1];
-    const int pieces = s.width * static_cast<int>(sizeof(T)) / 16, heads = layers * s.kv_heads;
-    const int64_t head_bytes = static_cast<int64_t>(s.page_tokens) * s.width * sizeof(T);
-    const int mask = s.page_tokens - 1;
-    const int64_t units = static_cast<int64_t>(heads) * (pieces + s.head_dim);
-    for (int64_t u = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x; u < units;
-         u += static_cast<int64_t>(gridDim.x) * kThreads) {
-        const bool key = u < static_cast<int64_t>(heads) * pieces;
-        const uint32_t of = static_cast<uint32_t>(key ? u : u - static_cast<int64_t>(heads) * pieces);
-        const uint32_t head = of / (key ? pieces : s.head_dim), part = of % (key ? pieces : s.head_dim);
-        uint8_t* base = s.pool + head / s.kv_heads * s.layer_bytes + head % s.kv_heads * head_bytes;
-        if (key) {
-            base += part * 16;
-            keep_moves<u32x4>(moves, begin, end, [&](int place) {
-                return base + (place >> s.page_shift) * s.page_bytes + (place & mask) * (s.width * static_cast<int>(sizeof(T)));
-            });
-        } else {
-            base += s.kv_heads * head_bytes + static_cast<int64_t>(part) * s.page_tokens * sizeof(T);
-            keep_moves<T>(moves, begin, end, [&](int place) {
-                return base + (place >> s.page_shift) * s.page_bytes + (place & mask) * static_cast<int>(sizeof(T));
-            });
+    typedef std::conditional_t<sizeof(T) == 2, uint16_t, uint32_t> Bits;
+    constexpr int kSize = sizeof(T), kMoves = 8, kSteps = 4, kBlock = 64 / kMoves * kSteps;  // lanes of a head a wave takes
+    const int begin = moves.begin[blockIdx.y], end = moves.begin[blockIdx.y + 1], lane = threadIdx.x & 63;
+    const int wave = blockIdx.x * (kThreads / 64) + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int pieces = s.width * kSize / 16, heads = layers * s.kv_heads, mask = s.page_tokens - 1;
+    const int key_waves = (heads * pieces + 63) / 64, blocks = (s.head_dim + kBlock - 1) / kBlock;
+    const int64_t head_bytes = static_cast<int64_t>(s.page_tokens) * s.width * kSize;
+    if (wave < key_waves) {
+        const int u = wave * 64 + lane;
+        if (u >= heads * pieces) return;
+        const int head = u / pieces;
+        uint8_t* base = s.pool + head / s.kv_heads * s.layer_bytes + head % s.kv_heads * head_bytes + u % pieces * 16;
+        const auto at = [&](int place) { return base + (place >> s.page_shift) * s.page_bytes + (place & mask) * (s.width * kSize); };
+        for (int i0 = begin; i0 < end; i0 += kMoves) {
+            u32x4 v[kMoves];
+#pragma unroll
+            for (int j = 0; j < kMoves; ++j) v[j] = *(const SATORI_GLOBAL u32x4*)(at(moves.source[min(i0 + j, end - 1)]));
+#pragma unroll
+            for (int j = 0; j < kMoves; ++j)
+                if (i0 + j < end) *(SATORI_GLOBAL u32x4*)(at(moves.destination[i0 + j])) = v[j];
         }
+        return;
+    }
+    const int head = (wave - key_waves) / blocks, first = (wave - key_waves) % blocks * kBlock;
+    if (head >= heads) return;
+    const int move = lane % kMoves, row = first + lane / kMoves, row_bytes = s.page_tokens * kSize;
+    uint8_t* base = s.pool + head / s.kv_heads * s.layer_bytes + (s.kv_heads + head % s.kv_heads) * head_bytes +
+                    static_cast<int64_t>(row) * row_bytes;
+    for (int i0 = begin; i0 < end; i0 += kMoves) {
+        // Each move's places are scalars, all read before any is chosen; those behind the last are the last, and not written.
+        int of[kMoves], to[kMoves];
+#pragma unroll
+        for (int j = 0; j < kMoves; ++j) {
+            of[j] = moves.source[min(i0 + j, end - 1)];
+            to[j] = moves.destination[min(i0 + j, end - 1)];
+        }
+        int source = 0, destination = 0;
+#pragma unroll
+        for (int j = 0; j < kMoves; ++j) {
+            const int x = unknown_scalar(of[j]), y = unknown_scalar(to[j]);
+            source = move == j ? x : source;
+            destination = move == j ? y : destination;
+        }
+        const auto at = [&](int place) { return base + (place >> s.page_shift) * s.page_bytes + (place & mask) * kSize; };
+        const uint8_t* from = at(source);
+        uint8_t* target = at(destination);
+        const int left = (s.head_dim - row + kMoves - 1) / kMoves;  // steps that have a lane
+        uint32_t v[kSteps];
+#pragma unroll
+        for (int j = 0; j < kSteps; ++j)
+            v[j] = *(const SATORI_GLOBAL Bits*)(from + (j < left ? j : 0) * kMoves * row_bytes);
+#pragma unroll
+        for (int j = 0; j < kSteps; ++j)
+            if (j < left && i0 + move < end) *(SATORI_GLOBAL Bits*)(target + j * kMoves * row_bytes) = static_cast<Bits>(v[j]);
     }
 }
 
@@ -628,10 +656,6 @@ __device__ __forceinline__ T scalar_load(const T* p) {
 // lane masks and addresses, moved out of the loop over items, would fill the registers).
 __device__ __forceinline__ int unknown(int v) {
     __asm__ volatile("" : "+v"(v));
-    return v;
-}
-__device__ __forceinline__ int unknown_scalar(int v) {
-    __asm__ volatile("" : "+s"(v));
     return v;
 }
 
@@ -1282,8 +1306,10 @@ hipError_t launch_cache_append(const CacheShape& s, const int* image, const Plan
 
 hipError_t launch_cache_keep(const CacheShape& s, int layers, const KeepMoves& moves, hipStream_t stream) {
     if (moves.sequences == 0) return hipSuccess;
-    const int64_t units = static_cast<int64_t>(layers) * s.kv_heads * (s.width * element_bytes(s.type) / 16 + s.head_dim);
-    const dim3 grid(static_cast<unsigned>(std::min<int64_t>((units + kThreads - 1) / kThreads, 1 << 16)), moves.sequences);
+    const int64_t heads = static_cast<int64_t>(layers) * s.kv_heads;
+    const int64_t waves = (heads * (s.width * element_bytes(s.type) / 16) + 63) / 64 + heads * ((s.head_dim + 31) / 32);
+    if (waves > INT32_MAX / 128) return hipErrorInvalidValue;
+    const dim3 grid(static_cast<unsigned>((waves + kThreads / 64 - 1) / (kThreads / 64)), moves.sequences);
     if (s.type == kF32)
         cache_keep_kernel<float><<<grid, kThreads, 0, stream>>>(s, layers, moves);
     else
