@@ -3076,8 +3076,8 @@ int satori_hip_logit_rules_apply(satori_hip_logit_rules* r, const satori_hip_log
             const void* at;
             int64_t bytes;
         };
-        const int64_t in = ((rows - 1) * b->logits_stride + v) * 4, out = ((rows - 1) * b->output_stride + v) * 4;
-        const Range logits{b->logits, in}, output{b->output, b->output ? out : 0}, best{b->best, rows * 4};
+        const int64_t in = ((rows - 1) * b->logits_stride + v) * 4, out = b->output ? ((rows - 1) * b->output_stride + v) * 4 : 0;
+        const Range logits{b->logits, in}, output{b->output, out}, best{b->best, b->best ? rows * 4 : 0};
         const Range others[] = {{b->rows, rows * static_cast<int64_t>(sizeof(LogitRow))},
                                 {b->history, b->histories * b->history_stride * 4},
                                 {b->lengths, b->histories * int64_t(4)},

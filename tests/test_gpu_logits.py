@@ -351,6 +351,16 @@ def test_refused_calls(context, device):
         rules.set_biases(0, [1], [1.0])
 
 
+def test_strides_of_what_is_not_there_are_not_looked_at(context, device):
+    rules = LogitRules(context, 100)
+    b = Batch(context, device, np.arange(300, dtype=np.float32).reshape(3, 100), [row()] * 3, [[1]], [np.ones(100, bool)])
+    for stride in (2 ** 63 - 1, -2 ** 63):
+        rules.apply(LogitBatch(**{**b.arguments, "output": 0, "output_stride": stride, "histories": 0, "history_stride": stride,
+                                  "mask_count": 0, "mask_stride": stride}))
+        assert context.download(np.zeros(3, np.int32), b.arguments["best"]).tolist() == [99] * 3
+    rules.dispose()
+
+
 def test_rules_keep_their_context(device):
     other = S.HipContext(0)
     rules = LogitRules(other, 10)
