@@ -164,13 +164,14 @@ __global__ __launch_bounds__(kThreads, 4) void logits_kernel(LogitArgs a) {
             walked = -1;
             if (history >= 0) {
                 const int* tokens = a.history + history * a.history_stride;
-                const int length = static_cast<int>(min(static_cast<int64_t>(max(a.lengths[history], 0)), a.history_stride));
+                // (unsigned: the last turn's places pass 2^31 where the longest history's tokens end just below it)
+                const uint32_t length = static_cast<uint32_t>(min(static_cast<int64_t>(max(a.lengths[history], 0)), a.history_stride));
                 // Sixteen tokens a thread and turn, all on their way at once.
-                for (int k0 = 0; k0 < length; k0 += kThreads * 16) {
+                for (uint32_t k0 = 0; k0 < length; k0 += kThreads * 16) {
                     i32x4_a4 had[4];
 #pragma unroll
                     for (int k = 0; k < 4; ++k) {
-                        const int at = k0 + (k * kThreads + thread) * 4;
+                        const uint32_t at = k0 + (k * kThreads + thread) * 4;
                         if (at + 4 <= length) {
                             had[k] = *(const SATORI_GLOBAL i32x4_a4*)(tokens + at);
                         } else {
