@@ -524,7 +524,8 @@ int satori_hip_cache_append(satori_hip_cache_plan* plan, int layer, const float*
                             const float* value_bias, double frequency_base, int rotary_dimensions,
                             const double* rope_table, int rope_positions, void* stream);
 /* satori_hip_cache_append with a rotation's layout, dimensions and frequencies (satori_hip_rotation_create) in place of
- * RopeHalf's: the values of satori_hip_rotation_apply over the biased rows. */
+ * RopeHalf's: the values of satori_hip_rotation_apply over the biased rows, in FP32 (F16 pages round keys once more, as
+ * satori_hip_cache_append's). */
 int satori_hip_cache_append_rotated(satori_hip_cache_plan* plan, int layer, const float* query, const float* query_bias,
                                     float* query_out, const float* key, const float* key_bias, const float* value,
                                     const float* value_bias, satori_hip_rotation* rotation, void* stream);

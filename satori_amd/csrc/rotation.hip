@@ -46,8 +46,29 @@ __device__ __forceinline__ void store_pack(T* p, const float (&v)[N]) {
 // cosine of one pair of one row each and leave them in LDS, while what they turn first is on its way: four accesses of 16 bytes
 // a thread and turn, each half a head apart its pairs' other one (two heads), or with whole pairs (four heads). Behind the
 // last whole pack of a head single pairs; the lanes behind the rotated ones are copied, unless the output is the input.
-// Bound by the launch (8 rows of 12 heads 3.2 us) or by memory: 4096 rows of 32 heads of 128 F16 lanes 13.0 us, 67 MB at 5.2 TB/s
-// (two accesses a thread 14.4, eight 13.8; angles read by every thread, 64 bytes a pack, 18).
+// Bound by the launch (8 rows of 12 heads 3.2 us) or by memory: 4096 rows of 32 heads of 128 F16 lanes 13.2 us, 67 MB at 5.1 TB/s
+// (13.0 where a sum was rounded by way of FP32's nearest number; with that two accesses a thread 14.4, eight 13.8; angles read by
+// every thread, 64 bytes a pack, 18).
+
+// A sum as an FP32 number that rounds to F16 as the sum itself does: its first 24 bits, the last of them set where any behind
+// them is. That lies on the sum's side of every border between F16's numbers, which have 13 bits fewer. (FP32's nearest number may be
+// such a border itself, and would round away from the sum.)
+__device__ __forceinline__ float once(double v) {
+    const uint64_t bits = __double_as_longlong(v);
+    const uint32_t low = static_cast<uint32_t>(bits), behind = low & 0x1fffffffu;
+    const uint32_t kept = (low | (behind + 0x1fffffffu)) & 0xe0000000u;
+    return static_cast<float>(__longlong_as_double(bits >> 32 << 32 | kept));
+}
+// FP32 lanes have the bits of the cache write's (rope_apply); F16 ones fuse a product into each sum.
+template <typename T>
+__device__ __forceinline__ void turn_pair(double x, double y, double sn, double cs, float& a, float& b) {
+    if constexpr (sizeof(T) == 4) {
+        rope_apply(x, y, sn, cs, a, b);
+    } else {
+        a = once(fma(-y, sn, x * cs));
+        b = once(fma(y, cs, x * sn));
+    }
+}
 
 // Where a pair's angle lies: a pack's 128 bytes start at other banks than the next one's.
 __device__ __forceinline__ int angle_at(int i) { return i + (i >> 3); }
@@ -109,8 +130,8 @@ __global__ __launch_bounds__(kThreads) void rotate_kernel(RotationShape s, Rotat
                 const int at = INTERLEAVED ? 2 * (k0 + i) : k0 + i, beside = INTERLEAVED ? 1 : s.pairs;
                 for (int h = 0; h < r.heads; ++h) {
                     float u, v;
-                    rope_apply(static_cast<float>(r.in[h * D + at]), static_cast<float>(r.in[h * D + at + beside]), angle[0],
-                               angle[1], u, v);
+                    turn_pair<T>(static_cast<float>(r.in[h * D + at]), static_cast<float>(r.in[h * D + at + beside]), angle[0],
+                                 angle[1], u, v);
                     r.out[h * D + at] = static_cast<T>(u);
                     r.out[h * D + at + beside] = static_cast<T>(v);
                 }
@@ -122,7 +143,7 @@ __global__ __launch_bounds__(kThreads) void rotate_kernel(RotationShape s, Rotat
 #pragma unroll
                 for (int h = 0; h < kHeads; ++h) {
                     float &u = INTERLEAVED ? x[h][2 * j] : x[h][j], &v = INTERLEAVED ? x[h][2 * j + 1] : y[INTERLEAVED ? 0 : h][j];
-                    rope_apply(u, v, angle[0], angle[1], u, v);
+                    turn_pair<T>(u, v, angle[0], angle[1], u, v);
                 }
             }
             const int at = INTERLEAVED ? 2 * (k0 + k) : k0 + k;
