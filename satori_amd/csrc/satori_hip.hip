@@ -2500,12 +2500,15 @@ void set_plan(satori_hip_context* c, satori_hip_cache_plan* p, satori_hip_pages*
     p->set = true;
 }
 
-// The attention inputs of every row of the plan into its pages: by satori_hip_cache_append's arguments, or a rotation.
-void append_plan(satori_hip_context* c, satori_hip_cache_plan* p, AppendArgs args, void* stream) {
+void require_inputs(const AppendArgs& args) {
     require(args.query, "query");
     require(args.query_out, "queryOut");
     require(args.key, "key");
     require(args.value, "value");
+}
+
+// The attention inputs of every row of the plan into its pages: by satori_hip_cache_append's arguments, or a rotation.
+void append_plan(satori_hip_context* c, satori_hip_cache_plan* p, const AppendArgs& args, void* stream) {
     const CacheShape& s = p->shape;
     const hipStream_t st = op_stream(c, stream);
     if (!p->set) fail(SATORI_HIP_E_INVALID_OPERATION, "Set the plan's batch first.");
@@ -2649,12 +2652,12 @@ int satori_hip_cache_append(satori_hip_cache_plan* p, int layer, const float* qu
                             const float* value_bias, double frequency_base, int rotary_dimensions,
                             const double* rope_table, int rope_positions, void* stream) {
     return plan_call(p, [&](satori_hip_context* c) {
+        const AppendArgs args{query, query_bias, key, key_bias, value, value_bias, query_out, frequency_base, rotary_dimensions,
+                              rope_table, rope_table ? rope_positions : 0, layer, nullptr, 1.0, false};
+        require_inputs(args);
         check_rotation(p->shape.head_dim, frequency_base, rotary_dimensions);
         if (rope_positions < 0) out_of_range("ropePositions");
-        append_plan(c, p,
-                    AppendArgs{query, query_bias, key, key_bias, value, value_bias, query_out, frequency_base,
-                               rotary_dimensions, rope_table, rope_table ? rope_positions : 0, layer, nullptr, 1.0, false},
-                    stream);
+        append_plan(c, p, args, stream);
     });
 }
 
@@ -2664,10 +2667,10 @@ int satori_hip_cache_append_rotated(satori_hip_cache_plan* p, int layer, const f
     return plan_call(p, [&](satori_hip_context* c) {
         require_rotation(rotation, c, p->shape.head_dim);
         const RotationShape& r = rotation->shape;
-        append_plan(c, p,
-                    AppendArgs{query, query_bias, key, key_bias, value, value_bias, query_out, 1.0, 2 * r.pairs, r.table,
-                               r.positions, layer, r.frequencies, r.magnitude, r.interleaved},
-                    stream);
+        const AppendArgs args{query, query_bias, key, key_bias, value, value_bias, query_out, 1.0, 2 * r.pairs, r.table,
+                              r.positions, layer, r.frequencies, r.magnitude, r.interleaved};
+        require_inputs(args);
+        append_plan(c, p, args, stream);
         note_handle(c, rotation, op_stream(c, stream));
     });
 }
