@@ -506,7 +506,7 @@ int satori_hip_cache_plan_set(satori_hip_cache_plan* plan, satori_hip_pages* pag
  * SATORI_HIP_E_ARGUMENT_OUT_OF_RANGE. Row j lies at the j-th new position; its rotation is that of the position that it stands for,
  * the context's length plus its depth, and its attention sees the context, the rows that it follows and itself. Rows that follow
  * one another in order are no tree and may be any number, those of a tree 1024 of a sequence (SATORI_HIP_E_NOT_SUPPORTED).
- * All that is said of satori_hip_cache_plan_set holds. A plan that has held a tree is launched with kernels that look for one:
+ * All that is said of satori_hip_cache_plan_set holds. Captured launches look for trees where the plan has held one by then:
  * for a captured step to take trees, set a batch of as many rows with as large a tree before the capture (else
  * SATORI_HIP_E_INVALID_OPERATION). */
 int satori_hip_cache_plan_set_tree(satori_hip_cache_plan* plan, satori_hip_pages* pages, const int* sequences,

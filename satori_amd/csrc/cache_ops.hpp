@@ -62,7 +62,7 @@ struct AppendArgs {
     bool interleaved;
 };
 // `image`: a plan's on the device, `now` its header. `all`: the launch is captured and replays may read any plan, so its
-// grid must do for any. `trees`: the plan may hold trees.
+// grid must do for any. `trees`: the launch looks for trees.
 hipError_t launch_cache_append(const CacheShape& shape, const int* image, const PlanLayout& layout, const PlanHeader& now,
                                bool all, bool trees, const AppendArgs& args, hipStream_t stream);
 

@@ -220,8 +220,7 @@ struct satori_hip_cache_plan {
     int turn = 0;
     int steps = 0;                   // captured steps that read the plan
     int appends = 0;                 // those of them that write its rows
-    // Whether it has held a tree: its launches then look for one (and captured ones take batches with and without).
-    bool trees = false;
+    bool trees = false;              // it has held one: captured launches then look for trees, as replays may meet batches with and without
     std::vector<int> first_row, places;  // of the batch: every sequence's rows, and where each lies (KeepMoves)
     // Another library's graph may read it, or write its rows (until the plan is destroyed: such a graph's end is not told).
     bool elsewhere = false, appended_elsewhere = false;
@@ -2417,6 +2416,9 @@ bool note_plan(satori_hip_context* c, satori_hip_cache_plan* p, int layer, hipSt
     return true;
 }
 
+// Whether a launch looks for trees.
+bool looks_for_trees(const satori_hip_cache_plan* p, bool captured) { return captured ? p->trees : p->header.tree_stride > 0; }
+
 // A live rotation of the context for heads of head_dim lanes.
 void require_rotation(const satori_hip_rotation* r, const satori_hip_context* c, int head_dim) {
     require(r, "rotation");
@@ -2522,7 +2524,8 @@ void append_plan(satori_hip_context* c, satori_hip_cache_plan* p, const AppendAr
         bytes_overlap(args.key, kb, s.pool, pool) || bytes_overlap(args.value, kb, s.pool, pool))
         fail(SATORI_HIP_E_ARGUMENT, "Partial overlap.");
     const bool captured = note_plan(c, p, args.layer, st, true);
-    check_hip(launch_cache_append(s, static_cast<const int*>(p->image.ptr), p->layout, p->header, captured, p->trees, args, st),
+    check_hip(launch_cache_append(s, static_cast<const int*>(p->image.ptr), p->layout, p->header, captured,
+                                  looks_for_trees(p, captured), args, st),
               "cache append launch");
 }
 
@@ -2736,8 +2739,8 @@ int satori_hip_cache_attention(satori_hip_cache_plan* p, int layer, const float*
         if (bytes_overlap(query, bytes, output, bytes) || bytes_overlap(output, bytes, s.pool, pool))
             fail(SATORI_HIP_E_ARGUMENT, "Attention output overlaps input.");
         const bool captured = note_plan(c, p, layer, st, false);
-        check_hip(launch_cache_attention(s, static_cast<const int*>(p->image.ptr), p->layout, p->header, captured, p->trees,
-                                         layer, query, output, static_cast<float*>(p->partials.ptr), p->partials.bytes, st),
+        check_hip(launch_cache_attention(s, static_cast<const int*>(p->image.ptr), p->layout, p->header, captured,
+                                         looks_for_trees(p, captured), layer, query, output, static_cast<float*>(p->partials.ptr), p->partials.bytes, st),
                   "cache attention launch");
     });
 }
