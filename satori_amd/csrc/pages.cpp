@@ -217,6 +217,7 @@ constexpr int64_t kNarrowBytes = 128 << 20;
 constexpr int kMostTokens = 1 << 20;  // of an item
 // A layout larger than this is not made larger still for plain divisions to come.
 constexpr int64_t kMostPlainWords = 64 << 20;
+constexpr int64_t kMostWords = INT32_MAX / 8;  // of an image
 
 // Tokens [begin, end) of the pages of `sequence`, seen by the rows of the sequences members[0 .. count).
 struct Node {
@@ -253,6 +254,8 @@ namespace {
 // The numbers of every row of a batch whose rows follow `parents` (PlanHeader::tree_stride of them each), and the context of
 // every sequence that is a tree; -1 for the others. Nothing where none is. Room for as many rows and as large a tree behind
 // any context goes with what plain divisions take.
+// (All rows have as many numbers, so that a launch finds a row's without reading where they are: a prompt of 16,000 rows beside
+// a tree of 1024 makes 2.3 MB of them.)
 void plan_trees(const PageTables& tables, const int* sequences, const int* new_tokens, int count, const int* parents,
                 PlanImage& image, std::vector<int>& contexts) {
     int64_t stride = 0, first = 0, largest = 0;
@@ -272,10 +275,10 @@ void plan_trees(const PageTables& tables, const int* sequences, const int* new_t
         stride = std::max<int64_t>(stride, 1 + (context % kTile + rows + kTile - 1) / kTile);
     }
     if (stride == 0) return;
-    const int64_t most = first * (1 + (largest + 2 * (kTile - 1)) / kTile);
-    if (most > INT32_MAX / 64) fail(SATORI_HIP_E_OVERFLOW, "Arithmetic operation resulted in an overflow.");
+    if (first * stride > kMostWords) fail(SATORI_HIP_E_OVERFLOW, "Arithmetic operation resulted in an overflow.");
     image.header.tree_stride = static_cast<int>(stride);
-    image.plain.trees = static_cast<int>(most);
+    // (past this many grow_plain makes no room)
+    image.plain.trees = static_cast<int>(std::min(first * (1 + (largest + 2 * (kTile - 1)) / kTile), kMostPlainWords));
     image.trees.resize(first * stride);
     int* row = image.trees.data();
     first = 0;
@@ -637,7 +640,7 @@ bool PlanLayout::grow(const PlanLayout& least) {
     const auto place = [&](int& where, int64_t entries, size_t size) {
         where = static_cast<int>(at);
         at = (at + entries * static_cast<int64_t>(size / 4) + 3) / 4 * 4;  // 16-byte aligned
-        if (at > INT32_MAX / 8) fail(SATORI_HIP_E_OVERFLOW, "Arithmetic operation resulted in an overflow.");
+        if (at > kMostWords) fail(SATORI_HIP_E_OVERFLOW, "Arithmetic operation resulted in an overflow.");
     };
     place(rows_at, rows, sizeof(PlanRow));
     place(narrow_at, narrow, sizeof(PlanItem));
