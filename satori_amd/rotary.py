@@ -53,7 +53,7 @@ class Rotation:
         """Turns `rows` rows of `heads` heads at device pointer x by positions[row] (32-bit, on the device), into `out` or in
         place. Strides are elements from row to row; 0: rows lie side by side (in place: x's own)."""
         width = heads * head_dim
-        if not out:
+        if not out or out == x:
             out, out_stride = x, out_stride or stride
         _check(_ffi.lib().satori_hip_rotation_apply(self._handle, type, x, stride or width, out, out_stride or width, rows, heads,
                                                     head_dim, positions, stream))
