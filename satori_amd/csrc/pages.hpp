@@ -136,7 +136,6 @@ struct PlanShape {
     int kv_heads, group;  // group: query heads of a key/value head
     int wide_pairs;       // pairs of a wide workgroup; a narrow one takes 16
     int token_bytes;      // a position's key and value of one head
-    int places = 512;     // workgroups that the card holds at once
 };
 
 // A plan's arrays, and what its launches need to know.
