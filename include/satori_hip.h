@@ -577,8 +577,8 @@ int satori_hip_adapters_destroy(satori_hip_adapters* adapters);
  *  SATORI_HIP_SCALING_YARN        (Peng et al., 2023) f_k (1 - s + s / factor), s rising from 0 to 1 between the pairs that turn `high`
  *                                 times and `low` times over original_positions, k = r ln(original_positions / (2 pi turns)) /
  *                                 (2 ln base), rounded down and up (32 and 1 usually; base > 1); magnitude 1 + 0.1 ln(factor);
- *  SATORI_HIP_SCALING_WAVELENGTH  f_k (s + (1 - s) / factor), s = (turns - low) / (high - low) within 0 .. 1, turns =
- *                                 original_positions f_k / (2 pi) (4 and 1 usually).
+ *  SATORI_HIP_SCALING_WAVELENGTH  (Llama 3.1's release, 2024) f_k (s + (1 - s) / factor), s = (turns - low) / (high - low) within
+ *                                 0 .. 1, turns = original_positions f_k / (2 pi) (4 and 1 usually).
  * What a kind does not name is ignored. 0 < low < high. */
 #define SATORI_HIP_SCALING_NONE 0
 #define SATORI_HIP_SCALING_LINEAR 1
@@ -603,7 +603,8 @@ int satori_hip_rotation_destroy(satori_hip_rotation* rotation);
 
 /* ---- logits of a batch ----
  * No counterpart in the reference, whose samplers take logits as they are. For every row, in this order: a token that the row has
- * had n > 0 times becomes l > 0 ? l / repetition : l * repetition, then l - (presence + frequency * n); the row's biases are added;
+ * had n > 0 times becomes l > 0 ? l / repetition : l * repetition, then l - (presence + frequency * n) (all three penalties count
+ * the same tokens); the row's biases are added (one of 0 leaves the bits);
  * what its mask does not allow becomes -infinity, whatever it was. FP32, every operation rounded; a token that nothing of
  * this concerns keeps its bits. A row has had the tokens of its history and, where it is a draft, its own and those of the rows
  * that it follows. The best token is the lowest of the greatest logits (zeros of either sign are equal), -1 where none is greater
