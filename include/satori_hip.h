@@ -505,8 +505,9 @@ int satori_hip_cache_plan_set(satori_hip_cache_plan* plan, satori_hip_pages* pag
  * from the sequence's first new one and before it, or -1 for the context (several rows may have it); anything else fails with
  * SATORI_HIP_E_ARGUMENT_OUT_OF_RANGE. Row j lies at the j-th new position; its rotation is that of the position that it stands for,
  * the context's length plus its depth, and its attention sees the context, the rows that it follows and itself. Rows that follow
- * one another in order are no tree and may be any number, those of a tree 1024 of a sequence (SATORI_HIP_E_NOT_SUPPORTED); the
- * batch's rows, of either kind, times two more than a 32nd of its largest tree's must stay below 2^28 (SATORI_HIP_E_OVERFLOW).
+ * one another in order are no tree and may be any number, those of a tree 1024 of a sequence (SATORI_HIP_E_NOT_SUPPORTED). The
+ * plan has fewer than 2^28 numbers (SATORI_HIP_E_OVERFLOW); beside a tree each row of the batch, of either kind, has a 32nd of the
+ * largest tree's rows and up to three of them.
  * All that is said of satori_hip_cache_plan_set holds. Captured launches look for trees where the plan has held one by then:
  * for a captured step to take trees, set a batch of as many rows with as large a tree before the capture (else
  * SATORI_HIP_E_INVALID_OPERATION). */

@@ -241,7 +241,8 @@ constexpr int kLeastShared = 128;
 // the number serves them no better: F16, 256 lanes, 32 + 8 heads over 256 shared positions, 30 sequences take 31.1 us with 512
 // here and 38.8 with 256, 32 take 30.8 and 23.7, 40 take 32.5 with either; FP32, 30 sequences, 45.4 and 73.7.
 // Of batches with trees, whose sequences have many rows each: what a token costs a wide workgroup and one of 16 pairs (ns, two
-// workgroups a CU; measured with F16 heads of 128 lanes and used for all). A node is wide from a quarter of a wide workgroup's pairs on, where two narrow ones cost less than it
+// workgroups a CU; measured with F16 heads of 128 lanes and used for all). A node is wide from a quarter of a wide workgroup's
+// pairs on, where two narrow ones cost less than it
 // (32 sequences of 16 rows and 64 pairs over 4096 and 100 to 1000 positions: from half 198 us, from a quarter 151), and a run is
 // also shared where that saves more of this time than its partial results take (the same: 101).
 constexpr int64_t kWideTokenTime = 62, kNarrowTokenTime = 26;
@@ -463,8 +464,9 @@ PlanImage plan_batch(const PageTables& tables, const int* sequences, const int* 
         // 64 rows over 4000 to 16384 positions, F16, 32 + 8 heads, 247 us in chunks for 256 workgroups, 196 for 512, 234 so for 256
         // places, 186 for 512; 16 over 500 to 4000 135, 146, 168, 120; FP32, 12 + 2 heads, 8 over 2000 to 8000 232, 140, 188, 141.)
         // Of heads of 192 and 256 lanes the card holds half as many workgroups, and half the number serves some better and some
-        // worse, 512 here and 256: 8 trees of 64 over 1000 to 4000, 28 + 4 heads of 256, F16, 154 us and 184; 8 of 32, 192 lanes, FP32, 208 and 209, F16
-        // 90 and 79; 2 of 64 over 3000 and 6000, 32 + 8 of 256, F16, 83 and 75; 16 of 16 over 500 to 6000, 8 + 2 of 256, FP32, 113 and 102.
+        // worse, 512 here and 256: 8 trees of 64 over 1000 to 4000, 28 + 4 heads of 256, F16, 154 us and 184; 8 of 32, 192 lanes,
+        // FP32, 208 and 209, F16 90 and 79; 2 of 64 over 3000 and 6000, 32 + 8 of 256, F16, 83 and 75; 16 of 16 over 500 to 6000,
+        // 8 + 2 of 256, FP32, 113 and 102.
         const int64_t step = kTile * kWaves, places = kPlaces * division.workgroups / 256;
         const auto items_of = [&](int64_t chunk) {
             int64_t items = 0;

@@ -220,7 +220,7 @@ struct satori_hip_cache_plan {
     int turn = 0;
     int steps = 0;                   // captured steps that read the plan
     int appends = 0;                 // those of them that write its rows
-    bool trees = false;              // it has held one: captured launches then look for trees, as replays may meet batches with and without
+    bool trees = false;              // it has held one: captured launches then look for trees (replays may meet any batch)
     std::vector<int> first_row, places;  // of the batch: every sequence's rows, and where each lies (KeepMoves)
     // Another library's graph may read it, or write its rows (until the plan is destroyed: such a graph's end is not told).
     bool elsewhere = false, appended_elsewhere = false;
@@ -2740,7 +2740,8 @@ int satori_hip_cache_attention(satori_hip_cache_plan* p, int layer, const float*
             fail(SATORI_HIP_E_ARGUMENT, "Attention output overlaps input.");
         const bool captured = note_plan(c, p, layer, st, false);
         check_hip(launch_cache_attention(s, static_cast<const int*>(p->image.ptr), p->layout, p->header, captured,
-                                         looks_for_trees(p, captured), layer, query, output, static_cast<float*>(p->partials.ptr), p->partials.bytes, st),
+                                         looks_for_trees(p, captured), layer, query, output,
+                                         static_cast<float*>(p->partials.ptr), p->partials.bytes, st),
                   "cache attention launch");
     });
 }
